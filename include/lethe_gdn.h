@@ -245,6 +245,116 @@ int lethe_gdn_gate_spread(const float* dg0, const float* db0, const float* dw0, 
 /* boundaries.  No counterpart in the reference.                                                                        */
 int lethe_gdn_convert(const void* src, void* dst, int64_t n, int32_t to_f32, void* cuda_stream);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * What stands beside a recurrence with a matrix state in a model: the recurrence with one state value per channel, and the
+ * norms on both sides of a block.  No counterpart in the reference.  These calls take tensors in the type they have
+ * (LETHE_F32, LETHE_BF16, LETHE_F16), compute in fp32 and round each result once.  Strides and offsets count elements;
+ * rows are read where they lie, the innermost dimension contiguous; pointers on a boundary of their element.  Like the
+ * calls above they allocate nothing, enqueue on the given stream and return non-zero where nothing was launched; they work
+ * on the GPU that owns `x`.
+ * ------------------------------------------------------------------------------------------------------------------ */
+enum { LETHE_F32 = 0, LETHE_BF16 = 1, LETHE_F16 = 2 };
+
+/* The element-wise gated recurrence, for every sequence b and channel d:
+ *   h_t = exp(g_t) h_{t-1} + x_t                       (complement != 0: exp(g_t) h_{t-1} + (1 - exp(g_t)) x_t)
+ * forward: h and hT from x, g, h0.  backward, with e_t the gradient of h_t: e_t = d_h_t + exp(g_{t+1}) e_{t+1},
+ *   dx_t = e_t (times 1 - exp(g_t)),  dg_t = exp(g_t) e_t (h_{t-1} (- x_t)),  dh0 = exp(g_0) e_0.
+ * g is a natural-log decay, <= 0; minus infinity starts anew.  States are fp32; the decay of a long memory keeps its
+ * precision (1 - exp(g) is formed without the cancellation that exp(g) next to one would bring).
+ * Types: x, h, d_h, dx are x_type; g, dg are g_type, which is LETHE_F32 or x_type.  h0, hT, dhT, dh0 fp32 [B, D].
+ * h, dx, dg are contiguous [B, L, D]; x, g, d_h have strides of their own for batch and token.
+ * states: fp32, lethe_gdn_diag_states_bytes; the forward writes it where it is not NULL, the backward reads it.
+ * work: lethe_gdn_diag_work_bytes bytes on a 16-byte boundary, scratch of one call (NULL where that is 0).
+ * status: as above; a device-side wait that gave up leaves a non-zero code there. */
+typedef struct LetheGdnDiagArgs {
+  int64_t B, L, D;
+  int32_t x_type, g_type, complement;
+  const void* x;
+  int64_t x_batch, x_token;
+  const void* g;
+  int64_t g_batch, g_token;
+  const float* h0;        /* NULL: zero                                                     */
+  void* h;                /* forward                                                        */
+  float* hT;              /* NULL: not wanted                                               */
+  float* states;          /* forward: NULL where no backward follows                        */
+  const void* d_h;        /* backward; NULL: zero                                           */
+  int64_t d_h_batch, d_h_token;
+  const float* dhT;       /* NULL: zero                                                     */
+  void* dx;               /* NULL: not wanted, as dg and dh0                                */
+  void* dg;
+  float* dh0;
+  void* work;
+  size_t work_bytes;
+  int32_t* status;
+} LetheGdnDiagArgs;
+size_t lethe_gdn_diag_states_bytes(int64_t B, int64_t L, int64_t D);
+size_t lethe_gdn_diag_work_bytes(int64_t B, int64_t L, int64_t D);
+int lethe_gdn_diag_forward(const LetheGdnDiagArgs* args, void* cuda_stream);
+int lethe_gdn_diag_backward(const LetheGdnDiagArgs* args, void* cuda_stream);
+
+/* One token of it for generation: state [B, D] fp32, contiguous, updated in place; h [B, D] contiguous in x_type.  Uses B, D,
+ * the types, x, g and their batch strides. */
+int lethe_gdn_diag_step(const LetheGdnDiagArgs* args, float* state, void* cuda_stream);
+
+/* The norm behind a block: y = x rsqrt(mean(x^2) + eps) weight act(gate), act the logistic function, or gate times it (silu != 0).
+ * Rows of D values, 1 <= D <= 8192: row r = i * inner + j lies at i * outer_stride + j * inner_stride, for x and gate each;
+ * y, dx, dgate are contiguous.  x, gate, y, dy, dx, dgate are x_type; weight and dweight LETHE_F32 or x_type (w_type).
+ * dy contiguous.  work (vjp): lethe_gdn_norm_work_bytes(rows, D, 1) bytes on a 16-byte boundary, needed where dweight is wanted. */
+typedef struct LetheGdnGatedNormArgs {
+  int64_t rows, inner;
+  int32_t D, x_type, w_type, silu;
+  float eps;
+  const void* x;
+  int64_t x_outer, x_inner;
+  const void* gate;
+  int64_t gate_outer, gate_inner;
+  const void* weight;
+  void* y;
+  const void* dy;
+  void* dx;               /* NULL: not wanted, as dgate and dweight                         */
+  void* dgate;
+  void* dweight;
+  void* work;
+  size_t work_bytes;
+} LetheGdnGatedNormArgs;
+int lethe_gdn_gated_norm(const LetheGdnGatedNormArgs* args, void* cuda_stream);
+int lethe_gdn_gated_norm_vjp(const LetheGdnGatedNormArgs* args, void* cuda_stream);
+
+/* The residual sum and the norm in front of the next block:
+ *   t = x  or, with post_weight,  x rsqrt(mean(x^2) + eps) post_weight;     r = residual + scale t, rounded to r_type;
+ *   y = r rsqrt(mean(r^2) + eps) weight       (of r as it was rounded, so that every later reader of r sees the same).
+ * scale: a vector of D values, or NULL for the number scale_value.  residual NULL: zero.
+ * x, y, dy, dx are x_type; residual, r, dr, dresidual r_type (LETHE_F32 or x_type); weight, post_weight, scale and their
+ * gradients w_type (LETHE_F32 or x_type).  Rows of D values, 1 <= D <= 8192; x and residual have a stride between rows, the rest is contiguous.
+ * vjp: reads r as the forward wrote it, x where post_weight or dscale needs it, dy and dr (either may be NULL: zero).
+ * work (vjp): lethe_gdn_norm_work_bytes(rows, D, n) bytes on a 16-byte boundary, n the number of vector gradients wanted. */
+typedef struct LetheGdnResidualNormArgs {
+  int64_t rows;
+  int32_t D, x_type, r_type, w_type;
+  float eps, scale_value;
+  const void* x;
+  int64_t x_stride;
+  const void* residual;
+  int64_t residual_stride;
+  const void* weight;
+  const void* post_weight;  /* NULL: no norm of x                                           */
+  const void* scale;
+  void* r;
+  void* y;
+  const void* dy;
+  const void* dr;
+  void* dx;                 /* NULL: not wanted, as the other gradients                     */
+  void* dresidual;
+  void* dweight;
+  void* dpost_weight;
+  void* dscale;
+  void* work;
+  size_t work_bytes;
+} LetheGdnResidualNormArgs;
+size_t lethe_gdn_norm_work_bytes(int64_t rows, int32_t D, int32_t vectors);
+int lethe_gdn_residual_norm(const LetheGdnResidualNormArgs* args, void* cuda_stream);
+int lethe_gdn_residual_norm_vjp(const LetheGdnResidualNormArgs* args, void* cuda_stream);
+
 /* Text for a return code of the calls above or for a device status code. */
 const char* lethe_gdn_strerror(int code);
 

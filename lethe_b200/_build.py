@@ -23,7 +23,7 @@ LIB = os.path.join(LIBDIR, "liblethe_gdn.so")
 PROBE_SRC = os.path.join(ROOT, "tests", "native", "probe.cu")
 PROBE_LIBDIR = os.path.join(ROOT, "tests", "native", "_lib")
 PROBE_LIB = os.path.join(PROBE_LIBDIR, "libletheprobe.so")
-TORCH_SRC = os.path.join(CSRC, "torch_ops.cpp")
+TORCH_SRCS = [os.path.join(CSRC, f) for f in ("torch_ops.cpp", "torch_block.cpp")]
 TORCH_LIB = os.path.join(LIBDIR, "lethe_gdn_torch.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 # -use_fast_math: subnormal results flush to zero and division / square root are the approximate forms.
@@ -32,6 +32,8 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 # move (decays that small are zero in the fp16 operands anyway) and results stay bit-deterministic.
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-use_fast_math",
          "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr", "-I", os.path.join(ROOT, "include"), "-I", CSRC]
+# Not for these: their exponentials and roots stand in fp32 results.
+EXACT_MATH = {"diag_scan.cu", "block_norm.cu", "residual_norm.cu"}
 FLAGS += os.environ.get("LETHE_NVCC_FLAGS", "").split()
 
 
@@ -72,7 +74,8 @@ def _run(cmd, what, verbose):
 
 def _compile(src, obj, verbose):
     tmp = f"{obj}.{os.getpid()}.tmp"
-    cmd = [NVCC, *FLAGS, "-c", src, "-o", tmp]
+    flags = [f for f in FLAGS if f != "-use_fast_math"] if os.path.basename(src) in EXACT_MATH else FLAGS
+    cmd = [NVCC, *flags, "-c", src, "-o", tmp]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")
     _run(cmd, f"nvcc {os.path.basename(src)}", verbose)
@@ -103,9 +106,9 @@ def build(force: bool = False, verbose: bool = False) -> str:
 
 
 def build_torch(force: bool = False, verbose: bool = False) -> str:
-    """The extension module that binds the CUDA library to PyTorch (``csrc/torch_ops.cpp``, host code only)."""
+    """The extension module that binds the CUDA library to PyTorch (``csrc/torch_*.cpp``, host code only)."""
     build()
-    deps = [TORCH_SRC, os.path.join(ROOT, "include", "lethe_gdn.h")]
+    deps = [*TORCH_SRCS, os.path.join(CSRC, "torch_util.h"), os.path.join(ROOT, "include", "lethe_gdn.h")]
     fresh = lambda: os.path.exists(TORCH_LIB) and os.path.getmtime(TORCH_LIB) >= max(map(os.path.getmtime, deps))
     if not force and fresh():
         return TORCH_LIB
@@ -120,12 +123,22 @@ def build_torch(force: bool = False, verbose: bool = False) -> str:
         tmp = f"{TORCH_LIB}.{os.getpid()}.tmp"
         incs = [os.path.join(t, "include"), os.path.join(t, "include", "torch", "csrc", "api", "include"),
                 os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
-        _run(["g++", "-shared", "-fPIC", "-O2", "-std=c++17", "-w",
-              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_EXTENSION_NAME=lethe_gdn_torch",
-              *[f"-I{i}" for i in incs], TORCH_SRC, "-o", tmp, f"-L{LIBDIR}", "-l:" + os.path.basename(LIB),
+        flags = ["-fPIC", "-O2", "-std=c++17", "-w", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                 "-DTORCH_EXTENSION_NAME=lethe_gdn_torch", *[f"-I{i}" for i in incs]]
+
+        def obj(src):
+            o = os.path.join(LIBDIR, f"{os.path.basename(src)[:-4]}.{os.getpid()}.tmp.o")
+            _run(["g++", *flags, "-c", src, "-o", o], f"g++ {os.path.basename(src)}", verbose)
+            return o
+
+        with ThreadPoolExecutor(max_workers=len(TORCH_SRCS)) as ex:
+            objs = list(ex.map(obj, TORCH_SRCS))
+        _run(["g++", "-shared", *objs, "-o", tmp, f"-L{LIBDIR}", "-l:" + os.path.basename(LIB),
               "-Wl,-rpath,$ORIGIN", "-L" + os.path.join(t, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
               "-L" + os.path.join(cuda, "lib64"), "-lcudart_static", "-ldl", "-lrt", "-lpthread"],
-             "g++ torch_ops.cpp", verbose)
+             "link " + os.path.basename(TORCH_LIB), verbose)
+        for o in objs:
+            os.remove(o)
         os.replace(tmp, TORCH_LIB)
     return TORCH_LIB
 

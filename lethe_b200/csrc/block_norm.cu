@@ -1,0 +1,217 @@
+// The norm behind a block, y = x / rms(x) * weight * act(gate), its vector-Jacobian product, and the column sums of both norms.
+//
+//   r = rsqrt(mean x^2 + eps), n = x r, a = act(gate) (logistic s, or gate s), y = n w a
+//   dgate = dy n w a',  a' = s (1 - s) or s (1 + gate (1 - s));   dweight = sum over rows of dy n a
+//   dn = dy w a,  dx = r (dn - n mean(dn n))
+//
+// Bound by HBM: 6 bytes a value forward and 10 backward in 16 bits.  mean(dn n) = r mean(dn x), so both row sums of the backward
+// are of what was loaded and are formed together.
+#include "block_norm.cuh"
+
+namespace lg {
+
+struct GatedProblem {
+  long long rows, inner;
+  int D, w_f32, silu;
+  float eps;
+  const void* x;
+  long long xo, xi;
+  const void* z;
+  long long zo, zi;
+  const void* w;
+  void* y;
+  const void* dy;
+  void *dx, *dz;
+  float* part;      // per CTA the sums for dweight; NULL: not wanted
+};
+
+// logistic function: the division's approximation is good to 2 ulp and the divisor is in [1, inf]
+__device__ __forceinline__ float logistic(float z) { return __fdividef(1.f, 1.f + expf(-z)); }
+
+template <int XT, typename S>
+__global__ void __launch_bounds__(S::kThreads) gated_norm_kernel(const GatedProblem p) {
+  __shared__ float sums[2][1][S::kWarps];
+  const int t = threadIdx.x % S::T;
+  const long long first = static_cast<long long>(blockIdx.x) * S::kRows + threadIdx.x / S::T, step = static_cast<long long>(gridDim.x) * S::kRows;
+  float w[S::N];
+  S::template vector<XT>(w, p.w, p.w_f32, t, p.D, 0.f);
+  RowWalk at(first, step, p.inner);
+  const float over = 1.f / p.D;
+  int flip = 0;
+  // every thread of a CTA takes as many turns: row sums are collective
+  for (long long row = first, base = first - threadIdx.x / S::T; base < p.rows; row += step, base += step, at.next(), flip ^= 1) {
+    const bool live = row < p.rows;
+    Raw<XT, 8> x[S::R], z[S::R];
+    if (live) {
+      S::template load<XT>(x, p.x, at.at(p.xo, p.xi), t, p.D);
+      S::template load<XT>(z, p.z, at.at(p.zo, p.zi), t, p.D);
+    } else {
+#pragma unroll
+      for (int i = 0; i < S::R; ++i) {
+        x[i].zero();
+        z[i].zero();
+      }
+    }
+    float s[1] = {0.f};
+#pragma unroll
+    for (int n = 0; n < S::N; ++n) s[0] = fmaf(x[n / 8].get(n % 8), x[n / 8].get(n % 8), s[0]);
+    S::template row_sums<1>(s, sums[flip]);
+    const float r = rsqrtf(fmaf(s[0], over, p.eps));
+    float y[S::N];
+#pragma unroll
+    for (int n = 0; n < S::N; ++n) {
+      const float zv = z[n / 8].get(n % 8), sg = logistic(zv);
+      y[n] = x[n / 8].get(n % 8) * r * w[n] * (p.silu ? zv * sg : sg);
+    }
+    if (live) S::template store<XT>(y, p.y, row * p.D, t, p.D);
+  }
+}
+
+template <int XT, typename S>
+__global__ void __launch_bounds__(S::kThreads) gated_norm_vjp_kernel(const GatedProblem p) {
+  __shared__ float sums[2][2][S::kWarps];
+  extern __shared__ float stage[];
+  const int t = threadIdx.x % S::T;
+  const long long first = static_cast<long long>(blockIdx.x) * S::kRows + threadIdx.x / S::T, step = static_cast<long long>(gridDim.x) * S::kRows;
+  float w[S::N], acc[S::N];
+  S::template vector<XT>(w, p.w, p.w_f32, t, p.D, 0.f);
+#pragma unroll
+  for (int n = 0; n < S::N; ++n) acc[n] = 0.f;
+  RowWalk at(first, step, p.inner);
+  const float over = 1.f / p.D;
+  int flip = 0;
+  for (long long row = first, base = first - threadIdx.x / S::T; base < p.rows; row += step, base += step, at.next(), flip ^= 1) {
+    const bool live = row < p.rows;
+    Raw<XT, 8> x[S::R], z[S::R], d[S::R];
+    if (live) {
+      S::template load<XT>(x, p.x, at.at(p.xo, p.xi), t, p.D);
+      S::template load<XT>(z, p.z, at.at(p.zo, p.zi), t, p.D);
+      S::template load<XT>(d, p.dy, row * p.D, t, p.D);
+    } else {
+#pragma unroll
+      for (int i = 0; i < S::R; ++i) {
+        x[i].zero();
+        z[i].zero();
+        d[i].zero();
+      }
+    }
+    float s[2] = {0.f, 0.f}, dn[S::N], slope[S::N];
+#pragma unroll
+    for (int n = 0; n < S::N; ++n) {
+      const float xv = x[n / 8].get(n % 8), zv = z[n / 8].get(n % 8), dv = d[n / 8].get(n % 8), sg = logistic(zv);
+      const float a = p.silu ? zv * sg : sg;
+      slope[n] = dv * (p.silu ? sg * fmaf(zv, 1.f - sg, 1.f) : sg * (1.f - sg));
+      dn[n] = dv * a;
+      s[0] = fmaf(xv, xv, s[0]);
+      s[1] = fmaf(dn[n] * w[n], xv, s[1]);
+    }
+    S::template row_sums<2>(s, sums[flip]);
+    const float r = rsqrtf(fmaf(s[0], over, p.eps)), c = s[1] * over * r * r;
+    float dx[S::N];
+#pragma unroll
+    for (int n = 0; n < S::N; ++n) {
+      const float xv = x[n / 8].get(n % 8);
+      dx[n] = r * (dn[n] * w[n] - xv * c);
+      acc[n] = fmaf(dn[n], xv * r, acc[n]);
+      slope[n] *= xv * r * w[n];
+    }
+    if (live) {
+      if (p.dx) S::template store<XT>(dx, p.dx, row * p.D, t, p.D);
+      if (p.dz) S::template store<XT>(slope, p.dz, row * p.D, t, p.D);
+    }
+  }
+  if (p.part) S::column_share(acc, p.part + static_cast<long long>(blockIdx.x) * p.D, stage, t, p.D);
+}
+
+// 32 columns a CTA; a warp takes every 32nd share, the warps' sums are added in their order.
+template <int XT>
+__global__ void __launch_bounds__(1024) column_sums_kernel(const ColumnSums c) {
+  __shared__ float s[32][33];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, v = blockIdx.y, col = blockIdx.x * 32 + lane;
+  float a = 0.f;
+  if (col < c.D) {
+    const float* p = c.part + static_cast<long long>(v) * c.D + col;
+    const long long line = static_cast<long long>(c.vectors) * c.D;
+#pragma unroll 8
+    for (int i = warp; i < c.parts; i += 32) a += p[i * line];
+  }
+  s[warp][lane] = a;
+  __syncthreads();
+  if (warp == 0 && col < c.D) {
+    a = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) a += s[i][lane];
+    if (c.f32[v]) static_cast<float*>(c.out[v])[col] = a;
+    else static_cast<typename Elem<XT>::T*>(c.out[v])[col] = from_f32<XT>(a);
+  }
+}
+
+int launch_column_sums(const ColumnSums& c, cudaStream_t st) {
+  return by_x_type(c.x_type, [&](auto x) {
+    column_sums_kernel<x.value><<<dim3((c.D + 31) / 32, c.vectors), 1024, 0, st>>>(c);
+    return launched_ok();
+  });
+}
+
+static int gated_problem(const LetheGdnGatedNormArgs* a, GatedProblem* p, bool backward) {
+  if (!a) return kErrNull;
+  if (a->rows <= 0 || a->inner <= 0 || a->D <= 0 || a->D > kNormMaxD || !norm_types_ok(a->x_type, a->w_type) || !(a->eps >= 0.f)) return kErrDims;
+  if (!a->x || !a->gate || !a->weight || (!backward && !a->y) || (backward && !a->dy)) return kErrNull;
+  *p = {a->rows, a->inner, a->D, a->w_type == LETHE_F32, a->silu, a->eps, a->x, a->x_outer, a->x_inner, a->gate, a->gate_outer, a->gate_inner,
+        a->weight, a->y, a->dy, a->dx, a->dgate, nullptr};
+  return kOk;
+}
+
+}  // namespace lg
+
+extern "C" size_t lethe_gdn_norm_work_bytes(int64_t rows, int32_t D, int32_t vectors) {
+  using namespace lg;
+  if (rows <= 0 || D <= 0 || D > kNormMaxD || vectors <= 0 || vectors > 3) return 0;
+  return static_cast<size_t>(std::min<int64_t>(rows, norm_parts_max(D))) * D * vectors * sizeof(float);
+}
+
+extern "C" int lethe_gdn_gated_norm(const LetheGdnGatedNormArgs* a, void* stream) {
+  using namespace lg;
+  GatedProblem p;
+  if (int e = gated_problem(a, &p, false)) return e;
+  DeviceGuard guard(a->x);
+  if (!guard.ok) return kErrDevice;
+  const bool vec = p.D % 8 == 0 && piece_aligned(p.x, a->x_type, p.xo, p.xi) && piece_aligned(p.z, a->x_type, p.zo, p.zi) && piece_aligned(p.y, a->x_type);
+  return by_x_type(a->x_type, [&](auto x) {
+    return by_row_shape(p.D, vec, [&](auto s) {
+      using S = decltype(s);
+      const int grid = norm_grid(p.rows, S::kRows, 2048 / S::kThreads);
+      gated_norm_kernel<x.value, S><<<grid, S::kThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+      return launched_ok();
+    });
+  });
+}
+
+extern "C" int lethe_gdn_gated_norm_vjp(const LetheGdnGatedNormArgs* a, void* stream) {
+  using namespace lg;
+  GatedProblem p;
+  if (int e = gated_problem(a, &p, true)) return e;
+  if (a->dweight) {
+    if (!a->work) return kErrNull;
+    if (a->work_bytes < lethe_gdn_norm_work_bytes(a->rows, a->D, 1)) return kErrWorkspace;
+    if (reinterpret_cast<uintptr_t>(a->work) & 15) return kErrAlign;
+    p.part = static_cast<float*>(a->work);
+  }
+  DeviceGuard guard(a->x);
+  if (!guard.ok) return kErrDevice;
+  const bool vec = p.D % 8 == 0 && piece_aligned(p.x, a->x_type, p.xo, p.xi) && piece_aligned(p.z, a->x_type, p.zo, p.zi) &&
+                   piece_aligned(p.dy, a->x_type) && piece_aligned(p.dx, a->x_type) && piece_aligned(p.dz, a->x_type);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int grid = 0;
+  const int e = by_x_type(a->x_type, [&](auto x) {
+    return by_row_shape(p.D, vec, [&](auto s) {
+      using S = decltype(s);
+      grid = std::min(norm_grid(p.rows, S::kRows, 1024 / S::kThreads), norm_parts_max(p.D));
+      constexpr int smem = S::kRows > 1 ? S::kThreads * S::N * 4 : 0;
+      gated_norm_vjp_kernel<x.value, S><<<grid, S::kThreads, smem, st>>>(p);
+      return launched_ok();
+    });
+  });
+  if (e || !p.part) return e;
+  return launch_column_sums({p.part, grid, 1, p.D, {a->dweight}, {p.w_f32}, a->x_type}, st);
+}

@@ -1,0 +1,182 @@
+// Rows of the norms in front of and behind a block: who holds what of a row, row sums, column sums over rows.
+//
+// A row of D values is held by T threads with R pieces of 8 values each (T R 8 >= D) and stays in registers from its loads to its
+// stores.  T <= 32: a CTA of 256 threads has 256 / T rows at a time, sums are butterflies.  T > 32: a CTA of T threads has one
+// row, sums go through shared memory.  CTAs go over the rows with the grid's stride, so that what belongs to a column (weights,
+// sums for their gradients) stays in registers as well.  Sums over rows: a CTA's share in the order of its rows, the CTAs'
+// shares by a kernel of its own in the order of the CTAs.  No atomics: two runs give the same bits.
+#pragma once
+#include <algorithm>
+#include <type_traits>
+
+#include "elem.cuh"
+#include "host_util.h"
+
+namespace lg {
+
+constexpr int kNormMaxD = 8192;
+
+// CTAs of a backward at most: what the work buffer holds partial sums of
+inline int norm_parts_max(int D) { return D <= 2048 ? 1024 : 320; }
+
+template <int T_, int R_, bool VEC_>
+struct RowShape {
+  static constexpr int T = T_, R = R_, N = R_ * 8;
+  static constexpr bool VEC = VEC_;
+  static constexpr int kThreads = T > 32 ? T : 256, kRows = kThreads / T;
+  static constexpr int kWarps = kThreads / 32;
+  // column of value n (of N) that thread t of a row holds
+  __device__ __forceinline__ static int col(int t, int n) { return VEC ? ((n / 8) * T + t) * 8 + n % 8 : n * T + t; }
+
+  template <int TY>
+  __device__ __forceinline__ static void load(Raw<TY, 8> (&r)[R], const void* base, long long row, int t, int D) {
+    const typename Elem<TY>::T* p = static_cast<const typename Elem<TY>::T*>(base) + row;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      r[i].zero();
+      if constexpr (VEC) {
+        if ((i * T + t) * 8 < D) r[i].load(p + (i * T + t) * 8);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (col(t, i * 8 + j) < D) raw_put(r[i], j, __ldg(p + col(t, i * 8 + j)));
+      }
+    }
+  }
+  template <int TY>
+  __device__ __forceinline__ static void store(const float (&v)[N], void* base, long long row, int t, int D) {
+    typename Elem<TY>::T* p = static_cast<typename Elem<TY>::T*>(base) + row;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      if constexpr (VEC) {
+        if ((i * T + t) * 8 < D) {
+          Raw<TY, 8> r;
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) r.set2(j, v[i * 8 + j], v[i * 8 + j + 1]);
+          r.store(p + (i * T + t) * 8);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (col(t, i * 8 + j) < D) p[col(t, i * 8 + j)] = from_f32<TY>(v[i * 8 + j]);
+      }
+    }
+  }
+  // a vector of D values (weight, scale), fp32 or XT; `none` where there is no vector
+  template <int XT>
+  __device__ __forceinline__ static void vector(float (&v)[N], const void* p, bool f32, int t, int D, float none) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int c = col(t, n);
+      v[n] = none;
+      if (p && c < D) v[n] = f32 ? __ldg(static_cast<const float*>(p) + c) : to_f32(__ldg(static_cast<const typename Elem<XT>::T*>(p) + c));
+    }
+  }
+  // sums of K values over the threads of a row, in all of them.  `buf`: this sum's place in shared memory, not that of the sum before.
+  template <int K>
+  __device__ __forceinline__ static void row_sums(float (&s)[K], float (*buf)[kWarps]) {
+#pragma unroll
+    for (int m = (T < 32 ? T : 32) / 2; m >= 1; m >>= 1)
+#pragma unroll
+      for (int k = 0; k < K; ++k) s[k] += __shfl_xor_sync(0xffffffffu, s[k], m);
+    if constexpr (T > 32) {
+      if (threadIdx.x % 32 == 0)
+#pragma unroll
+        for (int k = 0; k < K; ++k) buf[k][threadIdx.x / 32] = s[k];
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        float a = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) a += buf[k][w];
+        s[k] = a;
+      }
+    }
+  }
+  // the CTA's share of a sum over rows: out[col] of its line of the work buffer.  `stage`: kThreads * N floats where a CTA has several rows.
+  __device__ __forceinline__ static void column_share(const float (&acc)[N], float* out, float* stage, int t, int D) {
+    if constexpr (kRows == 1) {
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        if (col(t, n) < D) out[col(t, n)] = acc[n];
+    } else {
+      const int slot = threadIdx.x / T;
+      __syncthreads();
+#pragma unroll
+      for (int n = 0; n < N; ++n) stage[slot * (T * N) + col(t, n)] = acc[n];
+      __syncthreads();
+      for (int c = threadIdx.x; c < D; c += kThreads) {
+        float a = 0.f;
+        for (int i = 0; i < kRows; ++i) a += stage[i * (T * N) + c];
+        out[c] = a;
+      }
+    }
+  }
+};
+
+// Walks the rows of a tensor with two strides, row r = (r / inner, r % inner), by a fixed step: one division at the start.
+struct RowWalk {
+  long long o, i, step_o, step_i, inner;
+  __device__ __forceinline__ RowWalk(long long first, long long step, long long inner_) : inner(inner_) {
+    o = first / inner;
+    i = first - o * inner;
+    step_o = step / inner;
+    step_i = step - step_o * inner;
+  }
+  __device__ __forceinline__ void next() {
+    o += step_o;
+    i += step_i;
+    if (i >= inner) {
+      i -= inner;
+      ++o;
+    }
+  }
+  __device__ __forceinline__ long long at(long long outer_stride, long long inner_stride) const { return o * outer_stride + i * inner_stride; }
+};
+
+// f(RowShape) for rows of D values.  Where pieces of 8 cannot be loaded as such, fewer shapes: these loads are what bounds.
+template <typename F>
+int by_row_shape(int D, bool vec, F&& f) {
+  if (!vec) {
+    if (D <= 256) return f(RowShape<32, 1, false>());
+    if (D <= 2048) return f(RowShape<256, 1, false>());
+    return f(RowShape<512, 2, false>());
+  }
+  if (D <= 64) return f(RowShape<8, 1, true>());
+  if (D <= 128) return f(RowShape<16, 1, true>());
+  if (D <= 256) return f(RowShape<32, 1, true>());
+  if (D <= 512) return f(RowShape<32, 2, true>());
+  if (D <= 1024) return f(RowShape<128, 1, true>());
+  if (D <= 2048) return f(RowShape<256, 1, true>());
+  if (D <= 4096) return f(RowShape<512, 1, true>());
+  return f(RowShape<512, 2, true>());
+}
+
+template <typename F>
+int by_x_type(int xt, F&& f) {
+  if (xt == LETHE_F32) return f(std::integral_constant<int, LETHE_F32>());
+  if (xt == LETHE_BF16) return f(std::integral_constant<int, LETHE_BF16>());
+  return f(std::integral_constant<int, LETHE_F16>());
+}
+
+inline bool norm_types_ok(int xt, int other) { return xt >= LETHE_F32 && xt <= LETHE_F16 && (other == LETHE_F32 || other == xt); }
+// 8 elements of type ty from ptr on can be loaded as 16-byte pieces, in every row
+inline bool piece_aligned(const void* ptr, int, long long s0 = 0, long long s1 = 0) {
+  return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && s0 % 8 == 0 && s1 % 8 == 0;
+}
+inline int norm_grid(long long rows, int rows_per_cta, int ctas_per_sm) {
+  const long long need = (rows + rows_per_cta - 1) / rows_per_cta;
+  return static_cast<int>(std::min<long long>(need, static_cast<long long>(sm_count()) * ctas_per_sm));
+}
+inline int launched_ok() { return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch; }
+
+// Sums the CTAs' shares: part[cta][vector][D] -> out[vector][D].
+struct ColumnSums {
+  const float* part;
+  int parts, vectors, D;
+  void* out[3];
+  int f32[3], x_type;
+};
+int launch_column_sums(const ColumnSums& c, cudaStream_t st);
+
+}  // namespace lg

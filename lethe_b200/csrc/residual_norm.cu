@@ -1,0 +1,248 @@
+// The residual sum and the norm in front of the next block, and its vector-Jacobian product.
+//
+//   t = x, or n1 pw with n1 = x r1, r1 = rsqrt(mean x^2 + eps);   r = residual + scale t, rounded to the stream's type
+//   y = n2 w, n2 = r r2, r2 = rsqrt(mean r^2 + eps)
+//   d = dr + r2 (dy w - n2 mean(dy w n2)) = dresidual;   dweight = sum over rows of dy n2,  dscale = sum of d t
+//   dx = scale d,  or r1 (u pw - n1 mean(u pw n1)) with u = scale d;  dpost_weight = sum of u n1
+//
+// Bound by HBM.  The backward takes n2 from r as it was stored, so it reads the stream once and x only where the branch has
+// something to learn.
+#include "block_norm.cuh"
+
+namespace lg {
+
+struct ResidualProblem {
+  long long rows;
+  int D, w_f32;
+  float eps, scale_value;
+  const void* x;
+  long long x_stride;
+  const void* res;
+  long long res_stride;
+  const void *w, *pw, *scale;
+  void *r, *y;
+  const void *dy, *dr;
+  void *dx, *dres;
+  float *part;              // per CTA: the vectors that are wanted, in the order dweight, dpost_weight, dscale
+  int vectors, at[3];       // their number, and the place of each (-1: not wanted)
+};
+
+template <int XT, int RT, typename S, bool POST>
+__global__ void __launch_bounds__(S::kThreads) residual_norm_kernel(const ResidualProblem p) {
+  __shared__ float sums[2][1][S::kWarps];
+  const int t = threadIdx.x % S::T;
+  const long long first = static_cast<long long>(blockIdx.x) * S::kRows + threadIdx.x / S::T, step = static_cast<long long>(gridDim.x) * S::kRows;
+  float w[S::N], sc[S::N], pw[POST ? S::N : 1];
+  S::template vector<XT>(w, p.w, p.w_f32, t, p.D, 0.f);
+  S::template vector<XT>(sc, p.scale, p.w_f32, t, p.D, p.scale_value);
+  if constexpr (POST) S::template vector<XT>(pw, p.pw, p.w_f32, t, p.D, 0.f);
+  const float over = 1.f / p.D;
+  for (long long row = first, base = first - threadIdx.x / S::T; base < p.rows; row += step, base += step) {
+    const bool live = row < p.rows;
+    Raw<XT, 8> x[S::R];
+    Raw<RT, 8> res[S::R];
+#pragma unroll
+    for (int i = 0; i < S::R; ++i) {
+      x[i].zero();
+      res[i].zero();
+    }
+    if (live) {
+      S::template load<XT>(x, p.x, row * p.x_stride, t, p.D);
+      if (p.res) S::template load<RT>(res, p.res, row * p.res_stride, t, p.D);
+    }
+    float r1 = 1.f;
+    if constexpr (POST) {
+      float s[1] = {0.f};
+#pragma unroll
+      for (int n = 0; n < S::N; ++n) s[0] = fmaf(x[n / 8].get(n % 8), x[n / 8].get(n % 8), s[0]);
+      S::template row_sums<1>(s, sums[0]);
+      r1 = rsqrtf(fmaf(s[0], over, p.eps));
+    }
+    float v[S::N], s[1] = {0.f};
+#pragma unroll
+    for (int n = 0; n < S::N; ++n) {
+      float b = x[n / 8].get(n % 8);
+      if constexpr (POST) b = b * r1 * pw[n];
+      // product and sum are rounded each, as the formula reads: with one rounding a sum could fall to the other side of a tie of the stored type
+      v[n] = to_f32(from_f32<RT>(__fadd_rn(res[n / 8].get(n % 8), __fmul_rn(b, sc[n]))));
+      s[0] = fmaf(v[n], v[n], s[0]);
+    }
+    if (live) S::template store<RT>(v, p.r, row * p.D, t, p.D);
+    S::template row_sums<1>(s, sums[1]);
+    const float r2 = rsqrtf(fmaf(s[0], over, p.eps));
+#pragma unroll
+    for (int n = 0; n < S::N; ++n) v[n] = v[n] * r2 * w[n];
+    if (live) S::template store<XT>(v, p.y, row * p.D, t, p.D);
+    if constexpr (!POST && S::T > 32) __syncthreads();      // sums[1] is read by now (with POST the sum in between says so)
+  }
+}
+
+// BRANCH 0: nothing of x is needed.  1: x for dscale.  2: norm of x.
+template <int XT, int RT, typename S, int BRANCH>
+__global__ void __launch_bounds__(S::kThreads) residual_norm_vjp_kernel(const ResidualProblem p) {
+  __shared__ float sums[2][3][S::kWarps];
+  extern __shared__ float stage[];
+  const int t = threadIdx.x % S::T;
+  const long long first = static_cast<long long>(blockIdx.x) * S::kRows + threadIdx.x / S::T, step = static_cast<long long>(gridDim.x) * S::kRows;
+  constexpr int NB = BRANCH == 2 ? S::N : 1, NS = BRANCH >= 1 ? S::N : 1;
+  float w[S::N], sc[S::N], pw[NB], acc_w[S::N], acc_p[NB], acc_s[NS];
+  S::template vector<XT>(w, p.w, p.w_f32, t, p.D, 0.f);
+  S::template vector<XT>(sc, p.scale, p.w_f32, t, p.D, p.scale_value);
+  if constexpr (BRANCH == 2) S::template vector<XT>(pw, p.pw, p.w_f32, t, p.D, 0.f);
+#pragma unroll
+  for (int n = 0; n < S::N; ++n) {
+    acc_w[n] = 0.f;
+    if constexpr (BRANCH == 2) acc_p[n] = 0.f;
+    if constexpr (BRANCH >= 1) acc_s[n] = 0.f;
+  }
+  const float over = 1.f / p.D;
+  for (long long row = first, base = first - threadIdx.x / S::T; base < p.rows; row += step, base += step) {
+    const bool live = row < p.rows;
+    Raw<XT, 8> x[S::R], dy[S::R];
+    Raw<RT, 8> r[S::R], dr[S::R];
+#pragma unroll
+    for (int i = 0; i < S::R; ++i) {
+      x[i].zero();
+      dy[i].zero();
+      r[i].zero();
+      dr[i].zero();
+    }
+    if (live) {
+      S::template load<RT>(r, p.r, row * p.D, t, p.D);
+      if (p.dy) S::template load<XT>(dy, p.dy, row * p.D, t, p.D);
+      if (p.dr) S::template load<RT>(dr, p.dr, row * p.D, t, p.D);
+      if constexpr (BRANCH >= 1) S::template load<XT>(x, p.x, row * p.x_stride, t, p.D);
+    }
+    float s[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < S::N; ++n) {
+      const float rv = r[n / 8].get(n % 8);
+      s[0] = fmaf(rv, rv, s[0]);
+      s[1] = fmaf(dy[n / 8].get(n % 8) * w[n], rv, s[1]);
+      if constexpr (BRANCH == 2) s[2] = fmaf(x[n / 8].get(n % 8), x[n / 8].get(n % 8), s[2]);
+    }
+    S::template row_sums<3>(s, sums[0]);
+    const float r2 = rsqrtf(fmaf(s[0], over, p.eps)), c2 = s[1] * over * r2 * r2;
+    const float r1 = BRANCH == 2 ? rsqrtf(fmaf(s[2], over, p.eps)) : 1.f;
+    float d[S::N], q[1] = {0.f};
+#pragma unroll
+    for (int n = 0; n < S::N; ++n) {
+      const float rv = r[n / 8].get(n % 8), dyv = dy[n / 8].get(n % 8);
+      acc_w[n] = fmaf(dyv, rv * r2, acc_w[n]);
+      d[n] = fmaf(r2, dyv * w[n] - rv * c2, dr[n / 8].get(n % 8));
+      if constexpr (BRANCH == 1) acc_s[n] = fmaf(d[n], x[n / 8].get(n % 8), acc_s[n]);
+      if constexpr (BRANCH == 2) {
+        const float n1 = x[n / 8].get(n % 8) * r1, dn = d[n] * n1;
+        acc_s[n] = fmaf(dn, pw[n], acc_s[n]);
+        acc_p[n] = fmaf(dn, sc[n], acc_p[n]);
+        q[0] = fmaf(dn, sc[n] * pw[n], q[0]);
+      }
+    }
+    if (live && p.dres) S::template store<RT>(d, p.dres, row * p.D, t, p.D);
+    if constexpr (BRANCH == 2) {
+      S::template row_sums<1>(q, sums[1]);
+      const float c1 = q[0] * over;
+#pragma unroll
+      for (int n = 0; n < S::N; ++n) d[n] = r1 * (d[n] * (sc[n] * pw[n]) - x[n / 8].get(n % 8) * r1 * c1);
+    } else {
+#pragma unroll
+      for (int n = 0; n < S::N; ++n) d[n] *= sc[n];
+      if constexpr (S::T > 32) __syncthreads();      // sums[0] is read by now
+    }
+    if (live && p.dx) S::template store<XT>(d, p.dx, row * p.D, t, p.D);
+  }
+  if (!p.part) return;
+  float* line = p.part + static_cast<long long>(blockIdx.x) * p.vectors * p.D;
+  if (p.at[0] >= 0) S::column_share(acc_w, line + static_cast<long long>(p.at[0]) * p.D, stage, t, p.D);
+  if constexpr (BRANCH == 2)
+    if (p.at[1] >= 0) S::column_share(acc_p, line + static_cast<long long>(p.at[1]) * p.D, stage, t, p.D);
+  if constexpr (BRANCH >= 1)
+    if (p.at[2] >= 0) S::column_share(acc_s, line + static_cast<long long>(p.at[2]) * p.D, stage, t, p.D);
+}
+
+// f(XT, RT)
+template <typename F>
+static int by_stream_type(int xt, int rt, F&& f) {
+  using T32 = std::integral_constant<int, LETHE_F32>;
+  if (rt == LETHE_F32) return by_x_type(xt, [&](auto x) { return f(x, T32()); });
+  return by_x_type(xt, [&](auto x) { return f(x, x); });
+}
+
+static int residual_problem(const LetheGdnResidualNormArgs* a, ResidualProblem* p, bool backward) {
+  if (!a) return kErrNull;
+  if (a->rows <= 0 || a->D <= 0 || a->D > kNormMaxD || !norm_types_ok(a->x_type, a->w_type) || !norm_types_ok(a->x_type, a->r_type) || !(a->eps >= 0.f))
+    return kErrDims;
+  if (!a->r || !a->weight || (!backward && (!a->x || !a->y))) return kErrNull;
+  if (backward && !a->x && (a->post_weight || a->dscale)) return kErrNull;
+  *p = {a->rows, a->D, a->w_type == LETHE_F32, a->eps, a->scale_value, a->x, a->x_stride, a->residual, a->residual_stride, a->weight, a->post_weight,
+        a->scale, a->r, a->y, a->dy, a->dr, a->dx, a->dresidual, nullptr, 0, {-1, -1, -1}};
+  return kOk;
+}
+
+}  // namespace lg
+
+extern "C" int lethe_gdn_residual_norm(const LetheGdnResidualNormArgs* a, void* stream) {
+  using namespace lg;
+  ResidualProblem p;
+  if (int e = residual_problem(a, &p, false)) return e;
+  DeviceGuard guard(a->r);
+  if (!guard.ok) return kErrDevice;
+  const bool vec = p.D % 8 == 0 && piece_aligned(p.x, a->x_type, p.x_stride) && piece_aligned(p.res, a->r_type, p.res_stride) &&
+                   piece_aligned(p.r, a->r_type) && piece_aligned(p.y, a->x_type);
+  return by_stream_type(a->x_type, a->r_type, [&](auto x, auto r) {
+    return by_row_shape(p.D, vec, [&](auto s) {
+      using S = decltype(s);
+      const int grid = norm_grid(p.rows, S::kRows, 2048 / S::kThreads);
+      cudaStream_t st = static_cast<cudaStream_t>(stream);
+      if (p.pw) residual_norm_kernel<x.value, r.value, S, true><<<grid, S::kThreads, 0, st>>>(p);
+      else residual_norm_kernel<x.value, r.value, S, false><<<grid, S::kThreads, 0, st>>>(p);
+      return launched_ok();
+    });
+  });
+}
+
+extern "C" int lethe_gdn_residual_norm_vjp(const LetheGdnResidualNormArgs* a, void* stream) {
+  using namespace lg;
+  ResidualProblem p;
+  if (int e = residual_problem(a, &p, true)) return e;
+  if (a->dpost_weight && !a->post_weight) return kErrFlags;
+  ColumnSums c{};
+  void* const wanted[3] = {a->dweight, a->dpost_weight, a->dscale};
+  for (int i = 0; i < 3; ++i)
+    if (wanted[i]) {
+      p.at[i] = p.vectors;
+      c.out[p.vectors] = wanted[i];
+      c.f32[p.vectors++] = p.w_f32;
+    }
+  if (p.vectors) {
+    if (!a->work) return kErrNull;
+    if (a->work_bytes < lethe_gdn_norm_work_bytes(a->rows, a->D, p.vectors)) return kErrWorkspace;
+    if (reinterpret_cast<uintptr_t>(a->work) & 15) return kErrAlign;
+    p.part = static_cast<float*>(a->work);
+  }
+  DeviceGuard guard(a->r);
+  if (!guard.ok) return kErrDevice;
+  const int branch = p.pw ? 2 : a->dscale ? 1 : 0;
+  const bool vec = p.D % 8 == 0 && (!branch || piece_aligned(p.x, a->x_type, p.x_stride)) && piece_aligned(p.r, a->r_type) &&
+                   piece_aligned(p.dy, a->x_type) && piece_aligned(p.dr, a->r_type) && piece_aligned(p.dx, a->x_type) && piece_aligned(p.dres, a->r_type);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int grid = 0;
+  const int e = by_stream_type(a->x_type, a->r_type, [&](auto x, auto r) {
+    return by_row_shape(p.D, vec, [&](auto s) {
+      using S = decltype(s);
+      grid = std::min(norm_grid(p.rows, S::kRows, 1024 / S::kThreads), norm_parts_max(p.D));
+      constexpr int smem = S::kRows > 1 ? S::kThreads * S::N * 4 : 0;
+      if (branch == 2) residual_norm_vjp_kernel<x.value, r.value, S, 2><<<grid, S::kThreads, smem, st>>>(p);
+      else if (branch == 1) residual_norm_vjp_kernel<x.value, r.value, S, 1><<<grid, S::kThreads, smem, st>>>(p);
+      else residual_norm_vjp_kernel<x.value, r.value, S, 0><<<grid, S::kThreads, smem, st>>>(p);
+      return launched_ok();
+    });
+  });
+  if (e || !p.part) return e;
+  c.part = p.part;
+  c.parts = grid;
+  c.vectors = p.vectors;
+  c.D = p.D;
+  c.x_type = a->x_type;
+  return launch_column_sums(c, st);
+}

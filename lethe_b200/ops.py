@@ -538,10 +538,10 @@ class _Traced(torch.autograd.Function):
     only the allocations of its results; an autograd function it records as a call, so this one stands around it."""
 
     @staticmethod
-    def forward(ctx, call, scale, l2norm, *tensors):
+    def forward(ctx, call, first, second, *tensors):      # the call's two options behind its tensors; None: it has one
         inner = [None if t is None else t.detach().requires_grad_(t.requires_grad) for t in tensors]
         with torch.enable_grad():
-            out = getattr(native.ext(), call)(*inner, scale, l2norm)
+            out = getattr(native.ext(), call)(*inner, *(o for o in (first, second) if o is not None))
         outs = (out,) if isinstance(out, Tensor) else out
         ctx.outs, ctx.inner = outs, [t for t in inner if t is not None and t.requires_grad]
         ctx.wanted = [t is not None and t.requires_grad for t in inner]
@@ -607,6 +607,62 @@ def gdn_chunk_full(q: Tensor, k: Tensor, v: Tensor, g: Tensor, b: Tensor, w: Ten
     if torch._C._is_tracing():
         return _Traced.apply("chunk_full", float(scale), bool(use_qk_l2norm), q, k, v, g, b, w, h0)
     return native.ext().chunk_full(q, k, v, g, b, w, h0, scale, use_qk_l2norm)
+
+
+# ------------------------------------------------------------------------------------------------
+# What stands beside the recurrence in a model
+# ------------------------------------------------------------------------------------------------
+def diag_scan(x: Tensor, g: Tensor, h0: Tensor | None = None, *, complement: bool = False) -> tuple[Tensor, Tensor]:
+    """Element-wise gated recurrence over the second dimension, differentiable: the member of the family with one state value per
+    channel.  ``h_t = exp(g_t) h_{t-1} + x_t``, or with ``complement`` ``exp(g_t) h_{t-1} + (1 - exp(g_t)) x_t``.  Returns
+    ``(h, h_T)``: ``h`` in the shape and type of ``x``, the final state in fp32 without the second dimension.
+
+    ``x [B, L, ...]``: fp32, bf16 or fp16.  ``g`` in the same shape: log decay, <= 0, fp32 or the type of ``x`` (other floating
+    types are read as fp32); minus infinity starts anew, e.g. at the first token of a packed document.  ``h0 [B, ...]``: the
+    initial state, zero if None.  Batch and token may have any strides (a slice of a fused projection is read where it lies).
+    States and sums are fp32, each result is rounded once; the decay of a long memory (``g`` near zero) keeps its precision.
+    Gradients flow to x, g and h0, first order only.  A value that is not finite spreads to the later tokens of its channel."""
+    if torch._C._is_tracing():
+        return _Traced.apply("diag_scan", bool(complement), None, x, g, h0)
+    return native.ext().diag_scan(x, g, h0, complement)
+
+
+def diag_scan_step(x: Tensor, g: Tensor, state: Tensor, *, complement: bool = False) -> Tensor:
+    """One token of ``diag_scan`` for generation: ``x, g [B, ...]``, ``state [B, ...]`` fp32 contiguous, **updated in place**
+    (start from the ``h_T`` of the prompt).  Returns the new state in the type of ``x``.  Not differentiable."""
+    return native.ext().diag_scan_step(x, g, state, complement)
+
+
+ACTIVATIONS = ("silu", "sigmoid")
+
+
+def gated_norm(x: Tensor, gate: Tensor, weight: Tensor, *, eps: float = 1e-6, activation: str = "silu") -> Tensor:
+    """The norm behind a block, differentiable: ``x * rsqrt(mean(x^2) + eps) * weight * act(gate)`` over the last dimension, in
+    one pass.  ``x, gate [..., D]`` of one type (fp32, bf16 or fp16), for a recurrence's output ``[B, L, H, V]`` with the gate a
+    view of a projection; ``weight [D]``; ``activation`` "silu" (``gate * sigmoid(gate)``) or "sigmoid".  D from 1 to 8192.
+    Gradients flow to x, gate and weight, first order only."""
+    if activation not in ACTIVATIONS:
+        raise GdnError(f"lethe_gdn: activation must be one of {ACTIVATIONS}")
+    if torch._C._is_tracing():
+        return _Traced.apply("gated_norm", float(eps), activation == "silu", x, gate, weight)
+    return native.ext().gated_norm(x, gate, weight, eps, activation == "silu")
+
+
+def residual_norm(x: Tensor, residual: Tensor | None, weight: Tensor, *, scale: Tensor | float | None = None,
+                  post_weight: Tensor | None = None, eps: float = 1e-6) -> tuple[Tensor, Tensor]:
+    """The residual sum and the norm in front of the next block, differentiable, in one pass.  Returns ``(y, r)``:
+    ``r = residual + scale * t`` with ``t = x``, or ``t = x * rsqrt(mean(x^2) + eps) * post_weight`` where the block's output has a
+    norm of its own, and ``y = r * rsqrt(mean(r^2) + eps) * weight``.
+
+    ``x [..., D]``: the block's output, fp32, bf16 or fp16.  ``residual``: the stream in the same shape, fp32 or the type of
+    ``x``; None for the first block (zero).  ``scale``: a number or a learned vector ``[D]``.  ``r`` comes in the type of the stream
+    (of ``x`` without one), ``y`` in that of ``x``; the norm is that of ``r`` as it is returned.  D from 1 to 8192.
+    Gradients flow to all tensors, first order only."""
+    vec = scale if isinstance(scale, Tensor) else None
+    num = 1.0 if vec is not None or scale is None else float(scale)
+    if torch._C._is_tracing():
+        return _Traced.apply("residual_norm", float(eps), num, x, residual, weight, post_weight, vec)
+    return native.ext().residual_norm(x, residual, weight, post_weight, vec, eps, num)
 
 
 # ------------------------------------------------------------------------------------------------
