@@ -2,10 +2,11 @@
 //
 // Bound by HBM: some 10 to 20 operations for every 8 bytes forward (bf16 x and h, fp32 g) and 14 backward.
 //
-// A tile is kTokens tokens of kChannels channels of one sequence.  A thread holds kSteps tokens of four channels in registers; its
-// 16-lane group covers the channels, kGroups groups the tokens.  Two levels of the same scan: every thread runs its own tokens
-// from a zero state, the groups' results (sum of g, state) meet in shared memory and are folded in order, and every thread runs
-// its tokens again from the state that it really starts from.  The order of all sums is fixed, so two runs give the same bits.
+// A CTA does a tile of kTokens tokens of kChannels channels of one sequence, read once and held in registers: a thread has kSteps
+// tokens of four channels, its 16-lane group covers the channels, kGroups groups the tokens.  Every thread runs its own tokens from
+// a zero state, the groups' results (sum of g, state) meet in shared memory and are folded in order, the tile gets the state in
+// front of it from the tiles before (below), and every thread runs its tokens again from the state that it really starts from.
+// The order of all sums is fixed, so two runs give the same bits.
 //
 // The decay.  With memories of thousands of tokens e^g lies next to one, and fp32 rounds it by up to 2^-25: over n tokens the
 // state is off by up to n times that, always to the same side where g is constant.  So below |g| = 1/4 the step is taken with
@@ -43,6 +44,10 @@ __device__ __forceinline__ float decay_step(float c, float h, float x) {
 }
 __device__ __forceinline__ float forgotten(float c) { return is_diff(c) ? -c : 1.f - c; }      // 1 - e^g
 
+struct LookBuffer {
+  uint32_t* head;                   // ticket, and the word that lets everybody pass
+  unsigned long long* word[3];      // of tiles, groups of tiles, groups of groups
+};
 struct DiagProblem {
   long long B, L, D;
   const void* x;
@@ -59,7 +64,26 @@ struct DiagProblem {
   void *dx, *dg;
   float* dh0;
   int tiles, strips;      // tiles of kTokens tokens, strips of kChannels channels
+  uint32_t seqs;          // B strips
+  int* status;
+  LookBuffer look;
 };
+
+// What a thread keeps from its first run over its tokens to its second: the compiler would keep everything that it formed there as
+// well (fp32 copies, 1 - e^g), for twice the registers.
+template <int TY>
+__device__ __forceinline__ void forget_copies(Raw<TY, kPer> (&r)[kSteps]) {
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+    for (int i = 0; i < Raw<TY, kPer>::kWords; ++i) asm volatile("" : "+r"(r[s].w[i]));
+}
+__device__ __forceinline__ void forget_copies(float (&c)[kSteps][kPer]) {
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) asm volatile("" : "+f"(c[s][j]));
+}
 
 // Four channels of one token.  VEC: neighbours, one load; else every 16th channel, element by element, D and alignment as they are.
 template <bool VEC>
@@ -93,42 +117,190 @@ __device__ __forceinline__ Raw<TY, kPer> packed(const float (&v)[kPer]) {
   return r;
 }
 
+// ---------------------------------------------------------------------------------------------
+// What a tile hands on.  The state in front of a tile depends on all tiles before it; a tile leaves its own part, (sum of g, state
+// from zero), in the work buffer as soon as it has it, 64 bits per channel, stored and loaded as one, so a word that is there is
+// whole and needs no flag or fence beside it.  Unwritten words are all ones (the buffer is set so in front of the kernel).
+//
+// Three levels keep what a tile has to read at 31 words: the tiles of its group of 16 in front of it, the groups of its 16 groups in
+// front of it (the last tile of a group leaves that word, from the group's words alone), and the state behind the 256 tiles before
+// those (left by the last of them).  The order of the fold is that of the tokens whoever comes first.
+//
+// Tiles are taken by ticket, so a tile waits only for tiles whose CTAs run already and wait for earlier ones only.  Waits are
+// bounded all the same: one that runs out leaves a code in the status word and lets everybody pass.
+// ---------------------------------------------------------------------------------------------
+constexpr int kFan = 16;
+constexpr long long kLookLimitCycles = 2000000000LL;      // about one second
+enum : int { kSiteLook = 900 };
+
+constexpr size_t kLookHead = 128;
+struct LookSizes {
+  size_t count[3];
+  size_t bytes() const { return kLookHead + (count[0] + count[1] + count[2]) * kChannels * 8; }
+};
+static LookSizes look_sizes(long long seqs, long long tiles) {
+  if (tiles <= 1) return {{0, 0, 0}};
+  const long long groups = (tiles + kFan - 1) / kFan, supers = (groups + kFan - 1) / kFan;
+  return {{static_cast<size_t>(seqs * tiles), static_cast<size_t>(seqs * groups), static_cast<size_t>(seqs * supers)}};
+}
+
+__device__ __forceinline__ unsigned long long look_load(const unsigned long long* p) {
+  unsigned long long v;
+  asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ void look_store(unsigned long long* p, float sum, float state) {
+  unsigned long long v = (static_cast<unsigned long long>(__float_as_uint(state)) << 32) | __float_as_uint(sum);
+  if (v == ~0ull) v = 0x7fffffff7fffffffull;      // (another NaN)
+  asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
+}
+__device__ __noinline__ unsigned long long look_wait(const unsigned long long* p, uint32_t* head, int* status) {
+  const long long t0 = clock64();
+  for (int n = 1;; ++n) {
+    const unsigned long long v = look_load(p);
+    if (v != ~0ull) return v;
+    if (n % 32) continue;
+    if (*reinterpret_cast<volatile uint32_t*>(head + 1) == 0u) return 0;
+    if (clock64() - t0 > kLookLimitCycles) {
+      atomicCAS(status, 0, kSiteLook);
+      *reinterpret_cast<volatile uint32_t*>(head + 1) = 0u;
+      return 0;
+    }
+  }
+}
+
+struct LookShared {
+  float2 part[2 * kFan - 1][kChannels];      // (coefficient, state): groups, then tiles, in front
+  float sum[kFan - 1][kChannels];            // sums of g of those tiles
+  float base[kChannels];                     // state behind the 256 tiles before
+};
 struct ScanShared {
   float2 part[kGroups][kChannels];      // per group of tokens: (coefficient of its whole decay, state from zero)
-  float start[kGroups][kChannels];      // state in front of a group
-  float2 back[kGroups][kChannels];      // the same for the gradient, backwards in time
-  float end[kGroups][kChannels];        // gradient that comes into a group from the tokens behind it
-  float carry[2][kChannels];
+  float sum[kGroups][kChannels];        // sum of its g
+  float start[kGroups][kChannels];      // state in front of it
+  LookShared look;
+  uint32_t ticket;
+};
+struct ScanSharedBackward : ScanShared {
+  float back[kGroups][kChannels];       // per group the gradient that leaves it towards earlier tokens, from zero
+  float end[kGroups][kChannels];        // the gradient that comes into it
 };
 
-// One CTA goes through the tiles of a strip of channels of one sequence.
+// Where tile number `i` (in the order of the fold) of sequence `seq` stands among the three levels.
+struct LookPlace {
+  LookBuffer buf;
+  long long group0, tile0;      // first words of its level: groups of its super, tiles of its group
+  long long super;              // its super's word
+  int n_groups, n_tiles;        // how many in front of it
+  bool first_super, last;       // no tiles in front of its super; no tile behind it
+  __device__ LookPlace(const LookBuffer& b, long long seq, int tiles, int i) : buf(b) {
+    const int groups = (tiles + kFan - 1) / kFan, supers = (groups + kFan - 1) / kFan;
+    const int sup = i / (kFan * kFan);
+    n_groups = i / kFan % kFan;
+    n_tiles = i % kFan;
+    group0 = seq * groups + sup * kFan;
+    tile0 = seq * tiles + (i - n_tiles);
+    super = seq * supers + sup;
+    first_super = sup == 0;
+    last = i == tiles - 1;
+  }
+  __device__ unsigned long long* at(int level, long long n, int ch) const { return buf.word[level] + n * kChannels + ch; }
+};
+
+// All threads.  Leaves what the fold reads in `l`; in between the last tile of a group leaves the group's word: `sum`, `state` of
+// threads below kChannels are the tile's own.
+__device__ __forceinline__ void look_fetch(LookShared& l, const LookPlace& p, float sum, float state, int* status) {
+  const int ch = threadIdx.x % kChannels, q = threadIdx.x / kChannels;
+  constexpr int kQ = kScanThreads / kChannels, kEach = (kFan + kQ - 1) / kQ;
+  unsigned long long t[kEach], g[kEach], b = 0;
+#pragma unroll
+  for (int m = 0; m < kEach; ++m) {
+    const int k = q + m * kQ;
+    if (k < p.n_tiles) t[m] = look_load(p.at(0, p.tile0 + k, ch));
+    if (k < p.n_groups) g[m] = look_load(p.at(1, p.group0 + k, ch));
+  }
+  if (q == 0 && !p.first_super) b = look_load(p.at(2, p.super - 1, ch));
+#pragma unroll
+  for (int m = 0; m < kEach; ++m) {
+    const int k = q + m * kQ;
+    if (k < p.n_tiles) {
+      if (t[m] == ~0ull) t[m] = look_wait(p.at(0, p.tile0 + k, ch), p.buf.head, status);
+      const float s = __uint_as_float(static_cast<uint32_t>(t[m]));
+      l.sum[k][ch] = s;
+      l.part[p.n_groups + k][ch] = make_float2(decay_coef(s), __uint_as_float(static_cast<uint32_t>(t[m] >> 32)));
+    }
+  }
+  if (p.n_tiles == kFan - 1 && !p.last) {      // (the same for all threads of a CTA)
+    __syncthreads();
+    if (q == 0) {
+      float gs = 0.f, gh = 0.f;
+      for (int k = 0; k < kFan - 1; ++k) {
+        const float2 a = l.part[p.n_groups + k][ch];
+        gs += l.sum[k][ch];
+        gh = decay_step(a.x, gh, a.y);
+      }
+      look_store(p.at(1, p.group0 + p.n_groups, ch), gs + sum, decay_step(decay_coef(sum), gh, state));
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < kEach; ++m) {
+    const int k = q + m * kQ;
+    if (k < p.n_groups) {
+      if (g[m] == ~0ull) g[m] = look_wait(p.at(1, p.group0 + k, ch), p.buf.head, status);
+      l.part[k][ch] = make_float2(decay_coef(__uint_as_float(static_cast<uint32_t>(g[m]))), __uint_as_float(static_cast<uint32_t>(g[m] >> 32)));
+    }
+  }
+  if (q == 0 && !p.first_super) {
+    if (b == ~0ull) b = look_wait(p.at(2, p.super - 1, ch), p.buf.head, status);
+    l.base[ch] = __uint_as_float(static_cast<uint32_t>(b >> 32));
+  }
+  __syncthreads();
+}
+// Threads below kChannels: the state in front of the tile; `first`: that in front of the first tile.
+__device__ __forceinline__ float look_fold(const LookShared& l, const LookPlace& p, float first) {
+  float carry = p.first_super ? first : l.base[threadIdx.x];
+  for (int k = 0; k < p.n_groups + p.n_tiles; ++k) {
+    const float2 a = l.part[k][threadIdx.x];
+    carry = decay_step(a.x, carry, a.y);
+  }
+  return carry;
+}
+
+// One CTA does one tile of kTokens tokens x kChannels channels.
 template <int XT, int GT, bool VEC, bool COMP>
-__global__ void __launch_bounds__(kScanThreads) diag_forward_kernel(const DiagProblem p) {
+__global__ void __launch_bounds__(kScanThreads, 2) diag_forward_kernel(const DiagProblem p) {
   using X = typename Elem<XT>::T;
   using G = typename Elem<GT>::T;
   __shared__ ScanShared sh;
   const int lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
-  const long long b = blockIdx.x / p.strips, ch0 = static_cast<long long>(blockIdx.x % p.strips) * kChannels;
+  long long seq = blockIdx.x;
+  int tile = 0;
+  if (p.tiles > 1) {
+    if (threadIdx.x == 0) sh.ticket = atomicAdd(p.look.head, 1u) + 1u;
+    __syncthreads();
+    tile = static_cast<int>(sh.ticket / p.seqs);
+    seq = sh.ticket % p.seqs;
+  }
+  const long long b = seq / p.strips, ch0 = (seq % p.strips) * kChannels;
   const int room = static_cast<int>(p.D - ch0 < kChannels ? p.D - ch0 : kChannels);
-  const X* x = static_cast<const X*>(p.x) + b * p.x_batch + ch0;
-  const G* g = static_cast<const G*>(p.g) + b * p.g_batch + ch0;
-  X* h = static_cast<X*>(p.h) + b * p.L * p.D + ch0;
-  float carry = 0.f;                    // threads below kChannels: the state in front of the tile
-  if (threadIdx.x < room && p.h0) carry = p.h0[b * p.D + ch0 + threadIdx.x];
-  for (int tile = 0; tile < p.tiles; ++tile) {
-    const long long t0 = static_cast<long long>(tile) * kTokens + grp * kSteps;
-    Raw<XT, kPer> xr[kSteps];
+  const long long t0 = static_cast<long long>(tile) * kTokens + grp * kSteps;
+  const X* x = static_cast<const X*>(p.x) + b * p.x_batch + t0 * p.x_token + ch0;
+  const G* g = static_cast<const G*>(p.g) + b * p.g_batch + t0 * p.g_token + ch0;
+  X* h = static_cast<X*>(p.h) + (b * p.L + t0) * p.D + ch0;
+  const int live = static_cast<int>(p.L - t0 < kSteps ? p.L - t0 : kSteps);      // tokens of this thread (0 and less: none)
+  Raw<XT, kPer> xr[kSteps];
+  float c[kSteps][kPer], sum[kPer], st[kPer];
+  {
     Raw<GT, kPer> gr[kSteps];
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       xr[s].zero();
       gr[s].zero();
-      if (t0 + s < p.L) {
-        load_token<XT, VEC>(xr[s], x + (t0 + s) * p.x_token, lane, room);
-        load_token<GT, VEC>(gr[s], g + (t0 + s) * p.g_token, lane, room);
+      if (s < live) {
+        load_token<XT, VEC>(xr[s], x + s * p.x_token, lane, room);
+        load_token<GT, VEC>(gr[s], g + s * p.g_token, lane, room);
       }
     }
-    float c[kSteps][kPer], sum[kPer], st[kPer];
 #pragma unroll
     for (int j = 0; j < kPer; ++j) sum[j] = st[j] = 0.f;
 #pragma unroll
@@ -141,66 +313,101 @@ __global__ void __launch_bounds__(kScanThreads) diag_forward_kernel(const DiagPr
         const float u = COMP ? xr[s].get(j) * forgotten(c[s][j]) : xr[s].get(j);
         st[j] = decay_step(c[s][j], st[j], u);
       }
+  }
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) sh.part[grp][channel_of<VEC>(lane, j)] = make_float2(decay_coef(sum[j]), st[j]);
-    __syncthreads();
-    if (threadIdx.x < kChannels) {
-      if (p.states && threadIdx.x < room) p.states[(b * p.tiles + tile) * p.D + ch0 + threadIdx.x] = carry;
+  for (int j = 0; j < kPer; ++j) {
+    const int ch = channel_of<VEC>(lane, j);
+    sh.part[grp][ch] = make_float2(decay_coef(sum[j]), st[j]);
+    sh.sum[grp][ch] = sum[j];
+  }
+  forget_copies(xr);
+  forget_copies(c);
+  __syncthreads();
+  const int ch = threadIdx.x;      // of threads below kChannels
+  float carry = 0.f;
+  if (ch < room && p.h0) carry = p.h0[b * p.D + ch0 + ch];
+  if (p.tiles > 1) {
+    const LookPlace at(p.look, seq, p.tiles, tile);
+    float ts = 0.f, th = 0.f;
+    if (ch < kChannels) {
 #pragma unroll
       for (int i = 0; i < kGroups; ++i) {
-        sh.start[i][threadIdx.x] = carry;
-        const float2 a = sh.part[i][threadIdx.x];
-        carry = decay_step(a.x, carry, a.y);
+        const float2 a = sh.part[i][ch];
+        ts += sh.sum[i][ch];
+        th = decay_step(a.x, th, a.y);
       }
+      if (!at.last) look_store(at.at(0, at.tile0 + at.n_tiles, ch), ts, th);
     }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) st[j] = sh.start[grp][channel_of<VEC>(lane, j)];
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const float u = COMP ? xr[s].get(j) * forgotten(c[s][j]) : xr[s].get(j);
-        st[j] = decay_step(c[s][j], st[j], u);
-      }
-      if (t0 + s < p.L) store_token<XT, VEC>(packed<XT>(st), h + (t0 + s) * p.D, lane, room);
+    look_fetch(sh.look, at, ts, th, p.status);
+    if (ch < kChannels) {
+      carry = look_fold(sh.look, at, carry);
+      if (at.n_tiles == kFan - 1 && at.n_groups == kFan - 1 && !at.last) look_store(at.at(2, at.super, ch), 0.f, decay_step(decay_coef(ts), carry, th));
     }
   }
-  if (threadIdx.x < room && p.hT) p.hT[b * p.D + ch0 + threadIdx.x] = carry;
+  if (ch < kChannels) {
+    if (p.states && ch < room) p.states[(b * p.tiles + tile) * p.D + ch0 + ch] = carry;
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) {
+      sh.start[i][ch] = carry;
+      const float2 a = sh.part[i][ch];
+      carry = decay_step(a.x, carry, a.y);
+    }
+    if (p.hT && ch < room && tile == p.tiles - 1) p.hT[b * p.D + ch0 + ch] = carry;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) st[j] = sh.start[grp][channel_of<VEC>(lane, j)];
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const float u = COMP ? xr[s].get(j) * forgotten(c[s][j]) : xr[s].get(j);
+      st[j] = decay_step(c[s][j], st[j], u);
+    }
+    if (s < live) store_token<XT, VEC>(packed<XT>(st), h + s * p.D, lane, room);
+  }
 }
 
 template <int XT, int GT, bool VEC, bool COMP>
-__global__ void __launch_bounds__(kScanThreads) diag_backward_kernel(const DiagProblem p) {
+__global__ void __launch_bounds__(kScanThreads, 2) diag_backward_kernel(const DiagProblem p) {
   using X = typename Elem<XT>::T;
   using G = typename Elem<GT>::T;
-  __shared__ ScanShared sh;
+  __shared__ ScanSharedBackward sh;
   const int lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
-  const long long b = blockIdx.x / p.strips, ch0 = static_cast<long long>(blockIdx.x % p.strips) * kChannels;
+  long long seq = blockIdx.x;
+  int order = 0;                      // of the tile, from the last one on
+  if (p.tiles > 1) {
+    if (threadIdx.x == 0) sh.ticket = atomicAdd(p.look.head, 1u) + 1u;
+    __syncthreads();
+    order = static_cast<int>(sh.ticket / p.seqs);
+    seq = sh.ticket % p.seqs;
+  }
+  const int tile = p.tiles - 1 - order;
+  const long long b = seq / p.strips, ch0 = (seq % p.strips) * kChannels;
   const int room = static_cast<int>(p.D - ch0 < kChannels ? p.D - ch0 : kChannels);
-  const X* x = static_cast<const X*>(p.x) + b * p.x_batch + ch0;
-  const G* g = static_cast<const G*>(p.g) + b * p.g_batch + ch0;
-  const X* d = p.d_h ? static_cast<const X*>(p.d_h) + b * p.d_batch + ch0 : nullptr;
-  X* dx = p.dx ? static_cast<X*>(p.dx) + b * p.L * p.D + ch0 : nullptr;
-  G* dg = p.dg ? static_cast<G*>(p.dg) + b * p.L * p.D + ch0 : nullptr;
-  const int fold = threadIdx.x - kChannels;      // threads kChannels .. 2 kChannels - 1 fold the gradient
-  float carry = 0.f;
-  if (fold >= 0 && fold < room && p.dhT) carry = p.dhT[b * p.D + ch0 + fold];
-  for (int tile = p.tiles - 1; tile >= 0; --tile) {
-    const long long t0 = static_cast<long long>(tile) * kTokens + grp * kSteps;
-    Raw<XT, kPer> xr[kSteps], dr[kSteps];
+  const long long t0 = static_cast<long long>(tile) * kTokens + grp * kSteps;
+  const X* x = static_cast<const X*>(p.x) + b * p.x_batch + t0 * p.x_token + ch0;
+  const G* g = static_cast<const G*>(p.g) + b * p.g_batch + t0 * p.g_token + ch0;
+  const X* d = static_cast<const X*>(p.d_h) + b * p.d_batch + t0 * p.d_token + ch0;
+  X* dx = static_cast<X*>(p.dx) + (b * p.L + t0) * p.D + ch0;
+  G* dg = static_cast<G*>(p.dg) + (b * p.L + t0) * p.D + ch0;
+  const int live = static_cast<int>(p.L - t0 < kSteps ? p.L - t0 : kSteps);
+  Raw<XT, kPer> xr[kSteps], dr[kSteps];
+  float c[kSteps][kPer], st[kPer], e[kPer];
+  {
     Raw<GT, kPer> gr[kSteps];
+    float sum[kPer];
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       xr[s].zero();
       gr[s].zero();
       dr[s].zero();
-      if (t0 + s < p.L) {
-        load_token<XT, VEC>(xr[s], x + (t0 + s) * p.x_token, lane, room);
-        load_token<GT, VEC>(gr[s], g + (t0 + s) * p.g_token, lane, room);
-        if (d) load_token<XT, VEC>(dr[s], d + (t0 + s) * p.d_token, lane, room);
+      if (s < live) {
+        load_token<XT, VEC>(xr[s], x + s * p.x_token, lane, room);
+        load_token<GT, VEC>(gr[s], g + s * p.g_token, lane, room);
+        if (p.d_h) load_token<XT, VEC>(dr[s], d + s * p.d_token, lane, room);
       }
     }
-    float c[kSteps][kPer], sum[kPer], st[kPer], e[kPer];
 #pragma unroll
     for (int j = 0; j < kPer; ++j) sum[j] = st[j] = e[j] = 0.f;
 #pragma unroll
@@ -219,59 +426,83 @@ __global__ void __launch_bounds__(kScanThreads) diag_backward_kernel(const DiagP
       for (int j = 0; j < kPer; ++j) e[j] = decay_step(c[s][j], dr[s].get(j) + e[j], 0.f);
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-      const float whole = decay_coef(sum[j]);
-      sh.part[grp][channel_of<VEC>(lane, j)] = make_float2(whole, st[j]);
-      sh.back[grp][channel_of<VEC>(lane, j)] = make_float2(whole, e[j]);
-    }
-    __syncthreads();
-    if (threadIdx.x < kChannels) {
-      float s0 = threadIdx.x < room ? p.states[(b * p.tiles + tile) * p.D + ch0 + threadIdx.x] : 0.f;
-#pragma unroll
-      for (int i = 0; i < kGroups; ++i) {
-        sh.start[i][threadIdx.x] = s0;
-        const float2 a = sh.part[i][threadIdx.x];
-        s0 = decay_step(a.x, s0, a.y);
-      }
-    } else if (fold < kChannels) {
-#pragma unroll
-      for (int i = kGroups - 1; i >= 0; --i) {
-        sh.end[i][fold] = carry;
-        const float2 a = sh.back[i][fold];
-        carry = decay_step(a.x, carry, a.y);
-      }
-    }
-    __syncthreads();
-    float before[kSteps][kPer];
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      st[j] = sh.start[grp][channel_of<VEC>(lane, j)];
-      e[j] = sh.end[grp][channel_of<VEC>(lane, j)];
-    }
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const float xv = xr[s].get(j);
-        before[s][j] = COMP ? st[j] - xv : st[j];
-        st[j] = decay_step(c[s][j], st[j], COMP ? xv * forgotten(c[s][j]) : xv);
-      }
-#pragma unroll
-    for (int s = kSteps - 1; s >= 0; --s) {
-      float vx[kPer], vg[kPer];
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const float dv = dr[s].get(j) + e[j];
-        vx[j] = COMP ? dv * forgotten(c[s][j]) : dv;
-        e[j] = decay_step(c[s][j], dv, 0.f);
-        vg[j] = e[j] * before[s][j];
-      }
-      if (t0 + s < p.L) {
-        if (dx) store_token<XT, VEC>(packed<XT>(vx), dx + (t0 + s) * p.D, lane, room);
-        if (dg) store_token<GT, VEC>(packed<GT>(vg), dg + (t0 + s) * p.D, lane, room);
-      }
+      const int ch = channel_of<VEC>(lane, j);
+      sh.part[grp][ch] = make_float2(decay_coef(sum[j]), st[j]);
+      sh.sum[grp][ch] = sum[j];
+      sh.back[grp][ch] = e[j];
     }
   }
-  if (fold >= 0 && fold < room && p.dh0) p.dh0[b * p.D + ch0 + fold] = carry;
+  forget_copies(xr);
+  forget_copies(dr);
+  forget_copies(c);
+  __syncthreads();
+  const int ch = threadIdx.x, ch2 = threadIdx.x - kChannels;      // the gradient is folded by threads below kChannels, the state by the next ones
+  float carry = 0.f;
+  if (ch < room && p.dhT) carry = p.dhT[b * p.D + ch0 + ch];
+  if (ch2 >= 0 && ch2 < kChannels) {
+    float s0 = ch2 < room ? p.states[(b * p.tiles + tile) * p.D + ch0 + ch2] : 0.f;
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) {
+      sh.start[i][ch2] = s0;
+      const float2 a = sh.part[i][ch2];
+      s0 = decay_step(a.x, s0, a.y);
+    }
+  }
+  if (p.tiles > 1) {
+    const LookPlace at(p.look, seq, p.tiles, order);
+    float ts = 0.f, te = 0.f;
+    if (ch < kChannels) {
+#pragma unroll
+      for (int i = kGroups - 1; i >= 0; --i) {
+        ts += sh.sum[i][ch];
+        te = decay_step(sh.part[i][ch].x, te, sh.back[i][ch]);
+      }
+      if (!at.last) look_store(at.at(0, at.tile0 + at.n_tiles, ch), ts, te);
+    }
+    look_fetch(sh.look, at, ts, te, p.status);
+    if (ch < kChannels) {
+      carry = look_fold(sh.look, at, carry);
+      if (at.n_tiles == kFan - 1 && at.n_groups == kFan - 1 && !at.last) look_store(at.at(2, at.super, ch), 0.f, decay_step(decay_coef(ts), carry, te));
+    }
+  }
+  if (ch < kChannels) {
+#pragma unroll
+    for (int i = kGroups - 1; i >= 0; --i) {
+      sh.end[i][ch] = carry;
+      carry = decay_step(sh.part[i][ch].x, carry, sh.back[i][ch]);
+    }
+    if (p.dh0 && ch < room && tile == 0) p.dh0[b * p.D + ch0 + ch] = carry;
+  }
+  __syncthreads();
+  float before[kSteps][kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    st[j] = sh.start[grp][channel_of<VEC>(lane, j)];
+    e[j] = sh.end[grp][channel_of<VEC>(lane, j)];
+  }
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const float xv = xr[s].get(j);
+      before[s][j] = COMP ? st[j] - xv : st[j];
+      st[j] = decay_step(c[s][j], st[j], COMP ? xv * forgotten(c[s][j]) : xv);
+    }
+#pragma unroll
+  for (int s = kSteps - 1; s >= 0; --s) {
+    float vx[kPer], vg[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const float dv = dr[s].get(j) + e[j];
+      vx[j] = COMP ? dv * forgotten(c[s][j]) : dv;
+      e[j] = decay_step(c[s][j], dv, 0.f);
+      vg[j] = e[j] * before[s][j];
+    }
+    if (s < live) {
+      if (p.dx) store_token<XT, VEC>(packed<XT>(vx), dx + s * p.D, lane, room);
+      if (p.dg) store_token<GT, VEC>(packed<GT>(vg), dg + s * p.D, lane, room);
+    }
+  }
 }
 
 struct StepProblem {
@@ -348,10 +579,24 @@ static int diag_problem(const LetheGdnDiagArgs* a, DiagProblem* p, bool backward
   if (a->B <= 0 || a->L <= 0 || a->D <= 0 || !types_ok(a->x_type, a->g_type)) return kErrDims;
   if (!a->x || !a->g || !a->status || (!backward && !a->h) || (backward && !a->states)) return kErrNull;
   const long long tiles = (a->L + kTokens - 1) / kTokens, strips = (a->D + kChannels - 1) / kChannels;
-  if (tiles > INT32_MAX || strips > INT32_MAX || a->B > INT32_MAX / strips) return kErrDims;
+  if (strips > INT32_MAX || a->B > INT32_MAX / strips || tiles > INT32_MAX / (a->B * strips)) return kErrDims;
   *p = {a->B, a->L, a->D, a->x, a->x_batch, a->x_token, a->g, a->g_batch, a->g_token, a->h0, a->h, a->hT, a->states, a->d_h, a->d_h_batch,
-        a->d_h_token, a->dhT, a->dx, a->dg, a->dh0, static_cast<int>(tiles), static_cast<int>(strips)};
+        a->d_h_token, a->dhT, a->dx, a->dg, a->dh0, static_cast<int>(tiles), static_cast<int>(strips), static_cast<uint32_t>(a->B * strips), a->status, {}};
+  if (tiles > 1) {
+    if (!a->work) return kErrNull;
+    if (reinterpret_cast<uintptr_t>(a->work) & 15) return kErrAlign;
+    const LookSizes n = look_sizes(p->seqs, tiles);
+    if (a->work_bytes < n.bytes()) return kErrWorkspace;
+    p->look.head = static_cast<uint32_t*>(a->work);
+    p->look.word[0] = reinterpret_cast<unsigned long long*>(static_cast<char*>(a->work) + kLookHead);
+    for (int i = 1; i < 3; ++i) p->look.word[i] = p->look.word[i - 1] + n.count[i - 1] * kChannels;
+  }
   return kOk;
+}
+// all ones: no word is there yet, and the ticket before the first
+static int look_clear(const DiagProblem& p, cudaStream_t st) {
+  if (p.tiles <= 1) return kOk;
+  return cudaMemsetAsync(p.look.head, 0xff, look_sizes(p.seqs, p.tiles).bytes(), st) == cudaSuccess ? kOk : kErrLaunch;
 }
 
 }  // namespace lg
@@ -361,7 +606,11 @@ extern "C" size_t lethe_gdn_diag_states_bytes(int64_t B, int64_t L, int64_t D) {
   if (B <= 0 || L <= 0 || D <= 0) return 0;
   return static_cast<size_t>(B) * ((L + kTokens - 1) / kTokens) * D * sizeof(float);
 }
-extern "C" size_t lethe_gdn_diag_work_bytes(int64_t, int64_t, int64_t) { return 0; }
+extern "C" size_t lethe_gdn_diag_work_bytes(int64_t B, int64_t L, int64_t D) {
+  using namespace lg;
+  if (B <= 0 || L <= kTokens || D <= 0) return 0;
+  return look_sizes(B * ((D + kChannels - 1) / kChannels), (L + kTokens - 1) / kTokens).bytes();
+}
 
 extern "C" int lethe_gdn_diag_forward(const LetheGdnDiagArgs* a, void* stream) {
   using namespace lg;
@@ -371,9 +620,10 @@ extern "C" int lethe_gdn_diag_forward(const LetheGdnDiagArgs* a, void* stream) {
   if (!guard.ok) return kErrDevice;
   const bool vec = a->D % kPer == 0 && on_boundary(a->x, a->x_type, kPer, a->x_batch, a->x_token) &&
                    on_boundary(a->g, a->g_type, kPer, a->g_batch, a->g_token) && on_boundary(a->h, a->x_type, kPer);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (int e = look_clear(p, st)) return e;
   return by_type(a->x_type, a->g_type, vec, a->complement != 0, [&](auto x, auto g, auto v, auto c) {
-    diag_forward_kernel<x.value, g.value, v.value, c.value>
-        <<<static_cast<unsigned>(p.B * p.strips), kScanThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    diag_forward_kernel<x.value, g.value, v.value, c.value><<<p.seqs * p.tiles, kScanThreads, 0, st>>>(p);
     return launched();
   });
 }
@@ -388,9 +638,10 @@ extern "C" int lethe_gdn_diag_backward(const LetheGdnDiagArgs* a, void* stream) 
                    on_boundary(a->g, a->g_type, kPer, a->g_batch, a->g_token) &&
                    on_boundary(a->d_h, a->x_type, kPer, a->d_h_batch, a->d_h_token) && on_boundary(a->dx, a->x_type, kPer) &&
                    on_boundary(a->dg, a->g_type, kPer);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (int e = look_clear(p, st)) return e;
   return by_type(a->x_type, a->g_type, vec, a->complement != 0, [&](auto x, auto g, auto v, auto c) {
-    diag_backward_kernel<x.value, g.value, v.value, c.value>
-        <<<static_cast<unsigned>(p.B * p.strips), kScanThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    diag_backward_kernel<x.value, g.value, v.value, c.value><<<p.seqs * p.tiles, kScanThreads, 0, st>>>(p);
     return launched();
   });
 }
