@@ -26,21 +26,31 @@ constexpr int kScanThreads = kLanes * kGroups;
 
 // coefficient of a step over the log decay g
 __device__ __forceinline__ float decay_coef(float g) {
-  // e^g - 1 = g (1 + g/2 (1 + g/3 (... (1 + g/7)))): the first term left out is under 2e-9 of the result for |g| <= 1/4
-  float s = fmaf(g, 1.f / 7.f, 1.f);
-  s = fmaf(g * (1.f / 6.f), s, 1.f);
-  s = fmaf(g * (1.f / 5.f), s, 1.f);
-  s = fmaf(g * (1.f / 4.f), s, 1.f);
-  s = fmaf(g * (1.f / 3.f), s, 1.f);
-  s = fmaf(g * (1.f / 2.f), s, 1.f);
-  const float m = __uint_as_float(__float_as_uint(g * s) | 0x80000000u);      // (g = +0 too)
-  return g > -0.25f && g <= 0.f ? m : expf(g);
+  // e^g - 1 = g (1 + g/2 + g^2/6 + ... + g^6/5040): the first term left out is under 2e-9 of the result for |g| <= 1/4
+  float s = fmaf(g, 1.f / 5040.f, 1.f / 720.f);
+  s = fmaf(g, s, 1.f / 120.f);
+  s = fmaf(g, s, 1.f / 24.f);
+  s = fmaf(g, s, 1.f / 6.f);
+  s = fmaf(g, s, 0.5f);
+  s = fmaf(g, s, 1.f);
+  const float m = -fabsf(g) * s;      // (-0 for both zeros)
+  float e;      // 2 ulp and the rounding of the product: beyond -1/4 a memory is shorter than five tokens
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * 1.4426950408889634f));
+  return g > -0.25f && g <= 0.f ? m : e;
 }
 __device__ __forceinline__ bool is_diff(float c) { return static_cast<int>(__float_as_uint(c)) < 0; }
 // e^g h + x
 __device__ __forceinline__ float decay_step(float c, float h, float x) {
   const float t = fmaf(c, h, x);
   return is_diff(c) ? h + t : t;
+}
+// coefficient of two steps, one after the other
+__device__ __forceinline__ float decay_both(float c, float d) {
+  if (is_diff(c) && is_diff(d)) {
+    const float m = -fabsf(fmaf(c, d, c + d));
+    return m >= -0.5f ? m : 1.f + m;
+  }
+  return (is_diff(c) ? 1.f + c : c) * (is_diff(d) ? 1.f + d : d);
 }
 __device__ __forceinline__ float forgotten(float c) { return is_diff(c) ? -c : 1.f - c; }      // 1 - e^g
 
@@ -85,28 +95,64 @@ __device__ __forceinline__ void forget_copies(float (&c)[kSteps][kPer]) {
     for (int j = 0; j < kPer; ++j) asm volatile("" : "+f"(c[s][j]));
 }
 
-// Four channels of one token.  VEC: neighbours, one load; else every 16th channel, element by element, D and alignment as they are.
-template <bool VEC>
-__device__ __forceinline__ int channel_of(int lane, int j) { return VEC ? lane * kPer + j : lane + j * kLanes; }
+// Four channels of one token, W neighbours at a time: as many as D, strides and alignment let be loaded at once.
+template <int W>
+__device__ __forceinline__ int channel_of(int lane, int j) { return (j / W * kLanes + lane) * W + j % W; }
 
-template <int TY, bool VEC>
-__device__ __forceinline__ void load_token(Raw<TY, kPer>& r, const typename Elem<TY>::T* p, int lane, int room) {
-  if constexpr (VEC) {
-    if (lane * kPer < room) r.load(p + lane * kPer);
-  } else {
+// What a thread loads next lies in shared memory in places of its own, so that it is under way while the thread works on what it has
+// in registers; nobody else reads it, so nothing but the thread's own wait stands between.  [step][piece][thread]: no bank conflicts.
+template <int TY, int W> struct Staged {
+  static constexpr int kBytes = W * elem_bytes(TY), kPieces = kPer / W, kWords = kBytes / 4;
+  static constexpr bool kAsync = kBytes >= 4;      // (2 bytes are no asynchronous copy: loaded when they are wanted)
+  alignas(16) uint32_t w[kAsync ? kSteps : 1][kPieces][kAsync ? kScanThreads : 1][kAsync ? kWords : 1];      // (a copy's two ends lie on a boundary of its size)
+
+  // `base`: the tensor, an address that is good where nothing is read
+  __device__ __forceinline__ void fetch(const typename Elem<TY>::T* p, const void* base, long long stride, int lane, int live, int room) {
+    if constexpr (kAsync) {
 #pragma unroll
-    for (int j = 0; j < kPer; ++j)
-      if (lane + j * kLanes < room) raw_put(r, j, __ldg(p + lane + j * kLanes));
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+          const int ch = channel_of<W>(lane, i * W);
+          const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(&w[s][i][threadIdx.x][0]));
+          const bool there = s < live && ch < room;      // zeros otherwise
+          const void* from = there ? p + s * stride + ch : base;
+          if constexpr (kBytes == 16)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+          else
+            asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(kBytes), "r"(there ? kBytes : 0) : "memory");
+        }
+    }
   }
-}
-template <int TY, bool VEC>
-__device__ __forceinline__ void store_token(const Raw<TY, kPer>& r, typename Elem<TY>::T* p, int lane, int room) {
-  if constexpr (VEC) {
-    if (lane * kPer < room) r.store(p + lane * kPer);
-  } else {
+  __device__ __forceinline__ void take(Raw<TY, kPer> (&r)[kSteps], const typename Elem<TY>::T* p, long long stride, int lane, int live, int room) const {
 #pragma unroll
-    for (int j = 0; j < kPer; ++j)
-      if (lane + j * kLanes < room) p[lane + j * kLanes] = raw_take(r, j);
+    for (int s = 0; s < kSteps; ++s) {
+      if constexpr (kAsync) {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i)
+#pragma unroll
+          for (int k = 0; k < kWords; ++k) r[s].w[i * kWords + k] = w[s][i][threadIdx.x][k];
+      } else {
+        r[s].zero();
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+          if (s < live && channel_of<W>(lane, j) < room) raw_put(r[s], j, __ldg(p + s * stride + channel_of<W>(lane, j)));
+      }
+    }
+  }
+};
+template <int TY, int W>
+__device__ __forceinline__ void store_token(const Raw<TY, kPer>& r, typename Elem<TY>::T* p, int lane, int room) {
+  constexpr int kBytes = W * elem_bytes(TY), kWords = kBytes / 4;
+#pragma unroll
+  for (int i = 0; i < kPer / W; ++i) {
+    const int ch = channel_of<W>(lane, i * W);
+    if (ch >= room) continue;
+    uint32_t* d = reinterpret_cast<uint32_t*>(p + ch);
+    if constexpr (kWords == 4) *reinterpret_cast<uint4*>(d) = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
+    else if constexpr (kWords == 2) *reinterpret_cast<uint2*>(d) = make_uint2(r.w[i * 2], r.w[i * 2 + 1]);
+    else if constexpr (kWords == 1) *d = r.w[i];
+    else p[ch] = raw_take(r, i);
   }
 }
 template <int TY>
@@ -118,9 +164,9 @@ __device__ __forceinline__ Raw<TY, kPer> packed(const float (&v)[kPer]) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// What a tile hands on.  The state in front of a tile depends on all tiles before it; a tile leaves its own part, (sum of g, state
-// from zero), in the work buffer as soon as it has it, 64 bits per channel, stored and loaded as one, so a word that is there is
-// whole and needs no flag or fence beside it.  Unwritten words are all ones (the buffer is set so in front of the kernel).
+// What a tile hands on.  The state in front of a tile depends on all tiles before it; a tile leaves its own part, (coefficient
+// of its decay, state from zero), in the work buffer as soon as it has it, 64 bits per channel, stored and loaded as one, so a word
+// that is there is whole and needs no flag or fence beside it.  Unwritten words are all ones (the buffer is set so in front of the kernel).
 //
 // Three levels keep what a tile has to read at 31 words: the tiles of its group of 16 in front of it, the groups of its 16 groups in
 // front of it (the last tile of a group leaves that word, from the group's words alone), and the state behind the 256 tiles before
@@ -149,8 +195,8 @@ __device__ __forceinline__ unsigned long long look_load(const unsigned long long
   asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
   return v;
 }
-__device__ __forceinline__ void look_store(unsigned long long* p, float sum, float state) {
-  unsigned long long v = (static_cast<unsigned long long>(__float_as_uint(state)) << 32) | __float_as_uint(sum);
+__device__ __forceinline__ void look_store(unsigned long long* p, float coef, float state) {
+  unsigned long long v = (static_cast<unsigned long long>(__float_as_uint(state)) << 32) | __float_as_uint(coef);
   if (v == ~0ull) v = 0x7fffffff7fffffffull;      // (another NaN)
   asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
 }
@@ -171,7 +217,6 @@ __device__ __noinline__ unsigned long long look_wait(const unsigned long long* p
 
 struct LookShared {
   float2 part[2 * kFan - 1][kChannels];      // (coefficient, state): groups, then tiles, in front
-  float sum[kFan - 1][kChannels];            // sums of g of those tiles
   float base[kChannels];                     // state behind the 256 tiles before
 };
 struct ScanShared {
@@ -179,11 +224,20 @@ struct ScanShared {
   float sum[kGroups][kChannels];        // sum of its g
   float start[kGroups][kChannels];      // state in front of it
   LookShared look;
-  uint32_t ticket;
+  uint32_t ticket[2];
 };
 struct ScanSharedBackward : ScanShared {
   float back[kGroups][kChannels];       // per group the gradient that leaves it towards earlier tokens, from zero
   float end[kGroups][kChannels];        // the gradient that comes into it
+};
+template <int XT, int GT, int W> struct ForwardShared : ScanShared {
+  Staged<XT, W> x;
+  Staged<GT, W> g;
+};
+static_assert(alignof(Staged<LETHE_F32, 4>) == 16 && sizeof(Staged<LETHE_BF16, 4>) % 16 == 0, "asynchronous copies of 16 bytes");
+template <int XT, int GT, int W> struct BackwardShared : ScanSharedBackward {
+  Staged<XT, W> x, d;
+  Staged<GT, W> g;
 };
 
 // Where tile number `i` (in the order of the fold) of sequence `seq` stands among the three levels.
@@ -207,16 +261,21 @@ struct LookPlace {
   __device__ unsigned long long* at(int level, long long n, int ch) const { return buf.word[level] + n * kChannels + ch; }
 };
 
-// All threads.  Leaves what the fold reads in `l`; in between the last tile of a group leaves the group's word: `sum`, `state` of
+// All threads.  Leaves what the fold reads in `l`; in between the last tile of a group leaves the group's word: `coef`, `state` of
 // threads below kChannels are the tile's own.
-__device__ __forceinline__ void look_fetch(LookShared& l, const LookPlace& p, float sum, float state, int* status) {
+__device__ __forceinline__ void look_fetch(LookShared& l, const LookPlace& p, float coef, float state, int* status) {
   const int ch = threadIdx.x % kChannels, q = threadIdx.x / kChannels;
   constexpr int kQ = kScanThreads / kChannels, kEach = (kFan + kQ - 1) / kQ;
+  const auto as_pair = [](unsigned long long v) { return make_float2(__uint_as_float(static_cast<uint32_t>(v)), __uint_as_float(static_cast<uint32_t>(v >> 32))); };
   unsigned long long t[kEach], g[kEach], b = 0;
 #pragma unroll
   for (int m = 0; m < kEach; ++m) {
     const int k = q + m * kQ;
     if (k < p.n_tiles) t[m] = look_load(p.at(0, p.tile0 + k, ch));
+  }
+#pragma unroll
+  for (int m = 0; m < kEach; ++m) {
+    const int k = q + m * kQ;
     if (k < p.n_groups) g[m] = look_load(p.at(1, p.group0 + k, ch));
   }
   if (q == 0 && !p.first_super) b = look_load(p.at(2, p.super - 1, ch));
@@ -225,21 +284,19 @@ __device__ __forceinline__ void look_fetch(LookShared& l, const LookPlace& p, fl
     const int k = q + m * kQ;
     if (k < p.n_tiles) {
       if (t[m] == ~0ull) t[m] = look_wait(p.at(0, p.tile0 + k, ch), p.buf.head, status);
-      const float s = __uint_as_float(static_cast<uint32_t>(t[m]));
-      l.sum[k][ch] = s;
-      l.part[p.n_groups + k][ch] = make_float2(decay_coef(s), __uint_as_float(static_cast<uint32_t>(t[m] >> 32)));
+      l.part[p.n_groups + k][ch] = as_pair(t[m]);
     }
   }
   if (p.n_tiles == kFan - 1 && !p.last) {      // (the same for all threads of a CTA)
     __syncthreads();
     if (q == 0) {
-      float gs = 0.f, gh = 0.f;
+      float gc = -0.f, gh = 0.f;
       for (int k = 0; k < kFan - 1; ++k) {
         const float2 a = l.part[p.n_groups + k][ch];
-        gs += l.sum[k][ch];
+        gc = decay_both(gc, a.x);
         gh = decay_step(a.x, gh, a.y);
       }
-      look_store(p.at(1, p.group0 + p.n_groups, ch), gs + sum, decay_step(decay_coef(sum), gh, state));
+      look_store(p.at(1, p.group0 + p.n_groups, ch), decay_both(gc, coef), decay_step(coef, gh, state));
     }
   }
 #pragma unroll
@@ -247,12 +304,12 @@ __device__ __forceinline__ void look_fetch(LookShared& l, const LookPlace& p, fl
     const int k = q + m * kQ;
     if (k < p.n_groups) {
       if (g[m] == ~0ull) g[m] = look_wait(p.at(1, p.group0 + k, ch), p.buf.head, status);
-      l.part[k][ch] = make_float2(decay_coef(__uint_as_float(static_cast<uint32_t>(g[m]))), __uint_as_float(static_cast<uint32_t>(g[m] >> 32)));
+      l.part[k][ch] = as_pair(g[m]);
     }
   }
   if (q == 0 && !p.first_super) {
     if (b == ~0ull) b = look_wait(p.at(2, p.super - 1, ch), p.buf.head, status);
-    l.base[ch] = __uint_as_float(static_cast<uint32_t>(b >> 32));
+    l.base[ch] = as_pair(b).y;
   }
   __syncthreads();
 }
@@ -266,242 +323,288 @@ __device__ __forceinline__ float look_fold(const LookShared& l, const LookPlace&
   return carry;
 }
 
-// One CTA does one tile of kTokens tokens x kChannels channels.
-template <int XT, int GT, bool VEC, bool COMP>
+// Where a tile lies.
+struct TilePlace {
+  long long seq, b, ch0, t0;      // sequence (a strip of one), batch, first channel, first token of this thread
+  int tile, room, live;           // channels of the strip; tokens of this thread (0 and less: none)
+  __device__ __forceinline__ TilePlace(const DiagProblem& p, uint32_t ticket, int grp, bool backwards) {
+    const uint32_t order = ticket / p.seqs;
+    seq = ticket - order * p.seqs;
+    tile = backwards ? p.tiles - 1 - static_cast<int>(order) : static_cast<int>(order);
+    const uint32_t s = static_cast<uint32_t>(seq);
+    b = s / static_cast<uint32_t>(p.strips);
+    ch0 = static_cast<long long>(s % static_cast<uint32_t>(p.strips)) * kChannels;
+    room = static_cast<int>(p.D - ch0 < kChannels ? p.D - ch0 : kChannels);
+    t0 = static_cast<long long>(tile) * kTokens + grp * kSteps;
+    live = static_cast<int>(p.L - t0 < kSteps ? p.L - t0 : kSteps);
+  }
+};
+
+// The CTAs take tiles until there are none; a CTA's tickets ascend, and it takes the next one while it works on a tile: the tile of the
+// lowest ticket that is not done is the one that its CTA works on, so somebody always can go on.
+template <int XT, int GT, int W, bool COMP>
 __global__ void __launch_bounds__(kScanThreads, 2) diag_forward_kernel(const DiagProblem p) {
   using X = typename Elem<XT>::T;
   using G = typename Elem<GT>::T;
-  __shared__ ScanShared sh;
+  extern __shared__ __align__(16) unsigned char smem[];
+  auto& sh = *reinterpret_cast<ForwardShared<XT, GT, W>*>(smem);
   const int lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
-  long long seq = blockIdx.x;
-  int tile = 0;
-  if (p.tiles > 1) {
-    if (threadIdx.x == 0) sh.ticket = atomicAdd(p.look.head, 1u) + 1u;
-    __syncthreads();
-    tile = static_cast<int>(sh.ticket / p.seqs);
-    seq = sh.ticket % p.seqs;
+  const uint32_t total = p.seqs * static_cast<uint32_t>(p.tiles);
+  const auto take_ticket = [&](uint32_t have) { return p.tiles > 1 ? atomicAdd(p.look.head, 1u) + 1u : have + gridDim.x; };
+  const auto x_at = [&](const TilePlace& t) { return static_cast<const X*>(p.x) + t.b * p.x_batch + t.t0 * p.x_token + t.ch0; };
+  const auto g_at = [&](const TilePlace& t) { return static_cast<const G*>(p.g) + t.b * p.g_batch + t.t0 * p.g_token + t.ch0; };
+  const auto fetch = [&](uint32_t ticket) {
+    if (ticket < total) {
+      const TilePlace t(p, ticket, grp, false);
+      sh.x.fetch(x_at(t), p.x, p.x_token, lane, t.live, t.room);
+      sh.g.fetch(g_at(t), p.g, p.g_token, lane, t.live, t.room);
+    }
+  };
+  if (threadIdx.x == 0) {
+    const uint32_t first = p.tiles > 1 ? take_ticket(0) : blockIdx.x;
+    sh.ticket[0] = first;
+    sh.ticket[1] = take_ticket(first);
   }
-  const long long b = seq / p.strips, ch0 = (seq % p.strips) * kChannels;
-  const int room = static_cast<int>(p.D - ch0 < kChannels ? p.D - ch0 : kChannels);
-  const long long t0 = static_cast<long long>(tile) * kTokens + grp * kSteps;
-  const X* x = static_cast<const X*>(p.x) + b * p.x_batch + t0 * p.x_token + ch0;
-  const G* g = static_cast<const G*>(p.g) + b * p.g_batch + t0 * p.g_token + ch0;
-  X* h = static_cast<X*>(p.h) + (b * p.L + t0) * p.D + ch0;
-  const int live = static_cast<int>(p.L - t0 < kSteps ? p.L - t0 : kSteps);      // tokens of this thread (0 and less: none)
-  Raw<XT, kPer> xr[kSteps];
-  float c[kSteps][kPer], sum[kPer], st[kPer];
-  {
-    Raw<GT, kPer> gr[kSteps];
+  __syncthreads();
+  uint32_t ticket = sh.ticket[0];
+  fetch(ticket);
+  for (int turn = 0; ticket < total; turn ^= 1) {
+    const TilePlace at(p, ticket, grp, false);
+    const int room = at.room, live = at.live;
+    Raw<XT, kPer> xr[kSteps];
+    float c[kSteps][kPer], sum[kPer], st[kPer];
+    const uint32_t next = sh.ticket[turn ^ 1];
+    uint32_t after = 0;
+    {
+      Raw<GT, kPer> gr[kSteps];
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      sh.x.take(xr, x_at(at), p.x_token, lane, live, room);
+      sh.g.take(gr, g_at(at), p.g_token, lane, live, room);
+      fetch(next);
+      if (threadIdx.x == 0) after = take_ticket(next);
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      xr[s].zero();
-      gr[s].zero();
-      if (s < live) {
-        load_token<XT, VEC>(xr[s], x + s * p.x_token, lane, room);
-        load_token<GT, VEC>(gr[s], g + s * p.g_token, lane, room);
-      }
+      for (int j = 0; j < kPer; ++j) sum[j] = st[j] = 0.f;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          const float gv = gr[s].get(j);
+          c[s][j] = decay_coef(gv);
+          sum[j] += gv;
+          const float u = COMP ? xr[s].get(j) * forgotten(c[s][j]) : xr[s].get(j);
+          st[j] = decay_step(c[s][j], st[j], u);
+        }
     }
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) sum[j] = st[j] = 0.f;
+    for (int j = 0; j < kPer; ++j) {
+      const int ch = channel_of<W>(lane, j);
+      sh.part[grp][ch] = make_float2(decay_coef(sum[j]), st[j]);
+      sh.sum[grp][ch] = sum[j];
+    }
+    forget_copies(xr);
+    forget_copies(c);
+    __syncthreads();
+    if (threadIdx.x == 0) sh.ticket[turn] = after;      // (read behind the next barriers)
+    const int ch = threadIdx.x;      // of threads below kChannels
+    float carry = 0.f;
+    if (ch < room && p.h0) carry = p.h0[at.b * p.D + at.ch0 + ch];
+    if (p.tiles > 1) {
+      const LookPlace look(p.look, at.seq, p.tiles, at.tile);
+      float tc = -0.f, th = 0.f;
+      if (ch < kChannels) {
+        float ts = 0.f;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s)
+        for (int i = 0; i < kGroups; ++i) {
+          const float2 a = sh.part[i][ch];
+          ts += sh.sum[i][ch];
+          th = decay_step(a.x, th, a.y);
+        }
+        tc = decay_coef(ts);
+        if (!look.last) look_store(look.at(0, look.tile0 + look.n_tiles, ch), tc, th);
+      }
+      look_fetch(sh.look, look, tc, th, p.status);
+      if (ch < kChannels) {
+        carry = look_fold(sh.look, look, carry);
+        if (look.n_tiles == kFan - 1 && look.n_groups == kFan - 1 && !look.last) look_store(look.at(2, look.super, ch), 0.f, decay_step(tc, carry, th));
+      }
+    }
+    if (ch < kChannels) {
+      if (p.states && ch < room) p.states[(at.b * p.tiles + at.tile) * p.D + at.ch0 + ch] = carry;
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) {
+        sh.start[i][ch] = carry;
+        const float2 a = sh.part[i][ch];
+        carry = decay_step(a.x, carry, a.y);
+      }
+      if (p.hT && ch < room && at.tile == p.tiles - 1) p.hT[at.b * p.D + at.ch0 + ch] = carry;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) st[j] = sh.start[grp][channel_of<W>(lane, j)];
+    X* h = static_cast<X*>(p.h) + (at.b * p.L + at.t0) * p.D + at.ch0;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
-        const float gv = gr[s].get(j);
-        c[s][j] = decay_coef(gv);
-        sum[j] += gv;
         const float u = COMP ? xr[s].get(j) * forgotten(c[s][j]) : xr[s].get(j);
         st[j] = decay_step(c[s][j], st[j], u);
       }
-  }
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    const int ch = channel_of<VEC>(lane, j);
-    sh.part[grp][ch] = make_float2(decay_coef(sum[j]), st[j]);
-    sh.sum[grp][ch] = sum[j];
-  }
-  forget_copies(xr);
-  forget_copies(c);
-  __syncthreads();
-  const int ch = threadIdx.x;      // of threads below kChannels
-  float carry = 0.f;
-  if (ch < room && p.h0) carry = p.h0[b * p.D + ch0 + ch];
-  if (p.tiles > 1) {
-    const LookPlace at(p.look, seq, p.tiles, tile);
-    float ts = 0.f, th = 0.f;
-    if (ch < kChannels) {
-#pragma unroll
-      for (int i = 0; i < kGroups; ++i) {
-        const float2 a = sh.part[i][ch];
-        ts += sh.sum[i][ch];
-        th = decay_step(a.x, th, a.y);
-      }
-      if (!at.last) look_store(at.at(0, at.tile0 + at.n_tiles, ch), ts, th);
+      if (s < live) store_token<XT, W>(packed<XT>(st), h + s * p.D, lane, room);
     }
-    look_fetch(sh.look, at, ts, th, p.status);
-    if (ch < kChannels) {
-      carry = look_fold(sh.look, at, carry);
-      if (at.n_tiles == kFan - 1 && at.n_groups == kFan - 1 && !at.last) look_store(at.at(2, at.super, ch), 0.f, decay_step(decay_coef(ts), carry, th));
-    }
-  }
-  if (ch < kChannels) {
-    if (p.states && ch < room) p.states[(b * p.tiles + tile) * p.D + ch0 + ch] = carry;
-#pragma unroll
-    for (int i = 0; i < kGroups; ++i) {
-      sh.start[i][ch] = carry;
-      const float2 a = sh.part[i][ch];
-      carry = decay_step(a.x, carry, a.y);
-    }
-    if (p.hT && ch < room && tile == p.tiles - 1) p.hT[b * p.D + ch0 + ch] = carry;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) st[j] = sh.start[grp][channel_of<VEC>(lane, j)];
-#pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const float u = COMP ? xr[s].get(j) * forgotten(c[s][j]) : xr[s].get(j);
-      st[j] = decay_step(c[s][j], st[j], u);
-    }
-    if (s < live) store_token<XT, VEC>(packed<XT>(st), h + s * p.D, lane, room);
+    ticket = next;
   }
 }
 
-template <int XT, int GT, bool VEC, bool COMP>
+template <int XT, int GT, int W, bool COMP>
 __global__ void __launch_bounds__(kScanThreads, 2) diag_backward_kernel(const DiagProblem p) {
   using X = typename Elem<XT>::T;
   using G = typename Elem<GT>::T;
-  __shared__ ScanSharedBackward sh;
+  extern __shared__ __align__(16) unsigned char smem[];
+  auto& sh = *reinterpret_cast<BackwardShared<XT, GT, W>*>(smem);
   const int lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
-  long long seq = blockIdx.x;
-  int order = 0;                      // of the tile, from the last one on
-  if (p.tiles > 1) {
-    if (threadIdx.x == 0) sh.ticket = atomicAdd(p.look.head, 1u) + 1u;
-    __syncthreads();
-    order = static_cast<int>(sh.ticket / p.seqs);
-    seq = sh.ticket % p.seqs;
+  const uint32_t total = p.seqs * static_cast<uint32_t>(p.tiles);
+  const auto take_ticket = [&](uint32_t have) { return p.tiles > 1 ? atomicAdd(p.look.head, 1u) + 1u : have + gridDim.x; };
+  const auto x_at = [&](const TilePlace& t) { return static_cast<const X*>(p.x) + t.b * p.x_batch + t.t0 * p.x_token + t.ch0; };
+  const auto g_at = [&](const TilePlace& t) { return static_cast<const G*>(p.g) + t.b * p.g_batch + t.t0 * p.g_token + t.ch0; };
+  const auto d_at = [&](const TilePlace& t) { return static_cast<const X*>(p.d_h) + t.b * p.d_batch + t.t0 * p.d_token + t.ch0; };
+  const auto fetch = [&](uint32_t ticket) {
+    if (ticket < total) {
+      const TilePlace t(p, ticket, grp, true);
+      sh.x.fetch(x_at(t), p.x, p.x_token, lane, t.live, t.room);
+      sh.g.fetch(g_at(t), p.g, p.g_token, lane, t.live, t.room);
+      if (p.d_h) sh.d.fetch(d_at(t), p.d_h, p.d_token, lane, t.live, t.room);
+    }
+  };
+  if (threadIdx.x == 0) {
+    const uint32_t first = p.tiles > 1 ? take_ticket(0) : blockIdx.x;
+    sh.ticket[0] = first;
+    sh.ticket[1] = take_ticket(first);
   }
-  const int tile = p.tiles - 1 - order;
-  const long long b = seq / p.strips, ch0 = (seq % p.strips) * kChannels;
-  const int room = static_cast<int>(p.D - ch0 < kChannels ? p.D - ch0 : kChannels);
-  const long long t0 = static_cast<long long>(tile) * kTokens + grp * kSteps;
-  const X* x = static_cast<const X*>(p.x) + b * p.x_batch + t0 * p.x_token + ch0;
-  const G* g = static_cast<const G*>(p.g) + b * p.g_batch + t0 * p.g_token + ch0;
-  const X* d = static_cast<const X*>(p.d_h) + b * p.d_batch + t0 * p.d_token + ch0;
-  X* dx = static_cast<X*>(p.dx) + (b * p.L + t0) * p.D + ch0;
-  G* dg = static_cast<G*>(p.dg) + (b * p.L + t0) * p.D + ch0;
-  const int live = static_cast<int>(p.L - t0 < kSteps ? p.L - t0 : kSteps);
-  Raw<XT, kPer> xr[kSteps], dr[kSteps];
-  float c[kSteps][kPer], st[kPer], e[kPer];
-  {
-    Raw<GT, kPer> gr[kSteps];
-    float sum[kPer];
+  __syncthreads();
+  uint32_t ticket = sh.ticket[0];
+  fetch(ticket);
+  for (int turn = 0; ticket < total; turn ^= 1) {
+    const TilePlace at(p, ticket, grp, true);
+    const int room = at.room, live = at.live;
+    Raw<XT, kPer> xr[kSteps], dr[kSteps];
+    float c[kSteps][kPer], st[kPer], e[kPer];
+    const uint32_t next = sh.ticket[turn ^ 1];
+    uint32_t after = 0;
+    {
+      Raw<GT, kPer> gr[kSteps];
+      float sum[kPer];
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      sh.x.take(xr, x_at(at), p.x_token, lane, live, room);
+      sh.g.take(gr, g_at(at), p.g_token, lane, live, room);
+      if (p.d_h) {
+        sh.d.take(dr, d_at(at), p.d_token, lane, live, room);
+      } else {
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      xr[s].zero();
-      gr[s].zero();
-      dr[s].zero();
-      if (s < live) {
-        load_token<XT, VEC>(xr[s], x + s * p.x_token, lane, room);
-        load_token<GT, VEC>(gr[s], g + s * p.g_token, lane, room);
-        if (p.d_h) load_token<XT, VEC>(dr[s], d + s * p.d_token, lane, room);
+        for (int s = 0; s < kSteps; ++s) dr[s].zero();
+      }
+      fetch(next);
+      if (threadIdx.x == 0) after = take_ticket(next);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) sum[j] = st[j] = e[j] = 0.f;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          const float gv = gr[s].get(j);
+          c[s][j] = decay_coef(gv);
+          sum[j] += gv;
+          const float u = COMP ? xr[s].get(j) * forgotten(c[s][j]) : xr[s].get(j);
+          st[j] = decay_step(c[s][j], st[j], u);
+        }
+#pragma unroll
+      for (int s = kSteps - 1; s >= 0; --s)
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) e[j] = decay_step(c[s][j], dr[s].get(j) + e[j], 0.f);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const int ch = channel_of<W>(lane, j);
+        sh.part[grp][ch] = make_float2(decay_coef(sum[j]), st[j]);
+        sh.sum[grp][ch] = sum[j];
+        sh.back[grp][ch] = e[j];
       }
     }
+    forget_copies(xr);
+    forget_copies(dr);
+    forget_copies(c);
+    __syncthreads();
+    if (threadIdx.x == 0) sh.ticket[turn] = after;
+    const int ch = threadIdx.x, ch2 = threadIdx.x - kChannels;      // the gradient is folded by threads below kChannels, the state by the next ones
+    float carry = 0.f;
+    if (ch < room && p.dhT) carry = p.dhT[at.b * p.D + at.ch0 + ch];
+    if (ch2 >= 0 && ch2 < kChannels) {
+      float s0 = ch2 < room ? p.states[(at.b * p.tiles + at.tile) * p.D + at.ch0 + ch2] : 0.f;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) sum[j] = st[j] = e[j] = 0.f;
+      for (int i = 0; i < kGroups; ++i) {
+        sh.start[i][ch2] = s0;
+        const float2 a = sh.part[i][ch2];
+        s0 = decay_step(a.x, s0, a.y);
+      }
+    }
+    if (p.tiles > 1) {
+      const LookPlace look(p.look, at.seq, p.tiles, p.tiles - 1 - at.tile);
+      float tc = -0.f, te = 0.f;
+      if (ch < kChannels) {
+        float ts = 0.f;
+#pragma unroll
+        for (int i = kGroups - 1; i >= 0; --i) {
+          ts += sh.sum[i][ch];
+          te = decay_step(sh.part[i][ch].x, te, sh.back[i][ch]);
+        }
+        tc = decay_coef(ts);
+        if (!look.last) look_store(look.at(0, look.tile0 + look.n_tiles, ch), tc, te);
+      }
+      look_fetch(sh.look, look, tc, te, p.status);
+      if (ch < kChannels) {
+        carry = look_fold(sh.look, look, carry);
+        if (look.n_tiles == kFan - 1 && look.n_groups == kFan - 1 && !look.last) look_store(look.at(2, look.super, ch), 0.f, decay_step(tc, carry, te));
+      }
+    }
+    if (ch < kChannels) {
+#pragma unroll
+      for (int i = kGroups - 1; i >= 0; --i) {
+        sh.end[i][ch] = carry;
+        carry = decay_step(sh.part[i][ch].x, carry, sh.back[i][ch]);
+      }
+      if (p.dh0 && ch < room && at.tile == 0) p.dh0[at.b * p.D + at.ch0 + ch] = carry;
+    }
+    __syncthreads();
+    float before[kSteps][kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      st[j] = sh.start[grp][channel_of<W>(lane, j)];
+      e[j] = sh.end[grp][channel_of<W>(lane, j)];
+    }
 #pragma unroll
     for (int s = 0; s < kSteps; ++s)
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
-        const float gv = gr[s].get(j);
-        c[s][j] = decay_coef(gv);
-        sum[j] += gv;
-        const float u = COMP ? xr[s].get(j) * forgotten(c[s][j]) : xr[s].get(j);
-        st[j] = decay_step(c[s][j], st[j], u);
+        const float xv = xr[s].get(j);
+        before[s][j] = COMP ? st[j] - xv : st[j];
+        st[j] = decay_step(c[s][j], st[j], COMP ? xv * forgotten(c[s][j]) : xv);
       }
+    X* dx = static_cast<X*>(p.dx) + (at.b * p.L + at.t0) * p.D + at.ch0;
+    G* dg = static_cast<G*>(p.dg) + (at.b * p.L + at.t0) * p.D + at.ch0;
 #pragma unroll
-    for (int s = kSteps - 1; s >= 0; --s)
+    for (int s = kSteps - 1; s >= 0; --s) {
+      float vx[kPer], vg[kPer];
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) e[j] = decay_step(c[s][j], dr[s].get(j) + e[j], 0.f);
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int ch = channel_of<VEC>(lane, j);
-      sh.part[grp][ch] = make_float2(decay_coef(sum[j]), st[j]);
-      sh.sum[grp][ch] = sum[j];
-      sh.back[grp][ch] = e[j];
-    }
-  }
-  forget_copies(xr);
-  forget_copies(dr);
-  forget_copies(c);
-  __syncthreads();
-  const int ch = threadIdx.x, ch2 = threadIdx.x - kChannels;      // the gradient is folded by threads below kChannels, the state by the next ones
-  float carry = 0.f;
-  if (ch < room && p.dhT) carry = p.dhT[b * p.D + ch0 + ch];
-  if (ch2 >= 0 && ch2 < kChannels) {
-    float s0 = ch2 < room ? p.states[(b * p.tiles + tile) * p.D + ch0 + ch2] : 0.f;
-#pragma unroll
-    for (int i = 0; i < kGroups; ++i) {
-      sh.start[i][ch2] = s0;
-      const float2 a = sh.part[i][ch2];
-      s0 = decay_step(a.x, s0, a.y);
-    }
-  }
-  if (p.tiles > 1) {
-    const LookPlace at(p.look, seq, p.tiles, order);
-    float ts = 0.f, te = 0.f;
-    if (ch < kChannels) {
-#pragma unroll
-      for (int i = kGroups - 1; i >= 0; --i) {
-        ts += sh.sum[i][ch];
-        te = decay_step(sh.part[i][ch].x, te, sh.back[i][ch]);
+      for (int j = 0; j < kPer; ++j) {
+        const float dv = dr[s].get(j) + e[j];
+        vx[j] = COMP ? dv * forgotten(c[s][j]) : dv;
+        e[j] = decay_step(c[s][j], dv, 0.f);
+        vg[j] = e[j] * before[s][j];
       }
-      if (!at.last) look_store(at.at(0, at.tile0 + at.n_tiles, ch), ts, te);
+      if (s < live) {
+        if (p.dx) store_token<XT, W>(packed<XT>(vx), dx + s * p.D, lane, room);
+        if (p.dg) store_token<GT, W>(packed<GT>(vg), dg + s * p.D, lane, room);
+      }
     }
-    look_fetch(sh.look, at, ts, te, p.status);
-    if (ch < kChannels) {
-      carry = look_fold(sh.look, at, carry);
-      if (at.n_tiles == kFan - 1 && at.n_groups == kFan - 1 && !at.last) look_store(at.at(2, at.super, ch), 0.f, decay_step(decay_coef(ts), carry, te));
-    }
-  }
-  if (ch < kChannels) {
-#pragma unroll
-    for (int i = kGroups - 1; i >= 0; --i) {
-      sh.end[i][ch] = carry;
-      carry = decay_step(sh.part[i][ch].x, carry, sh.back[i][ch]);
-    }
-    if (p.dh0 && ch < room && tile == 0) p.dh0[b * p.D + ch0 + ch] = carry;
-  }
-  __syncthreads();
-  float before[kSteps][kPer];
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    st[j] = sh.start[grp][channel_of<VEC>(lane, j)];
-    e[j] = sh.end[grp][channel_of<VEC>(lane, j)];
-  }
-#pragma unroll
-  for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const float xv = xr[s].get(j);
-      before[s][j] = COMP ? st[j] - xv : st[j];
-      st[j] = decay_step(c[s][j], st[j], COMP ? xv * forgotten(c[s][j]) : xv);
-    }
-#pragma unroll
-  for (int s = kSteps - 1; s >= 0; --s) {
-    float vx[kPer], vg[kPer];
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const float dv = dr[s].get(j) + e[j];
-      vx[j] = COMP ? dv * forgotten(c[s][j]) : dv;
-      e[j] = decay_step(c[s][j], dv, 0.f);
-      vg[j] = e[j] * before[s][j];
-    }
-    if (s < live) {
-      if (p.dx) store_token<XT, VEC>(packed<XT>(vx), dx + s * p.D, lane, room);
-      if (p.dg) store_token<GT, VEC>(packed<GT>(vg), dg + s * p.D, lane, room);
-    }
+    ticket = next;
   }
 }
 
@@ -516,19 +619,19 @@ struct StepProblem {
   int blocks;      // CTAs of a sequence
 };
 
-// One token: state and h, four neighbouring channels a thread (VEC) or one.
-template <int XT, int GT, bool VEC, bool COMP>
+// One token: state and h, four neighbouring channels a thread (W = 4) or one.
+template <int XT, int GT, int W, bool COMP>
 __global__ void __launch_bounds__(256) diag_step_kernel(const StepProblem p) {
   using X = typename Elem<XT>::T;
   using G = typename Elem<GT>::T;
-  constexpr int N = VEC ? kPer : 1;
+  constexpr int N = W == kPer ? kPer : 1;
   const long long b = blockIdx.x / p.blocks, at = (static_cast<long long>(blockIdx.x % p.blocks) * 256 + threadIdx.x) * N;
   if (at >= p.D) return;
   const X* x = static_cast<const X*>(p.x) + b * p.x_batch + at;
   const G* g = static_cast<const G*>(p.g) + b * p.g_batch + at;
   X* h = static_cast<X*>(p.h) + b * p.D + at;
   float* st = p.state + b * p.D + at;
-  if constexpr (VEC) {
+  if constexpr (N > 1) {
     Raw<XT, N> xr;
     Raw<GT, N> gr;
     xr.load(x);
@@ -557,12 +660,14 @@ static bool on_boundary(const void* ptr, int ty, int n, long long s0 = 0, long l
   return reinterpret_cast<uintptr_t>(ptr) % (n * elem_bytes(ty)) == 0 && s0 % n == 0 && s1 % n == 0;
 }
 
-// f(XT, GT, VEC, COMP) as template arguments
+// f(XT, GT, W, COMP) as template arguments
 template <typename F>
-static int by_type(int xt, int gt, bool vec, bool comp, F&& f) {
-  auto flags = [&](auto x, auto g) {
-    if (vec) return comp ? f(x, g, std::true_type(), std::true_type()) : f(x, g, std::true_type(), std::false_type());
-    return comp ? f(x, g, std::false_type(), std::true_type()) : f(x, g, std::false_type(), std::false_type());
+static int by_type(int xt, int gt, int w, bool comp, F&& f) {
+  const auto flags = [&](auto x, auto g) {
+    const auto last = [&](auto n) { return comp ? f(x, g, n, std::true_type()) : f(x, g, n, std::false_type()); };
+    if (w == 4) return last(std::integral_constant<int, 4>());
+    if (w == 2) return last(std::integral_constant<int, 2>());
+    return last(std::integral_constant<int, 1>());
   };
   using T32 = std::integral_constant<int, LETHE_F32>;
   using TB = std::integral_constant<int, LETHE_BF16>;
@@ -593,10 +698,18 @@ static int diag_problem(const LetheGdnDiagArgs* a, DiagProblem* p, bool backward
   }
   return kOk;
 }
-// all ones: no word is there yet, and the ticket before the first
-static int look_clear(const DiagProblem& p, cudaStream_t st) {
-  if (p.tiles <= 1) return kOk;
-  return cudaMemsetAsync(p.look.head, 0xff, look_sizes(p.seqs, p.tiles).bytes(), st) == cudaSuccess ? kOk : kErrLaunch;
+// elements that can be moved at once
+template <typename F>
+static int widest(F&& fits) { return fits(4) ? 4 : fits(2) ? 2 : 1; }
+
+template <typename Shared>
+static int launch_scan_tiles(void (*kern)(DiagProblem), const DiagProblem& p, SmemAttr& attr, cudaStream_t st) {
+  if (int e = attr.set(kern, sizeof(Shared))) return e;
+  // all ones: no word is there yet, and the ticket before the first
+  if (p.tiles > 1 && cudaMemsetAsync(p.look.head, 0xff, look_sizes(p.seqs, p.tiles).bytes(), st) != cudaSuccess) return kErrLaunch;
+  const uint32_t total = p.seqs * static_cast<uint32_t>(p.tiles), room = 2u * static_cast<uint32_t>(sm_count());
+  kern<<<total < room ? total : room, kScanThreads, sizeof(Shared), st>>>(p);
+  return launched();
 }
 
 }  // namespace lg
@@ -618,13 +731,13 @@ extern "C" int lethe_gdn_diag_forward(const LetheGdnDiagArgs* a, void* stream) {
   if (int e = diag_problem(a, &p, false)) return e;
   DeviceGuard guard(a->x);
   if (!guard.ok) return kErrDevice;
-  const bool vec = a->D % kPer == 0 && on_boundary(a->x, a->x_type, kPer, a->x_batch, a->x_token) &&
-                   on_boundary(a->g, a->g_type, kPer, a->g_batch, a->g_token) && on_boundary(a->h, a->x_type, kPer);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (int e = look_clear(p, st)) return e;
-  return by_type(a->x_type, a->g_type, vec, a->complement != 0, [&](auto x, auto g, auto v, auto c) {
-    diag_forward_kernel<x.value, g.value, v.value, c.value><<<p.seqs * p.tiles, kScanThreads, 0, st>>>(p);
-    return launched();
+  const int w = widest([&](int n) {
+    return a->D % n == 0 && on_boundary(a->x, a->x_type, n, a->x_batch, a->x_token) && on_boundary(a->g, a->g_type, n, a->g_batch, a->g_token) &&
+           on_boundary(a->h, a->x_type, n);
+  });
+  return by_type(a->x_type, a->g_type, w, a->complement != 0, [&](auto x, auto g, auto n, auto c) {
+    static SmemAttr attr;
+    return launch_scan_tiles<ForwardShared<x.value, g.value, n.value>>(diag_forward_kernel<x.value, g.value, n.value, c.value>, p, attr, static_cast<cudaStream_t>(stream));
   });
 }
 
@@ -634,15 +747,13 @@ extern "C" int lethe_gdn_diag_backward(const LetheGdnDiagArgs* a, void* stream) 
   if (int e = diag_problem(a, &p, true)) return e;
   DeviceGuard guard(a->x);
   if (!guard.ok) return kErrDevice;
-  const bool vec = a->D % kPer == 0 && on_boundary(a->x, a->x_type, kPer, a->x_batch, a->x_token) &&
-                   on_boundary(a->g, a->g_type, kPer, a->g_batch, a->g_token) &&
-                   on_boundary(a->d_h, a->x_type, kPer, a->d_h_batch, a->d_h_token) && on_boundary(a->dx, a->x_type, kPer) &&
-                   on_boundary(a->dg, a->g_type, kPer);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (int e = look_clear(p, st)) return e;
-  return by_type(a->x_type, a->g_type, vec, a->complement != 0, [&](auto x, auto g, auto v, auto c) {
-    diag_backward_kernel<x.value, g.value, v.value, c.value><<<p.seqs * p.tiles, kScanThreads, 0, st>>>(p);
-    return launched();
+  const int w = widest([&](int n) {
+    return a->D % n == 0 && on_boundary(a->x, a->x_type, n, a->x_batch, a->x_token) && on_boundary(a->g, a->g_type, n, a->g_batch, a->g_token) &&
+           on_boundary(a->d_h, a->x_type, n, a->d_h_batch, a->d_h_token) && on_boundary(a->dx, a->x_type, n) && on_boundary(a->dg, a->g_type, n);
+  });
+  return by_type(a->x_type, a->g_type, w, a->complement != 0, [&](auto x, auto g, auto n, auto c) {
+    static SmemAttr attr;
+    return launch_scan_tiles<BackwardShared<x.value, g.value, n.value>>(diag_backward_kernel<x.value, g.value, n.value, c.value>, p, attr, static_cast<cudaStream_t>(stream));
   });
 }
 
@@ -658,8 +769,8 @@ extern "C" int lethe_gdn_diag_step(const LetheGdnDiagArgs* a, float* state, void
   DeviceGuard guard(a->x);
   if (!guard.ok) return kErrDevice;
   const StepProblem p{a->B, a->D, a->x, a->x_batch, a->g, a->g_batch, a->h, state, static_cast<int>(blocks)};
-  return by_type(a->x_type, a->g_type, vec, a->complement != 0, [&](auto x, auto g, auto v, auto c) {
-    diag_step_kernel<x.value, g.value, v.value, c.value>
+  return by_type(a->x_type, a->g_type, vec ? kPer : 1, a->complement != 0, [&](auto x, auto g, auto n, auto c) {
+    diag_step_kernel<x.value, g.value, n.value == kPer ? kPer : 1, c.value>
         <<<static_cast<unsigned>(p.B * blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
     return launched();
   });
