@@ -287,8 +287,8 @@ typedef struct LetheGdnDiagArgs {
   size_t work_bytes;
   int32_t* status;
 } LetheGdnDiagArgs;
-size_t lethe_gdn_diag_states_bytes(int64_t B, int64_t L, int64_t D);
-size_t lethe_gdn_diag_work_bytes(int64_t B, int64_t L, int64_t D);
+size_t lethe_gdn_diag_states_bytes(int64_t B, int64_t L, int64_t D, int32_t x_type);
+size_t lethe_gdn_diag_work_bytes(int64_t B, int64_t L, int64_t D, int32_t x_type, int32_t backward);
 int lethe_gdn_diag_forward(const LetheGdnDiagArgs* args, void* cuda_stream);
 int lethe_gdn_diag_backward(const LetheGdnDiagArgs* args, void* cuda_stream);
 

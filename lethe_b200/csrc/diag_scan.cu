@@ -2,11 +2,10 @@
 //
 // Bound by HBM: some 10 to 20 operations for every 8 bytes forward (bf16 x and h, fp32 g) and 14 backward.
 //
-// A CTA does a tile of kTokens tokens of kChannels channels of one sequence, read once and held in registers: a thread has kSteps
-// tokens of four channels, its 16-lane group covers the channels, kGroups groups the tokens.  Every thread runs its own tokens from
-// a zero state, the groups' results (sum of g, state) meet in shared memory and are folded in order, the tile gets the state in
-// front of it from the tiles before (below), and every thread runs its tokens again from the state that it really starts from.
-// The order of all sums is fixed, so two runs give the same bits.
+// A CTA does tiles, 16 groups of tokens x 64 channels of one sequence, each read once: a thread has 3 to 8 tokens of four channels, its
+// 16-lane group covers the channels.  Every thread runs its own tokens from a zero state, the groups' results (sum of g, state) meet in shared memory and are folded in order, the tile gets the state in front of it from the tiles before (below), and
+// every thread runs its tokens again from the state that it really starts from.  The order of all sums is fixed, so two runs give
+// the same bits.
 //
 // The decay.  With memories of thousands of tokens e^g lies next to one, and fp32 rounds it by up to 2^-25: over n tokens the
 // state is off by up to n times that, always to the same side where g is constant.  So below |g| = 1/4 the step is taken with
@@ -20,38 +19,36 @@
 
 namespace lg {
 
-constexpr int kLanes = 16, kPer = 4, kChannels = kLanes * kPer;
-constexpr int kGroups = 16, kSteps = 8, kTokens = kGroups * kSteps;
-constexpr int kScanThreads = kLanes * kGroups;
+constexpr int kLanes = 16, kPer = 4, kChannels = kLanes * kPer;      // a strip of channels
+constexpr int kGroups = 16, kRunners = kLanes * kGroups;              // threads that hold a tile
+constexpr int kPublisher = kRunners, kLooker = kPublisher + 32;         // first threads of the warp that hands on and of those that look back
+constexpr int kScanThreads = kLooker + kChannels;
+// Tokens of a thread: what two tiles of two CTAs take in shared memory decides.  The forward leaves a state for every tile of the backward.
+constexpr int forward_steps(int xt) { return xt == LETHE_F32 ? 6 : 8; }
+constexpr int backward_steps(int xt) { return forward_steps(xt) / 2; }
 
-// coefficient of a step over the log decay g
+// whether the step over the log decay g is taken with the difference: -1/4 < g <= -0 (as whole numbers, negative floats are ordered
+// backwards; +0 has the coefficient one)
+__device__ __forceinline__ bool by_diff(float g) { return __float_as_int(g) < static_cast<int>(0xbe800000u); }
+// coefficient of that step
 __device__ __forceinline__ float decay_coef(float g) {
-  // e^g - 1 = g (1 + g/2 + g^2/6 + ... + g^6/5040): the first term left out is under 2e-9 of the result for |g| <= 1/4
-  float s = fmaf(g, 1.f / 5040.f, 1.f / 720.f);
-  s = fmaf(g, s, 1.f / 120.f);
+  // e^g - 1 = g (1 + g/2 + g^2/6 + ... + g^5/720): the first term left out is under 5e-8 of the result
+  float s = fmaf(g, 1.f / 720.f, 1.f / 120.f);
   s = fmaf(g, s, 1.f / 24.f);
   s = fmaf(g, s, 1.f / 6.f);
   s = fmaf(g, s, 0.5f);
   s = fmaf(g, s, 1.f);
-  const float m = -fabsf(g) * s;      // (-0 for both zeros)
   float e;      // 2 ulp and the rounding of the product: beyond -1/4 a memory is shorter than five tokens
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * 1.4426950408889634f));
-  return g > -0.25f && g <= 0.f ? m : e;
+  return by_diff(g) ? g * s : e;
 }
 __device__ __forceinline__ bool is_diff(float c) { return static_cast<int>(__float_as_uint(c)) < 0; }
 // e^g h + x
-__device__ __forceinline__ float decay_step(float c, float h, float x) {
+__device__ __forceinline__ float decay_step(float c, bool diff, float h, float x) {
   const float t = fmaf(c, h, x);
-  return is_diff(c) ? h + t : t;
+  return diff ? h + t : t;
 }
-// coefficient of two steps, one after the other
-__device__ __forceinline__ float decay_both(float c, float d) {
-  if (is_diff(c) && is_diff(d)) {
-    const float m = -fabsf(fmaf(c, d, c + d));
-    return m >= -0.5f ? m : 1.f + m;
-  }
-  return (is_diff(c) ? 1.f + c : c) * (is_diff(d) ? 1.f + d : d);
-}
+__device__ __forceinline__ float decay_step(float c, float h, float x) { return decay_step(c, is_diff(c), h, x); }
 __device__ __forceinline__ float forgotten(float c) { return is_diff(c) ? -c : 1.f - c; }      // 1 - e^g
 
 struct LookBuffer {
@@ -73,72 +70,74 @@ struct DiagProblem {
   const float* dhT;
   void *dx, *dg;
   float* dh0;
-  int tiles, strips;      // tiles of kTokens tokens, strips of kChannels channels
+  int tiles, strips;      // tiles of tokens, strips of kChannels channels
+  long long records;      // states of a sequence that the forward keeps: one for every tile of the backward
   uint32_t seqs;          // B strips
   int* status;
   LookBuffer look;
 };
 
-// What a thread keeps from its first run over its tokens to its second: the compiler would keep everything that it formed there as
-// well (fp32 copies, 1 - e^g), for twice the registers.
-template <int TY>
-__device__ __forceinline__ void forget_copies(Raw<TY, kPer> (&r)[kSteps]) {
-#pragma unroll
-  for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-    for (int i = 0; i < Raw<TY, kPer>::kWords; ++i) asm volatile("" : "+r"(r[s].w[i]));
-}
-__device__ __forceinline__ void forget_copies(float (&c)[kSteps][kPer]) {
-#pragma unroll
-  for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) asm volatile("" : "+f"(c[s][j]));
-}
-
-// Four channels of one token, W neighbours at a time: as many as D, strides and alignment let be loaded at once.
+// Four channels of one token, W neighbours at a time: as many as D, strides and alignment let be moved at once.
 template <int W>
 __device__ __forceinline__ int channel_of(int lane, int j) { return (j / W * kLanes + lane) * W + j % W; }
 
-// What a thread loads next lies in shared memory in places of its own, so that it is under way while the thread works on what it has
-// in registers; nobody else reads it, so nothing but the thread's own wait stands between.  [step][piece][thread]: no bank conflicts.
-template <int TY, int W> struct Staged {
-  static constexpr int kBytes = W * elem_bytes(TY), kPieces = kPer / W, kWords = kBytes / 4;
-  static constexpr bool kAsync = kBytes >= 4;      // (2 bytes are no asynchronous copy: loaded when they are wanted)
-  alignas(16) uint32_t w[kAsync ? kSteps : 1][kPieces][kAsync ? kScanThreads : 1][kAsync ? kWords : 1];      // (a copy's two ends lie on a boundary of its size)
+// What a thread has of a tile lies in shared memory, four channels of a token in a cell of its own, [step][thread]: nobody else reads
+// or writes it, so nothing but the thread's own wait for its copies stands between them and their use.
+template <int S, int WORDS> struct Cells {
+  alignas(16) uint32_t w[S][kRunners][WORDS];      // (a copy's two ends lie on a boundary of its size)
 
-  // `base`: the tensor, an address that is good where nothing is read
-  __device__ __forceinline__ void fetch(const typename Elem<TY>::T* p, const void* base, long long stride, int lane, int live, int room) {
-    if constexpr (kAsync) {
+  template <int TY, int W>
+  __device__ __forceinline__ void fetch(const void* base, long long at, long long stride, int lane, int live, int room) {
+    using T = typename Elem<TY>::T;
+    constexpr int kBytes = W * elem_bytes(TY), kPieces = kPer / W;
+    const T* p = static_cast<const T*>(base) + at;
+    if constexpr (kBytes >= 4) {
+      const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(&w[0][threadIdx.x][0]));
+      const auto copy = [&](int s, int i, const void* from, int bytes) {      // (zeros beyond `bytes`)
+        const uint32_t d = to + s * (kRunners * WORDS * 4) + i * kBytes;
+        if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(from), "r"(bytes) : "memory");
+        else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(d), "l"(from), "n"(kBytes), "r"(bytes) : "memory");
+      };
+      if (live >= S && room == kChannels) {
+        p += channel_of<W>(lane, 0);
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s)
+        for (int s = 0; s < S; ++s, p += stride)
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-          const int ch = channel_of<W>(lane, i * W);
-          const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(&w[s][i][threadIdx.x][0]));
-          const bool there = s < live && ch < room;      // zeros otherwise
-          const void* from = there ? p + s * stride + ch : base;
-          if constexpr (kBytes == 16)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
-          else
-            asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(kBytes), "r"(there ? kBytes : 0) : "memory");
-        }
-    }
-  }
-  __device__ __forceinline__ void take(Raw<TY, kPer> (&r)[kSteps], const typename Elem<TY>::T* p, long long stride, int lane, int live, int room) const {
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      if constexpr (kAsync) {
-#pragma unroll
-        for (int i = 0; i < kPieces; ++i)
-#pragma unroll
-          for (int k = 0; k < kWords; ++k) r[s].w[i * kWords + k] = w[s][i][threadIdx.x][k];
+          for (int i = 0; i < kPieces; ++i) copy(s, i, p + channel_of<W>(0, i * W), kBytes);
       } else {
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+#pragma unroll
+          for (int i = 0; i < kPieces; ++i) {
+            const int ch = channel_of<W>(lane, i * W);
+            const bool there = s < live && ch < room;
+            copy(s, i, there ? p + s * stride + ch : base, there ? kBytes : 0);      // (an address that is good where nothing is read)
+          }
+      }
+    } else {      // 2 bytes are no asynchronous copy
+      Raw<TY, kPer> r[S];
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
         r[s].zero();
 #pragma unroll
         for (int j = 0; j < kPer; ++j)
           if (s < live && channel_of<W>(lane, j) < room) raw_put(r[s], j, __ldg(p + s * stride + channel_of<W>(lane, j)));
       }
+#pragma unroll
+      for (int s = 0; s < S; ++s) put(s, r[s]);
     }
+  }
+  template <int TY>
+  __device__ __forceinline__ Raw<TY, kPer> take(int s) const {
+    Raw<TY, kPer> r;
+#pragma unroll
+    for (int i = 0; i < Raw<TY, kPer>::kWords; ++i) r.w[i] = w[s][threadIdx.x][i];
+    return r;
+  }
+  template <int TY>
+  __device__ __forceinline__ void put(int s, const Raw<TY, kPer>& r) {
+#pragma unroll
+    for (int i = 0; i < Raw<TY, kPer>::kWords; ++i) w[s][threadIdx.x][i] = r.w[i];
   }
 };
 template <int TY, int W>
@@ -164,18 +163,18 @@ __device__ __forceinline__ Raw<TY, kPer> packed(const float (&v)[kPer]) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// What a tile hands on.  The state in front of a tile depends on all tiles before it; a tile leaves its own part, (coefficient
-// of its decay, state from zero), in the work buffer as soon as it has it, 64 bits per channel, stored and loaded as one, so a word
+// What a tile hands on.  The state in front of a tile depends on all tiles before it; a tile leaves its own part, (sum of g,
+// state from zero), in the work buffer as soon as it has it, 64 bits per channel, stored and loaded as one, so a word
 // that is there is whole and needs no flag or fence beside it.  Unwritten words are all ones (the buffer is set so in front of the kernel).
 //
-// Three levels keep what a tile has to read at 31 words: the tiles of its group of 16 in front of it, the groups of its 16 groups in
-// front of it (the last tile of a group leaves that word, from the group's words alone), and the state behind the 256 tiles before
+// Three levels keep what a tile has to read at 15 words: the tiles of its group of 8 in front of it, the groups of its 8 groups in
+// front of it (the last tile of a group leaves that word, from the group's words alone), and the state behind the 64 tiles before
 // those (left by the last of them).  The order of the fold is that of the tokens whoever comes first.
 //
 // Tiles are taken by ticket, so a tile waits only for tiles whose CTAs run already and wait for earlier ones only.  Waits are
 // bounded all the same: one that runs out leaves a code in the status word and lets everybody pass.
 // ---------------------------------------------------------------------------------------------
-constexpr int kFan = 16;
+constexpr int kFan = 8;
 constexpr long long kLookLimitCycles = 2000000000LL;      // about one second
 enum : int { kSiteLook = 900 };
 
@@ -195,8 +194,8 @@ __device__ __forceinline__ unsigned long long look_load(const unsigned long long
   asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
   return v;
 }
-__device__ __forceinline__ void look_store(unsigned long long* p, float coef, float state) {
-  unsigned long long v = (static_cast<unsigned long long>(__float_as_uint(state)) << 32) | __float_as_uint(coef);
+__device__ __forceinline__ void look_store(unsigned long long* p, float sum, float state) {
+  unsigned long long v = (static_cast<unsigned long long>(__float_as_uint(state)) << 32) | __float_as_uint(sum);
   if (v == ~0ull) v = 0x7fffffff7fffffffull;      // (another NaN)
   asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
 }
@@ -215,30 +214,30 @@ __device__ __noinline__ unsigned long long look_wait(const unsigned long long* p
   }
 }
 
-struct LookShared {
-  float2 part[2 * kFan - 1][kChannels];      // (coefficient, state): groups, then tiles, in front
-  float base[kChannels];                     // state behind the 256 tiles before
+struct Ticket {
+  int order;                     // of the tile in its sequence; from `tiles` on there is none
+  uint32_t seq, b, strip;
 };
-struct ScanShared {
-  float2 part[kGroups][kChannels];      // per group of tokens: (coefficient of its whole decay, state from zero)
-  float sum[kGroups][kChannels];        // sum of its g
-  float start[kGroups][kChannels];      // state in front of it
-  LookShared look;
-  uint32_t ticket[2];
+template <int XT, int S> struct ForwardShared {
+  struct Tile {
+    Cells<S, elem_bytes(XT)> x;
+    Cells<S, 4> c;                        // g, and over it the coefficients
+  } tile[2];
+  alignas(16) float2 part[2][kGroups][kChannels];      // per group of tokens: (sum of g, state from zero); the publisher puts the
+                                                       // coefficient in the sum's place, the lookers the state in front of the group
+  Ticket ticket[4];
 };
-struct ScanSharedBackward : ScanShared {
-  float back[kGroups][kChannels];       // per group the gradient that leaves it towards earlier tokens, from zero
-  float end[kGroups][kChannels];        // the gradient that comes into it
+template <int XT, int S> struct BackwardShared {
+  struct Tile {
+    Cells<S, elem_bytes(XT)> x, d;
+    Cells<S, 4> c;
+  } tile[2];
+  alignas(16) float2 part[2][kGroups][kChannels];      // as above
+  alignas(16) float back[2][kGroups][kChannels];       // the gradient that leaves a group towards earlier tokens, from zero; the lookers put that which comes into it
+  Ticket ticket[4];
 };
-template <int XT, int GT, int W> struct ForwardShared : ScanShared {
-  Staged<XT, W> x;
-  Staged<GT, W> g;
-};
-static_assert(alignof(Staged<LETHE_F32, 4>) == 16 && sizeof(Staged<LETHE_BF16, 4>) % 16 == 0, "asynchronous copies of 16 bytes");
-template <int XT, int GT, int W> struct BackwardShared : ScanSharedBackward {
-  Staged<XT, W> x, d;
-  Staged<GT, W> g;
-};
+static_assert(2 * sizeof(ForwardShared<LETHE_BF16, forward_steps(LETHE_BF16)>) <= 230400 && 2 * sizeof(ForwardShared<LETHE_F32, forward_steps(LETHE_F32)>) <= 230400 &&
+              2 * sizeof(BackwardShared<LETHE_BF16, backward_steps(LETHE_BF16)>) <= 230400 && 2 * sizeof(BackwardShared<LETHE_F32, backward_steps(LETHE_F32)>) <= 230400, "two CTAs on an SM");
 
 // Where tile number `i` (in the order of the fold) of sequence `seq` stands among the three levels.
 struct LookPlace {
@@ -247,6 +246,7 @@ struct LookPlace {
   long long super;              // its super's word
   int n_groups, n_tiles;        // how many in front of it
   bool first_super, last;       // no tiles in front of its super; no tile behind it
+  __device__ __forceinline__ bool closes_super() const { return n_tiles == kFan - 1 && n_groups == kFan - 1 && !last; }
   __device__ LookPlace(const LookBuffer& b, long long seq, int tiles, int i) : buf(b) {
     const int groups = (tiles + kFan - 1) / kFan, supers = (groups + kFan - 1) / kFan;
     const int sup = i / (kFan * kFan);
@@ -261,197 +261,252 @@ struct LookPlace {
   __device__ unsigned long long* at(int level, long long n, int ch) const { return buf.word[level] + n * kChannels + ch; }
 };
 
-// All threads.  Leaves what the fold reads in `l`; in between the last tile of a group leaves the group's word: `coef`, `state` of
-// threads below kChannels are the tile's own.
-__device__ __forceinline__ void look_fetch(LookShared& l, const LookPlace& p, float coef, float state, int* status) {
-  const int ch = threadIdx.x % kChannels, q = threadIdx.x / kChannels;
-  constexpr int kQ = kScanThreads / kChannels, kEach = (kFan + kQ - 1) / kQ;
-  const auto as_pair = [](unsigned long long v) { return make_float2(__uint_as_float(static_cast<uint32_t>(v)), __uint_as_float(static_cast<uint32_t>(v >> 32))); };
-  unsigned long long t[kEach], g[kEach], b = 0;
+// A looker: what comes in front of the tile in its channel; `first`: in front of the first tile.  The last tile of a group leaves the group's
+// word.  A straight line where all words are there: one that does not exist is (0, 0), which is a step that changes nothing.
+__device__ __forceinline__ float look_back(const LookPlace& p, int ch, float first, int* status) {
+  const auto upper = [](unsigned long long v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); };
+  const auto lower = [](unsigned long long v) { return __uint_as_float(static_cast<uint32_t>(v)); };
+  constexpr int N = kFan - 1;
+  const bool closes = p.n_tiles == N && !p.last;
+  unsigned long long t[N], g[N], b = 0, own = 0;
+  bool missing = false;
 #pragma unroll
-  for (int m = 0; m < kEach; ++m) {
-    const int k = q + m * kQ;
-    if (k < p.n_tiles) t[m] = look_load(p.at(0, p.tile0 + k, ch));
+  for (int k = 0; k < N; ++k) t[k] = k < p.n_tiles ? look_load(p.at(0, p.tile0 + k, ch)) : 0;
+#pragma unroll
+  for (int k = 0; k < N; ++k) g[k] = k < p.n_groups ? look_load(p.at(1, p.group0 + k, ch)) : 0;
+  if (!p.first_super) b = look_load(p.at(2, p.super - 1, ch));
+  if (closes) own = look_load(p.at(0, p.tile0 + N, ch));
+#pragma unroll
+  for (int k = 0; k < N; ++k) missing = missing || t[k] == ~0ull;
+  if (missing) {
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (t[k] == ~0ull) t[k] = look_wait(p.at(0, p.tile0 + k, ch), p.buf.head, status);
   }
+  float c[N];
 #pragma unroll
-  for (int m = 0; m < kEach; ++m) {
-    const int k = q + m * kQ;
-    if (k < p.n_groups) g[m] = look_load(p.at(1, p.group0 + k, ch));
-  }
-  if (q == 0 && !p.first_super) b = look_load(p.at(2, p.super - 1, ch));
+  for (int k = 0; k < N; ++k) c[k] = decay_coef(lower(t[k]));
+  if (closes) {
+    if (own == ~0ull) own = look_wait(p.at(0, p.tile0 + N, ch), p.buf.head, status);
+    float gs = 0.f, gh = 0.f;
 #pragma unroll
-  for (int m = 0; m < kEach; ++m) {
-    const int k = q + m * kQ;
-    if (k < p.n_tiles) {
-      if (t[m] == ~0ull) t[m] = look_wait(p.at(0, p.tile0 + k, ch), p.buf.head, status);
-      l.part[p.n_groups + k][ch] = as_pair(t[m]);
+    for (int k = 0; k < N; ++k) {
+      gs += lower(t[k]);
+      gh = decay_step(c[k], gh, upper(t[k]));
     }
+    look_store(p.at(1, p.group0 + p.n_groups, ch), gs + lower(own), decay_step(decay_coef(lower(own)), gh, upper(own)));
   }
-  if (p.n_tiles == kFan - 1 && !p.last) {      // (the same for all threads of a CTA)
-    __syncthreads();
-    if (q == 0) {
-      float gc = -0.f, gh = 0.f;
-      for (int k = 0; k < kFan - 1; ++k) {
-        const float2 a = l.part[p.n_groups + k][ch];
-        gc = decay_both(gc, a.x);
-        gh = decay_step(a.x, gh, a.y);
-      }
-      look_store(p.at(1, p.group0 + p.n_groups, ch), decay_both(gc, coef), decay_step(coef, gh, state));
-    }
-  }
+  missing = b == ~0ull;
 #pragma unroll
-  for (int m = 0; m < kEach; ++m) {
-    const int k = q + m * kQ;
-    if (k < p.n_groups) {
-      if (g[m] == ~0ull) g[m] = look_wait(p.at(1, p.group0 + k, ch), p.buf.head, status);
-      l.part[k][ch] = as_pair(g[m]);
-    }
-  }
-  if (q == 0 && !p.first_super) {
+  for (int k = 0; k < N; ++k) missing = missing || g[k] == ~0ull;
+  if (missing) {
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (g[k] == ~0ull) g[k] = look_wait(p.at(1, p.group0 + k, ch), p.buf.head, status);
     if (b == ~0ull) b = look_wait(p.at(2, p.super - 1, ch), p.buf.head, status);
-    l.base[ch] = as_pair(b).y;
   }
-  __syncthreads();
-}
-// Threads below kChannels: the state in front of the tile; `first`: that in front of the first tile.
-__device__ __forceinline__ float look_fold(const LookShared& l, const LookPlace& p, float first) {
-  float carry = p.first_super ? first : l.base[threadIdx.x];
-  for (int k = 0; k < p.n_groups + p.n_tiles; ++k) {
-    const float2 a = l.part[k][threadIdx.x];
-    carry = decay_step(a.x, carry, a.y);
-  }
+  float carry = p.first_super ? first : upper(b);
+#pragma unroll
+  for (int k = 0; k < N; ++k) carry = decay_step(decay_coef(lower(g[k])), carry, upper(g[k]));
+#pragma unroll
+  for (int k = 0; k < N; ++k) carry = decay_step(c[k], carry, upper(t[k]));
   return carry;
 }
 
-// Where a tile lies.
+// Where a thread's part of a tile lies.
 struct TilePlace {
-  long long seq, b, ch0, t0;      // sequence (a strip of one), batch, first channel, first token of this thread
-  int tile, room, live;           // channels of the strip; tokens of this thread (0 and less: none)
-  __device__ __forceinline__ TilePlace(const DiagProblem& p, uint32_t ticket, int grp, bool backwards) {
-    const uint32_t order = ticket / p.seqs;
-    seq = ticket - order * p.seqs;
-    tile = backwards ? p.tiles - 1 - static_cast<int>(order) : static_cast<int>(order);
-    const uint32_t s = static_cast<uint32_t>(seq);
-    b = s / static_cast<uint32_t>(p.strips);
-    ch0 = static_cast<long long>(s % static_cast<uint32_t>(p.strips)) * kChannels;
-    room = static_cast<int>(p.D - ch0 < kChannels ? p.D - ch0 : kChannels);
-    t0 = static_cast<long long>(tile) * kTokens + grp * kSteps;
-    live = static_cast<int>(p.L - t0 < kSteps ? p.L - t0 : kSteps);
+  long long b, ch0, t0;      // batch, first channel, first token of this thread
+  int tile, room, live;      // channels of the strip; tokens of this thread (0 and less: none)
+  template <int S>
+  __device__ __forceinline__ static TilePlace of(const DiagProblem& p, const Ticket& t, int grp, bool backwards) {
+    TilePlace r;
+    r.tile = backwards ? p.tiles - 1 - t.order : t.order;
+    r.b = t.b;
+    r.ch0 = static_cast<long long>(t.strip) * kChannels;
+    r.room = static_cast<int>(p.D - r.ch0 < kChannels ? p.D - r.ch0 : kChannels);
+    r.t0 = static_cast<long long>(r.tile) * (kGroups * S) + grp * S;
+    r.live = static_cast<int>(p.L - r.t0 < S ? p.L - r.t0 : S);
+    return r;
+  }
+};
+// One thread takes tickets, and says for all what they stand for.
+struct TicketTaker {
+  const DiagProblem& p;
+  uint32_t have;      // the last one
+  __device__ __forceinline__ void take() { have = p.tiles > 1 ? atomicAdd(p.look.head, 1u) + 1u : have + gridDim.x; }
+  __device__ __forceinline__ Ticket named() const {
+    Ticket t;
+    t.order = static_cast<int>(have / p.seqs);
+    t.seq = have - t.order * p.seqs;
+    t.b = t.seq / static_cast<uint32_t>(p.strips);
+    t.strip = t.seq - t.b * p.strips;
+    return t;
   }
 };
 
-// The CTAs take tiles until there are none; a CTA's tickets ascend, and it takes the next one while it works on a tile: the tile of the
-// lowest ticket that is not done is the one that its CTA works on, so somebody always can go on.
+// Barriers from one role to the next, two of each for even and odd tiles: a tile's parts are there (runners to publisher), its word has
+// gone out (publisher to lookers), its starts are there (lookers to runners).
+constexpr int kBarParts = 1, kBarOut = 3, kBarStarts = 5;
+template <int N> __device__ __forceinline__ void bar_sync(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory"); }
+template <int N> __device__ __forceinline__ void bar_arrive(int id) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(N) : "memory"); }
+constexpr int kPartsThreads = kRunners + 32, kOutThreads = 32 + kChannels, kStartsThreads = kChannels + kRunners;
+
+// The CTAs take tiles until there are none; a CTA's tickets ascend, and it takes tickets ahead: the tile of the lowest ticket that is not
+// done is one that its CTA has begun or begins next, so somebody always can go on.
+//
+// Runners go over a tile's tokens twice, and over those of the next tile the first time before they go over this one the second time.
+// A publisher folds a tile's parts and lets its word go out, lookers wait for the words of others.  So a tile's word waits for nobody,
+// and looking back has the time of a run.  Before, with all of it in one order, the CTAs ran in step, all computing or all waiting
+// (B1 L65536 D2048 bf16 forward 294 us, with issue slots half empty), and with folding and looking in the same warps a word
+// waited for the words that the tile before it waited for (299 us; the lookers of every second tile waited 16 k cycles).
 template <int XT, int GT, int W, bool COMP>
 __global__ void __launch_bounds__(kScanThreads, 2) diag_forward_kernel(const DiagProblem p) {
   using X = typename Elem<XT>::T;
-  using G = typename Elem<GT>::T;
+  constexpr int S = forward_steps(XT);
   extern __shared__ __align__(16) unsigned char smem[];
-  auto& sh = *reinterpret_cast<ForwardShared<XT, GT, W>*>(smem);
-  const int lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
-  const uint32_t total = p.seqs * static_cast<uint32_t>(p.tiles);
-  const auto take_ticket = [&](uint32_t have) { return p.tiles > 1 ? atomicAdd(p.look.head, 1u) + 1u : have + gridDim.x; };
-  const auto x_at = [&](const TilePlace& t) { return static_cast<const X*>(p.x) + t.b * p.x_batch + t.t0 * p.x_token + t.ch0; };
-  const auto g_at = [&](const TilePlace& t) { return static_cast<const G*>(p.g) + t.b * p.g_batch + t.t0 * p.g_token + t.ch0; };
-  const auto fetch = [&](uint32_t ticket) {
-    if (ticket < total) {
-      const TilePlace t(p, ticket, grp, false);
-      sh.x.fetch(x_at(t), p.x, p.x_token, lane, t.live, t.room);
-      sh.g.fetch(g_at(t), p.g, p.g_token, lane, t.live, t.room);
-    }
-  };
-  if (threadIdx.x == 0) {
-    const uint32_t first = p.tiles > 1 ? take_ticket(0) : blockIdx.x;
-    sh.ticket[0] = first;
-    sh.ticket[1] = take_ticket(first);
+  auto& sh = *reinterpret_cast<ForwardShared<XT, S>*>(smem);
+  TicketTaker tickets{p, blockIdx.x - gridDim.x};
+  const bool taker = threadIdx.x == kPublisher;
+  if (taker) {
+    tickets.take();
+    sh.ticket[0] = tickets.named();
+    tickets.take();
+    sh.ticket[1] = tickets.named();
   }
   __syncthreads();
-  uint32_t ticket = sh.ticket[0];
-  fetch(ticket);
-  for (int turn = 0; ticket < total; turn ^= 1) {
-    const TilePlace at(p, ticket, grp, false);
-    const int room = at.room, live = at.live;
-    Raw<XT, kPer> xr[kSteps];
-    float c[kSteps][kPer], sum[kPer], st[kPer];
-    const uint32_t next = sh.ticket[turn ^ 1];
-    uint32_t after = 0;
-    {
-      Raw<GT, kPer> gr[kSteps];
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      sh.x.take(xr, x_at(at), p.x_token, lane, live, room);
-      sh.g.take(gr, g_at(at), p.g_token, lane, live, room);
-      fetch(next);
-      if (threadIdx.x == 0) after = take_ticket(next);
+  if (threadIdx.x >= kLooker) {
+    const int ch = threadIdx.x - kLooker;
+    for (int n = 0;; ++n) {
+      const Ticket cur = sh.ticket[n & 3];
+      if (cur.order >= p.tiles) break;
+      const TilePlace at = TilePlace::of<S>(p, cur, 0, false);
+      const LookPlace look(p.look, cur.seq, p.tiles, cur.order);
+      auto& part = sh.part[n & 1];
+      const long long state_at = at.b * p.D + at.ch0 + ch;
+      float carry = ch < at.room && p.h0 ? p.h0[state_at] : 0.f;
+      bar_sync<kOutThreads>(kBarOut + (n & 1));
+      if (p.tiles > 1) carry = look_back(look, ch, carry, p.status);
+      const float entry = carry;
+      float middle = 0.f;
+      float2 own[kGroups];
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) sum[j] = st[j] = 0.f;
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-          const float gv = gr[s].get(j);
-          c[s][j] = decay_coef(gv);
-          sum[j] += gv;
-          const float u = COMP ? xr[s].get(j) * forgotten(c[s][j]) : xr[s].get(j);
-          st[j] = decay_step(c[s][j], st[j], u);
-        }
-    }
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int ch = channel_of<W>(lane, j);
-      sh.part[grp][ch] = make_float2(decay_coef(sum[j]), st[j]);
-      sh.sum[grp][ch] = sum[j];
-    }
-    forget_copies(xr);
-    forget_copies(c);
-    __syncthreads();
-    if (threadIdx.x == 0) sh.ticket[turn] = after;      // (read behind the next barriers)
-    const int ch = threadIdx.x;      // of threads below kChannels
-    float carry = 0.f;
-    if (ch < room && p.h0) carry = p.h0[at.b * p.D + at.ch0 + ch];
-    if (p.tiles > 1) {
-      const LookPlace look(p.look, at.seq, p.tiles, at.tile);
-      float tc = -0.f, th = 0.f;
-      if (ch < kChannels) {
-        float ts = 0.f;
-#pragma unroll
-        for (int i = 0; i < kGroups; ++i) {
-          const float2 a = sh.part[i][ch];
-          ts += sh.sum[i][ch];
-          th = decay_step(a.x, th, a.y);
-        }
-        tc = decay_coef(ts);
-        if (!look.last) look_store(look.at(0, look.tile0 + look.n_tiles, ch), tc, th);
-      }
-      look_fetch(sh.look, look, tc, th, p.status);
-      if (ch < kChannels) {
-        carry = look_fold(sh.look, look, carry);
-        if (look.n_tiles == kFan - 1 && look.n_groups == kFan - 1 && !look.last) look_store(look.at(2, look.super, ch), 0.f, decay_step(tc, carry, th));
-      }
-    }
-    if (ch < kChannels) {
-      if (p.states && ch < room) p.states[(at.b * p.tiles + at.tile) * p.D + at.ch0 + ch] = carry;
+      for (int i = 0; i < kGroups; ++i) own[i] = part[i][ch];
 #pragma unroll
       for (int i = 0; i < kGroups; ++i) {
-        sh.start[i][ch] = carry;
-        const float2 a = sh.part[i][ch];
-        carry = decay_step(a.x, carry, a.y);
+        if (i == kGroups / 2) middle = carry;
+        part[i][ch].x = carry;
+        carry = decay_step(own[i].x, carry, own[i].y);
       }
-      if (p.hT && ch < room && at.tile == p.tiles - 1) p.hT[at.b * p.D + at.ch0 + ch] = carry;
+      bar_arrive<kStartsThreads>(kBarStarts + (n & 1));
+      if (p.tiles > 1 && look.closes_super()) look_store(look.at(2, look.super, ch), 0.f, carry);
+      if (p.states && ch < at.room) {
+        float* to = p.states + (at.b * p.records + 2 * at.tile) * p.D + at.ch0 + ch;
+        to[0] = entry;
+        if (2 * at.tile + 1 < p.records) to[p.D] = middle;
+      }
+      if (p.hT && ch < at.room && at.tile == p.tiles - 1) p.hT[state_at] = carry;
     }
-    __syncthreads();
+    return;
+  }
+  if (threadIdx.x >= kPublisher) {
+    const int ch = 2 * (threadIdx.x - kPublisher);      // two channels a thread
+    for (int n = 0;; ++n) {
+      const Ticket cur = sh.ticket[n & 3];
+      if (cur.order >= p.tiles) break;
+      const LookPlace look(p.look, cur.seq, p.tiles, cur.order);
+      auto& part = sh.part[n & 1];
+      bar_sync<kPartsThreads>(kBarParts + (n & 1));
+      if (taker) tickets.take();
+      float ts[2] = {0.f, 0.f}, th[2] = {0.f, 0.f};
+      float4 v[kGroups];
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) st[j] = sh.start[grp][channel_of<W>(lane, j)];
-    X* h = static_cast<X*>(p.h) + (at.b * p.L + at.t0) * p.D + at.ch0;
+      for (int i = 0; i < kGroups; ++i) v[i] = *reinterpret_cast<const float4*>(&part[i][ch]);
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
+      for (int i = 0; i < kGroups; ++i) {
+        ts[0] += v[i].x;
+        ts[1] += v[i].z;
+        v[i].x = decay_coef(v[i].x);
+        v[i].z = decay_coef(v[i].z);
+        th[0] = decay_step(v[i].x, th[0], v[i].y);
+        th[1] = decay_step(v[i].z, th[1], v[i].w);
+        *reinterpret_cast<float4*>(&part[i][ch]) = v[i];
+      }
+      if (p.tiles > 1 && !look.last) {
+        look_store(look.at(0, look.tile0 + look.n_tiles, ch), ts[0], th[0]);
+        look_store(look.at(0, look.tile0 + look.n_tiles, ch + 1), ts[1], th[1]);
+      }
+      if (taker) sh.ticket[(n + 2) & 3] = tickets.named();
+      __syncwarp();
+      bar_arrive<kOutThreads>(kBarOut + (n & 1));
+    }
+    return;
+  }
+  const int lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
+  const auto fetch = [&](const Ticket& t, int slot) {
+    if (t.order < p.tiles) {
+      const TilePlace at = TilePlace::of<S>(p, t, grp, false);
+      sh.tile[slot].x.template fetch<XT, W>(p.x, at.b * p.x_batch + at.t0 * p.x_token + at.ch0, p.x_token, lane, at.live, at.room);
+      sh.tile[slot].c.template fetch<GT, W>(p.g, at.b * p.g_batch + at.t0 * p.g_token + at.ch0, p.g_token, lane, at.live, at.room);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  const auto first_run = [&](int slot) {
+    auto& tile = sh.tile[slot];
+    float sum[kPer], st[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) sum[j] = st[j] = 0.f;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const auto gr = tile.c.template take<GT>(s);
+      const auto xr = tile.x.template take<XT>(s);
+      Raw<LETHE_F32, kPer> cr;
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
-        const float u = COMP ? xr[s].get(j) * forgotten(c[s][j]) : xr[s].get(j);
-        st[j] = decay_step(c[s][j], st[j], u);
+        const float gv = gr.get(j), c = decay_coef(gv);
+        cr.w[j] = __float_as_uint(c);
+        sum[j] += gv;
+        st[j] = decay_step(c, by_diff(gv), st[j], COMP ? xr.get(j) * forgotten(c) : xr.get(j));
       }
-      if (s < live) store_token<XT, W>(packed<XT>(st), h + s * p.D, lane, room);
+      tile.c.put(s, cr);
     }
-    ticket = next;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) sh.part[slot][grp][channel_of<W>(lane, j)] = make_float2(sum[j], st[j]);
+    bar_arrive<kPartsThreads>(kBarParts + slot);
+  };
+  fetch(sh.ticket[0], 0);
+  fetch(sh.ticket[1], 1);
+  if (sh.ticket[0].order < p.tiles) {
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    first_run(0);
+  }
+  for (int n = 0;; ++n) {
+    const Ticket cur = sh.ticket[n & 3];
+    if (cur.order >= p.tiles) break;
+    const int slot = n & 1;
+    if (sh.ticket[(n + 1) & 3].order < p.tiles) {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      first_run(slot ^ 1);
+    }
+    const TilePlace at = TilePlace::of<S>(p, cur, grp, false);
+    auto& tile = sh.tile[slot];
+    X* h = static_cast<X*>(p.h) + (at.b * p.L + at.t0) * p.D + at.ch0;
+    float st[kPer];
+    bar_sync<kStartsThreads>(kBarStarts + slot);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) st[j] = sh.part[slot][grp][channel_of<W>(lane, j)].x;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const auto xr = tile.x.template take<XT>(s);
+      const auto cr = tile.c.template take<LETHE_F32>(s);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const float c = cr.get(j);
+        st[j] = decay_step(c, st[j], COMP ? xr.get(j) * forgotten(c) : xr.get(j));
+      }
+      if (s < at.live) store_token<XT, W>(packed<XT>(st), h, lane, at.room);
+      h += p.D;
+    }
+    fetch(sh.ticket[(n + 2) & 3], slot);
   }
 }
 
@@ -459,152 +514,193 @@ template <int XT, int GT, int W, bool COMP>
 __global__ void __launch_bounds__(kScanThreads, 2) diag_backward_kernel(const DiagProblem p) {
   using X = typename Elem<XT>::T;
   using G = typename Elem<GT>::T;
+  constexpr int S = backward_steps(XT);
   extern __shared__ __align__(16) unsigned char smem[];
-  auto& sh = *reinterpret_cast<BackwardShared<XT, GT, W>*>(smem);
-  const int lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
-  const uint32_t total = p.seqs * static_cast<uint32_t>(p.tiles);
-  const auto take_ticket = [&](uint32_t have) { return p.tiles > 1 ? atomicAdd(p.look.head, 1u) + 1u : have + gridDim.x; };
-  const auto x_at = [&](const TilePlace& t) { return static_cast<const X*>(p.x) + t.b * p.x_batch + t.t0 * p.x_token + t.ch0; };
-  const auto g_at = [&](const TilePlace& t) { return static_cast<const G*>(p.g) + t.b * p.g_batch + t.t0 * p.g_token + t.ch0; };
-  const auto d_at = [&](const TilePlace& t) { return static_cast<const X*>(p.d_h) + t.b * p.d_batch + t.t0 * p.d_token + t.ch0; };
-  const auto fetch = [&](uint32_t ticket) {
-    if (ticket < total) {
-      const TilePlace t(p, ticket, grp, true);
-      sh.x.fetch(x_at(t), p.x, p.x_token, lane, t.live, t.room);
-      sh.g.fetch(g_at(t), p.g, p.g_token, lane, t.live, t.room);
-      if (p.d_h) sh.d.fetch(d_at(t), p.d_h, p.d_token, lane, t.live, t.room);
-    }
-  };
-  if (threadIdx.x == 0) {
-    const uint32_t first = p.tiles > 1 ? take_ticket(0) : blockIdx.x;
-    sh.ticket[0] = first;
-    sh.ticket[1] = take_ticket(first);
+  auto& sh = *reinterpret_cast<BackwardShared<XT, S>*>(smem);
+  TicketTaker tickets{p, blockIdx.x - gridDim.x};
+  const bool taker = threadIdx.x == kPublisher;
+  if (taker) {
+    tickets.take();
+    sh.ticket[0] = tickets.named();
+    tickets.take();
+    sh.ticket[1] = tickets.named();
   }
   __syncthreads();
-  uint32_t ticket = sh.ticket[0];
-  fetch(ticket);
-  for (int turn = 0; ticket < total; turn ^= 1) {
-    const TilePlace at(p, ticket, grp, true);
-    const int room = at.room, live = at.live;
-    Raw<XT, kPer> xr[kSteps], dr[kSteps];
-    float c[kSteps][kPer], st[kPer], e[kPer];
-    const uint32_t next = sh.ticket[turn ^ 1];
-    uint32_t after = 0;
-    {
-      Raw<GT, kPer> gr[kSteps];
-      float sum[kPer];
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      sh.x.take(xr, x_at(at), p.x_token, lane, live, room);
-      sh.g.take(gr, g_at(at), p.g_token, lane, live, room);
-      if (p.d_h) {
-        sh.d.take(dr, d_at(at), p.d_token, lane, live, room);
-      } else {
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) dr[s].zero();
-      }
-      fetch(next);
-      if (threadIdx.x == 0) after = take_ticket(next);
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) sum[j] = st[j] = e[j] = 0.f;
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-          const float gv = gr[s].get(j);
-          c[s][j] = decay_coef(gv);
-          sum[j] += gv;
-          const float u = COMP ? xr[s].get(j) * forgotten(c[s][j]) : xr[s].get(j);
-          st[j] = decay_step(c[s][j], st[j], u);
-        }
-#pragma unroll
-      for (int s = kSteps - 1; s >= 0; --s)
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) e[j] = decay_step(c[s][j], dr[s].get(j) + e[j], 0.f);
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const int ch = channel_of<W>(lane, j);
-        sh.part[grp][ch] = make_float2(decay_coef(sum[j]), st[j]);
-        sh.sum[grp][ch] = sum[j];
-        sh.back[grp][ch] = e[j];
-      }
-    }
-    forget_copies(xr);
-    forget_copies(dr);
-    forget_copies(c);
-    __syncthreads();
-    if (threadIdx.x == 0) sh.ticket[turn] = after;
-    const int ch = threadIdx.x, ch2 = threadIdx.x - kChannels;      // the gradient is folded by threads below kChannels, the state by the next ones
-    float carry = 0.f;
-    if (ch < room && p.dhT) carry = p.dhT[at.b * p.D + at.ch0 + ch];
-    if (ch2 >= 0 && ch2 < kChannels) {
-      float s0 = ch2 < room ? p.states[(at.b * p.tiles + at.tile) * p.D + at.ch0 + ch2] : 0.f;
+  if (threadIdx.x >= kLooker) {
+    const int ch = threadIdx.x - kLooker;
+    for (int n = 0;; ++n) {
+      const Ticket cur = sh.ticket[n & 3];
+      if (cur.order >= p.tiles) break;
+      const TilePlace at = TilePlace::of<S>(p, cur, 0, true);
+      const LookPlace look(p.look, cur.seq, p.tiles, cur.order);
+      auto& part = sh.part[n & 1];
+      auto& back = sh.back[n & 1];
+      const long long state_at = at.b * p.D + at.ch0 + ch;
+      float carry = ch < at.room && p.dhT ? p.dhT[state_at] : 0.f;
+      float st = ch < at.room ? p.states[(at.b * p.records + at.tile) * p.D + at.ch0 + ch] : 0.f;
+      bar_sync<kOutThreads>(kBarOut + (n & 1));
+      if (p.tiles > 1) carry = look_back(look, ch, carry, p.status);
+      float2 own[kGroups];
+      float e[kGroups];
 #pragma unroll
       for (int i = 0; i < kGroups; ++i) {
-        sh.start[i][ch2] = s0;
-        const float2 a = sh.part[i][ch2];
-        s0 = decay_step(a.x, s0, a.y);
+        own[i] = part[i][ch];
+        e[i] = back[i][ch];
       }
-    }
-    if (p.tiles > 1) {
-      const LookPlace look(p.look, at.seq, p.tiles, p.tiles - 1 - at.tile);
-      float tc = -0.f, te = 0.f;
-      if (ch < kChannels) {
-        float ts = 0.f;
 #pragma unroll
-        for (int i = kGroups - 1; i >= 0; --i) {
-          ts += sh.sum[i][ch];
-          te = decay_step(sh.part[i][ch].x, te, sh.back[i][ch]);
-        }
-        tc = decay_coef(ts);
-        if (!look.last) look_store(look.at(0, look.tile0 + look.n_tiles, ch), tc, te);
+      for (int i = 0; i < kGroups; ++i) {      // (two chains, one from each end)
+        const int k = kGroups - 1 - i;
+        back[k][ch] = carry;
+        carry = decay_step(own[k].x, carry, e[k]);
+        part[i][ch].x = st;
+        st = decay_step(own[i].x, st, own[i].y);
       }
-      look_fetch(sh.look, look, tc, te, p.status);
-      if (ch < kChannels) {
-        carry = look_fold(sh.look, look, carry);
-        if (look.n_tiles == kFan - 1 && look.n_groups == kFan - 1 && !look.last) look_store(look.at(2, look.super, ch), 0.f, decay_step(tc, carry, te));
-      }
+      bar_arrive<kStartsThreads>(kBarStarts + (n & 1));
+      if (p.tiles > 1 && look.closes_super()) look_store(look.at(2, look.super, ch), 0.f, carry);
+      if (p.dh0 && ch < at.room && at.tile == 0) p.dh0[state_at] = carry;
     }
-    if (ch < kChannels) {
+    return;
+  }
+  if (threadIdx.x >= kPublisher) {
+    const int ch = 2 * (threadIdx.x - kPublisher);
+    for (int n = 0;; ++n) {
+      const Ticket cur = sh.ticket[n & 3];
+      if (cur.order >= p.tiles) break;
+      const LookPlace look(p.look, cur.seq, p.tiles, cur.order);
+      auto& part = sh.part[n & 1];
+      bar_sync<kPartsThreads>(kBarParts + (n & 1));
+      if (taker) tickets.take();
+      float ts[2] = {0.f, 0.f}, te[2] = {0.f, 0.f};
 #pragma unroll
       for (int i = kGroups - 1; i >= 0; --i) {
-        sh.end[i][ch] = carry;
-        carry = decay_step(sh.part[i][ch].x, carry, sh.back[i][ch]);
+        const float s0 = part[i][ch].x, s1 = part[i][ch + 1].x;
+        const float2 e = *reinterpret_cast<const float2*>(&sh.back[n & 1][i][ch]);
+        const float c0 = decay_coef(s0), c1 = decay_coef(s1);
+        ts[0] += s0;
+        ts[1] += s1;
+        te[0] = decay_step(c0, te[0], e.x);
+        te[1] = decay_step(c1, te[1], e.y);
+        part[i][ch].x = c0;
+        part[i][ch + 1].x = c1;
       }
-      if (p.dh0 && ch < room && at.tile == 0) p.dh0[at.b * p.D + at.ch0 + ch] = carry;
+      if (p.tiles > 1 && !look.last) {
+        look_store(look.at(0, look.tile0 + look.n_tiles, ch), ts[0], te[0]);
+        look_store(look.at(0, look.tile0 + look.n_tiles, ch + 1), ts[1], te[1]);
+      }
+      if (taker) sh.ticket[(n + 2) & 3] = tickets.named();
+      __syncwarp();
+      bar_arrive<kOutThreads>(kBarOut + (n & 1));
     }
-    __syncthreads();
-    float before[kSteps][kPer];
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      st[j] = sh.start[grp][channel_of<W>(lane, j)];
-      e[j] = sh.end[grp][channel_of<W>(lane, j)];
+    return;
+  }
+  const int lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
+  const auto fetch = [&](const Ticket& t, int slot) {
+    if (t.order < p.tiles) {
+      const TilePlace at = TilePlace::of<S>(p, t, grp, true);
+      sh.tile[slot].x.template fetch<XT, W>(p.x, at.b * p.x_batch + at.t0 * p.x_token + at.ch0, p.x_token, lane, at.live, at.room);
+      sh.tile[slot].c.template fetch<GT, W>(p.g, at.b * p.g_batch + at.t0 * p.g_token + at.ch0, p.g_token, lane, at.live, at.room);
+      if (p.d_h) sh.tile[slot].d.template fetch<XT, W>(p.d_h, at.b * p.d_batch + at.t0 * p.d_token + at.ch0, p.d_token, lane, at.live, at.room);
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  const auto first_run = [&](int slot) {
+    auto& tile = sh.tile[slot];
+    float c[S][kPer], sum[kPer], st[kPer], e[kPer];
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s)
+    for (int j = 0; j < kPer; ++j) sum[j] = st[j] = e[j] = 0.f;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const auto gr = tile.c.template take<GT>(s);
+      const auto xr = tile.x.template take<XT>(s);
+      Raw<LETHE_F32, kPer> cr;
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
-        const float xv = xr[s].get(j);
+        const float gv = gr.get(j);
+        c[s][j] = decay_coef(gv);
+        cr.w[j] = __float_as_uint(c[s][j]);
+        sum[j] += gv;
+        st[j] = decay_step(c[s][j], by_diff(gv), st[j], COMP ? xr.get(j) * forgotten(c[s][j]) : xr.get(j));
+      }
+      tile.c.put(s, cr);
+    }
+#pragma unroll
+    for (int s = S - 1; s >= 0; --s) {
+      const auto dr = tile.d.template take<XT>(s);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) e[j] = decay_step(c[s][j], dr.get(j) + e[j], 0.f);
+    }
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int ch = channel_of<W>(lane, j);
+      sh.part[slot][grp][ch] = make_float2(sum[j], st[j]);
+      sh.back[slot][grp][ch] = e[j];
+    }
+    bar_arrive<kPartsThreads>(kBarParts + slot);
+  };
+  if (!p.d_h) {      // no gradient of h: zeros, for good
+    Raw<XT, kPer> none;
+    none.zero();
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      sh.tile[0].d.put(s, none);
+      sh.tile[1].d.put(s, none);
+    }
+  }
+  fetch(sh.ticket[0], 0);
+  fetch(sh.ticket[1], 1);
+  if (sh.ticket[0].order < p.tiles) {
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    first_run(0);
+  }
+  for (int n = 0;; ++n) {
+    const Ticket cur = sh.ticket[n & 3];
+    if (cur.order >= p.tiles) break;
+    const int slot = n & 1;
+    if (sh.ticket[(n + 1) & 3].order < p.tiles) {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      first_run(slot ^ 1);
+    }
+    const TilePlace at = TilePlace::of<S>(p, cur, grp, true);
+    auto& tile = sh.tile[slot];
+    float before[S][kPer], c[S][kPer], st[kPer], e[kPer];
+    bar_sync<kStartsThreads>(kBarStarts + slot);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int ch = channel_of<W>(lane, j);
+      st[j] = sh.part[slot][grp][ch].x;
+      e[j] = sh.back[slot][grp][ch];
+    }
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const auto xr = tile.x.template take<XT>(s);
+      const auto cr = tile.c.template take<LETHE_F32>(s);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const float xv = xr.get(j);
+        c[s][j] = cr.get(j);
         before[s][j] = COMP ? st[j] - xv : st[j];
         st[j] = decay_step(c[s][j], st[j], COMP ? xv * forgotten(c[s][j]) : xv);
       }
+    }
     X* dx = static_cast<X*>(p.dx) + (at.b * p.L + at.t0) * p.D + at.ch0;
     G* dg = static_cast<G*>(p.dg) + (at.b * p.L + at.t0) * p.D + at.ch0;
 #pragma unroll
-    for (int s = kSteps - 1; s >= 0; --s) {
+    for (int s = S - 1; s >= 0; --s) {
+      const auto dr = tile.d.template take<XT>(s);
       float vx[kPer], vg[kPer];
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
-        const float dv = dr[s].get(j) + e[j];
+        const float dv = dr.get(j) + e[j];
         vx[j] = COMP ? dv * forgotten(c[s][j]) : dv;
         e[j] = decay_step(c[s][j], dv, 0.f);
         vg[j] = e[j] * before[s][j];
       }
-      if (s < live) {
-        if (p.dx) store_token<XT, W>(packed<XT>(vx), dx + s * p.D, lane, room);
-        if (p.dg) store_token<GT, W>(packed<GT>(vg), dg + s * p.D, lane, room);
+      if (s < at.live) {
+        if (p.dx) store_token<XT, W>(packed<XT>(vx), dx + s * p.D, lane, at.room);
+        if (p.dg) store_token<GT, W>(packed<GT>(vg), dg + s * p.D, lane, at.room);
       }
     }
-    ticket = next;
+    fetch(sh.ticket[(n + 2) & 3], slot);
   }
 }
 
@@ -679,14 +775,19 @@ static int by_type(int xt, int gt, int w, bool comp, F&& f) {
 
 static int launched() { return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch; }
 
+static long long tiles_of(long long L, int xt, bool backward) {
+  const int n = kGroups * (backward ? backward_steps(xt) : forward_steps(xt));
+  return (L + n - 1) / n;
+}
 static int diag_problem(const LetheGdnDiagArgs* a, DiagProblem* p, bool backward) {
   if (!a) return kErrNull;
   if (a->B <= 0 || a->L <= 0 || a->D <= 0 || !types_ok(a->x_type, a->g_type)) return kErrDims;
   if (!a->x || !a->g || !a->status || (!backward && !a->h) || (backward && !a->states)) return kErrNull;
-  const long long tiles = (a->L + kTokens - 1) / kTokens, strips = (a->D + kChannels - 1) / kChannels;
+  const long long tiles = tiles_of(a->L, a->x_type, backward), strips = (a->D + kChannels - 1) / kChannels;
   if (strips > INT32_MAX || a->B > INT32_MAX / strips || tiles > INT32_MAX / (a->B * strips)) return kErrDims;
   *p = {a->B, a->L, a->D, a->x, a->x_batch, a->x_token, a->g, a->g_batch, a->g_token, a->h0, a->h, a->hT, a->states, a->d_h, a->d_h_batch,
-        a->d_h_token, a->dhT, a->dx, a->dg, a->dh0, static_cast<int>(tiles), static_cast<int>(strips), static_cast<uint32_t>(a->B * strips), a->status, {}};
+        a->d_h_token, a->dhT, a->dx, a->dg, a->dh0, static_cast<int>(tiles), static_cast<int>(strips), tiles_of(a->L, a->x_type, true),
+        static_cast<uint32_t>(a->B * strips), a->status, {}};
   if (tiles > 1) {
     if (!a->work) return kErrNull;
     if (reinterpret_cast<uintptr_t>(a->work) & 15) return kErrAlign;
@@ -707,22 +808,23 @@ static int launch_scan_tiles(void (*kern)(DiagProblem), const DiagProblem& p, Sm
   if (int e = attr.set(kern, sizeof(Shared))) return e;
   // all ones: no word is there yet, and the ticket before the first
   if (p.tiles > 1 && cudaMemsetAsync(p.look.head, 0xff, look_sizes(p.seqs, p.tiles).bytes(), st) != cudaSuccess) return kErrLaunch;
-  const uint32_t total = p.seqs * static_cast<uint32_t>(p.tiles), room = 2u * static_cast<uint32_t>(sm_count());
+  const uint32_t total = p.seqs * static_cast<uint32_t>(p.tiles), room = static_cast<uint32_t>(2 * sm_count());
   kern<<<total < room ? total : room, kScanThreads, sizeof(Shared), st>>>(p);
   return launched();
 }
 
 }  // namespace lg
 
-extern "C" size_t lethe_gdn_diag_states_bytes(int64_t B, int64_t L, int64_t D) {
+extern "C" size_t lethe_gdn_diag_states_bytes(int64_t B, int64_t L, int64_t D, int32_t x_type) {
   using namespace lg;
-  if (B <= 0 || L <= 0 || D <= 0) return 0;
-  return static_cast<size_t>(B) * ((L + kTokens - 1) / kTokens) * D * sizeof(float);
+  if (B <= 0 || L <= 0 || D <= 0 || !types_ok(x_type, LETHE_F32)) return 0;
+  return static_cast<size_t>(B) * tiles_of(L, x_type, true) * D * sizeof(float);
 }
-extern "C" size_t lethe_gdn_diag_work_bytes(int64_t B, int64_t L, int64_t D) {
+extern "C" size_t lethe_gdn_diag_work_bytes(int64_t B, int64_t L, int64_t D, int32_t x_type, int32_t backward) {
   using namespace lg;
-  if (B <= 0 || L <= kTokens || D <= 0) return 0;
-  return look_sizes(B * ((D + kChannels - 1) / kChannels), (L + kTokens - 1) / kTokens).bytes();
+  if (B <= 0 || L <= 0 || D <= 0 || !types_ok(x_type, LETHE_F32)) return 0;
+  const long long tiles = tiles_of(L, x_type, backward != 0);
+  return tiles > 1 ? look_sizes(B * ((D + kChannels - 1) / kChannels), tiles).bytes() : 0;
 }
 
 extern "C" int lethe_gdn_diag_forward(const LetheGdnDiagArgs* a, void* stream) {
@@ -737,7 +839,7 @@ extern "C" int lethe_gdn_diag_forward(const LetheGdnDiagArgs* a, void* stream) {
   });
   return by_type(a->x_type, a->g_type, w, a->complement != 0, [&](auto x, auto g, auto n, auto c) {
     static SmemAttr attr;
-    return launch_scan_tiles<ForwardShared<x.value, g.value, n.value>>(diag_forward_kernel<x.value, g.value, n.value, c.value>, p, attr, static_cast<cudaStream_t>(stream));
+    return launch_scan_tiles<ForwardShared<x.value, forward_steps(x.value)>>(diag_forward_kernel<x.value, g.value, n.value, c.value>, p, attr, static_cast<cudaStream_t>(stream));
   });
 }
 
@@ -753,7 +855,7 @@ extern "C" int lethe_gdn_diag_backward(const LetheGdnDiagArgs* a, void* stream) 
   });
   return by_type(a->x_type, a->g_type, w, a->complement != 0, [&](auto x, auto g, auto n, auto c) {
     static SmemAttr attr;
-    return launch_scan_tiles<BackwardShared<x.value, g.value, n.value>>(diag_backward_kernel<x.value, g.value, n.value, c.value>, p, attr, static_cast<cudaStream_t>(stream));
+    return launch_scan_tiles<BackwardShared<x.value, backward_steps(x.value)>>(diag_backward_kernel<x.value, g.value, n.value, c.value>, p, attr, static_cast<cudaStream_t>(stream));
   });
 }
 

@@ -103,8 +103,8 @@ LetheGdnDiagArgs diag_args(const Tensor& x, const Tensor& g, bool complement) {
   a.status = status_word(x.device().index());
   return a;
 }
-Tensor diag_work(LetheGdnDiagArgs* a, const Tensor& like) {
-  a->work_bytes = lethe_gdn_diag_work_bytes(a->B, a->L, a->D);
+Tensor diag_work(LetheGdnDiagArgs* a, const Tensor& like, bool backward) {
+  a->work_bytes = lethe_gdn_diag_work_bytes(a->B, a->L, a->D, a->x_type, backward);
   Tensor w;
   if (a->work_bytes) {
     w = at::empty({static_cast<int64_t>(a->work_bytes)}, like.options().dtype(at::kByte));
@@ -144,7 +144,7 @@ struct DiagScanBackward : public FirstOrderNode {      // kept: x, g, states
       if (task_should_compute_output(0)) dx = at::empty(x.sizes(), x.options());
       if (task_should_compute_output(1)) dg = at::empty(g.sizes(), g.options());
       a.dx = ptr(dx); a.dg = ptr(dg); a.dh0 = ptr<float>(dh0);
-      const Tensor work = diag_work(&a, x);
+      const Tensor work = diag_work(&a, x, true);
       check(lethe_gdn_diag_backward(&a, stream_of(x)));
     }
     return {dx, dg.defined() ? cast_back(dg, g_type) : dg, dh0.defined() ? cast_back(dh0, h0_type) : dh0};
@@ -184,10 +184,10 @@ std::pair<Tensor, Tensor> diag_scan(const Tensor& x, const Tensor& g_in, const O
         a.h = ptr(h);
         a.hT = ptr<float>(hT);
         if (need) {
-          states = at::empty({static_cast<int64_t>(lethe_gdn_diag_states_bytes(a.B, a.L, a.D) / 4)}, o32);
+          states = at::empty({static_cast<int64_t>(lethe_gdn_diag_states_bytes(a.B, a.L, a.D, a.x_type) / 4)}, o32);
           a.states = ptr<float>(states);
         }
-        const Tensor work = diag_work(&a, x);
+        const Tensor work = diag_work(&a, x, false);
         check(lethe_gdn_diag_forward(&a, stream_of(x)));
       }
     }

@@ -30,9 +30,8 @@ class Residual(ctypes.Structure):
 def lib():
     _build.build()
     L = native.lib()
-    for n in ("diag_states_bytes", "diag_work_bytes"):
-        f = getattr(L, "lethe_gdn_" + n)
-        f.restype, f.argtypes = Z, [I64] * 3
+    L.lethe_gdn_diag_states_bytes.restype, L.lethe_gdn_diag_states_bytes.argtypes = Z, [I64, I64, I64, I32]
+    L.lethe_gdn_diag_work_bytes.restype, L.lethe_gdn_diag_work_bytes.argtypes = Z, [I64, I64, I64, I32, I32]
     L.lethe_gdn_norm_work_bytes.restype, L.lethe_gdn_norm_work_bytes.argtypes = Z, [I64, I32, I32]
     return L
 
@@ -68,10 +67,13 @@ def test_diag_step(lib):
 
 
 def test_sizes(lib):
-    assert lib.lethe_gdn_diag_states_bytes(2, 300, 10) == 2 * 3 * 10 * 4
+    assert lib.lethe_gdn_diag_states_bytes(2, 300, 10, 1) == 2 * 5 * 10 * 4          # one for every 64 tokens
+    assert lib.lethe_gdn_diag_states_bytes(2, 300, 10, 0) == 2 * 7 * 10 * 4          # fp32: 48
     for bad in ((0, 1, 1), (1, 0, 1), (1, 1, 0), (-1, 1, 1)):
-        assert lib.lethe_gdn_diag_states_bytes(*bad) == 0 and lib.lethe_gdn_diag_work_bytes(*bad) == 0
-    assert lib.lethe_gdn_diag_work_bytes(1, 1, 64) == 0                  # one tile: nothing to hand on
+        assert lib.lethe_gdn_diag_states_bytes(*bad, 1) == 0 and lib.lethe_gdn_diag_work_bytes(*bad, 1, 0) == 0
+    for back, tile in ((0, 128), (1, 64)):                                            # one tile: nothing to hand on
+        assert lib.lethe_gdn_diag_work_bytes(1, tile, 64, 1, back) == 0
+        assert lib.lethe_gdn_diag_work_bytes(1, tile + 1, 64, 1, back) == 128 + (2 + 1 + 1) * 64 * 8
     assert lib.lethe_gdn_norm_work_bytes(3, 100, 2) == 3 * 100 * 2 * 4
     assert lib.lethe_gdn_norm_work_bytes(1 << 40, 8192, 3) < 1 << 27     # bounded by the CTAs, not by the rows
     for bad in ((0, 8, 1), (4, 0, 1), (4, 8193, 1), (4, 8, 0), (4, 8, 4)):
