@@ -21,7 +21,7 @@ namespace lg {
 
 constexpr int kLanes = 16, kPer = 4, kChannels = kLanes * kPer;      // a strip of channels
 constexpr int kGroups = 16, kRunners = kLanes * kGroups;              // threads that hold a tile
-constexpr int kPublisher = kRunners, kLooker = kPublisher + 32;         // first threads of the warp that hands on and of those that look back
+constexpr int kPublisher = kRunners, kLooker = kPublisher + kChannels;  // first threads of those that hand on and of those that look back
 constexpr int kScanThreads = kLooker + kChannels;
 // Tokens of a thread: what two tiles of two CTAs take in shared memory decides.  The forward leaves a state for every tile of the backward.
 constexpr int forward_steps(int xt) { return xt == LETHE_F32 ? 6 : 8; }
@@ -86,45 +86,35 @@ __device__ __forceinline__ int channel_of(int lane, int j) { return (j / W * kLa
 template <int S, int WORDS> struct Cells {
   alignas(16) uint32_t w[S][kRunners][WORDS];      // (a copy's two ends lie on a boundary of its size)
 
+  // Step s of this thread from p, its strip of that token; `there`: the token exists, `whole`: so do all channels of the strip.  `base`: the
+  // tensor, an address that is good where nothing is read.  Two bytes are no asynchronous copy: those elements are loaded and put here.
   template <int TY, int W>
-  __device__ __forceinline__ void fetch(const void* base, long long at, long long stride, int lane, int live, int room) {
-    using T = typename Elem<TY>::T;
+  __device__ __forceinline__ void fetch(int s, const typename Elem<TY>::T* p, const void* base, int lane, bool there, bool whole, int room) {
     constexpr int kBytes = W * elem_bytes(TY), kPieces = kPer / W;
-    const T* p = static_cast<const T*>(base) + at;
     if constexpr (kBytes >= 4) {
-      const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(&w[0][threadIdx.x][0]));
-      const auto copy = [&](int s, int i, const void* from, int bytes) {      // (zeros beyond `bytes`)
-        const uint32_t d = to + s * (kRunners * WORDS * 4) + i * kBytes;
-        if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(from), "r"(bytes) : "memory");
-        else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(d), "l"(from), "n"(kBytes), "r"(bytes) : "memory");
+      const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(&w[s][threadIdx.x][0]));
+      const auto copy = [&](int i, const void* from, int bytes) {      // (zeros beyond `bytes`)
+        if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + i * kBytes), "l"(from), "r"(bytes) : "memory");
+        else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to + i * kBytes), "l"(from), "n"(kBytes), "r"(bytes) : "memory");
       };
-      if (live >= S && room == kChannels) {
-        p += channel_of<W>(lane, 0);
+      if (there && whole) {
 #pragma unroll
-        for (int s = 0; s < S; ++s, p += stride)
-#pragma unroll
-          for (int i = 0; i < kPieces; ++i) copy(s, i, p + channel_of<W>(0, i * W), kBytes);
+        for (int i = 0; i < kPieces; ++i) copy(i, p + channel_of<W>(lane, i * W), kBytes);
       } else {
 #pragma unroll
-        for (int s = 0; s < S; ++s)
-#pragma unroll
-          for (int i = 0; i < kPieces; ++i) {
-            const int ch = channel_of<W>(lane, i * W);
-            const bool there = s < live && ch < room;
-            copy(s, i, there ? p + s * stride + ch : base, there ? kBytes : 0);      // (an address that is good where nothing is read)
-          }
+        for (int i = 0; i < kPieces; ++i) {
+          const int ch = channel_of<W>(lane, i * W);
+          const bool any = there && ch < room;
+          copy(i, any ? p + ch : base, any ? kBytes : 0);
+        }
       }
-    } else {      // 2 bytes are no asynchronous copy
-      Raw<TY, kPer> r[S];
+    } else {
+      Raw<TY, kPer> r;
+      r.zero();
 #pragma unroll
-      for (int s = 0; s < S; ++s) {
-        r[s].zero();
-#pragma unroll
-        for (int j = 0; j < kPer; ++j)
-          if (s < live && channel_of<W>(lane, j) < room) raw_put(r[s], j, __ldg(p + s * stride + channel_of<W>(lane, j)));
-      }
-#pragma unroll
-      for (int s = 0; s < S; ++s) put(s, r[s]);
+      for (int j = 0; j < kPer; ++j)
+        if (there && channel_of<W>(lane, j) < room) raw_put(r, j, __ldg(p + channel_of<W>(lane, j)));
+      put(s, r);
     }
   }
   template <int TY>
@@ -329,6 +319,15 @@ struct TilePlace {
     return r;
   }
 };
+// A thread's rows of a tensor in a tile.
+template <int TY> struct Rows {
+  using T = typename Elem<TY>::T;
+  const void* base;
+  const T* p;
+  long long stride;
+  __device__ __forceinline__ Rows(const void* t, const TilePlace& at, long long batch, long long token)
+      : base(t), p(static_cast<const T*>(t) + at.b * batch + at.t0 * token + at.ch0), stride(token) {}
+};
 // One thread takes tickets, and says for all what they stand for.
 struct TicketTaker {
   const DiagProblem& p;
@@ -349,7 +348,7 @@ struct TicketTaker {
 constexpr int kBarParts = 1, kBarOut = 3, kBarStarts = 5;
 template <int N> __device__ __forceinline__ void bar_sync(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory"); }
 template <int N> __device__ __forceinline__ void bar_arrive(int id) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(N) : "memory"); }
-constexpr int kPartsThreads = kRunners + 32, kOutThreads = 32 + kChannels, kStartsThreads = kChannels + kRunners;
+constexpr int kPartsThreads = kRunners + kChannels, kOutThreads = 2 * kChannels, kStartsThreads = kChannels + kRunners;
 
 // The CTAs take tiles until there are none; a CTA's tickets ascend, and it takes tickets ahead: the tile of the lowest ticket that is not
 // done is one that its CTA has begun or begins next, so somebody always can go on.
@@ -409,7 +408,7 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_forward_kernel(const Dia
     return;
   }
   if (threadIdx.x >= kPublisher) {
-    const int ch = 2 * (threadIdx.x - kPublisher);      // two channels a thread
+    const int ch = threadIdx.x - kPublisher;
     for (int n = 0;; ++n) {
       const Ticket cur = sh.ticket[n & 3];
       if (cur.order >= p.tiles) break;
@@ -417,38 +416,38 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_forward_kernel(const Dia
       auto& part = sh.part[n & 1];
       bar_sync<kPartsThreads>(kBarParts + (n & 1));
       if (taker) tickets.take();
-      float ts[2] = {0.f, 0.f}, th[2] = {0.f, 0.f};
-      float4 v[kGroups];
+      float ts = 0.f, th = 0.f;
+      float2 v[kGroups];
 #pragma unroll
-      for (int i = 0; i < kGroups; ++i) v[i] = *reinterpret_cast<const float4*>(&part[i][ch]);
+      for (int i = 0; i < kGroups; ++i) v[i] = part[i][ch];
 #pragma unroll
       for (int i = 0; i < kGroups; ++i) {
-        ts[0] += v[i].x;
-        ts[1] += v[i].z;
+        ts += v[i].x;
         v[i].x = decay_coef(v[i].x);
-        v[i].z = decay_coef(v[i].z);
-        th[0] = decay_step(v[i].x, th[0], v[i].y);
-        th[1] = decay_step(v[i].z, th[1], v[i].w);
-        *reinterpret_cast<float4*>(&part[i][ch]) = v[i];
+        th = decay_step(v[i].x, th, v[i].y);
       }
-      if (p.tiles > 1 && !look.last) {
-        look_store(look.at(0, look.tile0 + look.n_tiles, ch), ts[0], th[0]);
-        look_store(look.at(0, look.tile0 + look.n_tiles, ch + 1), ts[1], th[1]);
-      }
+      if (p.tiles > 1 && !look.last) look_store(look.at(0, look.tile0 + look.n_tiles, ch), ts, th);
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) part[i][ch].x = v[i].x;
       if (taker) sh.ticket[(n + 2) & 3] = tickets.named();
-      __syncwarp();
       bar_arrive<kOutThreads>(kBarOut + (n & 1));
     }
     return;
   }
   const int lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
+  const auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
   const auto fetch = [&](const Ticket& t, int slot) {
     if (t.order < p.tiles) {
       const TilePlace at = TilePlace::of<S>(p, t, grp, false);
-      sh.tile[slot].x.template fetch<XT, W>(p.x, at.b * p.x_batch + at.t0 * p.x_token + at.ch0, p.x_token, lane, at.live, at.room);
-      sh.tile[slot].c.template fetch<GT, W>(p.g, at.b * p.g_batch + at.t0 * p.g_token + at.ch0, p.g_token, lane, at.live, at.room);
+      const Rows<XT> x(p.x, at, p.x_batch, p.x_token);
+      const Rows<GT> g(p.g, at, p.g_batch, p.g_token);
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        sh.tile[slot].x.template fetch<XT, W>(s, x.p + s * x.stride, x.base, lane, s < at.live, at.room == kChannels, at.room);
+        sh.tile[slot].c.template fetch<GT, W>(s, g.p + s * g.stride, g.base, lane, s < at.live, at.room == kChannels, at.room);
+      }
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    commit();
   };
   const auto first_run = [&](int slot) {
     auto& tile = sh.tile[slot];
@@ -494,10 +493,22 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_forward_kernel(const Dia
     bar_sync<kStartsThreads>(kBarStarts + slot);
 #pragma unroll
     for (int j = 0; j < kPer; ++j) st[j] = sh.part[slot][grp][channel_of<W>(lane, j)].x;
+    // a cell that has been read takes its step of the tile after the next
+    const Ticket after = sh.ticket[(n + 2) & 3];
+    const TilePlace to = TilePlace::of<S>(p, after, grp, false);
+    Rows<XT> x(p.x, to, p.x_batch, p.x_token);
+    Rows<GT> g(p.g, to, p.g_batch, p.g_token);
+    const bool more = after.order < p.tiles;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
       const auto xr = tile.x.template take<XT>(s);
       const auto cr = tile.c.template take<LETHE_F32>(s);
+      if (more) {
+        tile.x.template fetch<XT, W>(s, x.p, x.base, lane, s < to.live, to.room == kChannels, to.room);
+        tile.c.template fetch<GT, W>(s, g.p, g.base, lane, s < to.live, to.room == kChannels, to.room);
+      }
+      x.p += x.stride;
+      g.p += g.stride;
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
         const float c = cr.get(j);
@@ -506,7 +517,7 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_forward_kernel(const Dia
       if (s < at.live) store_token<XT, W>(packed<XT>(st), h, lane, at.room);
       h += p.D;
     }
-    fetch(sh.ticket[(n + 2) & 3], slot);
+    commit();
   }
 }
 
@@ -562,7 +573,7 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_backward_kernel(const Di
     return;
   }
   if (threadIdx.x >= kPublisher) {
-    const int ch = 2 * (threadIdx.x - kPublisher);
+    const int ch = threadIdx.x - kPublisher;
     for (int n = 0;; ++n) {
       const Ticket cur = sh.ticket[n & 3];
       if (cur.order >= p.tiles) break;
@@ -570,38 +581,41 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_backward_kernel(const Di
       auto& part = sh.part[n & 1];
       bar_sync<kPartsThreads>(kBarParts + (n & 1));
       if (taker) tickets.take();
-      float ts[2] = {0.f, 0.f}, te[2] = {0.f, 0.f};
+      float ts = 0.f, te = 0.f, c[kGroups], e[kGroups];
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) {
+        c[i] = part[i][ch].x;
+        e[i] = sh.back[n & 1][i][ch];
+      }
 #pragma unroll
       for (int i = kGroups - 1; i >= 0; --i) {
-        const float s0 = part[i][ch].x, s1 = part[i][ch + 1].x;
-        const float2 e = *reinterpret_cast<const float2*>(&sh.back[n & 1][i][ch]);
-        const float c0 = decay_coef(s0), c1 = decay_coef(s1);
-        ts[0] += s0;
-        ts[1] += s1;
-        te[0] = decay_step(c0, te[0], e.x);
-        te[1] = decay_step(c1, te[1], e.y);
-        part[i][ch].x = c0;
-        part[i][ch + 1].x = c1;
+        ts += c[i];
+        c[i] = decay_coef(c[i]);
+        te = decay_step(c[i], te, e[i]);
       }
-      if (p.tiles > 1 && !look.last) {
-        look_store(look.at(0, look.tile0 + look.n_tiles, ch), ts[0], te[0]);
-        look_store(look.at(0, look.tile0 + look.n_tiles, ch + 1), ts[1], te[1]);
-      }
+      if (p.tiles > 1 && !look.last) look_store(look.at(0, look.tile0 + look.n_tiles, ch), ts, te);
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) part[i][ch].x = c[i];
       if (taker) sh.ticket[(n + 2) & 3] = tickets.named();
-      __syncwarp();
       bar_arrive<kOutThreads>(kBarOut + (n & 1));
     }
     return;
   }
   const int lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
+  const auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
   const auto fetch = [&](const Ticket& t, int slot) {
     if (t.order < p.tiles) {
       const TilePlace at = TilePlace::of<S>(p, t, grp, true);
-      sh.tile[slot].x.template fetch<XT, W>(p.x, at.b * p.x_batch + at.t0 * p.x_token + at.ch0, p.x_token, lane, at.live, at.room);
-      sh.tile[slot].c.template fetch<GT, W>(p.g, at.b * p.g_batch + at.t0 * p.g_token + at.ch0, p.g_token, lane, at.live, at.room);
-      if (p.d_h) sh.tile[slot].d.template fetch<XT, W>(p.d_h, at.b * p.d_batch + at.t0 * p.d_token + at.ch0, p.d_token, lane, at.live, at.room);
+      const Rows<XT> x(p.x, at, p.x_batch, p.x_token), d(p.d_h, at, p.d_batch, p.d_token);
+      const Rows<GT> g(p.g, at, p.g_batch, p.g_token);
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        sh.tile[slot].x.template fetch<XT, W>(s, x.p + s * x.stride, x.base, lane, s < at.live, at.room == kChannels, at.room);
+        sh.tile[slot].c.template fetch<GT, W>(s, g.p + s * g.stride, g.base, lane, s < at.live, at.room == kChannels, at.room);
+        if (p.d_h) sh.tile[slot].d.template fetch<XT, W>(s, d.p + s * d.stride, d.base, lane, s < at.live, at.room == kChannels, at.room);
+      }
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    commit();
   };
   const auto first_run = [&](int slot) {
     auto& tile = sh.tile[slot];
@@ -670,10 +684,19 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_backward_kernel(const Di
       st[j] = sh.part[slot][grp][ch].x;
       e[j] = sh.back[slot][grp][ch];
     }
+    const Ticket after = sh.ticket[(n + 2) & 3];
+    const TilePlace to = TilePlace::of<S>(p, after, grp, true);
+    const Rows<XT> x(p.x, to, p.x_batch, p.x_token), d(p.d_h, to, p.d_batch, p.d_token);
+    const Rows<GT> g(p.g, to, p.g_batch, p.g_token);
+    const bool more = after.order < p.tiles;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
       const auto xr = tile.x.template take<XT>(s);
       const auto cr = tile.c.template take<LETHE_F32>(s);
+      if (more) {
+        tile.x.template fetch<XT, W>(s, x.p + s * x.stride, x.base, lane, s < to.live, to.room == kChannels, to.room);
+        tile.c.template fetch<GT, W>(s, g.p + s * g.stride, g.base, lane, s < to.live, to.room == kChannels, to.room);
+      }
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
         const float xv = xr.get(j);
@@ -687,6 +710,7 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_backward_kernel(const Di
 #pragma unroll
     for (int s = S - 1; s >= 0; --s) {
       const auto dr = tile.d.template take<XT>(s);
+      if (more && p.d_h) tile.d.template fetch<XT, W>(s, d.p + s * d.stride, d.base, lane, s < to.live, to.room == kChannels, to.room);
       float vx[kPer], vg[kPer];
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
@@ -700,7 +724,7 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_backward_kernel(const Di
         if (p.dg) store_token<GT, W>(packed<GT>(vg), dg + s * p.D, lane, at.room);
       }
     }
-    fetch(sh.ticket[(n + 2) & 3], slot);
+    commit();
   }
 }
 
