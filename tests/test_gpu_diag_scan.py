@@ -106,6 +106,14 @@ def test_decays(gates, complement):
     check(*make(2, 700, (96,), "f32", gates), complement)
 
 
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("complement", [False, True])
+@pytest.mark.parametrize("B,L,inner", [(400, 10, (8,)), (2, 5000, (264,)), (3, 1100, (1040,)), (350, 200, (72,)), (5, 4100, (6, 40))])
+def test_more_tiles_than_the_gpu_holds(types, complement, B, L, inner):
+    """Copies of whole tiles, and CTAs that do several of them."""
+    check(*make(B, L, inner, types, "kinds"), complement)
+
+
 @pytest.mark.parametrize("L", [2, 7, 8, 9, 255, 256, 257, 2048, 5000])
 def test_lengths(L):
     check(*make(1, L, (68,), "bf16", seed=L), False)
