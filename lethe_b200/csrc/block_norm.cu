@@ -25,32 +25,68 @@ struct GatedProblem {
   float* part;      // per CTA the sums for dweight; NULL: not wanted
 };
 
-// logistic function: the division's approximation is good to 2 ulp and the divisor is in [1, inf]
-__device__ __forceinline__ float logistic(float z) { return __fdividef(1.f, 1.f + expf(-z)); }
+// logistic function.  Results in 16 bits: exponential and reciprocal by the approximations, some 2^-21 off; in 32 bits the
+// exponential is expf, the quotient good to 2 ulp with a divisor in [1, inf].
+template <int XT>
+__device__ __forceinline__ float logistic(float z) {
+  if constexpr (XT == LETHE_F32) return __fdividef(1.f, 1.f + expf(-z));
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return r;
+}
+
+// CTAs on an SM: registers (64 a thread forward, 80 backward)
+template <typename S> constexpr int gated_ctas(bool backward) { return (backward ? 768 : 1024) / S::kThreads / S::R > 0 ? (backward ? 768 : 1024) / S::kThreads / S::R : 1; }
+template <int XT, typename S, bool BACK> using GatedRing = RowRing<S, (BACK ? 3 : 2) * S::R * 8 * elem_bytes(XT), gated_ctas<S>(BACK)>;
 
 template <int XT, typename S>
-__global__ void __launch_bounds__(S::kThreads) gated_norm_kernel(const GatedProblem p) {
+__global__ void __launch_bounds__(S::kThreads, gated_ctas<S>(false)) gated_norm_kernel(const GatedProblem p) {
+  using Ring = GatedRing<XT, S, false>;
+  constexpr int kX = 0, kZ = S::R * elem_bytes(XT) / 2;
   __shared__ float sums[2][1][S::kWarps];
+  extern __shared__ __align__(16) unsigned char smem[];
+  const Ring ring(smem);
   const int t = threadIdx.x % S::T;
   const long long first = static_cast<long long>(blockIdx.x) * S::kRows + threadIdx.x / S::T, step = static_cast<long long>(gridDim.x) * S::kRows;
+  RowWalk ahead(first, step, p.inner);      // of the copies, or of the rows themselves
+  long long far = first;
+  const auto fetch = [&](int stage) {
+    if (far < p.rows) {
+      ring.template copy<XT, kX>(stage, p.x, ahead.at(p.xo, p.xi), t, p.D);
+      ring.template copy<XT, kZ>(stage, p.z, ahead.at(p.zo, p.zi), t, p.D);
+    }
+    Ring::commit();
+    far += step;
+    ahead.next();
+  };
+  if constexpr (Ring::kOn)
+    for (int i = 0; i < Ring::kStages - 1; ++i) fetch(i);
   float w[S::N];
   S::template vector<XT>(w, p.w, p.w_f32, t, p.D, 0.f);
-  RowWalk at(first, step, p.inner);
   const float over = 1.f / p.D;
-  int flip = 0;
+  int flip = 0, stage = 0;
   // every thread of a CTA takes as many turns: row sums are collective
-  for (long long row = first, base = first - threadIdx.x / S::T; base < p.rows; row += step, base += step, at.next(), flip ^= 1) {
+  for (long long row = first, base = first - threadIdx.x / S::T; base < p.rows; row += step, base += step, flip ^= 1) {
     const bool live = row < p.rows;
     Raw<XT, 8> x[S::R], z[S::R];
-    if (live) {
-      S::template load<XT>(x, p.x, at.at(p.xo, p.xi), t, p.D);
-      S::template load<XT>(z, p.z, at.at(p.zo, p.zi), t, p.D);
+    if constexpr (Ring::kOn) {
+      Ring::wait();
+      ring.template take<XT, kX>(x, stage);
+      ring.template take<XT, kZ>(z, stage);
+      fetch(stage ? stage - 1 : Ring::kStages - 1);
+      stage = stage + 1 == Ring::kStages ? 0 : stage + 1;
     } else {
 #pragma unroll
       for (int i = 0; i < S::R; ++i) {
         x[i].zero();
         z[i].zero();
       }
+      if (live) {
+        S::template load<XT>(x, p.x, ahead.at(p.xo, p.xi), t, p.D);
+        S::template load<XT>(z, p.z, ahead.at(p.zo, p.zi), t, p.D);
+      }
+      ahead.next();
     }
     float s[1] = {0.f};
 #pragma unroll
@@ -60,7 +96,7 @@ __global__ void __launch_bounds__(S::kThreads) gated_norm_kernel(const GatedProb
     float y[S::N];
 #pragma unroll
     for (int n = 0; n < S::N; ++n) {
-      const float zv = z[n / 8].get(n % 8), sg = logistic(zv);
+      const float zv = z[n / 8].get(n % 8), sg = logistic<XT>(zv);
       y[n] = x[n / 8].get(n % 8) * r * w[n] * (p.silu ? zv * sg : sg);
     }
     if (live) S::template store<XT>(y, p.y, row * p.D, t, p.D);
@@ -68,26 +104,46 @@ __global__ void __launch_bounds__(S::kThreads) gated_norm_kernel(const GatedProb
 }
 
 template <int XT, typename S>
-__global__ void __launch_bounds__(S::kThreads) gated_norm_vjp_kernel(const GatedProblem p) {
+__global__ void __launch_bounds__(S::kThreads, gated_ctas<S>(true)) gated_norm_vjp_kernel(const GatedProblem p) {
+  using Ring = GatedRing<XT, S, true>;
+  constexpr int kEach = S::R * elem_bytes(XT) / 2, kX = 0, kZ = kEach, kD = 2 * kEach;
   __shared__ float sums[2][2][S::kWarps];
-  extern __shared__ float stage[];
+  extern __shared__ __align__(16) unsigned char smem[];
+  const Ring ring(smem);
   const int t = threadIdx.x % S::T;
   const long long first = static_cast<long long>(blockIdx.x) * S::kRows + threadIdx.x / S::T, step = static_cast<long long>(gridDim.x) * S::kRows;
+  RowWalk ahead(first, step, p.inner);
+  long long far = first;
+  const auto fetch = [&](int stage) {
+    if (far < p.rows) {
+      ring.template copy<XT, kX>(stage, p.x, ahead.at(p.xo, p.xi), t, p.D);
+      ring.template copy<XT, kZ>(stage, p.z, ahead.at(p.zo, p.zi), t, p.D);
+      ring.template copy<XT, kD>(stage, p.dy, far * p.D, t, p.D);
+    }
+    Ring::commit();
+    far += step;
+    ahead.next();
+  };
+  if constexpr (Ring::kOn)
+    for (int i = 0; i < Ring::kStages - 1; ++i) fetch(i);
   float w[S::N], acc[S::N];
   S::template vector<XT>(w, p.w, p.w_f32, t, p.D, 0.f);
 #pragma unroll
   for (int n = 0; n < S::N; ++n) acc[n] = 0.f;
-  RowWalk at(first, step, p.inner);
   const float over = 1.f / p.D;
-  int flip = 0;
-  for (long long row = first, base = first - threadIdx.x / S::T; base < p.rows; row += step, base += step, at.next(), flip ^= 1) {
+  int flip = 0, stage = 0;
+  for (long long row = first, base = first - threadIdx.x / S::T; base < p.rows; row += step, base += step, flip ^= 1) {
     const bool live = row < p.rows;
     Raw<XT, 8> x[S::R], z[S::R], d[S::R];
-    if (live) {
-      S::template load<XT>(x, p.x, at.at(p.xo, p.xi), t, p.D);
-      S::template load<XT>(z, p.z, at.at(p.zo, p.zi), t, p.D);
-      S::template load<XT>(d, p.dy, row * p.D, t, p.D);
-    } else {
+    if constexpr (Ring::kOn) {
+      Ring::wait();
+      ring.template take<XT, kX>(x, stage);
+      ring.template take<XT, kZ>(z, stage);
+      ring.template take<XT, kD>(d, stage);
+      fetch(stage ? stage - 1 : Ring::kStages - 1);
+      stage = stage + 1 == Ring::kStages ? 0 : stage + 1;
+    }
+    if (!Ring::kOn || !live) {      // (a row that is not there adds nothing)
 #pragma unroll
       for (int i = 0; i < S::R; ++i) {
         x[i].zero();
@@ -95,10 +151,18 @@ __global__ void __launch_bounds__(S::kThreads) gated_norm_vjp_kernel(const Gated
         d[i].zero();
       }
     }
+    if constexpr (!Ring::kOn) {
+      if (live) {
+        S::template load<XT>(x, p.x, ahead.at(p.xo, p.xi), t, p.D);
+        S::template load<XT>(z, p.z, ahead.at(p.zo, p.zi), t, p.D);
+        S::template load<XT>(d, p.dy, row * p.D, t, p.D);
+      }
+      ahead.next();
+    }
     float s[2] = {0.f, 0.f}, dn[S::N], slope[S::N];
 #pragma unroll
     for (int n = 0; n < S::N; ++n) {
-      const float xv = x[n / 8].get(n % 8), zv = z[n / 8].get(n % 8), dv = d[n / 8].get(n % 8), sg = logistic(zv);
+      const float xv = x[n / 8].get(n % 8), zv = z[n / 8].get(n % 8), dv = d[n / 8].get(n % 8), sg = logistic<XT>(zv);
       const float a = p.silu ? zv * sg : sg;
       slope[n] = dv * (p.silu ? sg * fmaf(zv, 1.f - sg, 1.f) : sg * (1.f - sg));
       dn[n] = dv * a;
@@ -120,7 +184,7 @@ __global__ void __launch_bounds__(S::kThreads) gated_norm_vjp_kernel(const Gated
       if (p.dz) S::template store<XT>(slope, p.dz, row * p.D, t, p.D);
     }
   }
-  if (p.part) S::column_share(acc, p.part + static_cast<long long>(blockIdx.x) * p.D, stage, t, p.D);
+  if (p.part) S::column_share(acc, p.part + static_cast<long long>(blockIdx.x) * p.D, reinterpret_cast<float*>(smem), t, p.D);
 }
 
 // 32 columns a CTA; a warp takes every 32nd share, the warps' sums are added in their order.
@@ -180,8 +244,11 @@ extern "C" int lethe_gdn_gated_norm(const LetheGdnGatedNormArgs* a, void* stream
   return by_x_type(a->x_type, [&](auto x) {
     return by_row_shape(p.D, vec, [&](auto s) {
       using S = decltype(s);
-      const int grid = norm_grid(p.rows, S::kRows, 2048 / S::kThreads);
-      gated_norm_kernel<x.value, S><<<grid, S::kThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+      static SmemAttr attr;
+      constexpr int smem = GatedRing<x.value, S, false>::kBytes;
+      if (int e = attr.set(gated_norm_kernel<x.value, S>, smem)) return e;
+      const int grid = norm_grid(p.rows, S::kRows, gated_ctas<S>(false));
+      gated_norm_kernel<x.value, S><<<grid, S::kThreads, smem, static_cast<cudaStream_t>(stream)>>>(p);
       return launched_ok();
     });
   });
@@ -206,8 +273,10 @@ extern "C" int lethe_gdn_gated_norm_vjp(const LetheGdnGatedNormArgs* a, void* st
   const int e = by_x_type(a->x_type, [&](auto x) {
     return by_row_shape(p.D, vec, [&](auto s) {
       using S = decltype(s);
-      grid = std::min(norm_grid(p.rows, S::kRows, 1024 / S::kThreads), norm_parts_max(p.D));
-      constexpr int smem = S::kRows > 1 ? S::kThreads * S::N * 4 : 0;
+      grid = std::min(norm_grid(p.rows, S::kRows, gated_ctas<S>(true)), norm_parts_max(p.D));
+      static SmemAttr attr;
+      constexpr int smem = std::max(GatedRing<x.value, S, true>::kBytes, S::kColumnBytes);
+      if (int e = attr.set(gated_norm_vjp_kernel<x.value, S>, smem)) return e;
       gated_norm_vjp_kernel<x.value, S><<<grid, S::kThreads, smem, st>>>(p);
       return launched_ok();
     });

@@ -27,35 +27,65 @@ struct ResidualProblem {
   int vectors, at[3];       // their number, and the place of each (-1: not wanted)
 };
 
+// CTAs on an SM: registers (64 a thread forward, 128 backward)
+template <typename S> constexpr int residual_ctas(bool backward) { return (backward ? 512 : 1024) / S::kThreads / (backward ? 1 : S::R); }
+template <int XT, int RT, typename S> using ResidualRing = RowRing<S, S::R * 8 * (elem_bytes(XT) + elem_bytes(RT)), residual_ctas<S>(false)>;
+template <int XT, int RT, typename S, int BRANCH>
+using ResidualRingBack = RowRing<S, S::R * 8 * (elem_bytes(XT) * (BRANCH ? 2 : 1) + 2 * elem_bytes(RT)), residual_ctas<S>(true)>;
+
 template <int XT, int RT, typename S, bool POST>
-__global__ void __launch_bounds__(S::kThreads) residual_norm_kernel(const ResidualProblem p) {
-  __shared__ float sums[2][1][S::kWarps];
+__global__ void __launch_bounds__(S::kThreads, residual_ctas<S>(false)) residual_norm_kernel(const ResidualProblem p) {
+  using Ring = ResidualRing<XT, RT, S>;
+  constexpr int kX = 0, kRes = S::R * elem_bytes(XT) / 2;
+  __shared__ float sums[2][2][1][S::kWarps];
+  extern __shared__ __align__(16) unsigned char smem[];
+  const Ring ring(smem);
   const int t = threadIdx.x % S::T;
   const long long first = static_cast<long long>(blockIdx.x) * S::kRows + threadIdx.x / S::T, step = static_cast<long long>(gridDim.x) * S::kRows;
+  long long far = first;
+  const auto fetch = [&](int stage) {
+    if (far < p.rows) {
+      ring.template copy<XT, kX>(stage, p.x, far * p.x_stride, t, p.D);
+      if (p.res) ring.template copy<RT, kRes>(stage, p.res, far * p.res_stride, t, p.D);      // (else the cells stay zeros)
+    }
+    Ring::commit();
+    far += step;
+  };
+  if constexpr (Ring::kOn)
+    for (int i = 0; i < Ring::kStages - 1; ++i) fetch(i);
   float w[S::N], sc[S::N], pw[POST ? S::N : 1];
   S::template vector<XT>(w, p.w, p.w_f32, t, p.D, 0.f);
   S::template vector<XT>(sc, p.scale, p.w_f32, t, p.D, p.scale_value);
   if constexpr (POST) S::template vector<XT>(pw, p.pw, p.w_f32, t, p.D, 0.f);
   const float over = 1.f / p.D;
-  for (long long row = first, base = first - threadIdx.x / S::T; base < p.rows; row += step, base += step) {
+  int flip = 0, stage = 0;
+  for (long long row = first, base = first - threadIdx.x / S::T; base < p.rows; row += step, base += step, flip ^= 1) {
     const bool live = row < p.rows;
     Raw<XT, 8> x[S::R];
     Raw<RT, 8> res[S::R];
+    if constexpr (Ring::kOn) {
+      Ring::wait();
+      ring.template take<XT, kX>(x, stage);
+      ring.template take<RT, kRes>(res, stage);
+      fetch(stage ? stage - 1 : Ring::kStages - 1);
+      stage = stage + 1 == Ring::kStages ? 0 : stage + 1;
+    } else {
 #pragma unroll
-    for (int i = 0; i < S::R; ++i) {
-      x[i].zero();
-      res[i].zero();
-    }
-    if (live) {
-      S::template load<XT>(x, p.x, row * p.x_stride, t, p.D);
-      if (p.res) S::template load<RT>(res, p.res, row * p.res_stride, t, p.D);
+      for (int i = 0; i < S::R; ++i) {
+        x[i].zero();
+        res[i].zero();
+      }
+      if (live) {
+        S::template load<XT>(x, p.x, row * p.x_stride, t, p.D);
+        if (p.res) S::template load<RT>(res, p.res, row * p.res_stride, t, p.D);
+      }
     }
     float r1 = 1.f;
     if constexpr (POST) {
       float s[1] = {0.f};
 #pragma unroll
       for (int n = 0; n < S::N; ++n) s[0] = fmaf(x[n / 8].get(n % 8), x[n / 8].get(n % 8), s[0]);
-      S::template row_sums<1>(s, sums[0]);
+      S::template row_sums<1>(s, sums[flip][0]);
       r1 = rsqrtf(fmaf(s[0], over, p.eps));
     }
     float v[S::N], s[1] = {0.f};
@@ -68,52 +98,87 @@ __global__ void __launch_bounds__(S::kThreads) residual_norm_kernel(const Residu
       s[0] = fmaf(v[n], v[n], s[0]);
     }
     if (live) S::template store<RT>(v, p.r, row * p.D, t, p.D);
-    S::template row_sums<1>(s, sums[1]);
+    S::template row_sums<1>(s, sums[flip][1]);
     const float r2 = rsqrtf(fmaf(s[0], over, p.eps));
 #pragma unroll
     for (int n = 0; n < S::N; ++n) v[n] = v[n] * r2 * w[n];
     if (live) S::template store<XT>(v, p.y, row * p.D, t, p.D);
-    if constexpr (!POST && S::T > 32) __syncthreads();      // sums[1] is read by now (with POST the sum in between says so)
   }
 }
 
-// BRANCH 0: nothing of x is needed.  1: x for dscale.  2: norm of x.
+// BRANCH 0: nothing of x is needed.  1: x for dscale.  2: norm of x.  Both gradients of the branch come from one sum over rows: with
+// q = sum of d n1, dscale = post_weight q and dpost_weight = scale q (without a norm of x: q = sum of d x = dscale).
 template <int XT, int RT, typename S, int BRANCH>
-__global__ void __launch_bounds__(S::kThreads) residual_norm_vjp_kernel(const ResidualProblem p) {
-  __shared__ float sums[2][3][S::kWarps];
-  extern __shared__ float stage[];
+__global__ void __launch_bounds__(S::kThreads, residual_ctas<S>(true)) residual_norm_vjp_kernel(const ResidualProblem p) {
+  using Ring = ResidualRingBack<XT, RT, S, BRANCH>;
+  constexpr int kR = 0, kDr = S::R * elem_bytes(RT) / 2, kDy = 2 * kDr, kX = kDy + S::R * elem_bytes(XT) / 2;
+  __shared__ float sums[2][2][3][S::kWarps];
+  extern __shared__ __align__(16) unsigned char smem[];
+  const Ring ring(smem);
   const int t = threadIdx.x % S::T;
   const long long first = static_cast<long long>(blockIdx.x) * S::kRows + threadIdx.x / S::T, step = static_cast<long long>(gridDim.x) * S::kRows;
+  long long far = first;
+  const auto fetch = [&](int stage) {
+    if (far < p.rows) {
+      ring.template copy<RT, kR>(stage, p.r, far * p.D, t, p.D);
+      if (p.dr) ring.template copy<RT, kDr>(stage, p.dr, far * p.D, t, p.D);
+      if (p.dy) ring.template copy<XT, kDy>(stage, p.dy, far * p.D, t, p.D);
+      if constexpr (BRANCH >= 1) ring.template copy<XT, kX>(stage, p.x, far * p.x_stride, t, p.D);
+    }
+    Ring::commit();
+    far += step;
+  };
+  if constexpr (Ring::kOn)
+    for (int i = 0; i < Ring::kStages - 1; ++i) fetch(i);
   constexpr int NB = BRANCH == 2 ? S::N : 1, NS = BRANCH >= 1 ? S::N : 1;
-  float w[S::N], sc[S::N], pw[NB], acc_w[S::N], acc_p[NB], acc_s[NS];
+  float w[S::N], sc[S::N], acc_w[S::N], acc_q[NS];      // sc: scale, times post_weight where there is one
   S::template vector<XT>(w, p.w, p.w_f32, t, p.D, 0.f);
   S::template vector<XT>(sc, p.scale, p.w_f32, t, p.D, p.scale_value);
-  if constexpr (BRANCH == 2) S::template vector<XT>(pw, p.pw, p.w_f32, t, p.D, 0.f);
+  if constexpr (BRANCH == 2) {
+    float pw[NB];
+    S::template vector<XT>(pw, p.pw, p.w_f32, t, p.D, 0.f);
+#pragma unroll
+    for (int n = 0; n < S::N; ++n) sc[n] *= pw[n];
+  }
 #pragma unroll
   for (int n = 0; n < S::N; ++n) {
     acc_w[n] = 0.f;
-    if constexpr (BRANCH == 2) acc_p[n] = 0.f;
-    if constexpr (BRANCH >= 1) acc_s[n] = 0.f;
+    if constexpr (BRANCH >= 1) acc_q[n] = 0.f;
   }
   const float over = 1.f / p.D;
-  for (long long row = first, base = first - threadIdx.x / S::T; base < p.rows; row += step, base += step) {
+  int flip = 0, stage = 0;
+  for (long long row = first, base = first - threadIdx.x / S::T; base < p.rows; row += step, base += step, flip ^= 1) {
     const bool live = row < p.rows;
     Raw<XT, 8> x[S::R], dy[S::R];
     Raw<RT, 8> r[S::R], dr[S::R];
+    if constexpr (Ring::kOn) {
+      Ring::wait();
+      ring.template take<RT, kR>(r, stage);
+      ring.template take<RT, kDr>(dr, stage);
+      ring.template take<XT, kDy>(dy, stage);
+      if constexpr (BRANCH >= 1) ring.template take<XT, kX>(x, stage);
+      fetch(stage ? stage - 1 : Ring::kStages - 1);
+      stage = stage + 1 == Ring::kStages ? 0 : stage + 1;
+    }
+    if (!Ring::kOn || !live) {      // (a row that is not there adds nothing)
 #pragma unroll
-    for (int i = 0; i < S::R; ++i) {
-      x[i].zero();
-      dy[i].zero();
-      r[i].zero();
-      dr[i].zero();
+      for (int i = 0; i < S::R; ++i) {
+        x[i].zero();
+        dy[i].zero();
+        r[i].zero();
+        dr[i].zero();
+      }
     }
-    if (live) {
-      S::template load<RT>(r, p.r, row * p.D, t, p.D);
-      if (p.dy) S::template load<XT>(dy, p.dy, row * p.D, t, p.D);
-      if (p.dr) S::template load<RT>(dr, p.dr, row * p.D, t, p.D);
-      if constexpr (BRANCH >= 1) S::template load<XT>(x, p.x, row * p.x_stride, t, p.D);
+    if constexpr (!Ring::kOn) {
+      if (live) {
+        S::template load<RT>(r, p.r, row * p.D, t, p.D);
+        if (p.dy) S::template load<XT>(dy, p.dy, row * p.D, t, p.D);
+        if (p.dr) S::template load<RT>(dr, p.dr, row * p.D, t, p.D);
+        if constexpr (BRANCH >= 1) S::template load<XT>(x, p.x, row * p.x_stride, t, p.D);
+      }
     }
-    float s[3] = {0.f, 0.f, 0.f};
+    constexpr int K = BRANCH == 2 ? 3 : 2;
+    float s[K] = {};
 #pragma unroll
     for (int n = 0; n < S::N; ++n) {
       const float rv = r[n / 8].get(n % 8);
@@ -121,43 +186,50 @@ __global__ void __launch_bounds__(S::kThreads) residual_norm_vjp_kernel(const Re
       s[1] = fmaf(dy[n / 8].get(n % 8) * w[n], rv, s[1]);
       if constexpr (BRANCH == 2) s[2] = fmaf(x[n / 8].get(n % 8), x[n / 8].get(n % 8), s[2]);
     }
-    S::template row_sums<3>(s, sums[0]);
+    S::template row_sums<K>(s, sums[flip][0]);
     const float r2 = rsqrtf(fmaf(s[0], over, p.eps)), c2 = s[1] * over * r2 * r2;
-    const float r1 = BRANCH == 2 ? rsqrtf(fmaf(s[2], over, p.eps)) : 1.f;
+    float r1 = 1.f;
+    if constexpr (BRANCH == 2) r1 = rsqrtf(fmaf(s[2], over, p.eps));
     float d[S::N], q[1] = {0.f};
 #pragma unroll
     for (int n = 0; n < S::N; ++n) {
       const float rv = r[n / 8].get(n % 8), dyv = dy[n / 8].get(n % 8);
       acc_w[n] = fmaf(dyv, rv * r2, acc_w[n]);
       d[n] = fmaf(r2, dyv * w[n] - rv * c2, dr[n / 8].get(n % 8));
-      if constexpr (BRANCH == 1) acc_s[n] = fmaf(d[n], x[n / 8].get(n % 8), acc_s[n]);
-      if constexpr (BRANCH == 2) {
-        const float n1 = x[n / 8].get(n % 8) * r1, dn = d[n] * n1;
-        acc_s[n] = fmaf(dn, pw[n], acc_s[n]);
-        acc_p[n] = fmaf(dn, sc[n], acc_p[n]);
-        q[0] = fmaf(dn, sc[n] * pw[n], q[0]);
+      if constexpr (BRANCH >= 1) {
+        const float dn = d[n] * (BRANCH == 2 ? x[n / 8].get(n % 8) * r1 : x[n / 8].get(n % 8));
+        acc_q[n] += dn;
+        if constexpr (BRANCH == 2) q[0] = fmaf(dn, sc[n], q[0]);
       }
     }
     if (live && p.dres) S::template store<RT>(d, p.dres, row * p.D, t, p.D);
     if constexpr (BRANCH == 2) {
-      S::template row_sums<1>(q, sums[1]);
-      const float c1 = q[0] * over;
+      S::template row_sums<1>(q, sums[flip][1]);
+      const float c1 = q[0] * over * r1;
 #pragma unroll
-      for (int n = 0; n < S::N; ++n) d[n] = r1 * (d[n] * (sc[n] * pw[n]) - x[n / 8].get(n % 8) * r1 * c1);
+      for (int n = 0; n < S::N; ++n) d[n] = r1 * (d[n] * sc[n] - x[n / 8].get(n % 8) * c1);
     } else {
 #pragma unroll
       for (int n = 0; n < S::N; ++n) d[n] *= sc[n];
-      if constexpr (S::T > 32) __syncthreads();      // sums[0] is read by now
     }
     if (live && p.dx) S::template store<XT>(d, p.dx, row * p.D, t, p.D);
   }
   if (!p.part) return;
   float* line = p.part + static_cast<long long>(blockIdx.x) * p.vectors * p.D;
-  if (p.at[0] >= 0) S::column_share(acc_w, line + static_cast<long long>(p.at[0]) * p.D, stage, t, p.D);
-  if constexpr (BRANCH == 2)
-    if (p.at[1] >= 0) S::column_share(acc_p, line + static_cast<long long>(p.at[1]) * p.D, stage, t, p.D);
+  float* columns = reinterpret_cast<float*>(smem);
+  if (p.at[0] >= 0) S::column_share(acc_w, line + static_cast<long long>(p.at[0]) * p.D, columns, t, p.D);
+  if constexpr (BRANCH == 2) {
+    float v[S::N];
+    S::template vector<XT>(v, p.scale, p.w_f32, t, p.D, p.scale_value);
+#pragma unroll
+    for (int n = 0; n < S::N; ++n) v[n] *= acc_q[n];
+    if (p.at[1] >= 0) S::column_share(v, line + static_cast<long long>(p.at[1]) * p.D, columns, t, p.D);
+    S::template vector<XT>(v, p.pw, p.w_f32, t, p.D, 0.f);
+#pragma unroll
+    for (int n = 0; n < S::N; ++n) acc_q[n] *= v[n];
+  }
   if constexpr (BRANCH >= 1)
-    if (p.at[2] >= 0) S::column_share(acc_s, line + static_cast<long long>(p.at[2]) * p.D, stage, t, p.D);
+    if (p.at[2] >= 0) S::column_share(acc_q, line + static_cast<long long>(p.at[2]) * p.D, columns, t, p.D);
 }
 
 // f(XT, RT)
@@ -192,11 +264,16 @@ extern "C" int lethe_gdn_residual_norm(const LetheGdnResidualNormArgs* a, void* 
   return by_stream_type(a->x_type, a->r_type, [&](auto x, auto r) {
     return by_row_shape(p.D, vec, [&](auto s) {
       using S = decltype(s);
-      const int grid = norm_grid(p.rows, S::kRows, 2048 / S::kThreads);
+      const int grid = norm_grid(p.rows, S::kRows, residual_ctas<S>(false));
+      constexpr int smem = ResidualRing<x.value, r.value, S>::kBytes;
       cudaStream_t st = static_cast<cudaStream_t>(stream);
-      if (p.pw) residual_norm_kernel<x.value, r.value, S, true><<<grid, S::kThreads, 0, st>>>(p);
-      else residual_norm_kernel<x.value, r.value, S, false><<<grid, S::kThreads, 0, st>>>(p);
-      return launched_ok();
+      const auto go = [&](auto kern, SmemAttr& attr) {
+        if (int e = attr.set(kern, smem)) return e;
+        kern<<<grid, S::kThreads, smem, st>>>(p);
+        return launched_ok();
+      };
+      static SmemAttr attr[2];
+      return p.pw ? go(residual_norm_kernel<x.value, r.value, S, true>, attr[1]) : go(residual_norm_kernel<x.value, r.value, S, false>, attr[0]);
     });
   });
 }
@@ -230,12 +307,17 @@ extern "C" int lethe_gdn_residual_norm_vjp(const LetheGdnResidualNormArgs* a, vo
   const int e = by_stream_type(a->x_type, a->r_type, [&](auto x, auto r) {
     return by_row_shape(p.D, vec, [&](auto s) {
       using S = decltype(s);
-      grid = std::min(norm_grid(p.rows, S::kRows, 1024 / S::kThreads), norm_parts_max(p.D));
-      constexpr int smem = S::kRows > 1 ? S::kThreads * S::N * 4 : 0;
-      if (branch == 2) residual_norm_vjp_kernel<x.value, r.value, S, 2><<<grid, S::kThreads, smem, st>>>(p);
-      else if (branch == 1) residual_norm_vjp_kernel<x.value, r.value, S, 1><<<grid, S::kThreads, smem, st>>>(p);
-      else residual_norm_vjp_kernel<x.value, r.value, S, 0><<<grid, S::kThreads, smem, st>>>(p);
-      return launched_ok();
+      grid = std::min(norm_grid(p.rows, S::kRows, residual_ctas<S>(true)), norm_parts_max(p.D));
+      static SmemAttr attr[3];
+      const auto go = [&](auto branch) {
+        constexpr int kBranch = decltype(branch)::value;
+        const auto kern = residual_norm_vjp_kernel<x.value, r.value, S, kBranch>;
+        constexpr int smem = std::max(ResidualRingBack<x.value, r.value, S, kBranch>::kBytes, S::kColumnBytes);
+        if (int e = attr[kBranch].set(kern, smem)) return e;
+        kern<<<grid, S::kThreads, smem, st>>>(p);
+        return launched_ok();
+      };
+      return branch == 2 ? go(std::integral_constant<int, 2>()) : branch == 1 ? go(std::integral_constant<int, 1>()) : go(std::integral_constant<int, 0>());
     });
   });
   if (e || !p.part) return e;
