@@ -28,12 +28,16 @@ struct GatedProblem {
 // logistic function.  Results in 16 bits: exponential and reciprocal by the approximations, some 2^-21 off; in 32 bits the
 // exponential is expf, the quotient good to 2 ulp with a divisor in [1, inf].
 template <int XT>
-__device__ __forceinline__ float logistic(float z) {
-  if constexpr (XT == LETHE_F32) return __fdividef(1.f, 1.f + expf(-z));
-  float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-  return r;
+__device__ __forceinline__ F2 logistic(F2 z) {
+  if constexpr (XT == LETHE_F32) return f2(__fdividef(1.f, 1.f + expf(-lo(z))), __fdividef(1.f, 1.f + expf(-hi(z))));
+  const F2 t = z * f2(-1.4426950408889634f);
+  float a, b;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(lo(t)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(hi(t)));
+  const F2 d = f2(a, b) + f2(1.f);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(lo(d)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(hi(d)));
+  return f2(a, b);
 }
 
 // CTAs on an SM: registers (64 a thread forward, 80 backward)
@@ -62,7 +66,7 @@ __global__ void __launch_bounds__(S::kThreads, gated_ctas<S>(false)) gated_norm_
   };
   if constexpr (Ring::kOn)
     for (int i = 0; i < Ring::kStages - 1; ++i) fetch(i);
-  float w[S::N];
+  F2 w[S::P];
   S::template vector<XT>(w, p.w, p.w_f32, t, p.D, 0.f);
   const float over = 1.f / p.D;
   int flip = 0, stage = 0;
@@ -88,16 +92,17 @@ __global__ void __launch_bounds__(S::kThreads, gated_ctas<S>(false)) gated_norm_
       }
       ahead.next();
     }
-    float s[1] = {0.f};
+    F2 xx = f2(0.f);
 #pragma unroll
-    for (int n = 0; n < S::N; ++n) s[0] = fmaf(x[n / 8].get(n % 8), x[n / 8].get(n % 8), s[0]);
+    for (int n = 0; n < S::P; ++n) xx = fma2(x[n / 4].get2(n % 4), x[n / 4].get2(n % 4), xx);
+    float s[1] = {lo(xx) + hi(xx)};
     S::template row_sums<1>(s, sums[flip]);
-    const float r = rsqrtf(fmaf(s[0], over, p.eps));
-    float y[S::N];
+    const F2 r = f2(rsqrtf(fmaf(s[0], over, p.eps)));
+    F2 y[S::P];
 #pragma unroll
-    for (int n = 0; n < S::N; ++n) {
-      const float zv = z[n / 8].get(n % 8), sg = logistic<XT>(zv);
-      y[n] = x[n / 8].get(n % 8) * r * w[n] * (p.silu ? zv * sg : sg);
+    for (int n = 0; n < S::P; ++n) {
+      const F2 zv = z[n / 4].get2(n % 4), sg = logistic<XT>(zv);
+      y[n] = x[n / 4].get2(n % 4) * r * w[n] * (p.silu ? zv * sg : sg);
     }
     if (live) S::template store<XT>(y, p.y, row * p.D, t, p.D);
   }
@@ -126,10 +131,10 @@ __global__ void __launch_bounds__(S::kThreads, gated_ctas<S>(true)) gated_norm_v
   };
   if constexpr (Ring::kOn)
     for (int i = 0; i < Ring::kStages - 1; ++i) fetch(i);
-  float w[S::N], acc[S::N];
+  F2 w[S::P], acc[S::P];
   S::template vector<XT>(w, p.w, p.w_f32, t, p.D, 0.f);
 #pragma unroll
-  for (int n = 0; n < S::N; ++n) acc[n] = 0.f;
+  for (int n = 0; n < S::P; ++n) acc[n] = f2(0.f);
   const float over = 1.f / p.D;
   int flip = 0, stage = 0;
   for (long long row = first, base = first - threadIdx.x / S::T; base < p.rows; row += step, base += step, flip ^= 1) {
@@ -159,25 +164,27 @@ __global__ void __launch_bounds__(S::kThreads, gated_ctas<S>(true)) gated_norm_v
       }
       ahead.next();
     }
-    float s[2] = {0.f, 0.f}, dn[S::N], slope[S::N];
+    F2 xx = f2(0.f), dx_sum = f2(0.f), dn[S::P], slope[S::P];
 #pragma unroll
-    for (int n = 0; n < S::N; ++n) {
-      const float xv = x[n / 8].get(n % 8), zv = z[n / 8].get(n % 8), dv = d[n / 8].get(n % 8), sg = logistic<XT>(zv);
-      const float a = p.silu ? zv * sg : sg;
-      slope[n] = dv * (p.silu ? sg * fmaf(zv, 1.f - sg, 1.f) : sg * (1.f - sg));
-      dn[n] = dv * a;
-      s[0] = fmaf(xv, xv, s[0]);
-      s[1] = fmaf(dn[n] * w[n], xv, s[1]);
+    for (int n = 0; n < S::P; ++n) {
+      const F2 xv = x[n / 4].get2(n % 4), zv = z[n / 4].get2(n % 4), dv = d[n / 4].get2(n % 4), sg = logistic<XT>(zv);
+      const F2 rest = fma2(sg, f2(-1.f), f2(1.f)), ds = dv * sg;      // 1 - s, dy s
+      dn[n] = p.silu ? ds * zv : ds;
+      slope[n] = ds * (p.silu ? fma2(zv, rest, f2(1.f)) : rest);
+      xx = fma2(xv, xv, xx);
+      dx_sum = fma2(dn[n] * w[n], xv, dx_sum);
     }
+    float s[2] = {lo(xx) + hi(xx), lo(dx_sum) + hi(dx_sum)};
     S::template row_sums<2>(s, sums[flip]);
-    const float r = rsqrtf(fmaf(s[0], over, p.eps)), c = s[1] * over * r * r;
-    float dx[S::N];
+    const float r1 = rsqrtf(fmaf(s[0], over, p.eps));
+    const F2 r = f2(r1), c = f2(-s[1] * over * r1 * r1);
+    F2 dx[S::P];
 #pragma unroll
-    for (int n = 0; n < S::N; ++n) {
-      const float xv = x[n / 8].get(n % 8);
-      dx[n] = r * (dn[n] * w[n] - xv * c);
-      acc[n] = fmaf(dn[n], xv * r, acc[n]);
-      slope[n] *= xv * r * w[n];
+    for (int n = 0; n < S::P; ++n) {
+      const F2 xv = x[n / 4].get2(n % 4), xr = xv * r;
+      dx[n] = r * fma2(xv, c, dn[n] * w[n]);
+      acc[n] = fma2(dn[n], xr, acc[n]);
+      slope[n] = slope[n] * (xr * w[n]);
     }
     if (live) {
       if (p.dx) S::template store<XT>(dx, p.dx, row * p.D, t, p.D);

@@ -22,7 +22,7 @@ inline int norm_parts_max(int D) { return D <= 2048 ? 1024 : 320; }
 
 template <int T_, int R_, bool VEC_>
 struct RowShape {
-  static constexpr int T = T_, R = R_, N = R_ * 8;
+  static constexpr int T = T_, R = R_, N = R_ * 8, P = N / 2;      // values and pairs of a thread
   static constexpr bool VEC = VEC_;
   static constexpr int kThreads = T > 32 ? T : 256, kRows = kThreads / T;
   static constexpr int kWarps = kThreads / 32;
@@ -46,33 +46,36 @@ struct RowShape {
     }
   }
   template <int TY>
-  __device__ __forceinline__ static void store(const float (&v)[N], void* base, long long row, int t, int D) {
+  __device__ __forceinline__ static void store(const Raw<TY, 8> (&r)[R], void* base, long long row, int t, int D) {
     typename Elem<TY>::T* p = static_cast<typename Elem<TY>::T*>(base) + row;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       if constexpr (VEC) {
-        if ((i * T + t) * 8 < D) {
-          Raw<TY, 8> r;
-#pragma unroll
-          for (int j = 0; j < 8; j += 2) r.set2(j, v[i * 8 + j], v[i * 8 + j + 1]);
-          r.store(p + (i * T + t) * 8);
-        }
+        if ((i * T + t) * 8 < D) r[i].store(p + (i * T + t) * 8);
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (col(t, i * 8 + j) < D) p[col(t, i * 8 + j)] = from_f32<TY>(v[i * 8 + j]);
+          if (col(t, i * 8 + j) < D) p[col(t, i * 8 + j)] = raw_take(r[i], j);
       }
     }
   }
+  template <int TY>
+  __device__ __forceinline__ static void store(const F2 (&v)[P], void* base, long long row, int t, int D) {
+    Raw<TY, 8> r[R];
+#pragma unroll
+    for (int n = 0; n < P; ++n) r[n / 4].set2(n % 4, v[n]);
+    store<TY>(r, base, row, t, D);
+  }
   // a vector of D values (weight, scale), fp32 or XT; `none` where there is no vector
   template <int XT>
-  __device__ __forceinline__ static void vector(float (&v)[N], const void* p, bool f32, int t, int D, float none) {
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
+  __device__ __forceinline__ static void vector(F2 (&v)[P], const void* p, bool f32, int t, int D, float none) {
+    const auto one = [&](int n) {
       const int c = col(t, n);
-      v[n] = none;
-      if (p && c < D) v[n] = f32 ? __ldg(static_cast<const float*>(p) + c) : to_f32(__ldg(static_cast<const typename Elem<XT>::T*>(p) + c));
-    }
+      if (!p || c >= D) return none;
+      return f32 ? __ldg(static_cast<const float*>(p) + c) : to_f32(__ldg(static_cast<const typename Elem<XT>::T*>(p) + c));
+    };
+#pragma unroll
+    for (int n = 0; n < P; ++n) v[n] = f2(one(2 * n), one(2 * n + 1));
   }
   // sums of K values over the threads of a row, in all of them.  `buf`: this sum's place in shared memory, not that of the sum before.
   template <int K>
@@ -96,7 +99,13 @@ struct RowShape {
     }
   }
   // the CTA's share of a sum over rows: out[col] of its line of the work buffer.  `stage`: kColumnBytes.
-  __device__ __forceinline__ static void column_share(const float (&acc)[N], float* out, float* stage, int t, int D) {
+  __device__ __forceinline__ static void column_share(const F2 (&acc2)[P], float* out, float* stage, int t, int D) {
+    float acc[N];
+#pragma unroll
+    for (int n = 0; n < P; ++n) {
+      acc[2 * n] = lo(acc2[n]);
+      acc[2 * n + 1] = hi(acc2[n]);
+    }
     if constexpr (kRows == 1) {
 #pragma unroll
       for (int n = 0; n < N; ++n)

@@ -24,6 +24,40 @@ template <> __device__ __forceinline__ float from_f32<LETHE_F32>(float x) { retu
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<LETHE_BF16>(float x) { return __float2bfloat16_rn(x); }
 template <> __device__ __forceinline__ __half from_f32<LETHE_F16>(float x) { return __float2half_rn(x); }
 
+// Two floats that go through one instruction: each product and sum is rounded as by itself.
+struct F2 { unsigned long long v; };
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ F2 f2(float a) { return f2(a, a); }
+__device__ __forceinline__ float lo(F2 a) {
+  float x, y;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a.v));
+  return x;
+}
+__device__ __forceinline__ float hi(F2 a) {
+  float x, y;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a.v));
+  return y;
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
 // N neighbours as they lie in memory: read once, so they do not take room in L1.  The address is a multiple of their size (16 bytes at most).
 template <int TY, int N> struct Raw {
   static constexpr int kWords = N * elem_bytes(TY) / 4;
@@ -57,6 +91,8 @@ template <int TY, int N> struct Raw {
     if constexpr (TY == LETHE_BF16) return __uint_as_float((i & 1) ? (w[i / 2] & 0xffff0000u) : (w[i / 2] << 16));
     if constexpr (TY == LETHE_F16) return __half2float(__ushort_as_half(static_cast<unsigned short>((i & 1) ? (w[i / 2] >> 16) : (w[i / 2] & 0xffffu))));
   }
+  __device__ __forceinline__ F2 get2(int i) const { return f2(get(2 * i), get(2 * i + 1)); }      // pair i
+  __device__ __forceinline__ void set2(int i, F2 a) { set2(2 * i, lo(a), hi(a)); }
   __device__ __forceinline__ void set2(int i, float a, float b) {      // elements i (even) and i + 1
     if constexpr (TY == LETHE_F32) {
       w[i] = __float_as_uint(a);

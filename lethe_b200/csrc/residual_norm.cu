@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(S::kThreads, residual_ctas<S>(false)) residual
   };
   if constexpr (Ring::kOn)
     for (int i = 0; i < Ring::kStages - 1; ++i) fetch(i);
-  float w[S::N], sc[S::N], pw[POST ? S::N : 1];
+  F2 w[S::P], sc[S::P], pw[S::P];
   S::template vector<XT>(w, p.w, p.w_f32, t, p.D, 0.f);
   S::template vector<XT>(sc, p.scale, p.w_f32, t, p.D, p.scale_value);
   if constexpr (POST) S::template vector<XT>(pw, p.pw, p.w_f32, t, p.D, 0.f);
@@ -80,29 +80,34 @@ __global__ void __launch_bounds__(S::kThreads, residual_ctas<S>(false)) residual
         if (p.res) S::template load<RT>(res, p.res, row * p.res_stride, t, p.D);
       }
     }
-    float r1 = 1.f;
+    F2 r1 = f2(1.f);
     if constexpr (POST) {
-      float s[1] = {0.f};
+      F2 xx = f2(0.f);
 #pragma unroll
-      for (int n = 0; n < S::N; ++n) s[0] = fmaf(x[n / 8].get(n % 8), x[n / 8].get(n % 8), s[0]);
+      for (int n = 0; n < S::P; ++n) xx = fma2(x[n / 4].get2(n % 4), x[n / 4].get2(n % 4), xx);
+      float s[1] = {lo(xx) + hi(xx)};
       S::template row_sums<1>(s, sums[flip][0]);
-      r1 = rsqrtf(fmaf(s[0], over, p.eps));
+      r1 = f2(rsqrtf(fmaf(s[0], over, p.eps)));
     }
-    float v[S::N], s[1] = {0.f};
+    Raw<RT, 8> kept[S::R];
+    F2 rr = f2(0.f);
 #pragma unroll
-    for (int n = 0; n < S::N; ++n) {
-      float b = x[n / 8].get(n % 8);
+    for (int n = 0; n < S::P; ++n) {
+      F2 b = x[n / 4].get2(n % 4);
       if constexpr (POST) b = b * r1 * pw[n];
       // product and sum are rounded each, as the formula reads: with one rounding a sum could fall to the other side of a tie of the stored type
-      v[n] = to_f32(from_f32<RT>(__fadd_rn(res[n / 8].get(n % 8), __fmul_rn(b, sc[n]))));
-      s[0] = fmaf(v[n], v[n], s[0]);
+      kept[n / 4].set2(n % 4, res[n / 4].get2(n % 4) + b * sc[n]);
+      const F2 v = kept[n / 4].get2(n % 4);
+      rr = fma2(v, v, rr);
     }
-    if (live) S::template store<RT>(v, p.r, row * p.D, t, p.D);
+    if (live) S::template store<RT>(kept, p.r, row * p.D, t, p.D);
+    float s[1] = {lo(rr) + hi(rr)};
     S::template row_sums<1>(s, sums[flip][1]);
-    const float r2 = rsqrtf(fmaf(s[0], over, p.eps));
+    const F2 r2 = f2(rsqrtf(fmaf(s[0], over, p.eps)));
+    F2 y[S::P];
 #pragma unroll
-    for (int n = 0; n < S::N; ++n) v[n] = v[n] * r2 * w[n];
-    if (live) S::template store<XT>(v, p.y, row * p.D, t, p.D);
+    for (int n = 0; n < S::P; ++n) y[n] = kept[n / 4].get2(n % 4) * r2 * w[n];
+    if (live) S::template store<XT>(y, p.y, row * p.D, t, p.D);
   }
 }
 
@@ -130,21 +135,17 @@ __global__ void __launch_bounds__(S::kThreads, residual_ctas<S>(true)) residual_
   };
   if constexpr (Ring::kOn)
     for (int i = 0; i < Ring::kStages - 1; ++i) fetch(i);
-  constexpr int NB = BRANCH == 2 ? S::N : 1, NS = BRANCH >= 1 ? S::N : 1;
-  float w[S::N], sc[S::N], acc_w[S::N], acc_q[NS];      // sc: scale, times post_weight where there is one
+  F2 w[S::P], sc[S::P], acc_w[S::P], acc_q[S::P];      // sc: scale, times post_weight where there is one
   S::template vector<XT>(w, p.w, p.w_f32, t, p.D, 0.f);
   S::template vector<XT>(sc, p.scale, p.w_f32, t, p.D, p.scale_value);
   if constexpr (BRANCH == 2) {
-    float pw[NB];
+    F2 pw[S::P];
     S::template vector<XT>(pw, p.pw, p.w_f32, t, p.D, 0.f);
 #pragma unroll
-    for (int n = 0; n < S::N; ++n) sc[n] *= pw[n];
+    for (int n = 0; n < S::P; ++n) sc[n] = sc[n] * pw[n];
   }
 #pragma unroll
-  for (int n = 0; n < S::N; ++n) {
-    acc_w[n] = 0.f;
-    if constexpr (BRANCH >= 1) acc_q[n] = 0.f;
-  }
+  for (int n = 0; n < S::P; ++n) acc_w[n] = acc_q[n] = f2(0.f);
   const float over = 1.f / p.D;
   int flip = 0, stage = 0;
   for (long long row = first, base = first - threadIdx.x / S::T; base < p.rows; row += step, base += step, flip ^= 1) {
@@ -178,39 +179,45 @@ __global__ void __launch_bounds__(S::kThreads, residual_ctas<S>(true)) residual_
       }
     }
     constexpr int K = BRANCH == 2 ? 3 : 2;
-    float s[K] = {};
+    F2 sum[3] = {f2(0.f), f2(0.f), f2(0.f)};
 #pragma unroll
-    for (int n = 0; n < S::N; ++n) {
-      const float rv = r[n / 8].get(n % 8);
-      s[0] = fmaf(rv, rv, s[0]);
-      s[1] = fmaf(dy[n / 8].get(n % 8) * w[n], rv, s[1]);
-      if constexpr (BRANCH == 2) s[2] = fmaf(x[n / 8].get(n % 8), x[n / 8].get(n % 8), s[2]);
+    for (int n = 0; n < S::P; ++n) {
+      const F2 rv = r[n / 4].get2(n % 4);
+      sum[0] = fma2(rv, rv, sum[0]);
+      sum[1] = fma2(dy[n / 4].get2(n % 4) * w[n], rv, sum[1]);
+      if constexpr (BRANCH == 2) sum[2] = fma2(x[n / 4].get2(n % 4), x[n / 4].get2(n % 4), sum[2]);
     }
-    S::template row_sums<K>(s, sums[flip][0]);
-    const float r2 = rsqrtf(fmaf(s[0], over, p.eps)), c2 = s[1] * over * r2 * r2;
-    float r1 = 1.f;
-    if constexpr (BRANCH == 2) r1 = rsqrtf(fmaf(s[2], over, p.eps));
-    float d[S::N], q[1] = {0.f};
+    float s[K];
 #pragma unroll
-    for (int n = 0; n < S::N; ++n) {
-      const float rv = r[n / 8].get(n % 8), dyv = dy[n / 8].get(n % 8);
-      acc_w[n] = fmaf(dyv, rv * r2, acc_w[n]);
-      d[n] = fmaf(r2, dyv * w[n] - rv * c2, dr[n / 8].get(n % 8));
-      if constexpr (BRANCH >= 1) {
-        const float dn = d[n] * (BRANCH == 2 ? x[n / 8].get(n % 8) * r1 : x[n / 8].get(n % 8));
-        acc_q[n] += dn;
-        if constexpr (BRANCH == 2) q[0] = fmaf(dn, sc[n], q[0]);
+    for (int k = 0; k < K; ++k) s[k] = lo(sum[k]) + hi(sum[k]);
+    S::template row_sums<K>(s, sums[flip][0]);
+    const float root = rsqrtf(fmaf(s[0], over, p.eps));
+    const F2 r2 = f2(root), c2 = f2(-s[1] * over * root * root);
+    F2 r1 = f2(1.f);
+    if constexpr (BRANCH == 2) r1 = f2(rsqrtf(fmaf(s[2], over, p.eps)));
+    F2 d[S::P], qq = f2(0.f);
+#pragma unroll
+    for (int n = 0; n < S::P; ++n) {
+      const F2 rv = r[n / 4].get2(n % 4), dyv = dy[n / 4].get2(n % 4);
+      acc_w[n] = fma2(dyv, rv * r2, acc_w[n]);
+      d[n] = fma2(r2, fma2(rv, c2, dyv * w[n]), dr[n / 4].get2(n % 4));
+      if constexpr (BRANCH == 1) acc_q[n] = fma2(d[n], x[n / 4].get2(n % 4), acc_q[n]);
+      if constexpr (BRANCH == 2) {
+        const F2 dn = d[n] * (x[n / 4].get2(n % 4) * r1);
+        acc_q[n] = acc_q[n] + dn;
+        qq = fma2(dn, sc[n], qq);
       }
     }
     if (live && p.dres) S::template store<RT>(d, p.dres, row * p.D, t, p.D);
     if constexpr (BRANCH == 2) {
+      float q[1] = {lo(qq) + hi(qq)};
       S::template row_sums<1>(q, sums[flip][1]);
-      const float c1 = q[0] * over * r1;
+      const F2 c1 = f2(-q[0] * over) * r1;
 #pragma unroll
-      for (int n = 0; n < S::N; ++n) d[n] = r1 * (d[n] * sc[n] - x[n / 8].get(n % 8) * c1);
+      for (int n = 0; n < S::P; ++n) d[n] = r1 * fma2(x[n / 4].get2(n % 4), c1, d[n] * sc[n]);
     } else {
 #pragma unroll
-      for (int n = 0; n < S::N; ++n) d[n] *= sc[n];
+      for (int n = 0; n < S::P; ++n) d[n] = d[n] * sc[n];
     }
     if (live && p.dx) S::template store<XT>(d, p.dx, row * p.D, t, p.D);
   }
@@ -219,14 +226,14 @@ __global__ void __launch_bounds__(S::kThreads, residual_ctas<S>(true)) residual_
   float* columns = reinterpret_cast<float*>(smem);
   if (p.at[0] >= 0) S::column_share(acc_w, line + static_cast<long long>(p.at[0]) * p.D, columns, t, p.D);
   if constexpr (BRANCH == 2) {
-    float v[S::N];
+    F2 v[S::P];
     S::template vector<XT>(v, p.scale, p.w_f32, t, p.D, p.scale_value);
 #pragma unroll
-    for (int n = 0; n < S::N; ++n) v[n] *= acc_q[n];
+    for (int n = 0; n < S::P; ++n) v[n] = v[n] * acc_q[n];
     if (p.at[1] >= 0) S::column_share(v, line + static_cast<long long>(p.at[1]) * p.D, columns, t, p.D);
     S::template vector<XT>(v, p.pw, p.w_f32, t, p.D, 0.f);
 #pragma unroll
-    for (int n = 0; n < S::N; ++n) acc_q[n] *= v[n];
+    for (int n = 0; n < S::P; ++n) acc_q[n] = acc_q[n] * v[n];
   }
   if constexpr (BRANCH >= 1)
     if (p.at[2] >= 0) S::column_share(acc_q, line + static_cast<long long>(p.at[2]) * p.D, columns, t, p.D);
