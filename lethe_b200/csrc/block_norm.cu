@@ -7,6 +7,7 @@
 // Bound by HBM: 6 bytes a value forward and 10 backward in 16 bits.  mean(dn n) = r mean(dn x), so both row sums of the backward
 // are of what was loaded and are formed together.
 #include "block_norm.cuh"
+#include "umma.cuh"
 
 namespace lg {
 
@@ -40,29 +41,36 @@ __device__ __forceinline__ F2 logistic(F2 z) {
   return f2(a, b);
 }
 
-// CTAs on an SM: registers (64 a thread forward, 80 backward)
-template <typename S> constexpr int gated_ctas(bool backward) { return (backward ? 768 : 1024) / S::kThreads / S::R > 0 ? (backward ? 768 : 1024) / S::kThreads / S::R : 1; }
+// CTAs on an SM: registers (64 a thread forward, 80 backward; twice that with two pieces)
+template <typename S> constexpr int gated_ctas(bool backward) { return S::R > 1 ? 512 / S::kThreads : (backward ? 768 : 1024) / S::kThreads; }
 template <int XT, typename S, bool BACK> using GatedRing = RowRing<S, (BACK ? 3 : 2) * S::R * 8 * elem_bytes(XT), gated_ctas<S>(BACK)>;
 
 template <int XT, typename S>
 __global__ void __launch_bounds__(S::kThreads, gated_ctas<S>(false)) gated_norm_kernel(const GatedProblem p) {
   using Ring = GatedRing<XT, S, false>;
   constexpr int kX = 0, kZ = S::R * elem_bytes(XT) / 2;
-  __shared__ float sums[2][1][S::kWarps];
+  __shared__ __align__(16) float sums[2][1][S::kWarps];
   extern __shared__ __align__(16) unsigned char smem[];
   const Ring ring(smem);
   const int t = threadIdx.x % S::T;
-  const long long first = static_cast<long long>(blockIdx.x) * S::kRows + threadIdx.x / S::T, step = static_cast<long long>(gridDim.x) * S::kRows;
-  RowWalk ahead(first, step, p.inner);      // of the copies, or of the rows themselves
-  long long far = first;
+  const Turns turns(p.rows, S::kRows, threadIdx.x / S::T);
+  RowWalk walk(turns, p.inner);
+  WalkPtr px(p.x, walk, p.xo, p.xi, elem_bytes(XT)), pz(p.z, walk, p.zo, p.zi, elem_bytes(XT));      // of the copies, or of the rows themselves
+  RowPtr py(p.y, turns, p.D, elem_bytes(XT));
+  const auto next = [&] {
+    const bool round = walk.next();
+    px.next(round);
+    pz.next(round);
+  };
+  int far = 0;
   const auto fetch = [&](int stage) {
-    if (far < p.rows) {
-      ring.template copy<XT, kX>(stage, p.x, ahead.at(p.xo, p.xi), t, p.D);
-      ring.template copy<XT, kZ>(stage, p.z, ahead.at(p.zo, p.zi), t, p.D);
+    if (far < turns.mine) {
+      ring.template copy<XT, kX>(stage, px.p, t, p.D);
+      ring.template copy<XT, kZ>(stage, pz.p, t, p.D);
     }
     Ring::commit();
-    far += step;
-    ahead.next();
+    ++far;
+    next();
   };
   if constexpr (Ring::kOn)
     for (int i = 0; i < Ring::kStages - 1; ++i) fetch(i);
@@ -70,9 +78,8 @@ __global__ void __launch_bounds__(S::kThreads, gated_ctas<S>(false)) gated_norm_
   S::template vector<XT>(w, p.w, p.w_f32, t, p.D, 0.f);
   const float over = 1.f / p.D;
   int flip = 0, stage = 0;
-  // every thread of a CTA takes as many turns: row sums are collective
-  for (long long row = first, base = first - threadIdx.x / S::T; base < p.rows; row += step, base += step, flip ^= 1) {
-    const bool live = row < p.rows;
+  for (int turn = 0; turn < turns.all; ++turn, flip ^= 1, py.next()) {
+    const bool live = turn < turns.mine;
     Raw<XT, 8> x[S::R], z[S::R];
     if constexpr (Ring::kOn) {
       Ring::wait();
@@ -87,10 +94,10 @@ __global__ void __launch_bounds__(S::kThreads, gated_ctas<S>(false)) gated_norm_
         z[i].zero();
       }
       if (live) {
-        S::template load<XT>(x, p.x, ahead.at(p.xo, p.xi), t, p.D);
-        S::template load<XT>(z, p.z, ahead.at(p.zo, p.zi), t, p.D);
+        S::template load<XT>(x, px.p, t, p.D);
+        S::template load<XT>(z, pz.p, t, p.D);
       }
-      ahead.next();
+      next();
     }
     F2 xx = f2(0.f);
 #pragma unroll
@@ -104,7 +111,7 @@ __global__ void __launch_bounds__(S::kThreads, gated_ctas<S>(false)) gated_norm_
       const F2 zv = z[n / 4].get2(n % 4), sg = logistic<XT>(zv);
       y[n] = x[n / 4].get2(n % 4) * r * w[n] * (p.silu ? zv * sg : sg);
     }
-    if (live) S::template store<XT>(y, p.y, row * p.D, t, p.D);
+    if (live) S::template store<XT>(y, py.p, t, p.D);
   }
 }
 
@@ -112,22 +119,30 @@ template <int XT, typename S>
 __global__ void __launch_bounds__(S::kThreads, gated_ctas<S>(true)) gated_norm_vjp_kernel(const GatedProblem p) {
   using Ring = GatedRing<XT, S, true>;
   constexpr int kEach = S::R * elem_bytes(XT) / 2, kX = 0, kZ = kEach, kD = 2 * kEach;
-  __shared__ float sums[2][2][S::kWarps];
+  __shared__ __align__(16) float sums[2][2][S::kWarps];
   extern __shared__ __align__(16) unsigned char smem[];
   const Ring ring(smem);
   const int t = threadIdx.x % S::T;
-  const long long first = static_cast<long long>(blockIdx.x) * S::kRows + threadIdx.x / S::T, step = static_cast<long long>(gridDim.x) * S::kRows;
-  RowWalk ahead(first, step, p.inner);
-  long long far = first;
+  const Turns turns(p.rows, S::kRows, threadIdx.x / S::T);
+  RowWalk walk(turns, p.inner);
+  WalkPtr px(p.x, walk, p.xo, p.xi, elem_bytes(XT)), pz(p.z, walk, p.zo, p.zi, elem_bytes(XT));
+  RowPtr pd(p.dy, turns, p.D, elem_bytes(XT)), pdx(p.dx, turns, p.D, elem_bytes(XT)), pdz(p.dz, turns, p.D, elem_bytes(XT));
+  const auto next = [&] {
+    const bool round = walk.next();
+    px.next(round);
+    pz.next(round);
+    pd.next();
+  };
+  int far = 0;
   const auto fetch = [&](int stage) {
-    if (far < p.rows) {
-      ring.template copy<XT, kX>(stage, p.x, ahead.at(p.xo, p.xi), t, p.D);
-      ring.template copy<XT, kZ>(stage, p.z, ahead.at(p.zo, p.zi), t, p.D);
-      ring.template copy<XT, kD>(stage, p.dy, far * p.D, t, p.D);
+    if (far < turns.mine) {
+      ring.template copy<XT, kX>(stage, px.p, t, p.D);
+      ring.template copy<XT, kZ>(stage, pz.p, t, p.D);
+      ring.template copy<XT, kD>(stage, pd.p, t, p.D);
     }
     Ring::commit();
-    far += step;
-    ahead.next();
+    ++far;
+    next();
   };
   if constexpr (Ring::kOn)
     for (int i = 0; i < Ring::kStages - 1; ++i) fetch(i);
@@ -137,8 +152,8 @@ __global__ void __launch_bounds__(S::kThreads, gated_ctas<S>(true)) gated_norm_v
   for (int n = 0; n < S::P; ++n) acc[n] = f2(0.f);
   const float over = 1.f / p.D;
   int flip = 0, stage = 0;
-  for (long long row = first, base = first - threadIdx.x / S::T; base < p.rows; row += step, base += step, flip ^= 1) {
-    const bool live = row < p.rows;
+  for (int turn = 0; turn < turns.all; ++turn, flip ^= 1, pdx.next(), pdz.next()) {
+    const bool live = turn < turns.mine;
     Raw<XT, 8> x[S::R], z[S::R], d[S::R];
     if constexpr (Ring::kOn) {
       Ring::wait();
@@ -158,11 +173,11 @@ __global__ void __launch_bounds__(S::kThreads, gated_ctas<S>(true)) gated_norm_v
     }
     if constexpr (!Ring::kOn) {
       if (live) {
-        S::template load<XT>(x, p.x, ahead.at(p.xo, p.xi), t, p.D);
-        S::template load<XT>(z, p.z, ahead.at(p.zo, p.zi), t, p.D);
-        S::template load<XT>(d, p.dy, row * p.D, t, p.D);
+        S::template load<XT>(x, px.p, t, p.D);
+        S::template load<XT>(z, pz.p, t, p.D);
+        S::template load<XT>(d, pd.p, t, p.D);
       }
-      ahead.next();
+      next();
     }
     F2 xx = f2(0.f), dx_sum = f2(0.f), dn[S::P], slope[S::P];
 #pragma unroll
@@ -187,11 +202,13 @@ __global__ void __launch_bounds__(S::kThreads, gated_ctas<S>(true)) gated_norm_v
       slope[n] = slope[n] * (xr * w[n]);
     }
     if (live) {
-      if (p.dx) S::template store<XT>(dx, p.dx, row * p.D, t, p.D);
-      if (p.dz) S::template store<XT>(slope, p.dz, row * p.D, t, p.D);
+      if (p.dx) S::template store<XT>(dx, pdx.p, t, p.D);
+      if (p.dz) S::template store<XT>(slope, pdz.p, t, p.D);
     }
   }
-  if (p.part) S::column_share(acc, p.part + static_cast<long long>(blockIdx.x) * p.D, reinterpret_cast<float*>(smem), t, p.D);
+  if (!p.part) return;
+  griddep_launch();      // (the kernel that adds the shares waits for their stores)
+  S::column_share(acc, p.part + static_cast<long long>(blockIdx.x) * p.D, reinterpret_cast<float*>(smem), t, p.D);
 }
 
 // 32 columns a CTA; a warp takes every 32nd share, the warps' sums are added in their order.
@@ -200,6 +217,7 @@ __global__ void __launch_bounds__(1024) column_sums_kernel(const ColumnSums c) {
   __shared__ float s[32][33];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, v = blockIdx.y, col = blockIdx.x * 32 + lane;
   float a = 0.f;
+  griddep_wait();
   if (col < c.D) {
     const float* p = c.part + static_cast<long long>(v) * c.D + col;
     const long long line = static_cast<long long>(c.vectors) * c.D;
@@ -219,14 +237,14 @@ __global__ void __launch_bounds__(1024) column_sums_kernel(const ColumnSums c) {
 
 int launch_column_sums(const ColumnSums& c, cudaStream_t st) {
   return by_x_type(c.x_type, [&](auto x) {
-    column_sums_kernel<x.value><<<dim3((c.D + 31) / 32, c.vectors), 1024, 0, st>>>(c);
-    return launched_ok();
+    const cudaError_t e = launch_dependent(column_sums_kernel<x.value>, dim3((c.D + 31) / 32, c.vectors), dim3(1024), 0, st, c);
+    return e == cudaSuccess ? kOk : kErrLaunch;
   });
 }
 
 static int gated_problem(const LetheGdnGatedNormArgs* a, GatedProblem* p, bool backward) {
   if (!a) return kErrNull;
-  if (a->rows <= 0 || a->inner <= 0 || a->D <= 0 || a->D > kNormMaxD || !norm_types_ok(a->x_type, a->w_type) || !(a->eps >= 0.f)) return kErrDims;
+  if (a->rows <= 0 || a->inner <= 0 || a->inner > INT32_MAX || a->D <= 0 || a->D > kNormMaxD || !norm_types_ok(a->x_type, a->w_type) || !(a->eps >= 0.f)) return kErrDims;
   if (!a->x || !a->gate || !a->weight || (!backward && !a->y) || (backward && !a->dy)) return kErrNull;
   *p = {a->rows, a->inner, a->D, a->w_type == LETHE_F32, a->silu, a->eps, a->x, a->x_outer, a->x_inner, a->gate, a->gate_outer, a->gate_inner,
         a->weight, a->y, a->dy, a->dx, a->dgate, nullptr};

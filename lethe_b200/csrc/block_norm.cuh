@@ -1,7 +1,7 @@
 // Rows of the norms in front of and behind a block: who holds what of a row, row sums, column sums over rows.
 //
 // A row of D values is held by T threads with R pieces of 8 values each (T R 8 >= D) and stays in registers from its loads to its
-// stores.  T <= 32: a CTA of 256 threads has 256 / T rows at a time, sums are butterflies.  T > 32: a CTA of T threads has one
+// stores; a CTA has one row at a time, or as many as fill 256 threads.  Sums over up to a warp are butterflies, beyond that the warps of a
 // row, sums go through shared memory.  CTAs go over the rows with the grid's stride, so that what belongs to a column (weights,
 // sums for their gradients) stays in registers as well, and the next rows are under way by asynchronous copies (RowRing): with loads at
 // the head of each turn instead, residual_norm of 16384 x 4096 bf16 took 132 us forward and 267 backward.  Sums over rows: a CTA's share in the order of its rows, the CTAs'
@@ -24,15 +24,15 @@ template <int T_, int R_, bool VEC_>
 struct RowShape {
   static constexpr int T = T_, R = R_, N = R_ * 8, P = N / 2;      // values and pairs of a thread
   static constexpr bool VEC = VEC_;
-  static constexpr int kThreads = T > 32 ? T : 256, kRows = kThreads / T;
+  static constexpr int kThreads = T > 256 ? T : 256, kRows = kThreads / T;
   static constexpr int kWarps = kThreads / 32;
   static constexpr int kColumnBytes = kRows > 1 ? kThreads * N * 4 : 0;      // what column_share wants
   // column of value n (of N) that thread t of a row holds
   __device__ __forceinline__ static int col(int t, int n) { return VEC ? ((n / 8) * T + t) * 8 + n % 8 : n * T + t; }
 
   template <int TY>
-  __device__ __forceinline__ static void load(Raw<TY, 8> (&r)[R], const void* base, long long row, int t, int D) {
-    const typename Elem<TY>::T* p = static_cast<const typename Elem<TY>::T*>(base) + row;
+  __device__ __forceinline__ static void load(Raw<TY, 8> (&r)[R], const void* row, int t, int D) {
+    const typename Elem<TY>::T* p = static_cast<const typename Elem<TY>::T*>(row);
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       r[i].zero();
@@ -46,8 +46,8 @@ struct RowShape {
     }
   }
   template <int TY>
-  __device__ __forceinline__ static void store(const Raw<TY, 8> (&r)[R], void* base, long long row, int t, int D) {
-    typename Elem<TY>::T* p = static_cast<typename Elem<TY>::T*>(base) + row;
+  __device__ __forceinline__ static void store(const Raw<TY, 8> (&r)[R], void* row, int t, int D) {
+    typename Elem<TY>::T* p = static_cast<typename Elem<TY>::T*>(row);
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       if constexpr (VEC) {
@@ -60,11 +60,11 @@ struct RowShape {
     }
   }
   template <int TY>
-  __device__ __forceinline__ static void store(const F2 (&v)[P], void* base, long long row, int t, int D) {
+  __device__ __forceinline__ static void store(const F2 (&v)[P], void* row, int t, int D) {
     Raw<TY, 8> r[R];
 #pragma unroll
     for (int n = 0; n < P; ++n) r[n / 4].set2(n % 4, v[n]);
-    store<TY>(r, base, row, t, D);
+    store<TY>(r, row, t, D);
   }
   // a vector of D values (weight, scale), fp32 or XT; `none` where there is no vector
   template <int XT>
@@ -85,16 +85,33 @@ struct RowShape {
 #pragma unroll
       for (int k = 0; k < K; ++k) s[k] += __shfl_xor_sync(0xffffffffu, s[k], m);
     if constexpr (T > 32) {
-      if (threadIdx.x % 32 == 0)
+      constexpr int kOfRow = T / 32;
+      const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+      if (lane == 0)
 #pragma unroll
-        for (int k = 0; k < K; ++k) buf[k][threadIdx.x / 32] = s[k];
+        for (int k = 0; k < K; ++k) buf[k][warp] = s[k];
       __syncthreads();
+      // one sum: every thread adds what the warps left, four chains of it; several: each lane one warp's, and butterflies (16384 x 4096 bf16
+      // in us, added / butterflies: forward, sums one by one, 96 / 103; backward, three together, 161 / 150)
+      if constexpr (K == 1 && kOfRow >= 4) {
+        const float4* p = reinterpret_cast<const float4*>(&buf[0][warp / kOfRow * kOfRow]);
+        float4 a = p[0];
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        float a = 0.f;
+        for (int i = 1; i < kOfRow / 4; ++i) {
+          const float4 c = p[i];
+          a.x += c.x;
+          a.y += c.y;
+          a.z += c.z;
+          a.w += c.w;
+        }
+        s[0] = (a.x + a.y) + (a.z + a.w);
+      } else {
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) a += buf[k][w];
-        s[k] = a;
+        for (int k = 0; k < K; ++k) s[k] = buf[k][warp / kOfRow * kOfRow + lane % kOfRow];
+#pragma unroll
+        for (int m = kOfRow / 2; m >= 1; m >>= 1)
+#pragma unroll
+          for (int k = 0; k < K; ++k) s[k] += __shfl_xor_sync(0xffffffffu, s[k], m);
       }
     }
   }
@@ -144,9 +161,9 @@ template <typename S, int B, int CTAS> struct RowRing {
   }
   // this thread's pieces of a row to cells AT and on of a stage
   template <int TY, int AT>
-  __device__ __forceinline__ void copy(int stage, const void* tensor, long long row, int t, int D) const {
+  __device__ __forceinline__ void copy(int stage, const void* row, int t, int D) const {
     constexpr int kEach = elem_bytes(TY) / 2;
-    const typename Elem<TY>::T* p = static_cast<const typename Elem<TY>::T*>(tensor) + row;
+    const typename Elem<TY>::T* p = static_cast<const typename Elem<TY>::T*>(row);
 #pragma unroll
     for (int i = 0; i < S::R; ++i)
       if ((i * S::T + t) * 8 < D)
@@ -174,27 +191,57 @@ template <typename S, int B, int CTAS> struct RowRing {
   __device__ __forceinline__ static void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kOn ? kStages - 2 : 0) : "memory"); }
 };
 
-// Walks the rows of a tensor with two strides, row r = (r / inner, r % inner), by a fixed step: one division at the start.
+// The turns of a thread: rows first, first + step, ...; all threads of a CTA take `all` of them, since row sums are collective, and
+// have a row in the first `mine`.
+struct Turns {
+  long long first, step;
+  int all, mine;
+  __device__ __forceinline__ Turns(long long rows, int rows_per_cta, int slot) {
+    const long long base = static_cast<long long>(blockIdx.x) * rows_per_cta;
+    first = base + slot;
+    step = static_cast<long long>(gridDim.x) * rows_per_cta;
+    all = base < rows ? static_cast<int>((rows - base + step - 1) / step) : 0;
+    mine = first < rows ? static_cast<int>((rows - first + step - 1) / step) : 0;
+  }
+};
+// The place of a tensor's row, from turn to turn: additions only.
+struct RowPtr {
+  char* p;
+  long long step;
+  __device__ __forceinline__ RowPtr(const void* base, const Turns& t, long long stride, int bytes)
+      : p(const_cast<char*>(static_cast<const char*>(base)) + t.first * stride * bytes), step(t.step * stride * bytes) {}
+  __device__ __forceinline__ void next() { p += step; }
+};
+// Rows (o, i), i below `inner`, of tensors with a stride for each of the two.
 struct RowWalk {
-  long long o, i, step_o, step_i, inner;
-  __device__ __forceinline__ RowWalk(long long first, long long step, long long inner_) : inner(inner_) {
-    o = first / inner;
-    i = first - o * inner;
-    step_o = step / inner;
-    step_i = step - step_o * inner;
+  int i, step_i, inner;
+  long long o, step_o;
+  __device__ __forceinline__ RowWalk(const Turns& t, long long inner_) : inner(static_cast<int>(inner_)) {
+    o = t.first / inner_;
+    i = static_cast<int>(t.first - o * inner_);
+    step_o = t.step / inner_;
+    step_i = static_cast<int>(t.step - step_o * inner_);
   }
-  __device__ __forceinline__ void next() {
-    o += step_o;
+  __device__ __forceinline__ bool next() {      // whether i has come round
     i += step_i;
-    if (i >= inner) {
-      i -= inner;
-      ++o;
-    }
+    const bool round = i >= inner;
+    if (round) i -= inner;
+    return round;
   }
-  __device__ __forceinline__ long long at(long long outer_stride, long long inner_stride) const { return o * outer_stride + i * inner_stride; }
+};
+struct WalkPtr {
+  char* p;
+  long long step, round;
+  __device__ __forceinline__ WalkPtr(const void* base, const RowWalk& w, long long outer, long long inner, int bytes)
+      : p(const_cast<char*>(static_cast<const char*>(base)) + (w.o * outer + w.i * inner) * bytes), step((w.step_o * outer + w.step_i * inner) * bytes),
+        round((outer - w.inner * inner) * bytes) {}
+  __device__ __forceinline__ void next(bool come_round) { p += step + (come_round ? round : 0); }
 };
 
-// f(RowShape) for rows of D values.  Where pieces of 8 cannot be loaded as such, fewer shapes: these loads are what bounds.
+// f(RowShape) for rows of D values: one piece of 8 a thread as far as a CTA goes.  With two, what a row costs beside its values (sums, places, loop)
+// is shared by 16 of them, but half the threads are there to cover one another (us, one / two: gated 4 x 4096 x 16 x 128 bf16 forward
+// 37.0 / 38.4, backward 66 / 71; residual 16384 x 4096 96 / 104; 64 rows of 2048 3.9 / 6.6).  Where pieces of 8 cannot be loaded as
+// such, fewer shapes: these loads are what bounds.
 template <typename F>
 int by_row_shape(int D, bool vec, F&& f) {
   if (!vec) {
@@ -205,7 +252,7 @@ int by_row_shape(int D, bool vec, F&& f) {
   if (D <= 64) return f(RowShape<8, 1, true>());
   if (D <= 128) return f(RowShape<16, 1, true>());
   if (D <= 256) return f(RowShape<32, 1, true>());
-  if (D <= 512) return f(RowShape<32, 2, true>());
+  if (D <= 512) return f(RowShape<64, 1, true>());
   if (D <= 1024) return f(RowShape<128, 1, true>());
   if (D <= 2048) return f(RowShape<256, 1, true>());
   if (D <= 4096) return f(RowShape<512, 1, true>());

@@ -8,6 +8,7 @@
 // Bound by HBM.  The backward takes n2 from r as it was stored, so it reads the stream once and x only where the branch has
 // something to learn.
 #include "block_norm.cuh"
+#include "umma.cuh"
 
 namespace lg {
 
@@ -27,8 +28,8 @@ struct ResidualProblem {
   int vectors, at[3];       // their number, and the place of each (-1: not wanted)
 };
 
-// CTAs on an SM: registers (64 a thread forward, 128 backward)
-template <typename S> constexpr int residual_ctas(bool backward) { return (backward ? 512 : 1024) / S::kThreads / (backward ? 1 : S::R); }
+// CTAs on an SM: registers (64 a thread forward, 128 backward and with two pieces)
+template <typename S> constexpr int residual_ctas(bool backward) { return (backward || S::R > 1 ? 512 : 1024) / S::kThreads; }
 template <int XT, int RT, typename S> using ResidualRing = RowRing<S, S::R * 8 * (elem_bytes(XT) + elem_bytes(RT)), residual_ctas<S>(false)>;
 template <int XT, int RT, typename S, int BRANCH>
 using ResidualRingBack = RowRing<S, S::R * 8 * (elem_bytes(XT) * (BRANCH ? 2 : 1) + 2 * elem_bytes(RT)), residual_ctas<S>(true)>;
@@ -37,19 +38,23 @@ template <int XT, int RT, typename S, bool POST>
 __global__ void __launch_bounds__(S::kThreads, residual_ctas<S>(false)) residual_norm_kernel(const ResidualProblem p) {
   using Ring = ResidualRing<XT, RT, S>;
   constexpr int kX = 0, kRes = S::R * elem_bytes(XT) / 2;
-  __shared__ float sums[2][2][1][S::kWarps];
+  __shared__ __align__(16) float sums[2][2][1][S::kWarps];
   extern __shared__ __align__(16) unsigned char smem[];
   const Ring ring(smem);
   const int t = threadIdx.x % S::T;
-  const long long first = static_cast<long long>(blockIdx.x) * S::kRows + threadIdx.x / S::T, step = static_cast<long long>(gridDim.x) * S::kRows;
-  long long far = first;
+  const Turns turns(p.rows, S::kRows, threadIdx.x / S::T);
+  RowPtr px(p.x, turns, p.x_stride, elem_bytes(XT)), pres(p.res, turns, p.res_stride, elem_bytes(RT));      // of the copies, or of the rows themselves
+  RowPtr pr(p.r, turns, p.D, elem_bytes(RT)), py(p.y, turns, p.D, elem_bytes(XT));
+  int far = 0;
   const auto fetch = [&](int stage) {
-    if (far < p.rows) {
-      ring.template copy<XT, kX>(stage, p.x, far * p.x_stride, t, p.D);
-      if (p.res) ring.template copy<RT, kRes>(stage, p.res, far * p.res_stride, t, p.D);      // (else the cells stay zeros)
+    if (far < turns.mine) {
+      ring.template copy<XT, kX>(stage, px.p, t, p.D);
+      if (p.res) ring.template copy<RT, kRes>(stage, pres.p, t, p.D);      // (else the cells stay zeros)
     }
     Ring::commit();
-    far += step;
+    ++far;
+    px.next();
+    pres.next();
   };
   if constexpr (Ring::kOn)
     for (int i = 0; i < Ring::kStages - 1; ++i) fetch(i);
@@ -59,8 +64,8 @@ __global__ void __launch_bounds__(S::kThreads, residual_ctas<S>(false)) residual
   if constexpr (POST) S::template vector<XT>(pw, p.pw, p.w_f32, t, p.D, 0.f);
   const float over = 1.f / p.D;
   int flip = 0, stage = 0;
-  for (long long row = first, base = first - threadIdx.x / S::T; base < p.rows; row += step, base += step, flip ^= 1) {
-    const bool live = row < p.rows;
+  for (int turn = 0; turn < turns.all; ++turn, flip ^= 1, pr.next(), py.next()) {
+    const bool live = turn < turns.mine;
     Raw<XT, 8> x[S::R];
     Raw<RT, 8> res[S::R];
     if constexpr (Ring::kOn) {
@@ -76,9 +81,11 @@ __global__ void __launch_bounds__(S::kThreads, residual_ctas<S>(false)) residual
         res[i].zero();
       }
       if (live) {
-        S::template load<XT>(x, p.x, row * p.x_stride, t, p.D);
-        if (p.res) S::template load<RT>(res, p.res, row * p.res_stride, t, p.D);
+        S::template load<XT>(x, px.p, t, p.D);
+        if (p.res) S::template load<RT>(res, pres.p, t, p.D);
       }
+      px.next();
+      pres.next();
     }
     F2 r1 = f2(1.f);
     if constexpr (POST) {
@@ -100,14 +107,14 @@ __global__ void __launch_bounds__(S::kThreads, residual_ctas<S>(false)) residual
       const F2 v = kept[n / 4].get2(n % 4);
       rr = fma2(v, v, rr);
     }
-    if (live) S::template store<RT>(kept, p.r, row * p.D, t, p.D);
+    if (live) S::template store<RT>(kept, pr.p, t, p.D);
     float s[1] = {lo(rr) + hi(rr)};
     S::template row_sums<1>(s, sums[flip][1]);
     const F2 r2 = f2(rsqrtf(fmaf(s[0], over, p.eps)));
     F2 y[S::P];
 #pragma unroll
     for (int n = 0; n < S::P; ++n) y[n] = kept[n / 4].get2(n % 4) * r2 * w[n];
-    if (live) S::template store<XT>(y, p.y, row * p.D, t, p.D);
+    if (live) S::template store<XT>(y, py.p, t, p.D);
   }
 }
 
@@ -117,21 +124,30 @@ template <int XT, int RT, typename S, int BRANCH>
 __global__ void __launch_bounds__(S::kThreads, residual_ctas<S>(true)) residual_norm_vjp_kernel(const ResidualProblem p) {
   using Ring = ResidualRingBack<XT, RT, S, BRANCH>;
   constexpr int kR = 0, kDr = S::R * elem_bytes(RT) / 2, kDy = 2 * kDr, kX = kDy + S::R * elem_bytes(XT) / 2;
-  __shared__ float sums[2][2][3][S::kWarps];
+  __shared__ __align__(16) float sums[2][2][3][S::kWarps];
   extern __shared__ __align__(16) unsigned char smem[];
   const Ring ring(smem);
   const int t = threadIdx.x % S::T;
-  const long long first = static_cast<long long>(blockIdx.x) * S::kRows + threadIdx.x / S::T, step = static_cast<long long>(gridDim.x) * S::kRows;
-  long long far = first;
+  const Turns turns(p.rows, S::kRows, threadIdx.x / S::T);
+  RowPtr pr(p.r, turns, p.D, elem_bytes(RT)), pdr(p.dr, turns, p.D, elem_bytes(RT)), pdy(p.dy, turns, p.D, elem_bytes(XT)), px(p.x, turns, p.x_stride, elem_bytes(XT));
+  RowPtr pdres(p.dres, turns, p.D, elem_bytes(RT)), pdx(p.dx, turns, p.D, elem_bytes(XT));
+  const auto next = [&] {
+    pr.next();
+    pdr.next();
+    pdy.next();
+    if constexpr (BRANCH >= 1) px.next();
+  };
+  int far = 0;
   const auto fetch = [&](int stage) {
-    if (far < p.rows) {
-      ring.template copy<RT, kR>(stage, p.r, far * p.D, t, p.D);
-      if (p.dr) ring.template copy<RT, kDr>(stage, p.dr, far * p.D, t, p.D);
-      if (p.dy) ring.template copy<XT, kDy>(stage, p.dy, far * p.D, t, p.D);
-      if constexpr (BRANCH >= 1) ring.template copy<XT, kX>(stage, p.x, far * p.x_stride, t, p.D);
+    if (far < turns.mine) {
+      ring.template copy<RT, kR>(stage, pr.p, t, p.D);
+      if (p.dr) ring.template copy<RT, kDr>(stage, pdr.p, t, p.D);
+      if (p.dy) ring.template copy<XT, kDy>(stage, pdy.p, t, p.D);
+      if constexpr (BRANCH >= 1) ring.template copy<XT, kX>(stage, px.p, t, p.D);
     }
     Ring::commit();
-    far += step;
+    ++far;
+    next();
   };
   if constexpr (Ring::kOn)
     for (int i = 0; i < Ring::kStages - 1; ++i) fetch(i);
@@ -148,8 +164,8 @@ __global__ void __launch_bounds__(S::kThreads, residual_ctas<S>(true)) residual_
   for (int n = 0; n < S::P; ++n) acc_w[n] = acc_q[n] = f2(0.f);
   const float over = 1.f / p.D;
   int flip = 0, stage = 0;
-  for (long long row = first, base = first - threadIdx.x / S::T; base < p.rows; row += step, base += step, flip ^= 1) {
-    const bool live = row < p.rows;
+  for (int turn = 0; turn < turns.all; ++turn, flip ^= 1, pdres.next(), pdx.next()) {
+    const bool live = turn < turns.mine;
     Raw<XT, 8> x[S::R], dy[S::R];
     Raw<RT, 8> r[S::R], dr[S::R];
     if constexpr (Ring::kOn) {
@@ -172,11 +188,12 @@ __global__ void __launch_bounds__(S::kThreads, residual_ctas<S>(true)) residual_
     }
     if constexpr (!Ring::kOn) {
       if (live) {
-        S::template load<RT>(r, p.r, row * p.D, t, p.D);
-        if (p.dy) S::template load<XT>(dy, p.dy, row * p.D, t, p.D);
-        if (p.dr) S::template load<RT>(dr, p.dr, row * p.D, t, p.D);
-        if constexpr (BRANCH >= 1) S::template load<XT>(x, p.x, row * p.x_stride, t, p.D);
+        S::template load<RT>(r, pr.p, t, p.D);
+        if (p.dy) S::template load<XT>(dy, pdy.p, t, p.D);
+        if (p.dr) S::template load<RT>(dr, pdr.p, t, p.D);
+        if constexpr (BRANCH >= 1) S::template load<XT>(x, px.p, t, p.D);
       }
+      next();
     }
     constexpr int K = BRANCH == 2 ? 3 : 2;
     F2 sum[3] = {f2(0.f), f2(0.f), f2(0.f)};
@@ -208,7 +225,7 @@ __global__ void __launch_bounds__(S::kThreads, residual_ctas<S>(true)) residual_
         qq = fma2(dn, sc[n], qq);
       }
     }
-    if (live && p.dres) S::template store<RT>(d, p.dres, row * p.D, t, p.D);
+    if (live && p.dres) S::template store<RT>(d, pdres.p, t, p.D);
     if constexpr (BRANCH == 2) {
       float q[1] = {lo(qq) + hi(qq)};
       S::template row_sums<1>(q, sums[flip][1]);
@@ -219,9 +236,10 @@ __global__ void __launch_bounds__(S::kThreads, residual_ctas<S>(true)) residual_
 #pragma unroll
       for (int n = 0; n < S::P; ++n) d[n] = d[n] * sc[n];
     }
-    if (live && p.dx) S::template store<XT>(d, p.dx, row * p.D, t, p.D);
+    if (live && p.dx) S::template store<XT>(d, pdx.p, t, p.D);
   }
   if (!p.part) return;
+  griddep_launch();      // (the kernel that adds the shares waits for their stores)
   float* line = p.part + static_cast<long long>(blockIdx.x) * p.vectors * p.D;
   float* columns = reinterpret_cast<float*>(smem);
   if (p.at[0] >= 0) S::column_share(acc_w, line + static_cast<long long>(p.at[0]) * p.D, columns, t, p.D);
@@ -311,22 +329,24 @@ extern "C" int lethe_gdn_residual_norm_vjp(const LetheGdnResidualNormArgs* a, vo
                    piece_aligned(p.dy, a->x_type) && piece_aligned(p.dr, a->r_type) && piece_aligned(p.dx, a->x_type) && piece_aligned(p.dres, a->r_type);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int grid = 0;
-  const int e = by_stream_type(a->x_type, a->r_type, [&](auto x, auto r) {
-    return by_row_shape(p.D, vec, [&](auto s) {
-      using S = decltype(s);
-      grid = std::min(norm_grid(p.rows, S::kRows, residual_ctas<S>(true)), norm_parts_max(p.D));
-      static SmemAttr attr[3];
-      const auto go = [&](auto branch) {
-        constexpr int kBranch = decltype(branch)::value;
+  const auto run = [&](auto kind) {
+    constexpr int kBranch = decltype(kind)::value;
+    return by_stream_type(a->x_type, a->r_type, [&](auto x, auto r) {
+      return by_row_shape(p.D, vec, [&](auto s) {
+        using S = decltype(s);
+        grid = std::min(norm_grid(p.rows, S::kRows, residual_ctas<S>(true)), norm_parts_max(p.D));
         const auto kern = residual_norm_vjp_kernel<x.value, r.value, S, kBranch>;
         constexpr int smem = std::max(ResidualRingBack<x.value, r.value, S, kBranch>::kBytes, S::kColumnBytes);
-        if (int e = attr[kBranch].set(kern, smem)) return e;
+        static SmemAttr attr;
+        if (int e = attr.set(kern, smem)) return e;
         kern<<<grid, S::kThreads, smem, st>>>(p);
         return launched_ok();
-      };
-      return branch == 2 ? go(std::integral_constant<int, 2>()) : branch == 1 ? go(std::integral_constant<int, 1>()) : go(std::integral_constant<int, 0>());
+      });
     });
-  });
+  };
+  const int e = branch == 2   ? run(std::integral_constant<int, 2>())
+                : branch == 1 ? run(std::integral_constant<int, 1>())
+                              : run(std::integral_constant<int, 0>());
   if (e || !p.part) return e;
   c.part = p.part;
   c.parts = grid;
