@@ -13,7 +13,7 @@ namespace lg {
 
 struct GatedProblem {
   long long rows, inner;
-  int D, w_f32, silu;
+  int D, w_f32;
   float eps;
   const void* x;
   long long xo, xi;
@@ -45,7 +45,7 @@ __device__ __forceinline__ F2 logistic(F2 z) {
 template <typename S> constexpr int gated_ctas(bool backward) { return S::R > 1 ? 512 / S::kThreads : (backward ? 768 : 1024) / S::kThreads; }
 template <int XT, typename S, bool BACK> using GatedRing = RowRing<S, (BACK ? 3 : 2) * S::R * 8 * elem_bytes(XT), gated_ctas<S>(BACK)>;
 
-template <int XT, typename S>
+template <int XT, bool SILU, typename S>
 __global__ void __launch_bounds__(S::kThreads, gated_ctas<S>(false)) gated_norm_kernel(const GatedProblem p) {
   using Ring = GatedRing<XT, S, false>;
   constexpr int kX = 0, kZ = S::R * elem_bytes(XT) / 2;
@@ -109,13 +109,13 @@ __global__ void __launch_bounds__(S::kThreads, gated_ctas<S>(false)) gated_norm_
 #pragma unroll
     for (int n = 0; n < S::P; ++n) {
       const F2 zv = z[n / 4].get2(n % 4), sg = logistic<XT>(zv);
-      y[n] = x[n / 4].get2(n % 4) * r * w[n] * (p.silu ? zv * sg : sg);
+      y[n] = x[n / 4].get2(n % 4) * r * w[n] * (SILU ? zv * sg : sg);
     }
     if (live) S::template store<XT>(y, py.p, t, p.D);
   }
 }
 
-template <int XT, typename S>
+template <int XT, bool SILU, typename S>
 __global__ void __launch_bounds__(S::kThreads, gated_ctas<S>(true)) gated_norm_vjp_kernel(const GatedProblem p) {
   using Ring = GatedRing<XT, S, true>;
   constexpr int kEach = S::R * elem_bytes(XT) / 2, kX = 0, kZ = kEach, kD = 2 * kEach;
@@ -184,8 +184,8 @@ __global__ void __launch_bounds__(S::kThreads, gated_ctas<S>(true)) gated_norm_v
     for (int n = 0; n < S::P; ++n) {
       const F2 xv = x[n / 4].get2(n % 4), zv = z[n / 4].get2(n % 4), dv = d[n / 4].get2(n % 4), sg = logistic<XT>(zv);
       const F2 rest = fma2(sg, f2(-1.f), f2(1.f)), ds = dv * sg;      // 1 - s, dy s
-      dn[n] = p.silu ? ds * zv : ds;
-      slope[n] = ds * (p.silu ? fma2(zv, rest, f2(1.f)) : rest);
+      dn[n] = SILU ? ds * zv : ds;
+      slope[n] = ds * (SILU ? fma2(zv, rest, f2(1.f)) : rest);
       xx = fma2(xv, xv, xx);
       dx_sum = fma2(dn[n] * w[n], xv, dx_sum);
     }
@@ -246,7 +246,7 @@ static int gated_problem(const LetheGdnGatedNormArgs* a, GatedProblem* p, bool b
   if (!a) return kErrNull;
   if (a->rows <= 0 || a->inner <= 0 || a->inner > INT32_MAX || a->D <= 0 || a->D > kNormMaxD || !norm_types_ok(a->x_type, a->w_type) || !(a->eps >= 0.f)) return kErrDims;
   if (!a->x || !a->gate || !a->weight || (!backward && !a->y) || (backward && !a->dy)) return kErrNull;
-  *p = {a->rows, a->inner, a->D, a->w_type == LETHE_F32, a->silu, a->eps, a->x, a->x_outer, a->x_inner, a->gate, a->gate_outer, a->gate_inner,
+  *p = {a->rows, a->inner, a->D, a->w_type == LETHE_F32, a->eps, a->x, a->x_outer, a->x_inner, a->gate, a->gate_outer, a->gate_inner,
         a->weight, a->y, a->dy, a->dx, a->dgate, nullptr};
   return kOk;
 }
@@ -269,11 +269,11 @@ extern "C" int lethe_gdn_gated_norm(const LetheGdnGatedNormArgs* a, void* stream
   return by_x_type(a->x_type, [&](auto x) {
     return by_row_shape(p.D, vec, [&](auto s) {
       using S = decltype(s);
-      static SmemAttr attr;
       constexpr int smem = GatedRing<x.value, S, false>::kBytes;
-      if (int e = attr.set(gated_norm_kernel<x.value, S>, smem)) return e;
-      const int grid = norm_grid(p.rows, S::kRows, gated_ctas<S>(false));
-      gated_norm_kernel<x.value, S><<<grid, S::kThreads, smem, static_cast<cudaStream_t>(stream)>>>(p);
+      static SmemAttr attr[2];
+      const auto kern = a->silu ? gated_norm_kernel<x.value, true, S> : gated_norm_kernel<x.value, false, S>;
+      if (int e = attr[a->silu != 0].set(kern, smem)) return e;
+      kern<<<norm_grid(p.rows, S::kRows, gated_ctas<S>(false)), S::kThreads, smem, static_cast<cudaStream_t>(stream)>>>(p);
       return launched_ok();
     });
   });
@@ -299,10 +299,11 @@ extern "C" int lethe_gdn_gated_norm_vjp(const LetheGdnGatedNormArgs* a, void* st
     return by_row_shape(p.D, vec, [&](auto s) {
       using S = decltype(s);
       grid = std::min(norm_grid(p.rows, S::kRows, gated_ctas<S>(true)), norm_parts_max(p.D));
-      static SmemAttr attr;
       constexpr int smem = std::max(GatedRing<x.value, S, true>::kBytes, S::kColumnBytes);
-      if (int e = attr.set(gated_norm_vjp_kernel<x.value, S>, smem)) return e;
-      gated_norm_vjp_kernel<x.value, S><<<grid, S::kThreads, smem, st>>>(p);
+      static SmemAttr attr[2];
+      const auto kern = a->silu ? gated_norm_vjp_kernel<x.value, true, S> : gated_norm_vjp_kernel<x.value, false, S>;
+      if (int e = attr[a->silu != 0].set(kern, smem)) return e;
+      kern<<<grid, S::kThreads, smem, st>>>(p);
       return launched_ok();
     });
   });
