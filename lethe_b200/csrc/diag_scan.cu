@@ -42,6 +42,21 @@ __device__ __forceinline__ float decay_coef(float g) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * 1.4426950408889634f));
   return by_diff(g) ? g * s : e;
 }
+// the same for two at a time, in place: c[i] becomes the coefficient over c[i]
+__device__ __forceinline__ void decay_coefs(float& g0, float& g1) {
+  const F2 g = f2(g0, g1);
+  F2 s = fma2(g, f2(1.f / 720.f), f2(1.f / 120.f));
+  s = fma2(g, s, f2(1.f / 24.f));
+  s = fma2(g, s, f2(1.f / 6.f));
+  s = fma2(g, s, f2(0.5f));
+  s = g * fma2(g, s, f2(1.f));
+  const F2 t = g * f2(1.4426950408889634f);
+  float e0, e1;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(lo(t)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(hi(t)));
+  g0 = by_diff(g0) ? lo(s) : e0;
+  g1 = by_diff(g1) ? hi(s) : e1;
+}
 __device__ __forceinline__ bool is_diff(float c) { return static_cast<int>(__float_as_uint(c)) < 0; }
 // e^g h + x
 __device__ __forceinline__ float decay_step(float c, bool diff, float h, float x) {
@@ -49,6 +64,23 @@ __device__ __forceinline__ float decay_step(float c, bool diff, float h, float x
   return diff ? h + t : t;
 }
 __device__ __forceinline__ float decay_step(float c, float h, float x) { return decay_step(c, is_diff(c), h, x); }
+__device__ __forceinline__ void add_to(float& a0, float& a1, float b0, float b1) {
+  const F2 s = f2(a0, a1) + f2(b0, b1);
+  a0 = lo(s);
+  a1 = hi(s);
+}
+// two steps side by side
+__device__ __forceinline__ void decay_steps(float c0, float c1, bool diff0, bool diff1, float& h0, float& h1, float x0, float x1) {
+  const F2 t = fma2(f2(c0, c1), f2(h0, h1), f2(x0, x1));
+  h0 = diff0 ? h0 + lo(t) : lo(t);
+  h1 = diff1 ? h1 + hi(t) : hi(t);
+}
+// the same without x
+__device__ __forceinline__ void decay_over(float c0, float c1, float& h0, float& h1) {
+  const F2 t = f2(c0, c1) * f2(h0, h1);
+  h0 = is_diff(c0) ? h0 + lo(t) : lo(t);
+  h1 = is_diff(c1) ? h1 + hi(t) : hi(t);
+}
 __device__ __forceinline__ float forgotten(float c) { return is_diff(c) ? -c : 1.f - c; }      // 1 - e^g
 
 struct LookBuffer {
@@ -421,11 +453,13 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_forward_kernel(const Dia
 #pragma unroll
       for (int i = 0; i < kGroups; ++i) v[i] = part[i][ch];
 #pragma unroll
-      for (int i = 0; i < kGroups; ++i) {
+      for (int i = 0; i < kGroups; i += 2) {
         ts += v[i].x;
-        v[i].x = decay_coef(v[i].x);
-        th = decay_step(v[i].x, th, v[i].y);
+        ts += v[i + 1].x;
+        decay_coefs(v[i].x, v[i + 1].x);
       }
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) th = decay_step(v[i].x, th, v[i].y);
       if (p.tiles > 1 && !look.last) look_store(look.at(0, look.tile0 + look.n_tiles, ch), ts, th);
 #pragma unroll
       for (int i = 0; i < kGroups; ++i) part[i][ch].x = v[i].x;
@@ -460,11 +494,14 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_forward_kernel(const Dia
       const auto xr = tile.x.template take<XT>(s);
       Raw<LETHE_F32, kPer> cr;
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const float gv = gr.get(j), c = decay_coef(gv);
-        cr.w[j] = __float_as_uint(c);
-        sum[j] += gv;
-        st[j] = decay_step(c, by_diff(gv), st[j], COMP ? xr.get(j) * forgotten(c) : xr.get(j));
+      for (int j = 0; j < kPer; j += 2) {
+        const float g0 = gr.get(j), g1 = gr.get(j + 1);
+        float c0 = g0, c1 = g1;
+        decay_coefs(c0, c1);
+        cr.set2(j, c0, c1);
+        add_to(sum[j], sum[j + 1], g0, g1);
+        const float x0 = xr.get(j), x1 = xr.get(j + 1);
+        decay_steps(c0, c1, by_diff(g0), by_diff(g1), st[j], st[j + 1], COMP ? x0 * forgotten(c0) : x0, COMP ? x1 * forgotten(c1) : x1);
       }
       tile.c.put(s, cr);
     }
@@ -510,9 +547,9 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_forward_kernel(const Dia
       x.p += x.stride;
       g.p += g.stride;
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const float c = cr.get(j);
-        st[j] = decay_step(c, st[j], COMP ? xr.get(j) * forgotten(c) : xr.get(j));
+      for (int j = 0; j < kPer; j += 2) {
+        const float c0 = cr.get(j), c1 = cr.get(j + 1), x0 = xr.get(j), x1 = xr.get(j + 1);
+        decay_steps(c0, c1, is_diff(c0), is_diff(c1), st[j], st[j + 1], COMP ? x0 * forgotten(c0) : x0, COMP ? x1 * forgotten(c1) : x1);
       }
       if (s < at.live) store_token<XT, W>(packed<XT>(st), h, lane, at.room);
       h += p.D;
@@ -588,11 +625,13 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_backward_kernel(const Di
         e[i] = sh.back[n & 1][i][ch];
       }
 #pragma unroll
-      for (int i = kGroups - 1; i >= 0; --i) {
+      for (int i = 0; i < kGroups; i += 2) {
         ts += c[i];
-        c[i] = decay_coef(c[i]);
-        te = decay_step(c[i], te, e[i]);
+        ts += c[i + 1];
+        decay_coefs(c[i], c[i + 1]);
       }
+#pragma unroll
+      for (int i = kGroups - 1; i >= 0; --i) te = decay_step(c[i], te, e[i]);
       if (p.tiles > 1 && !look.last) look_store(look.at(0, look.tile0 + look.n_tiles, ch), ts, te);
 #pragma unroll
       for (int i = 0; i < kGroups; ++i) part[i][ch].x = c[i];
@@ -628,12 +667,16 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_backward_kernel(const Di
       const auto xr = tile.x.template take<XT>(s);
       Raw<LETHE_F32, kPer> cr;
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const float gv = gr.get(j);
-        c[s][j] = decay_coef(gv);
-        cr.w[j] = __float_as_uint(c[s][j]);
-        sum[j] += gv;
-        st[j] = decay_step(c[s][j], by_diff(gv), st[j], COMP ? xr.get(j) * forgotten(c[s][j]) : xr.get(j));
+      for (int j = 0; j < kPer; j += 2) {
+        const float g0 = gr.get(j), g1 = gr.get(j + 1);
+        float c0 = g0, c1 = g1;
+        decay_coefs(c0, c1);
+        cr.set2(j, c0, c1);
+        c[s][j] = c0;
+        c[s][j + 1] = c1;
+        add_to(sum[j], sum[j + 1], g0, g1);
+        const float x0 = xr.get(j), x1 = xr.get(j + 1);
+        decay_steps(c0, c1, by_diff(g0), by_diff(g1), st[j], st[j + 1], COMP ? x0 * forgotten(c0) : x0, COMP ? x1 * forgotten(c1) : x1);
       }
       tile.c.put(s, cr);
     }
@@ -641,7 +684,10 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_backward_kernel(const Di
     for (int s = S - 1; s >= 0; --s) {
       const auto dr = tile.d.template take<XT>(s);
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) e[j] = decay_step(c[s][j], dr.get(j) + e[j], 0.f);
+      for (int j = 0; j < kPer; j += 2) {
+        add_to(e[j], e[j + 1], dr.get(j), dr.get(j + 1));
+        decay_over(c[s][j], c[s][j + 1], e[j], e[j + 1]);
+      }
     }
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
@@ -698,11 +744,13 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_backward_kernel(const Di
         tile.c.template fetch<GT, W>(s, g.p + s * g.stride, g.base, lane, s < to.live, to.room == kChannels, to.room);
       }
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const float xv = xr.get(j);
-        c[s][j] = cr.get(j);
-        before[s][j] = COMP ? st[j] - xv : st[j];
-        st[j] = decay_step(c[s][j], st[j], COMP ? xv * forgotten(c[s][j]) : xv);
+      for (int j = 0; j < kPer; j += 2) {
+        const float c0 = cr.get(j), c1 = cr.get(j + 1), x0 = xr.get(j), x1 = xr.get(j + 1);
+        c[s][j] = c0;
+        c[s][j + 1] = c1;
+        before[s][j] = COMP ? st[j] - x0 : st[j];
+        before[s][j + 1] = COMP ? st[j + 1] - x1 : st[j + 1];
+        decay_steps(c0, c1, is_diff(c0), is_diff(c1), st[j], st[j + 1], COMP ? x0 * forgotten(c0) : x0, COMP ? x1 * forgotten(c1) : x1);
       }
     }
     X* dx = static_cast<X*>(p.dx) + (at.b * p.L + at.t0) * p.D + at.ch0;
@@ -713,11 +761,14 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_backward_kernel(const Di
       if (more && p.d_h) tile.d.template fetch<XT, W>(s, d.p + s * d.stride, d.base, lane, s < to.live, to.room == kChannels, to.room);
       float vx[kPer], vg[kPer];
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const float dv = dr.get(j) + e[j];
-        vx[j] = COMP ? dv * forgotten(c[s][j]) : dv;
-        e[j] = decay_step(c[s][j], dv, 0.f);
-        vg[j] = e[j] * before[s][j];
+      for (int j = 0; j < kPer; j += 2) {
+        add_to(e[j], e[j + 1], dr.get(j), dr.get(j + 1));
+        vx[j] = COMP ? e[j] * forgotten(c[s][j]) : e[j];
+        vx[j + 1] = COMP ? e[j + 1] * forgotten(c[s][j + 1]) : e[j + 1];
+        decay_over(c[s][j], c[s][j + 1], e[j], e[j + 1]);
+        const F2 v = f2(e[j], e[j + 1]) * f2(before[s][j], before[s][j + 1]);
+        vg[j] = lo(v);
+        vg[j + 1] = hi(v);
       }
       if (s < at.live) {
         if (p.dx) store_token<XT, W>(packed<XT>(vx), dx + s * p.D, lane, at.room);
