@@ -118,36 +118,42 @@ __device__ __forceinline__ int channel_of(int lane, int j) { return (j / W * kLa
 template <int S, int WORDS> struct Cells {
   alignas(16) uint32_t w[S][kRunners][WORDS];      // (a copy's two ends lie on a boundary of its size)
 
-  // Step s of this thread from p, its strip of that token; `there`: the token exists, `whole`: so do all channels of the strip.  `base`: the
-  // tensor, an address that is good where nothing is read.  Two bytes are no asynchronous copy: those elements are loaded and put here.
+  // Step s of this thread from p, its first channel of that token, where all channels of the strip exist ...
   template <int TY, int W>
-  __device__ __forceinline__ void fetch(int s, const typename Elem<TY>::T* p, const void* base, int lane, bool there, bool whole, int room) {
-    constexpr int kBytes = W * elem_bytes(TY), kPieces = kPer / W;
+  __device__ __forceinline__ void fetch(int s, const typename Elem<TY>::T* p) {
+    constexpr int kBytes = W * elem_bytes(TY);
     if constexpr (kBytes >= 4) {
-      const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(&w[s][threadIdx.x][0]));
-      const auto copy = [&](int i, const void* from, int bytes) {      // (zeros beyond `bytes`)
-        if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + i * kBytes), "l"(from), "r"(bytes) : "memory");
-        else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to + i * kBytes), "l"(from), "n"(kBytes), "r"(bytes) : "memory");
-      };
-      if (there && whole) {
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) copy(i, p + channel_of<W>(lane, i * W), kBytes);
-      } else {
+      for (int i = 0; i < kPer / W; ++i) copy<kBytes>(s, i, p + i * (kLanes * W), kBytes);
+    } else {
+      fetch<TY, W>(s, p, p, kChannels);
+    }
+  }
+  // ... and where `room` channels do, from this thread's first on (0: no token); `base`: the tensor, an address that is good where nothing is
+  // read.  Two bytes are no asynchronous copy: those elements are loaded and put here.
+  template <int TY, int W>
+  __device__ __forceinline__ void fetch(int s, const typename Elem<TY>::T* p, const void* base, int room) {
+    constexpr int kBytes = W * elem_bytes(TY);
+    if constexpr (kBytes >= 4) {
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-          const int ch = channel_of<W>(lane, i * W);
-          const bool any = there && ch < room;
-          copy(i, any ? p + ch : base, any ? kBytes : 0);
-        }
+      for (int i = 0; i < kPer / W; ++i) {
+        const bool any = i * (kLanes * W) < room;
+        copy<kBytes>(s, i, any ? p + i * (kLanes * W) : base, any ? kBytes : 0);
       }
     } else {
       Raw<TY, kPer> r;
       r.zero();
 #pragma unroll
       for (int j = 0; j < kPer; ++j)
-        if (there && channel_of<W>(lane, j) < room) raw_put(r, j, __ldg(p + channel_of<W>(lane, j)));
+        if (j * kLanes < room) raw_put(r, j, __ldg(p + j * kLanes));
       put(s, r);
     }
+  }
+  template <int BYTES>
+  __device__ __forceinline__ void copy(int s, int i, const void* from, int bytes) {      // (zeros beyond `bytes`)
+    const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(&w[s][threadIdx.x][0])) + i * BYTES;
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(BYTES), "r"(bytes) : "memory");
   }
   template <int TY>
   __device__ __forceinline__ Raw<TY, kPer> take(int s) const {
@@ -162,18 +168,18 @@ template <int S, int WORDS> struct Cells {
     for (int i = 0; i < Raw<TY, kPer>::kWords; ++i) w[s][threadIdx.x][i] = r.w[i];
   }
 };
+// p: this thread's first channel; room: channels from there on
 template <int TY, int W>
-__device__ __forceinline__ void store_token(const Raw<TY, kPer>& r, typename Elem<TY>::T* p, int lane, int room) {
+__device__ __forceinline__ void store_token(const Raw<TY, kPer>& r, typename Elem<TY>::T* p, int room) {
   constexpr int kBytes = W * elem_bytes(TY), kWords = kBytes / 4;
 #pragma unroll
   for (int i = 0; i < kPer / W; ++i) {
-    const int ch = channel_of<W>(lane, i * W);
-    if (ch >= room) continue;
-    uint32_t* d = reinterpret_cast<uint32_t*>(p + ch);
+    if (i * (kLanes * W) >= room) continue;
+    uint32_t* d = reinterpret_cast<uint32_t*>(p + i * (kLanes * W));
     if constexpr (kWords == 4) *reinterpret_cast<uint4*>(d) = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
     else if constexpr (kWords == 2) *reinterpret_cast<uint2*>(d) = make_uint2(r.w[i * 2], r.w[i * 2 + 1]);
     else if constexpr (kWords == 1) *d = r.w[i];
-    else p[ch] = raw_take(r, i);
+    else p[i * kLanes] = raw_take(r, i);
   }
 }
 template <int TY>
@@ -237,8 +243,11 @@ __device__ __noinline__ unsigned long long look_wait(const unsigned long long* p
 }
 
 struct Ticket {
-  int order;                     // of the tile in its sequence; from `tiles` on there is none
-  uint32_t seq, b, strip;
+  int order, tile;               // of the tile in its sequence, as it is folded (from `tiles` on there is none) and from the first token on
+  uint32_t seq;                  // sequence: strip of channels of a batch
+  int room, live;                // channels of the strip, tokens of the tile
+  long long state;               // where its strip begins in a state [B, D], its first element in x, g, d_h and in what is contiguous
+  long long x, g, d, h;
 };
 template <int XT, int S> struct ForwardShared {
   struct Tile {
@@ -335,45 +344,33 @@ __device__ __forceinline__ float look_back(const LookPlace& p, int ch, float fir
   return carry;
 }
 
-// Where a thread's part of a tile lies.
-struct TilePlace {
-  long long b, ch0, t0;      // batch, first channel, first token of this thread
-  int tile, room, live;      // channels of the strip; tokens of this thread (0 and less: none)
-  template <int S>
-  __device__ __forceinline__ static TilePlace of(const DiagProblem& p, const Ticket& t, int grp, bool backwards) {
-    TilePlace r;
-    r.tile = backwards ? p.tiles - 1 - t.order : t.order;
-    r.b = t.b;
-    r.ch0 = static_cast<long long>(t.strip) * kChannels;
-    r.room = static_cast<int>(p.D - r.ch0 < kChannels ? p.D - r.ch0 : kChannels);
-    r.t0 = static_cast<long long>(r.tile) * (kGroups * S) + grp * S;
-    r.live = static_cast<int>(p.L - r.t0 < S ? p.L - r.t0 : S);
-    return r;
-  }
-};
-// A thread's rows of a tensor in a tile.
-template <int TY> struct Rows {
-  using T = typename Elem<TY>::T;
-  const void* base;
-  const T* p;
-  long long stride;
-  __device__ __forceinline__ Rows(const void* t, const TilePlace& at, long long batch, long long token)
-      : base(t), p(static_cast<const T*>(t) + at.b * batch + at.t0 * token + at.ch0), stride(token) {}
-};
 // One thread takes tickets, and says for all what they stand for.
-struct TicketTaker {
+template <int S, bool BACK> struct TicketTaker {
   const DiagProblem& p;
   uint32_t have;      // the last one
   __device__ __forceinline__ void take() { have = p.tiles > 1 ? atomicAdd(p.look.head, 1u) + 1u : have + gridDim.x; }
   __device__ __forceinline__ Ticket named() const {
     Ticket t;
     t.order = static_cast<int>(have / p.seqs);
+    t.tile = BACK ? p.tiles - 1 - t.order : t.order;
     t.seq = have - t.order * p.seqs;
-    t.b = t.seq / static_cast<uint32_t>(p.strips);
-    t.strip = t.seq - t.b * p.strips;
+    const uint32_t b = t.seq / static_cast<uint32_t>(p.strips);
+    const long long ch0 = static_cast<long long>(t.seq - b * p.strips) * kChannels, t0 = static_cast<long long>(t.tile) * (kGroups * S);
+    t.room = static_cast<int>(p.D - ch0 < kChannels ? p.D - ch0 : kChannels);
+    t.live = static_cast<int>(p.L - t0 < kGroups * S ? p.L - t0 : kGroups * S);
+    t.state = b * p.D + ch0;
+    t.x = b * p.x_batch + t0 * p.x_token + ch0;
+    t.g = b * p.g_batch + t0 * p.g_token + ch0;
+    t.d = b * p.d_batch + t0 * p.d_token + ch0;
+    t.h = (b * p.L + t0) * p.D + ch0;
     return t;
   }
 };
+// This thread's first element of a tensor, in a tile whose first element is the tensor's.
+template <int TY>
+__device__ __forceinline__ typename Elem<TY>::T* own_part(const void* tensor, long long token, int first_token, int first_channel) {
+  return static_cast<typename Elem<TY>::T*>(const_cast<void*>(tensor)) + first_token * token + first_channel;
+}
 
 // Barriers from one role to the next, two of each for even and odd tiles: a tile's parts are there (runners to publisher), its word has
 // gone out (publisher to lookers), its starts are there (lookers to runners).
@@ -396,7 +393,7 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_forward_kernel(const Dia
   constexpr int S = forward_steps(XT);
   extern __shared__ __align__(16) unsigned char smem[];
   auto& sh = *reinterpret_cast<ForwardShared<XT, S>*>(smem);
-  TicketTaker tickets{p, blockIdx.x - gridDim.x};
+  TicketTaker<S, false> tickets{p, blockIdx.x - gridDim.x};
   const bool taker = threadIdx.x == kPublisher;
   if (taker) {
     tickets.take();
@@ -410,11 +407,10 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_forward_kernel(const Dia
     for (int n = 0;; ++n) {
       const Ticket cur = sh.ticket[n & 3];
       if (cur.order >= p.tiles) break;
-      const TilePlace at = TilePlace::of<S>(p, cur, 0, false);
       const LookPlace look(p.look, cur.seq, p.tiles, cur.order);
       auto& part = sh.part[n & 1];
-      const long long state_at = at.b * p.D + at.ch0 + ch;
-      float carry = ch < at.room && p.h0 ? p.h0[state_at] : 0.f;
+      const long long state_at = cur.state + ch;
+      float carry = ch < cur.room && p.h0 ? p.h0[state_at] : 0.f;
       bar_sync<kOutThreads>(kBarOut + (n & 1));
       if (p.tiles > 1) carry = look_back(look, ch, carry, p.status);
       const float entry = carry;
@@ -430,12 +426,12 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_forward_kernel(const Dia
       }
       bar_arrive<kStartsThreads>(kBarStarts + (n & 1));
       if (p.tiles > 1 && look.closes_super()) look_store(look.at(2, look.super, ch), 0.f, carry);
-      if (p.states && ch < at.room) {
-        float* to = p.states + (at.b * p.records + 2 * at.tile) * p.D + at.ch0 + ch;
+      if (p.states && ch < cur.room) {
+        float* to = p.states + (cur.seq / p.strips * p.records + 2 * cur.tile) * p.D + cur.seq % p.strips * kChannels + ch;
         to[0] = entry;
-        if (2 * at.tile + 1 < p.records) to[p.D] = middle;
+        if (2 * cur.tile + 1 < p.records) to[p.D] = middle;
       }
-      if (p.hT && ch < at.room && at.tile == p.tiles - 1) p.hT[state_at] = carry;
+      if (p.hT && ch < cur.room && cur.tile == p.tiles - 1) p.hT[state_at] = carry;
     }
     return;
   }
@@ -470,15 +466,18 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_forward_kernel(const Dia
   }
   const int lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
   const auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+  using GE = typename Elem<GT>::T;
+  const X* const x0 = own_part<XT>(p.x, p.x_token, grp * S, lane * W);
+  const GE* const g0 = own_part<GT>(p.g, p.g_token, grp * S, lane * W);
+  X* const h0 = own_part<XT>(p.h, p.D, grp * S, lane * W);
   const auto fetch = [&](const Ticket& t, int slot) {
     if (t.order < p.tiles) {
-      const TilePlace at = TilePlace::of<S>(p, t, grp, false);
-      const Rows<XT> x(p.x, at, p.x_batch, p.x_token);
-      const Rows<GT> g(p.g, at, p.g_batch, p.g_token);
+      auto& tile = sh.tile[slot];
 #pragma unroll
       for (int s = 0; s < S; ++s) {
-        sh.tile[slot].x.template fetch<XT, W>(s, x.p + s * x.stride, x.base, lane, s < at.live, at.room == kChannels, at.room);
-        sh.tile[slot].c.template fetch<GT, W>(s, g.p + s * g.stride, g.base, lane, s < at.live, at.room == kChannels, at.room);
+        const int room = s < t.live - grp * S ? t.room - lane * W : 0;
+        tile.x.template fetch<XT, W>(s, x0 + t.x + s * p.x_token, p.x, room);
+        tile.c.template fetch<GT, W>(s, g0 + t.g + s * p.g_token, p.g, room);
       }
     }
     commit();
@@ -495,13 +494,13 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_forward_kernel(const Dia
       Raw<LETHE_F32, kPer> cr;
 #pragma unroll
       for (int j = 0; j < kPer; j += 2) {
-        const float g0 = gr.get(j), g1 = gr.get(j + 1);
-        float c0 = g0, c1 = g1;
+        const float a0 = gr.get(j), a1 = gr.get(j + 1);
+        float c0 = a0, c1 = a1;
         decay_coefs(c0, c1);
         cr.set2(j, c0, c1);
-        add_to(sum[j], sum[j + 1], g0, g1);
-        const float x0 = xr.get(j), x1 = xr.get(j + 1);
-        decay_steps(c0, c1, by_diff(g0), by_diff(g1), st[j], st[j + 1], COMP ? x0 * forgotten(c0) : x0, COMP ? x1 * forgotten(c1) : x1);
+        add_to(sum[j], sum[j + 1], a0, a1);
+        const float v0 = xr.get(j), v1 = xr.get(j + 1);
+        decay_steps(c0, c1, by_diff(a0), by_diff(a1), st[j], st[j + 1], COMP ? v0 * forgotten(c0) : v0, COMP ? v1 * forgotten(c1) : v1);
       }
       tile.c.put(s, cr);
     }
@@ -516,42 +515,48 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_forward_kernel(const Dia
     first_run(0);
   }
   for (int n = 0;; ++n) {
-    const Ticket cur = sh.ticket[n & 3];
+    const Ticket& cur = sh.ticket[n & 3];
     if (cur.order >= p.tiles) break;
     const int slot = n & 1;
     if (sh.ticket[(n + 1) & 3].order < p.tiles) {
       asm volatile("cp.async.wait_group 0;" ::: "memory");
       first_run(slot ^ 1);
     }
-    const TilePlace at = TilePlace::of<S>(p, cur, grp, false);
     auto& tile = sh.tile[slot];
-    X* h = static_cast<X*>(p.h) + (at.b * p.L + at.t0) * p.D + at.ch0;
+    X* h = h0 + cur.h;
+    const int live = cur.live - grp * S, room = cur.room - lane * W;
+    const bool whole = live >= S && cur.room == kChannels;
     float st[kPer];
     bar_sync<kStartsThreads>(kBarStarts + slot);
 #pragma unroll
     for (int j = 0; j < kPer; ++j) st[j] = sh.part[slot][grp][channel_of<W>(lane, j)].x;
     // a cell that has been read takes its step of the tile after the next
-    const Ticket after = sh.ticket[(n + 2) & 3];
-    const TilePlace to = TilePlace::of<S>(p, after, grp, false);
-    Rows<XT> x(p.x, to, p.x_batch, p.x_token);
-    Rows<GT> g(p.g, to, p.g_batch, p.g_token);
+    const Ticket& after = sh.ticket[(n + 2) & 3];
+    const X* xn = x0 + after.x;
+    const GE* gn = g0 + after.g;
     const bool more = after.order < p.tiles;
+    const int live_n = after.live - grp * S, room_n = after.room - lane * W;
+    const bool whole_n = more && live_n >= S && after.room == kChannels;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
       const auto xr = tile.x.template take<XT>(s);
       const auto cr = tile.c.template take<LETHE_F32>(s);
-      if (more) {
-        tile.x.template fetch<XT, W>(s, x.p, x.base, lane, s < to.live, to.room == kChannels, to.room);
-        tile.c.template fetch<GT, W>(s, g.p, g.base, lane, s < to.live, to.room == kChannels, to.room);
+      if (whole_n) {
+        tile.x.template fetch<XT, W>(s, xn);
+        tile.c.template fetch<GT, W>(s, gn);
+      } else if (more) {
+        tile.x.template fetch<XT, W>(s, xn, p.x, s < live_n ? room_n : 0);
+        tile.c.template fetch<GT, W>(s, gn, p.g, s < live_n ? room_n : 0);
       }
-      x.p += x.stride;
-      g.p += g.stride;
+      xn += p.x_token;
+      gn += p.g_token;
 #pragma unroll
       for (int j = 0; j < kPer; j += 2) {
-        const float c0 = cr.get(j), c1 = cr.get(j + 1), x0 = xr.get(j), x1 = xr.get(j + 1);
-        decay_steps(c0, c1, is_diff(c0), is_diff(c1), st[j], st[j + 1], COMP ? x0 * forgotten(c0) : x0, COMP ? x1 * forgotten(c1) : x1);
+        const float c0 = cr.get(j), c1 = cr.get(j + 1), v0 = xr.get(j), v1 = xr.get(j + 1);
+        decay_steps(c0, c1, is_diff(c0), is_diff(c1), st[j], st[j + 1], COMP ? v0 * forgotten(c0) : v0, COMP ? v1 * forgotten(c1) : v1);
       }
-      if (s < at.live) store_token<XT, W>(packed<XT>(st), h, lane, at.room);
+      if (whole) store_token<XT, W>(packed<XT>(st), h, kChannels);
+      else if (s < live) store_token<XT, W>(packed<XT>(st), h, room);
       h += p.D;
     }
     commit();
@@ -565,7 +570,7 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_backward_kernel(const Di
   constexpr int S = backward_steps(XT);
   extern __shared__ __align__(16) unsigned char smem[];
   auto& sh = *reinterpret_cast<BackwardShared<XT, S>*>(smem);
-  TicketTaker tickets{p, blockIdx.x - gridDim.x};
+  TicketTaker<S, true> tickets{p, blockIdx.x - gridDim.x};
   const bool taker = threadIdx.x == kPublisher;
   if (taker) {
     tickets.take();
@@ -579,13 +584,12 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_backward_kernel(const Di
     for (int n = 0;; ++n) {
       const Ticket cur = sh.ticket[n & 3];
       if (cur.order >= p.tiles) break;
-      const TilePlace at = TilePlace::of<S>(p, cur, 0, true);
       const LookPlace look(p.look, cur.seq, p.tiles, cur.order);
       auto& part = sh.part[n & 1];
       auto& back = sh.back[n & 1];
-      const long long state_at = at.b * p.D + at.ch0 + ch;
-      float carry = ch < at.room && p.dhT ? p.dhT[state_at] : 0.f;
-      float st = ch < at.room ? p.states[(at.b * p.records + at.tile) * p.D + at.ch0 + ch] : 0.f;
+      const long long state_at = cur.state + ch;
+      float carry = ch < cur.room && p.dhT ? p.dhT[state_at] : 0.f;
+      float st = ch < cur.room ? p.states[(cur.seq / p.strips * p.records + cur.tile) * p.D + cur.seq % p.strips * kChannels + ch] : 0.f;
       bar_sync<kOutThreads>(kBarOut + (n & 1));
       if (p.tiles > 1) carry = look_back(look, ch, carry, p.status);
       float2 own[kGroups];
@@ -605,7 +609,7 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_backward_kernel(const Di
       }
       bar_arrive<kStartsThreads>(kBarStarts + (n & 1));
       if (p.tiles > 1 && look.closes_super()) look_store(look.at(2, look.super, ch), 0.f, carry);
-      if (p.dh0 && ch < at.room && at.tile == 0) p.dh0[state_at] = carry;
+      if (p.dh0 && ch < cur.room && cur.tile == 0) p.dh0[state_at] = carry;
     }
     return;
   }
@@ -642,16 +646,21 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_backward_kernel(const Di
   }
   const int lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
   const auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+  using GE = typename Elem<GT>::T;
+  const X* const x0 = own_part<XT>(p.x, p.x_token, grp * S, lane * W);
+  const GE* const g0 = own_part<GT>(p.g, p.g_token, grp * S, lane * W);
+  const X* const d0 = own_part<XT>(p.d_h, p.d_token, grp * S, lane * W);
+  X* const dx0 = own_part<XT>(p.dx, p.D, grp * S, lane * W);
+  G* const dg0 = own_part<GT>(p.dg, p.D, grp * S, lane * W);
   const auto fetch = [&](const Ticket& t, int slot) {
     if (t.order < p.tiles) {
-      const TilePlace at = TilePlace::of<S>(p, t, grp, true);
-      const Rows<XT> x(p.x, at, p.x_batch, p.x_token), d(p.d_h, at, p.d_batch, p.d_token);
-      const Rows<GT> g(p.g, at, p.g_batch, p.g_token);
+      auto& tile = sh.tile[slot];
 #pragma unroll
       for (int s = 0; s < S; ++s) {
-        sh.tile[slot].x.template fetch<XT, W>(s, x.p + s * x.stride, x.base, lane, s < at.live, at.room == kChannels, at.room);
-        sh.tile[slot].c.template fetch<GT, W>(s, g.p + s * g.stride, g.base, lane, s < at.live, at.room == kChannels, at.room);
-        if (p.d_h) sh.tile[slot].d.template fetch<XT, W>(s, d.p + s * d.stride, d.base, lane, s < at.live, at.room == kChannels, at.room);
+        const int room = s < t.live - grp * S ? t.room - lane * W : 0;
+        tile.x.template fetch<XT, W>(s, x0 + t.x + s * p.x_token, p.x, room);
+        tile.c.template fetch<GT, W>(s, g0 + t.g + s * p.g_token, p.g, room);
+        if (p.d_h) tile.d.template fetch<XT, W>(s, d0 + t.d + s * p.d_token, p.d_h, room);
       }
     }
     commit();
@@ -668,15 +677,15 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_backward_kernel(const Di
       Raw<LETHE_F32, kPer> cr;
 #pragma unroll
       for (int j = 0; j < kPer; j += 2) {
-        const float g0 = gr.get(j), g1 = gr.get(j + 1);
-        float c0 = g0, c1 = g1;
+        const float a0 = gr.get(j), a1 = gr.get(j + 1);
+        float c0 = a0, c1 = a1;
         decay_coefs(c0, c1);
         cr.set2(j, c0, c1);
         c[s][j] = c0;
         c[s][j + 1] = c1;
-        add_to(sum[j], sum[j + 1], g0, g1);
-        const float x0 = xr.get(j), x1 = xr.get(j + 1);
-        decay_steps(c0, c1, by_diff(g0), by_diff(g1), st[j], st[j + 1], COMP ? x0 * forgotten(c0) : x0, COMP ? x1 * forgotten(c1) : x1);
+        add_to(sum[j], sum[j + 1], a0, a1);
+        const float v0 = xr.get(j), v1 = xr.get(j + 1);
+        decay_steps(c0, c1, by_diff(a0), by_diff(a1), st[j], st[j + 1], COMP ? v0 * forgotten(c0) : v0, COMP ? v1 * forgotten(c1) : v1);
       }
       tile.c.put(s, cr);
     }
@@ -713,15 +722,16 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_backward_kernel(const Di
     first_run(0);
   }
   for (int n = 0;; ++n) {
-    const Ticket cur = sh.ticket[n & 3];
+    const Ticket& cur = sh.ticket[n & 3];
     if (cur.order >= p.tiles) break;
     const int slot = n & 1;
     if (sh.ticket[(n + 1) & 3].order < p.tiles) {
       asm volatile("cp.async.wait_group 0;" ::: "memory");
       first_run(slot ^ 1);
     }
-    const TilePlace at = TilePlace::of<S>(p, cur, grp, true);
     auto& tile = sh.tile[slot];
+    const int live = cur.live - grp * S, room = cur.room - lane * W;
+    const bool whole = live >= S && cur.room == kChannels && p.dx && p.dg;
     float before[S][kPer], c[S][kPer], st[kPer], e[kPer];
     bar_sync<kStartsThreads>(kBarStarts + slot);
 #pragma unroll
@@ -730,35 +740,44 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_backward_kernel(const Di
       st[j] = sh.part[slot][grp][ch].x;
       e[j] = sh.back[slot][grp][ch];
     }
-    const Ticket after = sh.ticket[(n + 2) & 3];
-    const TilePlace to = TilePlace::of<S>(p, after, grp, true);
-    const Rows<XT> x(p.x, to, p.x_batch, p.x_token), d(p.d_h, to, p.d_batch, p.d_token);
-    const Rows<GT> g(p.g, to, p.g_batch, p.g_token);
+    const Ticket& after = sh.ticket[(n + 2) & 3];
+    const X* xn = x0 + after.x;
+    const GE* gn = g0 + after.g;
     const bool more = after.order < p.tiles;
+    const int live_n = after.live - grp * S, room_n = after.room - lane * W;
+    const bool whole_n = more && live_n >= S && after.room == kChannels && p.d_h;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
       const auto xr = tile.x.template take<XT>(s);
       const auto cr = tile.c.template take<LETHE_F32>(s);
-      if (more) {
-        tile.x.template fetch<XT, W>(s, x.p + s * x.stride, x.base, lane, s < to.live, to.room == kChannels, to.room);
-        tile.c.template fetch<GT, W>(s, g.p + s * g.stride, g.base, lane, s < to.live, to.room == kChannels, to.room);
+      if (whole_n) {
+        tile.x.template fetch<XT, W>(s, xn);
+        tile.c.template fetch<GT, W>(s, gn);
+      } else if (more) {
+        tile.x.template fetch<XT, W>(s, xn, p.x, s < live_n ? room_n : 0);
+        tile.c.template fetch<GT, W>(s, gn, p.g, s < live_n ? room_n : 0);
       }
+      xn += p.x_token;
+      gn += p.g_token;
 #pragma unroll
       for (int j = 0; j < kPer; j += 2) {
-        const float c0 = cr.get(j), c1 = cr.get(j + 1), x0 = xr.get(j), x1 = xr.get(j + 1);
+        const float c0 = cr.get(j), c1 = cr.get(j + 1), v0 = xr.get(j), v1 = xr.get(j + 1);
         c[s][j] = c0;
         c[s][j + 1] = c1;
-        before[s][j] = COMP ? st[j] - x0 : st[j];
-        before[s][j + 1] = COMP ? st[j + 1] - x1 : st[j + 1];
-        decay_steps(c0, c1, is_diff(c0), is_diff(c1), st[j], st[j + 1], COMP ? x0 * forgotten(c0) : x0, COMP ? x1 * forgotten(c1) : x1);
+        before[s][j] = COMP ? st[j] - v0 : st[j];
+        before[s][j + 1] = COMP ? st[j + 1] - v1 : st[j + 1];
+        decay_steps(c0, c1, is_diff(c0), is_diff(c1), st[j], st[j + 1], COMP ? v0 * forgotten(c0) : v0, COMP ? v1 * forgotten(c1) : v1);
       }
     }
-    X* dx = static_cast<X*>(p.dx) + (at.b * p.L + at.t0) * p.D + at.ch0;
-    G* dg = static_cast<G*>(p.dg) + (at.b * p.L + at.t0) * p.D + at.ch0;
+    const X* dn = d0 + after.d + (S - 1) * p.d_token;
+    X* dx = dx0 + cur.h + (S - 1) * p.D;
+    G* dg = dg0 + cur.h + (S - 1) * p.D;
 #pragma unroll
     for (int s = S - 1; s >= 0; --s) {
       const auto dr = tile.d.template take<XT>(s);
-      if (more && p.d_h) tile.d.template fetch<XT, W>(s, d.p + s * d.stride, d.base, lane, s < to.live, to.room == kChannels, to.room);
+      if (whole_n) tile.d.template fetch<XT, W>(s, dn);
+      else if (more && p.d_h) tile.d.template fetch<XT, W>(s, dn, p.d_h, s < live_n ? room_n : 0);
+      dn -= p.d_token;
       float vx[kPer], vg[kPer];
 #pragma unroll
       for (int j = 0; j < kPer; j += 2) {
@@ -770,10 +789,15 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_backward_kernel(const Di
         vg[j] = lo(v);
         vg[j + 1] = hi(v);
       }
-      if (s < at.live) {
-        if (p.dx) store_token<XT, W>(packed<XT>(vx), dx + s * p.D, lane, at.room);
-        if (p.dg) store_token<GT, W>(packed<GT>(vg), dg + s * p.D, lane, at.room);
+      if (whole) {
+        store_token<XT, W>(packed<XT>(vx), dx, kChannels);
+        store_token<GT, W>(packed<GT>(vg), dg, kChannels);
+      } else if (s < live) {
+        if (p.dx) store_token<XT, W>(packed<XT>(vx), dx, room);
+        if (p.dg) store_token<GT, W>(packed<GT>(vg), dg, room);
       }
+      dx -= p.D;
+      dg -= p.D;
     }
     commit();
   }
