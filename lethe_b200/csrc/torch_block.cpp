@@ -93,13 +93,16 @@ int64_t joint_stride(const Tensor& t, int64_t from, int64_t to) {
 // readable as [B, L, D] with strides for batch and token
 Tensor tokens(const Tensor& t) { return lazy(t) || !packed_from(t, 2) ? as(t, t.scalar_type()) : t; }
 
+// stride of a dimension; one of a single index is never gone by, and its stride says nothing
+int64_t step_of(const Tensor& t, int64_t dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
+
 LetheGdnDiagArgs diag_args(const Tensor& x, const Tensor& g, bool complement) {
   LetheGdnDiagArgs a;
   memset(&a, 0, sizeof(a));
   a.B = x.size(0); a.L = x.size(1); a.D = x.numel() / (a.B * a.L);
   a.x_type = code(x.scalar_type()); a.g_type = code(g.scalar_type()); a.complement = complement;
-  a.x = ptr(x); a.x_batch = x.stride(0); a.x_token = x.stride(1);
-  a.g = ptr(g); a.g_batch = g.stride(0); a.g_token = g.stride(1);
+  a.x = ptr(x); a.x_batch = step_of(x, 0); a.x_token = step_of(x, 1);
+  a.g = ptr(g); a.g_batch = step_of(g, 0); a.g_token = step_of(g, 1);
   a.status = status_word(x.device().index());
   return a;
 }
@@ -138,7 +141,7 @@ struct DiagScanBackward : public FirstOrderNode {      // kept: x, g, states
       const Tensor at_states = reinterpret_cast<uintptr_t>(states.data_ptr()) % 4 || !states.is_contiguous() ? states.clone() : states;
       a.states = ptr<float>(at_states);
       if (d.defined()) {
-        a.d_h = ptr(d); a.d_h_batch = d.stride(0); a.d_h_token = d.stride(1);
+        a.d_h = ptr(d); a.d_h_batch = step_of(d, 0); a.d_h_token = step_of(d, 1);
       }
       a.dhT = ptr<float>(dhT);
       if (task_should_compute_output(0)) dx = at::empty(x.sizes(), x.options());
@@ -234,8 +237,8 @@ Tensor diag_scan_step(const Tensor& x, const Tensor& g_in, const Tensor& state, 
     memset(&a, 0, sizeof(a));
     a.B = state.size(0); a.L = 1; a.D = state.numel() / a.B;
     a.x_type = code(x.scalar_type()); a.g_type = code(g.scalar_type()); a.complement = complement;
-    a.x = ptr(xt); a.x_batch = xt.stride(0);
-    a.g = ptr(g); a.g_batch = g.stride(0);
+    a.x = ptr(xt); a.x_batch = step_of(xt, 0);
+    a.g = ptr(g); a.g_batch = step_of(g, 0);
     a.h = ptr(h);
     check(lethe_gdn_diag_step(&a, ptr<float>(state), stream_of(state)));
     if (!state.is_inference()) torch::autograd::impl::bump_version(state);
@@ -269,7 +272,7 @@ Rows rows_of(const Tensor& t) {
   r.t = lazy(t) || !packed_from(t, t.dim() - 1) || joint_stride(t, 0, t.dim() - 2) < 0 ? as(t, t.scalar_type()) : t;
   if (t.dim() >= 2) {
     r.inner = t.size(-2);
-    r.inner_stride = r.t.stride(-2);
+    r.inner_stride = t.size(-2) > 1 ? r.t.stride(-2) : 0;
     r.outer_stride = joint_stride(r.t, 0, t.dim() - 2);
   }
   return r;
