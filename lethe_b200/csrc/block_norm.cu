@@ -43,7 +43,7 @@ __device__ __forceinline__ F2 logistic(F2 z) {
 
 // CTAs on an SM: registers (64 a thread forward, 80 backward; twice that with two pieces)
 template <typename S> constexpr int gated_ctas(bool backward) { return S::R > 1 ? 512 / S::kThreads : (backward ? 768 : 1024) / S::kThreads; }
-template <int XT, typename S, bool BACK> using GatedRing = RowRing<S, (BACK ? 3 : 2) * S::R * 8 * elem_bytes(XT), gated_ctas<S>(BACK)>;
+template <int XT, typename S, bool BACK> using GatedRing = RowRing<S, (BACK ? 3 : 2) * S::R * 8 * elem_bytes(XT), gated_ctas<S>(BACK), elem_bytes(XT)>;
 
 template <int XT, bool SILU, typename S>
 __global__ void __launch_bounds__(S::kThreads, gated_ctas<S>(false)) gated_norm_kernel(const GatedProblem p) {
@@ -265,9 +265,11 @@ extern "C" int lethe_gdn_gated_norm(const LetheGdnGatedNormArgs* a, void* stream
   if (int e = gated_problem(a, &p, false)) return e;
   DeviceGuard guard(a->x);
   if (!guard.ok) return kErrDevice;
-  const bool vec = p.D % 8 == 0 && piece_aligned(p.x, a->x_type, p.xo, p.xi) && piece_aligned(p.z, a->x_type, p.zo, p.zi) && piece_aligned(p.y, a->x_type);
+  const int w = widest_piece(widest_of(a->x_type, a->x_type), p.D, [&](int n) {
+    return piece_aligned(n, p.x, a->x_type, p.xo, p.xi) && piece_aligned(n, p.z, a->x_type, p.zo, p.zi) && piece_aligned(n, p.y, a->x_type);
+  });
   return by_x_type(a->x_type, [&](auto x) {
-    return by_row_shape(p.D, vec, [&](auto s) {
+    return by_row_shape<widest_of(x.value, x.value)>(p.D, w, [&](auto s) {
       using S = decltype(s);
       constexpr int smem = GatedRing<x.value, S, false>::kBytes;
       static SmemAttr attr[2];
@@ -291,12 +293,14 @@ extern "C" int lethe_gdn_gated_norm_vjp(const LetheGdnGatedNormArgs* a, void* st
   }
   DeviceGuard guard(a->x);
   if (!guard.ok) return kErrDevice;
-  const bool vec = p.D % 8 == 0 && piece_aligned(p.x, a->x_type, p.xo, p.xi) && piece_aligned(p.z, a->x_type, p.zo, p.zi) &&
-                   piece_aligned(p.dy, a->x_type) && piece_aligned(p.dx, a->x_type) && piece_aligned(p.dz, a->x_type);
+  const int w = widest_piece(widest_of(a->x_type, a->x_type), p.D, [&](int n) {
+    return piece_aligned(n, p.x, a->x_type, p.xo, p.xi) && piece_aligned(n, p.z, a->x_type, p.zo, p.zi) && piece_aligned(n, p.dy, a->x_type) &&
+           piece_aligned(n, p.dx, a->x_type) && piece_aligned(n, p.dz, a->x_type);
+  });
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int grid = 0;
   const int e = by_x_type(a->x_type, [&](auto x) {
-    return by_row_shape(p.D, vec, [&](auto s) {
+    return by_row_shape<widest_of(x.value, x.value)>(p.D, w, [&](auto s) {
       using S = decltype(s);
       grid = std::min(norm_grid(p.rows, S::kRows, gated_ctas<S>(true)), norm_parts_max(p.D));
       constexpr int smem = std::max(GatedRing<x.value, S, true>::kBytes, S::kColumnBytes);

@@ -20,28 +20,48 @@ constexpr int kNormMaxD = 8192;
 // CTAs of a backward at most: what the work buffer holds partial sums of
 inline int norm_parts_max(int D) { return D <= 2048 ? 1024 : 320; }
 
-template <int T_, int R_, bool VEC_>
+// W: neighbours that are moved at once: 16 bytes of the widest type (8 or 4 values) where D, strides and boundaries allow it, else fewer.  With
+// 8 values of fp32, in two moves, every move of a warp would take half of each sector it touches.
+template <int T_, int R_, int W_>
 struct RowShape {
   static constexpr int T = T_, R = R_, N = R_ * 8, P = N / 2;      // values and pairs of a thread
-  static constexpr bool VEC = VEC_;
+  static constexpr int W = W_, kMoves = N / W;
   static constexpr int kThreads = T > 256 ? T : 256, kRows = kThreads / T;
   static constexpr int kWarps = kThreads / 32;
   static constexpr int kColumnBytes = kRows > 1 ? kThreads * N * 4 : 0;      // what column_share wants
   // column of value n (of N) that thread t of a row holds
-  __device__ __forceinline__ static int col(int t, int n) { return VEC ? ((n / 8) * T + t) * 8 + n % 8 : n * T + t; }
+  __device__ __forceinline__ static int col(int t, int n) { return (n / W * T + t) * W + n % W; }
 
   template <int TY>
   __device__ __forceinline__ static void load(Raw<TY, 8> (&r)[R], const void* row, int t, int D) {
     const typename Elem<TY>::T* p = static_cast<const typename Elem<TY>::T*>(row);
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      r[i].zero();
-      if constexpr (VEC) {
-        if ((i * T + t) * 8 < D) r[i].load(p + (i * T + t) * 8);
-      } else {
+    for (int i = 0; i < R; ++i) r[i].zero();
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (col(t, i * 8 + j) < D) raw_put(r[i], j, __ldg(p + col(t, i * 8 + j)));
+    for (int m = 0; m < kMoves; ++m) {
+      const int c = col(t, m * W);
+      if (c >= D) continue;
+      constexpr int kWords = W * elem_bytes(TY) / 4;
+      if constexpr (kWords == 0) {
+        raw_put(r[m / 8], m % 8, __ldg(p + c));
+      } else {
+        uint32_t* to = &r[m * W / 8].w[m * W % 8 * elem_bytes(TY) / 4];
+        const uint32_t* from = reinterpret_cast<const uint32_t*>(p + c);
+        if constexpr (kWords == 1) to[0] = __ldg(from);
+        else if constexpr (kWords == 2) {
+          const uint2 v = __ldg(reinterpret_cast<const uint2*>(from));
+          to[0] = v.x;
+          to[1] = v.y;
+        } else {
+#pragma unroll
+          for (int k = 0; k < kWords; k += 4) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(from + k));
+            to[k] = v.x;
+            to[k + 1] = v.y;
+            to[k + 2] = v.z;
+            to[k + 3] = v.w;
+          }
+        }
       }
     }
   }
@@ -49,13 +69,20 @@ struct RowShape {
   __device__ __forceinline__ static void store(const Raw<TY, 8> (&r)[R], void* row, int t, int D) {
     typename Elem<TY>::T* p = static_cast<typename Elem<TY>::T*>(row);
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      if constexpr (VEC) {
-        if ((i * T + t) * 8 < D) r[i].store(p + (i * T + t) * 8);
+    for (int m = 0; m < kMoves; ++m) {
+      const int c = col(t, m * W);
+      if (c >= D) continue;
+      constexpr int kWords = W * elem_bytes(TY) / 4;
+      if constexpr (kWords == 0) {
+        p[c] = raw_take(r[m / 8], m % 8);
       } else {
+        const uint32_t* from = &r[m * W / 8].w[m * W % 8 * elem_bytes(TY) / 4];
+        uint32_t* to = reinterpret_cast<uint32_t*>(p + c);
+        if constexpr (kWords == 1) to[0] = from[0];
+        else if constexpr (kWords == 2) *reinterpret_cast<uint2*>(to) = make_uint2(from[0], from[1]);
+        else
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (col(t, i * 8 + j) < D) p[col(t, i * 8 + j)] = raw_take(r[i], j);
+          for (int k = 0; k < kWords; k += 4) *reinterpret_cast<uint4*>(to + k) = make_uint4(from[k], from[k + 1], from[k + 2], from[k + 3]);
       }
     }
   }
@@ -148,8 +175,8 @@ constexpr int ring_stages(int b, int threads_sm) {
   const int n = 196 * 1024 / (b * threads_sm);
   return n > 4 ? 4 : n;      // (three rows of 32 to 48 KB under way cover the latency)
 }
-template <typename S, int B, int CTAS> struct RowRing {
-  static constexpr int kStages = S::VEC ? ring_stages(B, S::kThreads * CTAS) : 0;
+template <typename S, int B, int CTAS, int SMALLEST> struct RowRing {      // SMALLEST: bytes of the smallest type of value
+  static constexpr int kStages = S::W * SMALLEST >= 4 ? ring_stages(B, S::kThreads * CTAS) : 0;      // (2 bytes are no asynchronous copy)
   static constexpr bool kOn = kStages >= 2;      // else rows are loaded at the head of their turn
   static constexpr int kBytes = kOn ? kStages * B * S::kThreads : 0;
   unsigned char* base;
@@ -162,15 +189,21 @@ template <typename S, int B, int CTAS> struct RowRing {
   // this thread's pieces of a row to cells AT and on of a stage
   template <int TY, int AT>
   __device__ __forceinline__ void copy(int stage, const void* row, int t, int D) const {
-    constexpr int kEach = elem_bytes(TY) / 2;
-    const typename Elem<TY>::T* p = static_cast<const typename Elem<TY>::T*>(row);
+    constexpr int kAll = S::W * elem_bytes(TY), kBytes = kAll > 16 ? 16 : kAll;
+    const char* p = static_cast<const char*>(row);
 #pragma unroll
-    for (int i = 0; i < S::R; ++i)
-      if ((i * S::T + t) * 8 < D)
+    for (int m = 0; m < S::kMoves; ++m) {
+      const int c = S::col(t, m * S::W);
+      if (c >= D) continue;
 #pragma unroll
-        for (int k = 0; k < kEach; ++k)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(cell(stage, AT + i * kEach + k)))),
-                       "l"(p + (i * S::T + t) * 8 + k * (16 / elem_bytes(TY))) : "memory");
+      for (int k = 0; k < kAll; k += kBytes) {
+        const int at = m * kAll + k;
+        const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(cell(stage, AT + at / 16))) + at % 16;
+        const char* from = p + static_cast<long long>(c) * elem_bytes(TY) + k;
+        if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+        else if constexpr (kBytes >= 4) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(kBytes) : "memory");
+      }
+    }
   }
   template <int TY, int AT>
   __device__ __forceinline__ void take(Raw<TY, 8> (&r)[S::R], int stage) const {
@@ -240,24 +273,30 @@ struct WalkPtr {
 
 // f(RowShape) for rows of D values: one piece of 8 a thread as far as a CTA goes.  With two, what a row costs beside its values (sums, places, loop)
 // is shared by 16 of them, but half the threads are there to cover one another (us, one / two: gated 4 x 4096 x 16 x 128 bf16 forward
-// 37.0 / 38.4, backward 66 / 71; residual 16384 x 4096 96 / 104; 64 rows of 2048 3.9 / 6.6).  Where pieces of 8 cannot be loaded as
-// such, fewer shapes: these loads are what bounds.
-template <typename F>
-int by_row_shape(int D, bool vec, F&& f) {
-  if (!vec) {
-    if (D <= 256) return f(RowShape<32, 1, false>());
-    if (D <= 2048) return f(RowShape<256, 1, false>());
-    return f(RowShape<512, 2, false>());
-  }
-  if (D <= 64) return f(RowShape<8, 1, true>());
-  if (D <= 128) return f(RowShape<16, 1, true>());
-  if (D <= 256) return f(RowShape<32, 1, true>());
-  if (D <= 512) return f(RowShape<64, 1, true>());
-  if (D <= 1024) return f(RowShape<128, 1, true>());
-  if (D <= 2048) return f(RowShape<256, 1, true>());
-  if (D <= 4096) return f(RowShape<512, 1, true>());
-  return f(RowShape<512, 2, true>());
+// 37.0 / 38.4, backward 66 / 71; residual 16384 x 4096 96 / 104; 64 rows of 2048 3.9 / 6.6).  Where 8 cannot be
+// moved at once, fewer shapes.
+template <int WIDEST, typename F>
+int by_row_shape(int D, int w, F&& f) {
+  const auto few = [&](auto n) {
+    constexpr int W = decltype(n)::value;
+    if (D <= 256) return f(RowShape<32, 1, W>());
+    if (D <= 1024) return f(RowShape<128, 1, W>());
+    if (D <= 4096) return f(RowShape<512, 1, W>());
+    return f(RowShape<512, 2, W>());
+  };
+  if (w == 1) return few(std::integral_constant<int, 1>());
+  if (w == 2) return few(std::integral_constant<int, 2>());
+  if (w < WIDEST) return few(std::integral_constant<int, 4>());
+  if (D <= 64) return f(RowShape<8, 1, WIDEST>());
+  if (D <= 128) return f(RowShape<16, 1, WIDEST>());
+  if (D <= 256) return f(RowShape<32, 1, WIDEST>());
+  if (D <= 512) return f(RowShape<64, 1, WIDEST>());
+  if (D <= 1024) return f(RowShape<128, 1, WIDEST>());
+  if (D <= 2048) return f(RowShape<256, 1, WIDEST>());
+  if (D <= 4096) return f(RowShape<512, 1, WIDEST>());
+  return f(RowShape<512, 2, WIDEST>());
 }
+constexpr int widest_of(int t0, int t1) { return t0 == LETHE_F32 || t1 == LETHE_F32 ? 4 : 8; }
 
 template <typename F>
 int by_x_type(int xt, F&& f) {
@@ -267,9 +306,15 @@ int by_x_type(int xt, F&& f) {
 }
 
 inline bool norm_types_ok(int xt, int other) { return xt >= LETHE_F32 && xt <= LETHE_F16 && (other == LETHE_F32 || other == xt); }
-// 8 elements of type ty from ptr on can be loaded as 16-byte pieces, in every row
-inline bool piece_aligned(const void* ptr, int, long long s0 = 0, long long s1 = 0) {
-  return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && s0 % 8 == 0 && s1 % 8 == 0;
+// n values of type ty from ptr on can be moved at once, in every row
+inline bool piece_aligned(int n, const void* ptr, int ty, long long s0 = 0, long long s1 = 0) {
+  return reinterpret_cast<uintptr_t>(ptr) % (n * elem_bytes(ty)) == 0 && s0 % n == 0 && s1 % n == 0;
+}
+template <typename F>
+int widest_piece(int widest, int D, F&& fits) {
+  for (int n = widest; n > 1; n /= 2)
+    if (D % n == 0 && fits(n)) return n;
+  return 1;
 }
 inline int norm_grid(long long rows, int rows_per_cta, int ctas_per_sm) {
   const long long need = (rows + rows_per_cta - 1) / rows_per_cta;

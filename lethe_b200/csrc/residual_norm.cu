@@ -30,9 +30,9 @@ struct ResidualProblem {
 
 // CTAs on an SM: registers (64 a thread forward, 128 backward and with two pieces)
 template <typename S> constexpr int residual_ctas(bool backward) { return (backward || S::R > 1 ? 512 : 1024) / S::kThreads; }
-template <int XT, int RT, typename S> using ResidualRing = RowRing<S, S::R * 8 * (elem_bytes(XT) + elem_bytes(RT)), residual_ctas<S>(false)>;
+template <int XT, int RT, typename S> using ResidualRing = RowRing<S, S::R * 8 * (elem_bytes(XT) + elem_bytes(RT)), residual_ctas<S>(false), std::min(elem_bytes(XT), elem_bytes(RT))>;
 template <int XT, int RT, typename S, int BRANCH>
-using ResidualRingBack = RowRing<S, S::R * 8 * (elem_bytes(XT) * (BRANCH ? 2 : 1) + 2 * elem_bytes(RT)), residual_ctas<S>(true)>;
+using ResidualRingBack = RowRing<S, S::R * 8 * (elem_bytes(XT) * (BRANCH ? 2 : 1) + 2 * elem_bytes(RT)), residual_ctas<S>(true), std::min(elem_bytes(XT), elem_bytes(RT))>;
 
 template <int XT, int RT, typename S, bool POST>
 __global__ void __launch_bounds__(S::kThreads, residual_ctas<S>(false)) residual_norm_kernel(const ResidualProblem p) {
@@ -284,10 +284,12 @@ extern "C" int lethe_gdn_residual_norm(const LetheGdnResidualNormArgs* a, void* 
   if (int e = residual_problem(a, &p, false)) return e;
   DeviceGuard guard(a->r);
   if (!guard.ok) return kErrDevice;
-  const bool vec = p.D % 8 == 0 && piece_aligned(p.x, a->x_type, p.x_stride) && piece_aligned(p.res, a->r_type, p.res_stride) &&
-                   piece_aligned(p.r, a->r_type) && piece_aligned(p.y, a->x_type);
+  const int w = widest_piece(widest_of(a->x_type, a->r_type), p.D, [&](int n) {
+    return piece_aligned(n, p.x, a->x_type, p.x_stride) && piece_aligned(n, p.res, a->r_type, p.res_stride) && piece_aligned(n, p.r, a->r_type) &&
+           piece_aligned(n, p.y, a->x_type);
+  });
   return by_stream_type(a->x_type, a->r_type, [&](auto x, auto r) {
-    return by_row_shape(p.D, vec, [&](auto s) {
+    return by_row_shape<widest_of(x.value, r.value)>(p.D, w, [&](auto s) {
       using S = decltype(s);
       const int grid = norm_grid(p.rows, S::kRows, residual_ctas<S>(false));
       constexpr int smem = ResidualRing<x.value, r.value, S>::kBytes;
@@ -325,14 +327,16 @@ extern "C" int lethe_gdn_residual_norm_vjp(const LetheGdnResidualNormArgs* a, vo
   DeviceGuard guard(a->r);
   if (!guard.ok) return kErrDevice;
   const int branch = p.pw ? 2 : a->dscale ? 1 : 0;
-  const bool vec = p.D % 8 == 0 && (!branch || piece_aligned(p.x, a->x_type, p.x_stride)) && piece_aligned(p.r, a->r_type) &&
-                   piece_aligned(p.dy, a->x_type) && piece_aligned(p.dr, a->r_type) && piece_aligned(p.dx, a->x_type) && piece_aligned(p.dres, a->r_type);
+  const int w = widest_piece(widest_of(a->x_type, a->r_type), p.D, [&](int n) {
+    return (!branch || piece_aligned(n, p.x, a->x_type, p.x_stride)) && piece_aligned(n, p.r, a->r_type) && piece_aligned(n, p.dy, a->x_type) &&
+           piece_aligned(n, p.dr, a->r_type) && piece_aligned(n, p.dx, a->x_type) && piece_aligned(n, p.dres, a->r_type);
+  });
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int grid = 0;
   const auto run = [&](auto kind) {
     constexpr int kBranch = decltype(kind)::value;
     return by_stream_type(a->x_type, a->r_type, [&](auto x, auto r) {
-      return by_row_shape(p.D, vec, [&](auto s) {
+      return by_row_shape<widest_of(x.value, r.value)>(p.D, w, [&](auto s) {
         using S = decltype(s);
         grid = std::min(norm_grid(p.rows, S::kRows, residual_ctas<S>(true)), norm_parts_max(p.D));
         const auto kern = residual_norm_vjp_kernel<x.value, r.value, S, kBranch>;
