@@ -279,6 +279,7 @@ template <int WIDEST, typename F>
 int by_row_shape(int D, int w, F&& f) {
   const auto few = [&](auto n) {
     constexpr int W = decltype(n)::value;
+    if (D <= 128) return f(RowShape<16, 1, W>());
     if (D <= 256) return f(RowShape<32, 1, W>());
     if (D <= 1024) return f(RowShape<128, 1, W>());
     if (D <= 4096) return f(RowShape<512, 1, W>());
