@@ -125,12 +125,10 @@ template <int S, int WORDS> struct Cells {
     if constexpr (kBytes >= 4) {
 #pragma unroll
       for (int i = 0; i < kPer / W; ++i) copy<kBytes>(s, i, p + i * (kLanes * W), kBytes);
-    } else {
-      fetch<TY, W>(s, p, p, kChannels);
     }
   }
   // ... and where `room` channels do, from this thread's first on (0: no token); `base`: the tensor, an address that is good where nothing is
-  // read.  Two bytes are no asynchronous copy: those elements are loaded and put here.
+  // read.  (Two bytes are no asynchronous copy: load_all.)
   template <int TY, int W>
   __device__ __forceinline__ void fetch(int s, const typename Elem<TY>::T* p, const void* base, int room) {
     constexpr int kBytes = W * elem_bytes(TY);
@@ -140,13 +138,22 @@ template <int S, int WORDS> struct Cells {
         const bool any = i * (kLanes * W) < room;
         copy<kBytes>(s, i, any ? p + i * (kLanes * W) : base, any ? kBytes : 0);
       }
-    } else {
-      Raw<TY, kPer> r;
-      r.zero();
+    }
+  }
+  // All steps of a thread element by element, loads first.
+  template <int TY, int W>
+  __device__ __forceinline__ void load_all(const typename Elem<TY>::T* p, long long stride, int live, int room) {
+    if constexpr (W * elem_bytes(TY) < 4) {
+      Raw<TY, kPer> r[S];
 #pragma unroll
-      for (int j = 0; j < kPer; ++j)
-        if (j * kLanes < room) raw_put(r, j, __ldg(p + j * kLanes));
-      put(s, r);
+      for (int s = 0; s < S; ++s) {
+        r[s].zero();
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+          if (s < live && j * kLanes < room) raw_put(r[s], j, __ldg(p + s * stride + j * kLanes));
+      }
+#pragma unroll
+      for (int s = 0; s < S; ++s) put(s, r[s]);
     }
   }
   template <int BYTES>
@@ -479,6 +486,8 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_forward_kernel(const Dia
         tile.x.template fetch<XT, W>(s, x0 + t.x + s * p.x_token, p.x, room);
         tile.c.template fetch<GT, W>(s, g0 + t.g + s * p.g_token, p.g, room);
       }
+      tile.x.template load_all<XT, W>(x0 + t.x, p.x_token, t.live - grp * S, t.room - lane * W);
+      tile.c.template load_all<GT, W>(g0 + t.g, p.g_token, t.live - grp * S, t.room - lane * W);
     }
     commit();
   };
@@ -558,6 +567,10 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_forward_kernel(const Dia
       if (whole) store_token<XT, W>(packed<XT>(st), h, kChannels);
       else if (s < live) store_token<XT, W>(packed<XT>(st), h, room);
       h += p.D;
+    }
+    if (more) {
+      tile.x.template load_all<XT, W>(x0 + after.x, p.x_token, live_n, room_n);
+      tile.c.template load_all<GT, W>(g0 + after.g, p.g_token, live_n, room_n);
     }
     commit();
   }
@@ -662,6 +675,9 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_backward_kernel(const Di
         tile.c.template fetch<GT, W>(s, g0 + t.g + s * p.g_token, p.g, room);
         if (p.d_h) tile.d.template fetch<XT, W>(s, d0 + t.d + s * p.d_token, p.d_h, room);
       }
+      tile.x.template load_all<XT, W>(x0 + t.x, p.x_token, t.live - grp * S, t.room - lane * W);
+      tile.c.template load_all<GT, W>(g0 + t.g, p.g_token, t.live - grp * S, t.room - lane * W);
+      if (p.d_h) tile.d.template load_all<XT, W>(d0 + t.d, p.d_token, t.live - grp * S, t.room - lane * W);
     }
     commit();
   };
@@ -798,6 +814,11 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_backward_kernel(const Di
       }
       dx -= p.D;
       dg -= p.D;
+    }
+    if (more) {
+      tile.x.template load_all<XT, W>(x0 + after.x, p.x_token, live_n, room_n);
+      tile.c.template load_all<GT, W>(g0 + after.g, p.g_token, live_n, room_n);
+      if (p.d_h) tile.d.template load_all<XT, W>(d0 + after.d, p.d_token, live_n, room_n);
     }
     commit();
   }
