@@ -2,10 +2,11 @@
 //
 // A row of D values is held by T threads with R pieces of 8 values each (T R 8 >= D) and stays in registers from its loads to its
 // stores; a CTA has one row at a time, or as many as fill 256 threads.  Sums over up to a warp are butterflies, beyond that the warps of a
-// row, sums go through shared memory.  CTAs go over the rows with the grid's stride, so that what belongs to a column (weights,
-// sums for their gradients) stays in registers as well, and the next rows are under way by asynchronous copies (RowRing): with loads at
-// the head of each turn instead, residual_norm of 16384 x 4096 bf16 took 132 us forward and 267 backward.  Sums over rows: a CTA's share in the order of its rows, the CTAs'
-// shares by a kernel of its own in the order of the CTAs.  No atomics: two runs give the same bits.
+// row meet in shared memory.  CTAs go over the rows with the grid's stride, so that what belongs to a column (weights, sums for their
+// gradients) stays in registers as well, and the next rows are under way by asynchronous copies (RowRing): with loads at the head of
+// each turn instead, residual_norm of 16384 x 4096 bf16 took 132 us forward and 267 backward, against 92 and 167 with the ring alone.
+// Sums over rows: a CTA's share in the order of its rows, the CTAs' shares by a kernel of its own in the order of the CTAs.  No
+// atomics: two runs give the same bits.
 #pragma once
 #include <algorithm>
 #include <type_traits>

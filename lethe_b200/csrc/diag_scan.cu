@@ -1,11 +1,13 @@
 // The element-wise gated recurrence h_t = e^{g_t} h_{t-1} + x_t (or + (1 - e^{g_t}) x_t), its backward, and one token of it.
 //
-// Bound by HBM: some 10 to 20 operations for every 8 bytes forward (bf16 x and h, fp32 g) and 14 backward.
+// Bound by HBM on paper: 8 bytes an element forward (bf16 x and h, fp32 g), 14 backward.  Measured (B1 L65536 D2048): 226 us forward, 0.73 of the
+// measured copy bandwidth, 425 backward, 0.68; without any tile waiting for another (1024 sequences of 128 tokens) 209 and 404, so
+// most of what is missing is the runs themselves, some 33 and 60 operations an element by 16 warps of an SM, not the handing on.
 //
 // A CTA does tiles, 16 groups of tokens x 64 channels of one sequence, each read once: a thread has 3 to 8 tokens of four channels, its
-// 16-lane group covers the channels.  Every thread runs its own tokens from a zero state, the groups' results (sum of g, state) meet in shared memory and are folded in order, the tile gets the state in front of it from the tiles before (below), and
-// every thread runs its tokens again from the state that it really starts from.  The order of all sums is fixed, so two runs give
-// the same bits.
+// 16-lane group covers the channels.  Every thread runs its own tokens from a zero state, the groups' results (sum of g, state) meet in
+// shared memory and are folded in order, the tile gets the state in front of it from the tiles before (below), and every thread runs
+// its tokens again from the state that it really starts from.  The order of all sums is fixed, so two runs give the same bits.
 //
 // The decay.  With memories of thousands of tokens e^g lies next to one, and fp32 rounds it by up to 2^-25: over n tokens the
 // state is off by up to n times that, always to the same side where g is constant.  So below |g| = 1/4 the step is taken with
@@ -390,10 +392,13 @@ constexpr int kPartsThreads = kRunners + kChannels, kOutThreads = 2 * kChannels,
 // done is one that its CTA has begun or begins next, so somebody always can go on.
 //
 // Runners go over a tile's tokens twice, and over those of the next tile the first time before they go over this one the second time.
-// A publisher folds a tile's parts and lets its word go out, lookers wait for the words of others.  So a tile's word waits for nobody,
-// and looking back has the time of a run.  Before, with all of it in one order, the CTAs ran in step, all computing or all waiting
-// (B1 L65536 D2048 bf16 forward 294 us, with issue slots half empty), and with folding and looking in the same warps a word
-// waited for the words that the tile before it waited for (299 us; the lookers of every second tile waited 16 k cycles).
+// Publishers fold a tile's parts and let its word go out, lookers wait for the words of others.  So a tile's word waits for nobody,
+// and looking back has the time of a run.  Steps on the way (B1 L65536 D2048 bf16, forward / backward in us): tiles in registers, two CTAs on
+// an SM, 462 / 651; the next tile by asynchronous copies and fewer operations 344 / 462; folding and looking in warps of their own,
+// a word behind the looking of the tile before it, 299 / 700; as it is 239 / 475; two channels by one instruction and the places of a
+// tile worked out once 226 / 425.  Left: whole tiles by tensor-map copies 240 / 490, four small CTAs without roles 627 / 569, one
+// more ticket ahead 255 / 506, tiles fetched to L2 row by row 388 / 638, tickets dealt out beforehand in a cooperative launch 228 / 470
+// (B2 L2048 D1024 14.5 + 21.1 against 15.6 + 23).
 template <int XT, int GT, int W, bool COMP>
 __global__ void __launch_bounds__(kScanThreads, 2) diag_forward_kernel(const DiagProblem p) {
   using X = typename Elem<XT>::T;

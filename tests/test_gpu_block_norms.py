@@ -247,6 +247,42 @@ def test_residual_norm_strides():
             assert all(torch.equal(got[n], want[n]) for n in want)
 
 
+def test_one_row_without_further_dimensions():
+    x, w = randn(96, seed=1), randn(96, seed=2)
+    assert torch.equal(ops.gated_norm(x, x, w), ops.gated_norm(x[None], x[None], w)[0])
+    for a, b in zip(ops.residual_norm(x, x, w), ops.residual_norm(x[None], x[None], w)):
+        assert torch.equal(a, b[0])
+
+
+def test_the_same_tensor_twice():
+    x, w, dy, dr = randn(7, 64, seed=1, dt=torch.bfloat16), randn(64, seed=2, dt=torch.bfloat16), randn(7, 64, seed=3, dt=torch.bfloat16), randn(7, 64, seed=4, dt=torch.bfloat16)
+    a, b, leaf = x.clone().requires_grad_(True), x.clone().requires_grad_(True), x.clone().requires_grad_(True)
+    for f, d in ((lambda s, t: ops.residual_norm(s, t, w), (dy, dr)), (lambda s, t: (ops.gated_norm(s, t, w),), (dy,))):
+        da, db = torch.autograd.grad(f(a, b), (a, b), d)
+        both, = torch.autograd.grad(f(leaf, leaf), leaf, d)
+        assert torch.equal(both, da + db)
+
+
+def test_second_derivatives_are_refused():
+    x, w = randn(5, 64).requires_grad_(True), randn(64)
+    for f in (lambda: ops.gated_norm(x, x.detach(), w), lambda: ops.residual_norm(x, None, w)[0]):
+        d, = torch.autograd.grad(f(), x, torch.ones_like(x).requires_grad_(True), create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            d.sum().backward()
+
+
+def test_what_is_not_finite_stays_in_its_row():
+    x, z, w, dy = (randn(9, 200, seed=i, dt=torch.bfloat16) for i in range(4))
+    w = w[0].float()
+    want, wantr = ops.gated_norm(x, z, w), ops.residual_norm(x, z, w, scale=w, post_weight=w)
+    x[4, 3] = float("nan")
+    got, gotr = ops.gated_norm(x, z, w), ops.residual_norm(x, z, w, scale=w, post_weight=w)
+    keep = [i for i in range(9) if i != 4]
+    assert bool(got[4].isnan().all()) and torch.equal(got[keep], want[keep])
+    for a, b in zip(gotr, wantr):
+        assert bool(a[4].isnan().all()) and torch.equal(a[keep], b[keep])
+
+
 def test_empty_rows():
     x = torch.zeros(0, 3, 64, device="cuda", requires_grad=True)
     w = torch.ones(64, device="cuda", requires_grad=True)

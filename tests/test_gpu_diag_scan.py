@@ -230,6 +230,46 @@ def test_a_reset_forgets_the_tokens_before():
         assert bool((whole["dg"][:, cut] == 0).all())
 
 
+def test_what_is_not_finite_stays_in_its_channel():
+    x, g, h0, dh, dhT = make(2, 700, (70,), "f32")
+    want = run(x, g, h0, dh, dhT, True)
+    for bad in (float("nan"), float("inf")):
+        xb, db = x.clone(), dh.clone()
+        xb[1, 300, 7] = bad
+        db[0, 400, 65] = bad
+        got = run(xb, g, h0, db, dhT, True)
+        clean = torch.ones(2, 70, dtype=torch.bool, device="cuda")
+        clean[1, 7] = clean[0, 65] = False
+        for n in ("h", "dx", "dg"):
+            assert torch.equal(got[n].transpose(1, 2)[clean], want[n].transpose(1, 2)[clean]), n
+        for n in ("hT", "dh0"):
+            assert torch.equal(got[n][clean], want[n][clean]), n
+        assert torch.equal(got["h"][1, :300, 7], want["h"][1, :300, 7]) and not bool(got["h"][1, 300:, 7].isfinite().any())
+        assert torch.equal(got["dx"][0, 401:, 65], want["dx"][0, 401:, 65]) and not bool(got["dx"][0, :401, 65].isfinite().any())
+
+
+def test_padding_leaves_the_state():
+    """x = 0 and g = 0 behind a sequence's end; with the complement any x."""
+    x, g, h0, _, _ = make(1, 500, (64,), "bf16")
+    for complement in (False, True):
+        for end in (1, 130, 384, 499):
+            xp, gp = x.clone(), g.clone()
+            gp[:, end:] = 0
+            if not complement:
+                xp[:, end:] = 0
+            h, hT = ops.diag_scan(xp, gp, h0, complement=complement)
+            # as many tokens, so the same tiles
+            assert torch.equal(h[:, :end], ops.diag_scan(x, g, h0, complement=complement)[0][:, :end])
+            assert torch.equal(hT.to(h.dtype), h[:, -1]) and float((h[:, end - 1].float() - hT).abs().max()) <= 2 ** -7 * float(hT.abs().max())
+
+
+def test_long_and_many():
+    """Groups of groups of tiles, and more sequences than 65535."""
+    x, g, h0, dh, dhT = make(1, 20000, (8,), "f32", "long")
+    check(x, g, h0, dh, dhT, False)
+    check(*make(70000, 2, (3,), "bf16", "kinds"), True)
+
+
 def test_two_runs_and_captured_replays_give_the_same_bits():
     x, g, h0, dh, dhT = make(2, 3000, (200,))
     want = run(x, g, h0, dh, dhT, True)
