@@ -33,7 +33,7 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-use_fast_math",
          "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr", "-I", os.path.join(ROOT, "include"), "-I", CSRC]
 # Not for these: their exponentials and roots stand in fp32 results.
-EXACT_MATH = {"diag_scan.cu", "block_norm.cu", "residual_norm.cu"}
+EXACT_MATH = {"diag_scan.cu", "block_norm.cu", "residual_norm.cu", "residual_norm_vjp.cu"}
 FLAGS += os.environ.get("LETHE_NVCC_FLAGS", "").split()
 
 
