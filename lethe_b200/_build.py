@@ -1,7 +1,7 @@
 """Build recipe for the CUDA library: every ``csrc/*.cu`` is compiled for sm_100a and linked into
 ``lethe_b200/_lib/liblethe_gdn.so`` (kept in-tree so that it travels with the checkout).
 
-``build_probe()`` builds the test-only self-test kernels of ``tests/native/probe.cu`` into
+``build_probe()`` builds the test-only self-test kernels of ``tests/native/*probe.cu`` into
 ``tests/native/_lib/libletheprobe.so``; the product library does not contain them.
 
 Several processes may call ``build()`` at once (one rank per GPU under ``torchrun``): the work is done
@@ -21,6 +21,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "_lib")
 LIB = os.path.join(LIBDIR, "liblethe_gdn.so")
 PROBE_SRC = os.path.join(ROOT, "tests", "native", "probe.cu")
+PROBE_SRCS = [PROBE_SRC, os.path.join(ROOT, "tests", "native", "look_probe.cu")]
 PROBE_LIBDIR = os.path.join(ROOT, "tests", "native", "_lib")
 PROBE_LIB = os.path.join(PROBE_LIBDIR, "libletheprobe.so")
 TORCH_SRCS = [os.path.join(CSRC, f) for f in ("torch_ops.cpp", "torch_block.cpp")]
@@ -153,8 +154,9 @@ def build_probe(force: bool = False, verbose: bool = False) -> str:
     with _Lock(os.path.join(PROBE_LIBDIR, ".build.lock")):
         if not force and fresh():
             return PROBE_LIB
-        obj = _compile(PROBE_SRC, os.path.join(PROBE_LIBDIR, "probe.o"), verbose)
-        _link([obj], PROBE_LIB)
+        with ThreadPoolExecutor(max_workers=len(PROBE_SRCS)) as ex:
+            objs = list(ex.map(lambda s: _compile(s, os.path.join(PROBE_LIBDIR, os.path.basename(s)[:-3] + ".o"), verbose), PROBE_SRCS))
+        _link(objs, PROBE_LIB)
     return PROBE_LIB
 
 

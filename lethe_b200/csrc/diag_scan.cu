@@ -16,6 +16,7 @@
 // coefficient whose sign bit says whether h is added (c <= -0) or not (e^g >= +0).  Decays of several tokens are kept as sums of g.
 #include <type_traits>
 
+#include "diag_look.cuh"
 #include "elem.cuh"
 #include "host_util.h"
 
@@ -85,10 +86,6 @@ __device__ __forceinline__ void decay_over(float c0, float c1, float& h0, float&
 }
 __device__ __forceinline__ float forgotten(float c) { return is_diff(c) ? -c : 1.f - c; }      // 1 - e^g
 
-struct LookBuffer {
-  uint32_t* head;                   // ticket, and the word that lets everybody pass
-  unsigned long long* word[3];      // of tiles, groups of tiles, groups of groups
-};
 struct DiagProblem {
   long long B, L, D;
   const void* x;
@@ -212,9 +209,6 @@ __device__ __forceinline__ Raw<TY, kPer> packed(const float (&v)[kPer]) {
 // bounded all the same: one that runs out leaves a code in the status word and lets everybody pass.
 // ---------------------------------------------------------------------------------------------
 constexpr int kFan = 8;
-constexpr long long kLookLimitCycles = 2000000000LL;      // about one second
-enum : int { kSiteLook = 900 };
-
 constexpr size_t kLookHead = 128;
 struct LookSizes {
   size_t count[3];
@@ -224,31 +218,6 @@ static LookSizes look_sizes(long long seqs, long long tiles) {
   if (tiles <= 1) return {{0, 0, 0}};
   const long long groups = (tiles + kFan - 1) / kFan, supers = (groups + kFan - 1) / kFan;
   return {{static_cast<size_t>(seqs * tiles), static_cast<size_t>(seqs * groups), static_cast<size_t>(seqs * supers)}};
-}
-
-__device__ __forceinline__ unsigned long long look_load(const unsigned long long* p) {
-  unsigned long long v;
-  asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
-  return v;
-}
-__device__ __forceinline__ void look_store(unsigned long long* p, float sum, float state) {
-  unsigned long long v = (static_cast<unsigned long long>(__float_as_uint(state)) << 32) | __float_as_uint(sum);
-  if (v == ~0ull) v = 0x7fffffff7fffffffull;      // (another NaN)
-  asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
-}
-__device__ __noinline__ unsigned long long look_wait(const unsigned long long* p, uint32_t* head, int* status) {
-  const long long t0 = clock64();
-  for (int n = 1;; ++n) {
-    const unsigned long long v = look_load(p);
-    if (v != ~0ull) return v;
-    if (n % 32) continue;
-    if (*reinterpret_cast<volatile uint32_t*>(head + 1) == 0u) return 0;
-    if (clock64() - t0 > kLookLimitCycles) {
-      atomicCAS(status, 0, kSiteLook);
-      *reinterpret_cast<volatile uint32_t*>(head + 1) = 0u;
-      return 0;
-    }
-  }
 }
 
 struct Ticket {
