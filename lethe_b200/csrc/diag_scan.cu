@@ -23,6 +23,7 @@
 namespace lg {
 
 constexpr int kLanes = 16, kPer = 4, kChannels = kLanes * kPer;      // a strip of channels
+constexpr int kPacked = 16;      // among the widths of the kernels: four channels at once, several batches in a strip
 constexpr int kGroups = 16, kRunners = kLanes * kGroups;              // threads that hold a tile
 constexpr int kPublisher = kRunners, kLooker = kPublisher + kChannels;  // first threads of those that hand on and of those that look back
 constexpr int kScanThreads = kLooker + kChannels;
@@ -103,7 +104,9 @@ struct DiagProblem {
   float* dh0;
   int tiles, strips;      // tiles of tokens, strips of kChannels channels
   long long records;      // states of a sequence that the forward keeps: one for every tile of the backward
-  uint32_t seqs;          // B strips
+  uint32_t seqs;          // strips of all batches: B strips, or fewer where a strip holds `pack` batches of D <= 32 channels
+  int pack;
+  size_t look_bytes;
   int* status;
   LookBuffer look;
 };
@@ -224,8 +227,8 @@ struct Ticket {
   int order, tile;               // of the tile in its sequence, as it is folded (from `tiles` on there is none) and from the first token on
   uint32_t seq;                  // sequence: strip of channels of a batch
   int room, live;                // channels of the strip, tokens of the tile
-  long long state;               // where its strip begins in a state [B, D], its first element in x, g, d_h and in what is contiguous
-  long long x, g, d, h;
+  long long state, record;       // where its strip begins in a state [B, D] and among the states that are kept
+  long long x, g, d, h;          // its first element in x, g, d_h and in what is contiguous
 };
 template <int XT, int S> struct ForwardShared {
   struct Tile {
@@ -323,7 +326,7 @@ __device__ __forceinline__ float look_back(const LookPlace& p, int ch, float fir
 }
 
 // One thread takes tickets, and says for all what they stand for.
-template <int S, bool BACK> struct TicketTaker {
+template <int S, bool BACK, bool PACK> struct TicketTaker {
   const DiagProblem& p;
   uint32_t have;      // the last one
   __device__ __forceinline__ void take() { have = p.tiles > 1 ? atomicAdd(p.look.head, 1u) + 1u : have + gridDim.x; }
@@ -332,11 +335,13 @@ template <int S, bool BACK> struct TicketTaker {
     t.order = static_cast<int>(have / p.seqs);
     t.tile = BACK ? p.tiles - 1 - t.order : t.order;
     t.seq = have - t.order * p.seqs;
-    const uint32_t b = t.seq / static_cast<uint32_t>(p.strips);
-    const long long ch0 = static_cast<long long>(t.seq - b * p.strips) * kChannels, t0 = static_cast<long long>(t.tile) * (kGroups * S);
-    t.room = static_cast<int>(p.D - ch0 < kChannels ? p.D - ch0 : kChannels);
+    const long long b = PACK ? static_cast<long long>(t.seq) * p.pack : t.seq / static_cast<uint32_t>(p.strips);
+    const long long ch0 = PACK ? 0 : (t.seq - b * p.strips) * kChannels, t0 = static_cast<long long>(t.tile) * (kGroups * S);
+    const long long there = PACK ? (p.B - b < p.pack ? p.B - b : p.pack) * p.D : p.D - ch0;
+    t.room = static_cast<int>(there < kChannels ? there : kChannels);
     t.live = static_cast<int>(p.L - t0 < kGroups * S ? p.L - t0 : kGroups * S);
     t.state = b * p.D + ch0;
+    t.record = (b * p.records + (BACK ? t.tile : 2 * t.tile)) * p.D + ch0;
     t.x = b * p.x_batch + t0 * p.x_token + ch0;
     t.g = b * p.g_batch + t0 * p.g_token + ch0;
     t.d = b * p.d_batch + t0 * p.d_token + ch0;
@@ -344,10 +349,17 @@ template <int S, bool BACK> struct TicketTaker {
     return t;
   }
 };
+// Where channel `ch` of a strip lies, from the strip's first one on, in a tensor with a stride between batches.
+template <bool PACK>
+__device__ __forceinline__ long long channel_place(const DiagProblem& p, int ch, long long batch) {
+  if constexpr (!PACK) return ch;
+  const int D = static_cast<int>(p.D);
+  return ch / D * batch + ch % D;
+}
 // This thread's first element of a tensor, in a tile whose first element is the tensor's.
 template <int TY>
-__device__ __forceinline__ typename Elem<TY>::T* own_part(const void* tensor, long long token, int first_token, int first_channel) {
-  return static_cast<typename Elem<TY>::T*>(const_cast<void*>(tensor)) + first_token * token + first_channel;
+__device__ __forceinline__ typename Elem<TY>::T* own_part(const void* tensor, long long token, int first_token, long long place) {
+  return static_cast<typename Elem<TY>::T*>(const_cast<void*>(tensor)) + first_token * token + place;
 }
 
 // Barriers from one role to the next, two of each for even and odd tiles: a tile's parts are there (runners to publisher), its word has
@@ -368,13 +380,15 @@ constexpr int kPartsThreads = kRunners + kChannels, kOutThreads = 2 * kChannels,
 // tile worked out once 226 / 425.  Left: whole tiles by tensor-map copies 240 / 490, four small CTAs without roles 627 / 569, one
 // more ticket ahead 255 / 506, tiles fetched to L2 row by row 388 / 638, tickets dealt out beforehand in a cooperative launch 228 / 470
 // (B2 L2048 D1024 14.5 + 21.1 against 15.6 + 23).
-template <int XT, int GT, int W, bool COMP>
+template <int XT, int GT, int WIDTH, bool COMP>
 __global__ void __launch_bounds__(kScanThreads, 2) diag_forward_kernel(const DiagProblem p) {
+  constexpr bool PACK = WIDTH == kPacked;
+  constexpr int W = PACK ? kPer : WIDTH;
   using X = typename Elem<XT>::T;
   constexpr int S = forward_steps(XT);
   extern __shared__ __align__(16) unsigned char smem[];
   auto& sh = *reinterpret_cast<ForwardShared<XT, S>*>(smem);
-  TicketTaker<S, false> tickets{p, blockIdx.x - gridDim.x};
+  TicketTaker<S, false, PACK> tickets{p, blockIdx.x - gridDim.x};
   const bool taker = threadIdx.x == kPublisher;
   if (taker) {
     tickets.take();
@@ -385,6 +399,7 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_forward_kernel(const Dia
   __syncthreads();
   if (threadIdx.x >= kLooker) {
     const int ch = threadIdx.x - kLooker;
+    const long long record_of = channel_place<PACK>(p, ch, p.records * p.D);
     for (int n = 0;; ++n) {
       const Ticket cur = sh.ticket[n & 3];
       if (cur.order >= p.tiles) break;
@@ -408,7 +423,7 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_forward_kernel(const Dia
       bar_arrive<kStartsThreads>(kBarStarts + (n & 1));
       if (p.tiles > 1 && look.closes_super()) look_store(look.at(2, look.super, ch), 0.f, carry);
       if (p.states && ch < cur.room) {
-        float* to = p.states + (cur.seq / p.strips * p.records + 2 * cur.tile) * p.D + cur.seq % p.strips * kChannels + ch;
+        float* to = p.states + cur.record + record_of;
         to[0] = entry;
         if (2 * cur.tile + 1 < p.records) to[p.D] = middle;
       }
@@ -448,9 +463,9 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_forward_kernel(const Dia
   const int lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
   const auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
   using GE = typename Elem<GT>::T;
-  const X* const x0 = own_part<XT>(p.x, p.x_token, grp * S, lane * W);
-  const GE* const g0 = own_part<GT>(p.g, p.g_token, grp * S, lane * W);
-  X* const h0 = own_part<XT>(p.h, p.D, grp * S, lane * W);
+  const X* const x0 = own_part<XT>(p.x, p.x_token, grp * S, channel_place<PACK>(p, lane * W, p.x_batch));
+  const GE* const g0 = own_part<GT>(p.g, p.g_token, grp * S, channel_place<PACK>(p, lane * W, p.g_batch));
+  X* const h0 = own_part<XT>(p.h, p.D, grp * S, channel_place<PACK>(p, lane * W, p.L * p.D));
   const auto fetch = [&](const Ticket& t, int slot) {
     if (t.order < p.tiles) {
       auto& tile = sh.tile[slot];
@@ -550,14 +565,16 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_forward_kernel(const Dia
   }
 }
 
-template <int XT, int GT, int W, bool COMP>
+template <int XT, int GT, int WIDTH, bool COMP>
 __global__ void __launch_bounds__(kScanThreads, 2) diag_backward_kernel(const DiagProblem p) {
+  constexpr bool PACK = WIDTH == kPacked;
+  constexpr int W = PACK ? kPer : WIDTH;
   using X = typename Elem<XT>::T;
   using G = typename Elem<GT>::T;
   constexpr int S = backward_steps(XT);
   extern __shared__ __align__(16) unsigned char smem[];
   auto& sh = *reinterpret_cast<BackwardShared<XT, S>*>(smem);
-  TicketTaker<S, true> tickets{p, blockIdx.x - gridDim.x};
+  TicketTaker<S, true, PACK> tickets{p, blockIdx.x - gridDim.x};
   const bool taker = threadIdx.x == kPublisher;
   if (taker) {
     tickets.take();
@@ -568,6 +585,7 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_backward_kernel(const Di
   __syncthreads();
   if (threadIdx.x >= kLooker) {
     const int ch = threadIdx.x - kLooker;
+    const long long record_of = channel_place<PACK>(p, ch, p.records * p.D);
     for (int n = 0;; ++n) {
       const Ticket cur = sh.ticket[n & 3];
       if (cur.order >= p.tiles) break;
@@ -576,7 +594,7 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_backward_kernel(const Di
       auto& back = sh.back[n & 1];
       const long long state_at = cur.state + ch;
       float carry = ch < cur.room && p.dhT ? p.dhT[state_at] : 0.f;
-      float st = ch < cur.room ? p.states[(cur.seq / p.strips * p.records + cur.tile) * p.D + cur.seq % p.strips * kChannels + ch] : 0.f;
+      float st = ch < cur.room ? p.states[cur.record + record_of] : 0.f;
       bar_sync<kOutThreads>(kBarOut + (n & 1));
       if (p.tiles > 1) carry = look_back(look, ch, carry, p.status);
       float2 own[kGroups];
@@ -634,11 +652,11 @@ __global__ void __launch_bounds__(kScanThreads, 2) diag_backward_kernel(const Di
   const int lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
   const auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
   using GE = typename Elem<GT>::T;
-  const X* const x0 = own_part<XT>(p.x, p.x_token, grp * S, lane * W);
-  const GE* const g0 = own_part<GT>(p.g, p.g_token, grp * S, lane * W);
-  const X* const d0 = own_part<XT>(p.d_h, p.d_token, grp * S, lane * W);
-  X* const dx0 = own_part<XT>(p.dx, p.D, grp * S, lane * W);
-  G* const dg0 = own_part<GT>(p.dg, p.D, grp * S, lane * W);
+  const X* const x0 = own_part<XT>(p.x, p.x_token, grp * S, channel_place<PACK>(p, lane * W, p.x_batch));
+  const GE* const g0 = own_part<GT>(p.g, p.g_token, grp * S, channel_place<PACK>(p, lane * W, p.g_batch));
+  const X* const d0 = own_part<XT>(p.d_h, p.d_token, grp * S, channel_place<PACK>(p, lane * W, p.d_batch));
+  X* const dx0 = own_part<XT>(p.dx, p.D, grp * S, channel_place<PACK>(p, lane * W, p.L * p.D));
+  G* const dg0 = own_part<GT>(p.dg, p.D, grp * S, channel_place<PACK>(p, lane * W, p.L * p.D));
   const auto fetch = [&](const Ticket& t, int slot) {
     if (t.order < p.tiles) {
       auto& tile = sh.tile[slot];
@@ -855,6 +873,7 @@ template <typename F>
 static int by_type(int xt, int gt, int w, bool comp, F&& f) {
   const auto flags = [&](auto x, auto g) {
     const auto last = [&](auto n) { return comp ? f(x, g, n, std::true_type()) : f(x, g, n, std::false_type()); };
+    if (w == kPacked) return last(std::integral_constant<int, kPacked>());
     if (w == 4) return last(std::integral_constant<int, 4>());
     if (w == 2) return last(std::integral_constant<int, 2>());
     return last(std::integral_constant<int, 1>());
@@ -881,12 +900,13 @@ static int diag_problem(const LetheGdnDiagArgs* a, DiagProblem* p, bool backward
   if (strips > INT32_MAX || a->B > INT32_MAX / strips || tiles > INT32_MAX / (a->B * strips)) return kErrDims;
   *p = {a->B, a->L, a->D, a->x, a->x_batch, a->x_token, a->g, a->g_batch, a->g_token, a->h0, a->h, a->hT, a->states, a->d_h, a->d_h_batch,
         a->d_h_token, a->dhT, a->dx, a->dg, a->dh0, static_cast<int>(tiles), static_cast<int>(strips), tiles_of(a->L, a->x_type, true),
-        static_cast<uint32_t>(a->B * strips), a->status, {}};
+        static_cast<uint32_t>(a->B * strips), 1, 0, a->status, {}};
   if (tiles > 1) {
     if (!a->work) return kErrNull;
     if (reinterpret_cast<uintptr_t>(a->work) & 15) return kErrAlign;
     const LookSizes n = look_sizes(p->seqs, tiles);
     if (a->work_bytes < n.bytes()) return kErrWorkspace;
+    p->look_bytes = n.bytes();
     p->look.head = static_cast<uint32_t*>(a->work);
     p->look.word[0] = reinterpret_cast<unsigned long long*>(static_cast<char*>(a->work) + kLookHead);
     for (int i = 1; i < 3; ++i) p->look.word[i] = p->look.word[i - 1] + n.count[i - 1] * kChannels;
@@ -897,11 +917,21 @@ static int diag_problem(const LetheGdnDiagArgs* a, DiagProblem* p, bool backward
 template <typename F>
 static int widest(F&& fits) { return fits(4) ? 4 : fits(2) ? 2 : 1; }
 
+// Few channels: a strip of 64 takes those of as many batches as fit (bf16, forward + backward in us, one batch / as many: 64 x 16384 x 8
+// 104 + 191 / 39 + 56, 16 x 16384 x 32 37 + 62 / 27 + 42).  A kernel of its own: with the places of a channel open at run time the others
+// spill (B1 L65536 D2048 backward 424 / 442).
+static int pack_batches(DiagProblem* p, int w) {
+  if (w != kPer || p->D > kChannels / 2 || p->B < 2) return w;
+  p->pack = static_cast<int>(kChannels / p->D);
+  p->seqs = static_cast<uint32_t>((p->B + p->pack - 1) / p->pack);
+  return kPacked;
+}
+
 template <typename Shared>
 static int launch_scan_tiles(void (*kern)(DiagProblem), const DiagProblem& p, SmemAttr& attr, cudaStream_t st) {
   if (int e = attr.set(kern, sizeof(Shared))) return e;
   // all ones: no word is there yet, and the ticket before the first
-  if (p.tiles > 1 && cudaMemsetAsync(p.look.head, 0xff, look_sizes(p.seqs, p.tiles).bytes(), st) != cudaSuccess) return kErrLaunch;
+  if (p.tiles > 1 && cudaMemsetAsync(p.look.head, 0xff, p.look_bytes, st) != cudaSuccess) return kErrLaunch;
   const uint32_t total = p.seqs * static_cast<uint32_t>(p.tiles), room = static_cast<uint32_t>(2 * sm_count());
   kern<<<total < room ? total : room, kScanThreads, sizeof(Shared), st>>>(p);
   return launched();
@@ -931,7 +961,8 @@ extern "C" int lethe_gdn_diag_forward(const LetheGdnDiagArgs* a, void* stream) {
     return a->D % n == 0 && on_boundary(a->x, a->x_type, n, a->x_batch, a->x_token) && on_boundary(a->g, a->g_type, n, a->g_batch, a->g_token) &&
            on_boundary(a->h, a->x_type, n);
   });
-  return by_type(a->x_type, a->g_type, w, a->complement != 0, [&](auto x, auto g, auto n, auto c) {
+  const int width = pack_batches(&p, w);
+  return by_type(a->x_type, a->g_type, width, a->complement != 0, [&](auto x, auto g, auto n, auto c) {
     static SmemAttr attr;
     return launch_scan_tiles<ForwardShared<x.value, forward_steps(x.value)>>(diag_forward_kernel<x.value, g.value, n.value, c.value>, p, attr, static_cast<cudaStream_t>(stream));
   });
@@ -947,7 +978,8 @@ extern "C" int lethe_gdn_diag_backward(const LetheGdnDiagArgs* a, void* stream) 
     return a->D % n == 0 && on_boundary(a->x, a->x_type, n, a->x_batch, a->x_token) && on_boundary(a->g, a->g_type, n, a->g_batch, a->g_token) &&
            on_boundary(a->d_h, a->x_type, n, a->d_h_batch, a->d_h_token) && on_boundary(a->dx, a->x_type, n) && on_boundary(a->dg, a->g_type, n);
   });
-  return by_type(a->x_type, a->g_type, w, a->complement != 0, [&](auto x, auto g, auto n, auto c) {
+  const int width = pack_batches(&p, w);
+  return by_type(a->x_type, a->g_type, width, a->complement != 0, [&](auto x, auto g, auto n, auto c) {
     static SmemAttr attr;
     return launch_scan_tiles<BackwardShared<x.value, backward_steps(x.value)>>(diag_backward_kernel<x.value, g.value, n.value, c.value>, p, attr, static_cast<cudaStream_t>(stream));
   });

@@ -176,6 +176,24 @@ def test_strided_inputs_are_read_where_they_lie():
     assert torch.allclose(dg, each.sum((0, 2), keepdim=True), rtol=1e-4, atol=1e-3)      # (torch's sum over 144 values)
 
 
+@pytest.mark.parametrize("types", ["f32", "bf16", "f16 g"])
+@pytest.mark.parametrize("B,L,D", [(2, 300, 32), (5, 257, 8), (17, 130, 4), (7, 1000, 24), (3, 64, 28), (40, 500, 12), (900, 40, 16), (2, 2000, 20)])
+def test_few_channels_of_many_sequences(types, B, L, D):
+    """Batches side by side in a strip, the last strip not full."""
+    check(*make(B, L, (D,), types, "kinds"), True)
+    x, g, h0, dh, dhT = make(B, L, (D,), types)
+    proj = torch.zeros(B, L + 3, 2 * D + 8, dtype=x.dtype, device="cuda")       # another stride for every tensor
+    proj[:, 2:L + 2, 8:D + 8] = x
+    want, got = run(x, g, h0, dh, dhT, False), {}
+    leaves = [proj[:, 2:L + 2, 8:D + 8].detach().requires_grad_(True), g.transpose(0, 1).contiguous().transpose(0, 1).requires_grad_(True), h0.clone().requires_grad_(True)]
+    h, hT = ops.diag_scan(*leaves)
+    got.update(h=h, hT=hT, **dict(zip(("dx", "dg", "dh0"), torch.autograd.grad((h, hT), leaves, (dh, dhT)))))
+    assert all(torch.equal(got[n], want[n]) for n in want)
+    # a sequence by itself gives the bits that it has among others
+    one = run(x[1:2], g[1:2], h0[1:2], dh[1:2], dhT[1:2], False)
+    assert all(torch.equal(one[n], want[n][1:2]) for n in want)
+
+
 def test_offsets_beyond_32_bits():
     big = torch.empty(3 * (1 << 30) + 64, dtype=torch.bfloat16, device="cuda")
     x, g, h0, dh, dhT = make(1, 3, (64,))
