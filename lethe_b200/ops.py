@@ -555,6 +555,20 @@ class _Traced(torch.autograd.Function):
         return (None, None, None, *(next(got) if w else None for w in ctx.wanted))
 
 
+class _TracedStep(torch.autograd.Function):
+    """The same for one token: the call updates its last tensor in place and has no gradient."""
+
+    @staticmethod
+    def forward(ctx, call, option, *tensors):
+        out = getattr(native.ext(), call)(*tensors, option)
+        ctx.mark_non_differentiable(out)
+        return out
+
+    @staticmethod
+    def backward(ctx, grad):      # (never asked for)
+        return (None,) * len(ctx.needs_input_grad)
+
+
 def gdn_chunk(q: Tensor, k: Tensor, v: Tensor, g: Tensor | None, beta: Tensor | None,
               h0: Tensor | None = None, *, scale: float | None = None,
               use_qk_l2norm: bool = False) -> tuple[Tensor, Tensor]:
@@ -630,6 +644,8 @@ def diag_scan(x: Tensor, g: Tensor, h0: Tensor | None = None, *, complement: boo
 def diag_scan_step(x: Tensor, g: Tensor, state: Tensor, *, complement: bool = False) -> Tensor:
     """One token of ``diag_scan`` for generation: ``x, g [B, ...]``, ``state [B, ...]`` fp32 contiguous, **updated in place**
     (start from the ``h_T`` of the prompt).  Returns the new state in the type of ``x``.  Not differentiable."""
+    if torch._C._is_tracing():
+        return _TracedStep.apply("diag_scan_step", bool(complement), x, g, state)
     return native.ext().diag_scan_step(x, g, state, complement)
 
 
