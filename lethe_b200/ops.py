@@ -609,6 +609,9 @@ def gdn_decode_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor | None, beta: Ten
     (start from the ``h_T`` that ``gdn_chunk`` returned for the prompt).  Returns ``o [B,H,V]`` bf16.
     Not differentiable.  K must be 128, V 64 or 128.
     """
+    if torch._C._is_tracing():
+        scale = int(state.shape[2]) ** -0.5 if scale is None else scale      # (a traced size is a tensor)
+        return _TracedStep.apply("decode_step", float(scale), q, k, v, g, beta, state)
     return native.ext().decode_step(q, k, v, g, beta, state, state.shape[2] ** -0.5 if scale is None else scale)
 
 

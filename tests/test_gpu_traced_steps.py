@@ -60,3 +60,27 @@ def test_diag_scan_step_has_no_gradient_and_refuses_as_ever():
             torch.jit.trace(f, bad)
         with pytest.raises(Exception, match=what):
             traced(*bad)
+
+
+def matrix(seed, gate, delta):
+    gen = torch.Generator().manual_seed(seed)
+    q, k, v = (torch.randn(2, 3, n, generator=gen).to("cuda", torch.bfloat16) for n in (128, 128, 64))
+    g = {"none": None, "scalar": -torch.rand(2, 3, generator=gen), "channel": -torch.rand(2, 3, 128, generator=gen)}[gate]
+    beta = torch.rand(2, 3, generator=gen) if delta else None
+    return [None if t is None else t.cuda() for t in (q, k * 128 ** -0.5, v, g, beta, torch.randn(2, 3, 128, 64, generator=gen))]
+
+
+@pytest.mark.parametrize("scale", [None, 0.5])
+@pytest.mark.parametrize("gate,delta", [("scalar", True), ("channel", True), ("scalar", False), ("none", False)])
+def test_gdn_decode_step(gate, delta, scale):
+    def call(*given):
+        it = iter(given)
+        full = [None if t is None else next(it) for t in matrix(1, gate, delta)]
+        return ops.gdn_decode_step(*full, scale=scale)
+    there = lambda seed: tuple(t for t in matrix(seed, gate, delta) if t is not None)
+    traced = torch.jit.trace(call, there(1))
+    a, b = there(2), there(2)
+    for _ in range(2):
+        want = call(*b)
+        poison(want)
+        assert torch.equal(traced(*a), want) and torch.equal(a[-1], b[-1])
