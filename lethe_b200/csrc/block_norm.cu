@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(S::kThreads, gated_ctas<S>(true)) gated_norm_v
     }
     float s[2] = {lo(xx) + hi(xx), lo(dx_sum) + hi(dx_sum)};
     S::template row_sums<2>(s, sums[flip]);
-    const float r1 = rsqrtf(fmaf(s[0], over, p.eps));
+    const float r1 = live ? rsqrtf(fmaf(s[0], over, p.eps)) : 0.f;      // (with eps = 0 a row that is not there would have an infinite root)
     const F2 r = f2(r1), c = f2(-s[1] * over * r1 * r1);
     F2 dx[S::P];
 #pragma unroll
