@@ -98,10 +98,10 @@ __global__ void __launch_bounds__(S::kThreads, residual_ctas<S>(true)) residual_
 #pragma unroll
     for (int k = 0; k < K; ++k) s[k] = lo(sum[k]) + hi(sum[k]);
     S::template row_sums<K>(s, sums[flip][0]);
-    const float root = rsqrtf(fmaf(s[0], over, p.eps));
+    const float root = live ? rsqrtf(fmaf(s[0], over, p.eps)) : 0.f;      // (with eps = 0 a row that is not there would have an infinite root)
     const F2 r2 = f2(root), c2 = f2(-s[1] * over * root * root);
     F2 r1 = f2(1.f);
-    if constexpr (BRANCH == 2) r1 = f2(rsqrtf(fmaf(s[2], over, p.eps)));
+    if constexpr (BRANCH == 2) r1 = f2(live ? rsqrtf(fmaf(s[2], over, p.eps)) : 0.f);
     F2 d[S::P], qq = f2(0.f);
 #pragma unroll
     for (int n = 0; n < S::P; ++n) {

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from .test_gpu_block_norms import gated_check, randn
+from .test_gpu_block_norms import gated_check, randn, residual_check, residual_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -17,3 +17,11 @@ def test_gated_norm_without_eps(rows, D, types, eps):
     xt, wt = types
     for act in ("silu", "sigmoid"):
         gated_check(randn(rows, D, seed=1, dt=xt), randn(rows, D, seed=2, dt=xt), randn(D, seed=3, dt=wt), randn(rows, D, seed=4, dt=xt), eps=eps, act=act)
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-60])
+@pytest.mark.parametrize("scale,post", [("none", False), ("number", True), ("vector", False), ("vector", True)])
+@pytest.mark.parametrize("rows,D", SPARE)
+def test_residual_norm_without_eps(rows, D, scale, post, eps):
+    for types in ((torch.float32, torch.float32, torch.float32), (torch.bfloat16, torch.float32, torch.float32), (torch.float16, torch.float16, torch.float16)):
+        residual_check(*residual_inputs((rows, D), *types, scale, post), eps=eps)
