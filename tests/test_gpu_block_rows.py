@@ -2,6 +2,8 @@
 import pytest
 import torch
 
+from lethe_b200 import ops
+
 from .test_gpu_block_norms import gated_check, randn, residual_check, residual_inputs
 
 pytestmark = pytest.mark.gpu
@@ -25,3 +27,26 @@ def test_gated_norm_without_eps(rows, D, types, eps):
 def test_residual_norm_without_eps(rows, D, scale, post, eps):
     for types in ((torch.float32, torch.float32, torch.float32), (torch.bfloat16, torch.float32, torch.float32), (torch.float16, torch.float16, torch.float16)):
         residual_check(*residual_inputs((rows, D), *types, scale, post), eps=eps)
+
+
+# several turns of the CTAs, the last one not full, and every number of rows of a CTA
+MANY = [(70001, 16), (20011, 64), (9001, 250), (2501, 1024), (2501, 700), (1501, 2048), (601, 8192)]
+
+
+@pytest.mark.parametrize("rows,D", MANY)
+def test_every_row_counts_once_in_the_sums_over_rows(rows, D):
+    """A gradient that is zero but for one row: the sums are that row's terms, to the bit (what is added to them is zeros)."""
+    x, z = randn(rows, D, seed=1, dt=torch.bfloat16), randn(rows, D, seed=2, dt=torch.bfloat16)
+    vectors = [randn(D, seed=i) for i in (3, 4, 5)]
+
+    def sums(x, z, dy):
+        w, sc, pw = (v.clone().requires_grad_(True) for v in vectors)
+        y, r = ops.residual_norm(x, z, w, scale=sc, post_weight=pw)
+        plain, _ = ops.residual_norm(x, z, w, scale=sc)
+        return [*torch.autograd.grad(ops.gated_norm(x, z, w), w, dy), *torch.autograd.grad((y, r), (w, sc, pw), (dy, dy)), *torch.autograd.grad(plain, (w, sc), dy)]
+    dy = torch.zeros_like(x)
+    for i in (0, 1, 31, rows // 3, rows // 2, rows - 17, rows - 2, rows - 1):
+        dy[i] = 1
+        for got, want in zip(sums(x, z, dy), sums(x[i:i + 1].clone(), z[i:i + 1].clone(), dy[i:i + 1].clone())):
+            assert bool((want != 0).any()) and torch.equal(got, want), i
+        dy[i] = 0
