@@ -27,20 +27,29 @@ struct GatedProblem {
   float* part;      // per CTA the sums for dweight; NULL: not wanted
 };
 
-// logistic function.  Results in 16 bits: exponential and reciprocal by the approximations, some 2^-21 off; in 32 bits the
-// exponential is expf, the quotient good to 2 ulp with a divisor in [1, inf].
+// logistic function s = 1 / (1 + e), e = exp(-z).  Results in 32 bits: the exponential is expf, the quotient good to 2 ulp up to a divisor of
+// 2^126 and 0 beyond, that is for gates below -87.3.  In 16 bits: exponential and reciprocal by the approximations, 2^-22 off each, and with the
+// rounding of its argument the exponential is off by |z| 2^-24 of itself more.
 template <int XT>
-__device__ __forceinline__ F2 logistic(F2 z) {
-  if constexpr (XT == LETHE_F32) return f2(__fdividef(1.f, 1.f + expf(-lo(z))), __fdividef(1.f, 1.f + expf(-hi(z))));
-  const F2 t = z * f2(-1.4426950408889634f);
+__device__ __forceinline__ F2 logistic(F2 z, F2& e) {
   float a, b;
+  if constexpr (XT == LETHE_F32) {
+    a = expf(-lo(z));
+    b = expf(-hi(z));
+    e = f2(a, b);
+    return f2(__fdividef(1.f, 1.f + a), __fdividef(1.f, 1.f + b));
+  }
+  const F2 t = z * f2(-1.4426950408889634f);
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(lo(t)));
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(hi(t)));
-  const F2 d = f2(a, b) + f2(1.f);
+  e = f2(a, b);
+  const F2 d = e + f2(1.f);
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(lo(d)));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(hi(d)));
   return f2(a, b);
 }
+// 1 - s = e s: by subtraction a gate of 12 would leave percents of it.  (Where e is infinite, s is 0.)
+__device__ __forceinline__ F2 one_less(F2 s, F2 e) { return f2(fminf(lo(e), 3e38f), fminf(hi(e), 3e38f)) * s; }
 
 // CTAs on an SM: registers (64 a thread forward, 80 backward; twice that with two pieces)
 template <typename S> constexpr int gated_ctas(bool backward) { return S::R > 1 ? 512 / S::kThreads : (backward ? 768 : 1024) / S::kThreads; }
@@ -109,7 +118,8 @@ __global__ void __launch_bounds__(S::kThreads, gated_ctas<S>(false)) gated_norm_
     F2 y[S::P];
 #pragma unroll
     for (int n = 0; n < S::P; ++n) {
-      const F2 zv = z[n / 4].get2(n % 4), sg = logistic<XT>(zv);
+      F2 e;
+      const F2 zv = z[n / 4].get2(n % 4), sg = logistic<XT>(zv, e);
       y[n] = x[n / 4].get2(n % 4) * r * w[n] * (SILU ? zv * sg : sg);
     }
     if (live) S::template store<XT>(y, py.p, t, p.D);
@@ -183,10 +193,10 @@ __global__ void __launch_bounds__(S::kThreads, gated_ctas<S>(true)) gated_norm_v
     F2 xx = f2(0.f), dx_sum = f2(0.f), dn[S::P], slope[S::P];
 #pragma unroll
     for (int n = 0; n < S::P; ++n) {
-      const F2 xv = x[n / 4].get2(n % 4), zv = z[n / 4].get2(n % 4), dv = d[n / 4].get2(n % 4), sg = logistic<XT>(zv);
-      const F2 rest = fma2(sg, f2(-1.f), f2(1.f)), ds = dv * sg;      // 1 - s, dy s
+      F2 e;
+      const F2 xv = x[n / 4].get2(n % 4), zv = z[n / 4].get2(n % 4), dv = d[n / 4].get2(n % 4), sg = logistic<XT>(zv, e), ds = dv * sg;
       dn[n] = SILU ? ds * zv : ds;
-      slope[n] = ds * (SILU ? fma2(zv, rest, f2(1.f)) : rest);
+      slope[n] = ds * (SILU ? fma2(zv, fma2(sg, f2(-1.f), f2(1.f)), f2(1.f)) : one_less(sg, e));      // (beside the 1 of silu the subtraction does no harm)
       xx = fma2(xv, xv, xx);
       dx_sum = fma2(dn[n] * w[n], xv, dx_sum);
     }
