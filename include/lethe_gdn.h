@@ -303,7 +303,7 @@ int lethe_gdn_diag_step(const LetheGdnDiagArgs* args, float* state, void* cuda_s
 typedef struct LetheGdnGatedNormArgs {
   int64_t rows, inner;
   int32_t D, x_type, w_type, silu;
-  float eps;
+  float eps;              /* finite, zero or more                                           */
   const void* x;
   int64_t x_outer, x_inner;
   const void* gate;
@@ -331,7 +331,7 @@ int lethe_gdn_gated_norm_vjp(const LetheGdnGatedNormArgs* args, void* cuda_strea
 typedef struct LetheGdnResidualNormArgs {
   int64_t rows;
   int32_t D, x_type, r_type, w_type;
-  float eps, scale_value;
+  float eps, scale_value;   /* eps: finite, zero or more                                      */
   const void* x;
   int64_t x_stride;
   const void* residual;

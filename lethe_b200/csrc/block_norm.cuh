@@ -9,6 +9,7 @@
 // atomics: two runs give the same bits.
 #pragma once
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "elem.cuh"

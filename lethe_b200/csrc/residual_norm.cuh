@@ -41,7 +41,7 @@ int by_stream_type(int xt, int rt, F&& f) {
 
 inline int residual_problem(const LetheGdnResidualNormArgs* a, ResidualProblem* p, bool backward) {
   if (!a) return kErrNull;
-  if (a->rows <= 0 || a->D <= 0 || a->D > kNormMaxD || !norm_types_ok(a->x_type, a->w_type) || !norm_types_ok(a->x_type, a->r_type) || !(a->eps >= 0.f))
+  if (a->rows <= 0 || a->D <= 0 || a->D > kNormMaxD || !norm_types_ok(a->x_type, a->w_type) || !norm_types_ok(a->x_type, a->r_type) || !(a->eps >= 0.f) || !std::isfinite(a->eps))
     return kErrDims;
   if (!a->r || !a->weight || (!backward && (!a->x || !a->y))) return kErrNull;
   if (backward && !a->x && (a->post_weight || a->dscale)) return kErrNull;

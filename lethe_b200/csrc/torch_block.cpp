@@ -255,7 +255,7 @@ void check_row(const Tensor& x, double eps) {
   need_shape(x.dim() >= 1, "rows [..., D]");
   if (x.size(-1) < 1 || x.size(-1) > kMaxRow)
     fail("unsupported row length " + std::to_string(x.size(-1)) + " (need 1 to " + std::to_string(kMaxRow) + ")");
-  if (!(eps >= 0.) || !std::isfinite(eps)) fail("eps must be a finite number, zero or more");
+  if (!(eps >= 0.) || !std::isfinite(static_cast<float>(eps))) fail("eps must be a finite number in fp32, zero or more");
 }
 void check_vector(const Tensor& v, const Tensor& x, const char* name) {
   if (!v.defined()) return;
@@ -455,6 +455,7 @@ std::pair<Tensor, Tensor> residual_norm(const Tensor& x, const OptTensor& residu
     need_device(x, residual, weight, post, scale);
     need_type(x, "x");
     check_row(x, eps);
+    if (std::isfinite(scale_value) && !std::isfinite(static_cast<float>(scale_value))) fail("scale lies beyond what fp32 holds");
     if (residual.defined()) {
       need_shape(residual.sizes() == x.sizes(), "x, residual [..., D]");
       if (residual.scalar_type() != at::kFloat && residual.scalar_type() != x.scalar_type())
