@@ -257,6 +257,7 @@ static int gated_problem(const LetheGdnGatedNormArgs* a, GatedProblem* p, bool b
   if (!a) return kErrNull;
   if (a->rows <= 0 || a->inner <= 0 || a->inner > INT32_MAX || a->D <= 0 || a->D > kNormMaxD || !norm_types_ok(a->x_type, a->w_type) || !(a->eps >= 0.f) || !std::isfinite(a->eps)) return kErrDims;
   if (!a->x || !a->gate || !a->weight || (!backward && !a->y) || (backward && !a->dy)) return kErrNull;
+  if (!on_elements(a->x_type, a->x, a->gate, a->y, a->dy, a->dx, a->dgate) || !on_elements(a->w_type, a->weight, a->dweight)) return kErrAlign;
   *p = {a->rows, a->inner, a->D, a->w_type == LETHE_F32, a->eps, a->x, a->x_outer, a->x_inner, a->gate, a->gate_outer, a->gate_inner,
         a->weight, a->y, a->dy, a->dx, a->dgate, nullptr};
   return kOk;

@@ -898,6 +898,8 @@ static int diag_problem(const LetheGdnDiagArgs* a, DiagProblem* p, bool backward
   if (!a->x || !a->g || !a->status || (!backward && !a->h) || (backward && !a->states)) return kErrNull;
   const long long tiles = tiles_of(a->L, a->x_type, backward), strips = (a->D + kChannels - 1) / kChannels;
   if (strips > INT32_MAX || a->B > INT32_MAX / strips || tiles > INT32_MAX / (a->B * strips)) return kErrDims;
+  if (!on_elements(a->x_type, a->x, a->h, a->d_h, a->dx) || !on_elements(a->g_type, a->g, a->dg) ||
+      !on_elements(LETHE_F32, a->h0, a->hT, a->states, a->dhT, a->dh0, a->status)) return kErrAlign;
   *p = {a->B, a->L, a->D, a->x, a->x_batch, a->x_token, a->g, a->g_batch, a->g_token, a->h0, a->h, a->hT, a->states, a->d_h, a->d_h_batch,
         a->d_h_token, a->dhT, a->dx, a->dg, a->dh0, static_cast<int>(tiles), static_cast<int>(strips), tiles_of(a->L, a->x_type, true),
         static_cast<uint32_t>(a->B * strips), 1, 0, a->status, {}};
@@ -990,6 +992,7 @@ extern "C" int lethe_gdn_diag_step(const LetheGdnDiagArgs* a, float* state, void
   if (!a) return kErrNull;
   if (a->B <= 0 || a->D <= 0 || !types_ok(a->x_type, a->g_type)) return kErrDims;
   if (!a->x || !a->g || !a->h || !state) return kErrNull;
+  if (!on_elements(a->x_type, a->x, a->h) || !on_elements(a->g_type, a->g) || !on_elements(LETHE_F32, state)) return kErrAlign;
   const bool vec = a->D % kPer == 0 && on_boundary(a->x, a->x_type, kPer, a->x_batch) && on_boundary(a->g, a->g_type, kPer, a->g_batch) &&
                    on_boundary(a->h, a->x_type, kPer) && on_boundary(state, LETHE_F32, kPer);
   const long long blocks = (a->D + 256 * (vec ? kPer : 1) - 1) / (256 * (vec ? kPer : 1));

@@ -14,6 +14,8 @@ template <> struct Elem<LETHE_BF16> { using T = __nv_bfloat16; };
 template <> struct Elem<LETHE_F16> { using T = __half; };
 
 inline __host__ __device__ constexpr int elem_bytes(int ty) { return ty == LETHE_F32 ? 4 : 2; }
+// whether all these pointers lie on a boundary of an element (null does)
+template <typename... P> inline bool on_elements(int ty, const P*... p) { return ((reinterpret_cast<uintptr_t>(p) % elem_bytes(ty) == 0) && ...); }
 
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }

@@ -45,6 +45,8 @@ inline int residual_problem(const LetheGdnResidualNormArgs* a, ResidualProblem* 
     return kErrDims;
   if (!a->r || !a->weight || (!backward && (!a->x || !a->y))) return kErrNull;
   if (backward && !a->x && (a->post_weight || a->dscale)) return kErrNull;
+  if (!on_elements(a->x_type, a->x, a->y, a->dy, a->dx) || !on_elements(a->r_type, a->residual, a->r, a->dr, a->dresidual) ||
+      !on_elements(a->w_type, a->weight, a->post_weight, a->scale, a->dweight, a->dpost_weight, a->dscale)) return kErrAlign;
   *p = {a->rows, a->D, a->w_type == LETHE_F32, a->eps, a->scale_value, a->x, a->x_stride, a->residual, a->residual_stride, a->weight, a->post_weight,
         a->scale, a->r, a->y, a->dy, a->dr, a->dx, a->dresidual, nullptr, 0, {-1, -1, -1}};
   return kOk;
