@@ -890,14 +890,19 @@ static int launched() { return cudaGetLastError() == cudaSuccess ? kOk : kErrLau
 
 static long long tiles_of(long long L, int xt, bool backward) {
   const int n = kGroups * (backward ? backward_steps(xt) : forward_steps(xt));
-  return (L + n - 1) / n;
+  return (L - 1) / n + 1;      // (L + n - 1 need not fit)
+}
+static long long strips_of(long long D) { return (D - 1) / kChannels + 1; }
+// tiles and what they hand on are counted in 32 bits
+static bool countable(long long B, long long strips, long long tiles) {
+  return strips <= INT32_MAX && B <= INT32_MAX / strips && tiles <= INT32_MAX / (B * strips);
 }
 static int diag_problem(const LetheGdnDiagArgs* a, DiagProblem* p, bool backward) {
   if (!a) return kErrNull;
   if (a->B <= 0 || a->L <= 0 || a->D <= 0 || !types_ok(a->x_type, a->g_type)) return kErrDims;
   if (!a->x || !a->g || !a->status || (!backward && !a->h) || (backward && !a->states)) return kErrNull;
-  const long long tiles = tiles_of(a->L, a->x_type, backward), strips = (a->D + kChannels - 1) / kChannels;
-  if (strips > INT32_MAX || a->B > INT32_MAX / strips || tiles > INT32_MAX / (a->B * strips)) return kErrDims;
+  const long long tiles = tiles_of(a->L, a->x_type, backward), strips = strips_of(a->D);
+  if (!countable(a->B, strips, tiles)) return kErrDims;
   if (!on_elements(a->x_type, a->x, a->h, a->d_h, a->dx) || !on_elements(a->g_type, a->g, a->dg) ||
       !on_elements(LETHE_F32, a->h0, a->hT, a->states, a->dhT, a->dh0, a->status)) return kErrAlign;
   *p = {a->B, a->L, a->D, a->x, a->x_batch, a->x_token, a->g, a->g_batch, a->g_token, a->h0, a->h, a->hT, a->states, a->d_h, a->d_h_batch,
@@ -949,8 +954,8 @@ extern "C" size_t lethe_gdn_diag_states_bytes(int64_t B, int64_t L, int64_t D, i
 extern "C" size_t lethe_gdn_diag_work_bytes(int64_t B, int64_t L, int64_t D, int32_t x_type, int32_t backward) {
   using namespace lg;
   if (B <= 0 || L <= 0 || D <= 0 || !types_ok(x_type, LETHE_F32)) return 0;
-  const long long tiles = tiles_of(L, x_type, backward != 0);
-  return tiles > 1 ? look_sizes(B * ((D + kChannels - 1) / kChannels), tiles).bytes() : 0;
+  const long long tiles = tiles_of(L, x_type, backward != 0), strips = strips_of(D);
+  return tiles > 1 && countable(B, strips, tiles) ? look_sizes(B * strips, tiles).bytes() : 0;      // (0 too where the call itself refuses)
 }
 
 extern "C" int lethe_gdn_diag_forward(const LetheGdnDiagArgs* a, void* stream) {
@@ -995,7 +1000,7 @@ extern "C" int lethe_gdn_diag_step(const LetheGdnDiagArgs* a, float* state, void
   if (!on_elements(a->x_type, a->x, a->h) || !on_elements(a->g_type, a->g) || !on_elements(LETHE_F32, state)) return kErrAlign;
   const bool vec = a->D % kPer == 0 && on_boundary(a->x, a->x_type, kPer, a->x_batch) && on_boundary(a->g, a->g_type, kPer, a->g_batch) &&
                    on_boundary(a->h, a->x_type, kPer) && on_boundary(state, LETHE_F32, kPer);
-  const long long blocks = (a->D + 256 * (vec ? kPer : 1) - 1) / (256 * (vec ? kPer : 1));
+  const long long blocks = (a->D - 1) / (256 * (vec ? kPer : 1)) + 1;
   if (blocks > INT32_MAX || a->B > INT32_MAX / blocks) return kErrDims;
   DeviceGuard guard(a->x);
   if (!guard.ok) return kErrDevice;

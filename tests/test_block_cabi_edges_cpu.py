@@ -56,3 +56,22 @@ def test_residual_pointers_between_elements(lib, call):      # noqa: F811
             refused(lib, call, off(residual, n, 2 if types["r_type"] == 0 else 1, **types), b"align")
         for n in ("weight", "post_weight", "scale", "dweight", "dpost_weight", "dscale"):
             refused(lib, call, off(residual, n, 2 if types["w_type"] == 0 else 1, **types), b"align")
+
+
+END = (1 << 63) - 1
+
+
+@pytest.mark.parametrize("call", ["lethe_gdn_diag_forward", "lethe_gdn_diag_backward"])
+def test_diag_sizes_at_the_end_of_64_bits(lib, call):      # noqa: F811
+    for bad in (dict(L=END), dict(L=END - 60), dict(D=END), dict(D=END - 60), dict(B=END), dict(B=END, L=END, D=END)):
+        refused(lib, call, diag(**bad), b"sizes")
+
+
+def test_diag_step_sizes_at_the_end_of_64_bits(lib):      # noqa: F811
+    for bad in (dict(D=END), dict(D=END - 200), dict(B=END), dict(B=END, D=END)):
+        refused(lib, "lethe_gdn_diag_step", diag(**bad), b"sizes", ctypes.c_void_p(0x70000))
+
+
+def test_diag_work_of_sizes_that_are_refused(lib):      # noqa: F811
+    for bad in ((END, 1000, 64), (1, END, 64), (1, 1000, END), (1 << 40, 1 << 40, 1)):
+        assert lib.lethe_gdn_diag_work_bytes(*bad, 1, 0) == 0
