@@ -249,13 +249,13 @@ struct RowPtr {
 };
 // Rows (o, i), i below `inner`, of tensors with a stride for each of the two.
 struct RowWalk {
-  int i, step_i, inner;
+  uint32_t i, step_i, inner;      // (the sum of two numbers below inner < 2^31)
   long long o, step_o;
-  __device__ __forceinline__ RowWalk(const Turns& t, long long inner_) : inner(static_cast<int>(inner_)) {
+  __device__ __forceinline__ RowWalk(const Turns& t, long long inner_) : inner(static_cast<uint32_t>(inner_)) {
     o = t.first / inner_;
-    i = static_cast<int>(t.first - o * inner_);
+    i = static_cast<uint32_t>(t.first - o * inner_);
     step_o = t.step / inner_;
-    step_i = static_cast<int>(t.step - step_o * inner_);
+    step_i = static_cast<uint32_t>(t.step - step_o * inner_);
   }
   __device__ __forceinline__ bool next() {      // whether i has come round
     i += step_i;

@@ -50,3 +50,24 @@ def test_every_row_counts_once_in_the_sums_over_rows(rows, D):
         for got, want in zip(sums(x, z, dy), sums(x[i:i + 1].clone(), z[i:i + 1].clone(), dy[i:i + 1].clone())):
             assert bool((want != 0).any()) and torch.equal(got, want), i
         dy[i] = 0
+
+
+def test_as_many_inner_rows_as_32_bits_count():
+    """Close to 2^31 rows of each of two: places are summed beyond what a signed number holds, and the step from one to the other comes behind that."""
+    inner = (1 << 31) - 1000
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("40 GB of memory")
+    gate = torch.empty(2, 1 << 31, 1, dtype=torch.bfloat16, device="cuda")
+    for part in gate.view(-1).split(1 << 28):
+        part.uniform_(-3, 3)
+    z = gate[:, 1000:]
+    x = torch.ones(2, inner, 1, dtype=torch.bfloat16, device="cuda")
+    with torch.no_grad():
+        y = ops.gated_norm(x, z, torch.ones(1, device="cuda"), activation="sigmoid")
+    for o in (0, 1):
+        for part in (slice(0, 30000), slice(1 << 30, (1 << 30) + 30000), slice(inner - 30000, inner)):
+            want = torch.sigmoid(z[o, part].double()) / (1 + 1e-6) ** 0.5
+            assert bool(((y[o, part].double() - want).abs() <= 2 ** -8 * 1.01 * want).all()), (o, part)
+    del gate, z, x, y
+    torch.cuda.empty_cache()
