@@ -249,7 +249,7 @@ int lethe_gdn_convert(const void* src, void* dst, int64_t n, int32_t to_f32, voi
  * What stands beside a recurrence with a matrix state in a model: the recurrence with one state value per channel, and the
  * norms on both sides of a block.  No counterpart in the reference.  These calls take tensors in the type they have
  * (LETHE_F32, LETHE_BF16, LETHE_F16), compute in fp32 and round each result once.  Strides and offsets count elements;
- * rows are read where they lie, the innermost dimension contiguous; pointers on a boundary of their element.  Like the
+ * rows are read where they lie, the innermost dimension contiguous; pointers on a boundary of their element (else refused).  Like the
  * calls above they allocate nothing, enqueue on the given stream and return non-zero where nothing was launched; they work
  * on the GPU that owns `x`.
  * ------------------------------------------------------------------------------------------------------------------ */
@@ -259,7 +259,8 @@ enum { LETHE_F32 = 0, LETHE_BF16 = 1, LETHE_F16 = 2 };
  *   h_t = exp(g_t) h_{t-1} + x_t                       (complement != 0: exp(g_t) h_{t-1} + (1 - exp(g_t)) x_t)
  * forward: h and hT from x, g, h0.  backward, with e_t the gradient of h_t: e_t = d_h_t + exp(g_{t+1}) e_{t+1},
  *   dx_t = e_t (times 1 - exp(g_t)),  dg_t = exp(g_t) e_t (h_{t-1} (- x_t)),  dh0 = exp(g_0) e_0.
- * g is a natural-log decay, <= 0; minus infinity starts anew.  States are fp32; the decay of a long memory keeps its
+ * g is a natural-log decay, <= 0; minus infinity starts anew.  What is not finite reaches all later tokens of its channel, also
+ * past such a start, and an infinite state may go on as NaN.  States are fp32; the decay of a long memory keeps its
  * precision (1 - exp(g) is formed without the cancellation that exp(g) next to one would bring).
  * Types: x, h, d_h, dx are x_type; g, dg are g_type, which is LETHE_F32 or x_type.  h0, hT, dhT, dh0 fp32 [B, D].
  * h, dx, dg are contiguous [B, L, D]; x, g, d_h have strides of their own for batch and token.
@@ -297,7 +298,7 @@ int lethe_gdn_diag_backward(const LetheGdnDiagArgs* args, void* cuda_stream);
 int lethe_gdn_diag_step(const LetheGdnDiagArgs* args, float* state, void* cuda_stream);
 
 /* The norm behind a block: y = x rsqrt(mean(x^2) + eps) weight act(gate), act the logistic function, or gate times it (silu != 0).
- * Rows of D values, 1 <= D <= 8192: row r = i * inner + j lies at i * outer_stride + j * inner_stride, for x and gate each;
+ * Norm first, gate behind.  Rows of D values, 1 <= D <= 8192: row r = i * inner + j (inner below 2^31) lies at i * outer_stride + j * inner_stride, for x and gate each;
  * y, dx, dgate are contiguous.  x, gate, y, dy, dx, dgate are x_type; weight and dweight LETHE_F32 or x_type (w_type).
  * dy contiguous.  work (vjp): lethe_gdn_norm_work_bytes(rows, D, 1) bytes on a 16-byte boundary, needed where dweight is wanted. */
 typedef struct LetheGdnGatedNormArgs {

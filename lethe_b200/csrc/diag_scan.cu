@@ -1,8 +1,9 @@
 // The element-wise gated recurrence h_t = e^{g_t} h_{t-1} + x_t (or + (1 - e^{g_t}) x_t), its backward, and one token of it.
 //
 // Bound by HBM on paper: 8 bytes an element forward (bf16 x and h, fp32 g), 14 backward.  Measured (B1 L65536 D2048): 226 us forward, 0.73 of the
-// measured copy bandwidth, 425 backward, 0.68; without any tile waiting for another (1024 sequences of 128 tokens) 209 and 404, so
-// most of what is missing is the runs themselves, some 33 and 60 operations an element by 16 warps of an SM, not the handing on.
+// measured copy bandwidth, 425 backward, 0.68; without any tile waiting for another (a tile a sequence: 1024 of 128 tokens forward, 2048 of 64
+// backward) 210 and 403, so most of what is missing is the runs themselves, some 33 and 60 operations an element by 16 warps of an SM, not
+// the handing on.  With the complement 246 and 505: its backward holds a value more for every step and spills 32 to 72 bytes a thread in 16 bits.
 //
 // A CTA does tiles, 16 groups of tokens x 64 channels of one sequence, each read once: a thread has 3 to 8 tokens of four channels, its
 // 16-lane group covers the channels.  Every thread runs its own tokens from a zero state, the groups' results (sum of g, state) meet in
@@ -377,7 +378,7 @@ constexpr int kPartsThreads = kRunners + kChannels, kOutThreads = 2 * kChannels,
 // and looking back has the time of a run.  Steps on the way (B1 L65536 D2048 bf16, forward / backward in us): tiles in registers, two CTAs on
 // an SM, 462 / 651; the next tile by asynchronous copies and fewer operations 344 / 462; folding and looking in warps of their own,
 // a word behind the looking of the tile before it, 299 / 700; as it is 239 / 475; two channels by one instruction and the places of a
-// tile worked out once 226 / 425.  Left: whole tiles by tensor-map copies 240 / 490, four small CTAs without roles 627 / 569, one
+// tile worked out once 226 / 425.  Tried beside 239 / 475 and left (not measured again since): whole tiles by tensor-map copies 240 / 490, four small CTAs without roles 627 / 569, one
 // more ticket ahead 255 / 506, tiles fetched to L2 row by row 388 / 638, tickets dealt out beforehand in a cooperative launch 228 / 470
 // (B2 L2048 D1024 14.5 + 21.1 against 15.6 + 23).
 template <int XT, int GT, int WIDTH, bool COMP>
@@ -926,7 +927,7 @@ static int widest(F&& fits) { return fits(4) ? 4 : fits(2) ? 2 : 1; }
 
 // Few channels: a strip of 64 takes those of as many batches as fit (bf16, forward + backward in us, one batch / as many: 64 x 16384 x 8
 // 104 + 191 / 39 + 56, 16 x 16384 x 32 37 + 62 / 27 + 42).  A kernel of its own: with the places of a channel open at run time the others
-// spill (B1 L65536 D2048 backward 424 / 442).
+// spill more (B1 L65536 D2048 backward 424 / 442).  The work buffer is that of a strip for each batch, all of it cleared.
 static int pack_batches(DiagProblem* p, int w) {
   if (w != kPer || p->D > kChannels / 2 || p->B < 2) return w;
   p->pack = static_cast<int>(kChannels / p->D);

@@ -638,7 +638,8 @@ def diag_scan(x: Tensor, g: Tensor, h0: Tensor | None = None, *, complement: boo
     types are read as fp32); minus infinity starts anew, e.g. at the first token of a packed document.  ``h0 [B, ...]``: the
     initial state, zero if None.  Batch and token may have any strides (a slice of a fused projection is read where it lies).
     States and sums are fp32, each result is rounded once; the decay of a long memory (``g`` near zero) keeps its precision.
-    Gradients flow to x, g and h0, first order only.  A value that is not finite spreads to the later tokens of its channel."""
+    Gradients flow to x, g and h0, first order only.  A value that is not finite spreads to the later tokens of its channel, also past
+    a start anew (zero times infinity); an infinite state may go on as NaN."""
     if torch._C._is_tracing():
         return _Traced.apply("diag_scan", bool(complement), None, x, g, h0)
     return native.ext().diag_scan(x, g, h0, complement)
@@ -658,7 +659,8 @@ ACTIVATIONS = ("silu", "sigmoid")
 def gated_norm(x: Tensor, gate: Tensor, weight: Tensor, *, eps: float = 1e-6, activation: str = "silu") -> Tensor:
     """The norm behind a block, differentiable: ``x * rsqrt(mean(x^2) + eps) * weight * act(gate)`` over the last dimension, in
     one pass.  ``x, gate [..., D]`` of one type (fp32, bf16 or fp16), for a recurrence's output ``[B, L, H, V]`` with the gate a
-    view of a projection; ``weight [D]``; ``activation`` "silu" (``gate * sigmoid(gate)``) or "sigmoid".  D from 1 to 8192.
+    view of a projection; ``weight [D]``; ``activation`` "silu" (``gate * sigmoid(gate)``) or "sigmoid".  The gate comes behind the
+    norm; the other order (norm of ``x * act(gate)``) is not offered.  D from 1 to 8192.
     Gradients flow to x, gate and weight, first order only."""
     if activation not in ACTIVATIONS:
         raise GdnError(f"lethe_gdn: activation must be one of {ACTIVATIONS}")
