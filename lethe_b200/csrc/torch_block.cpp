@@ -212,6 +212,15 @@ std::pair<Tensor, Tensor> diag_scan(const Tensor& x, const Tensor& g_in, const O
   });
 }
 
+// whether some of t's memory may be some of the contiguous tensor `whole`'s: by addresses, since two storages can stand for the same memory
+bool touches(const Tensor& t, const Tensor& whole) {
+  if (t.numel() == 0 || lazy(t)) return false;      // (lazy: written out elsewhere)
+  int64_t last = 0;
+  for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+  const char *a = static_cast<const char*>(t.data_ptr()), *b = static_cast<const char*>(whole.data_ptr());
+  return a < b + whole.nbytes() && b < a + (last + 1) * t.element_size();
+}
+
 Tensor diag_scan_step(const Tensor& x, const Tensor& g_in, const Tensor& state, bool complement) {
   return guarded([&] {
     need_cuda(state);
@@ -225,9 +234,9 @@ Tensor diag_scan_step(const Tensor& x, const Tensor& g_in, const Tensor& state, 
     refuse_tangents({x, g_in, state});
     at::NoGradGuard no_grad;
     c10::cuda::CUDAGuard guard(state.device());
-    // a view of the state is read before any of it is written
+    // what lies in the state's memory is read before any of it is written
     const auto readable = [&](const Tensor& t) {
-      if (t.is_alias_of(state)) return t.clone(at::MemoryFormat::Contiguous);
+      if (touches(t, state)) return t.clone(at::MemoryFormat::Contiguous);
       return lazy(t) || !packed_from(t, 1) ? as(t, t.scalar_type()) : t;
     };
     Tensor h = at::empty(x.sizes(), x.options());

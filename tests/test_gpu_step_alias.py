@@ -44,3 +44,26 @@ def test_rows_of_the_state_one_further():
     state = other[:-1].clone()
     wh = ops.diag_scan_step(x, other[1:].clone(), state)
     assert torch.equal(h, wh) and torch.equal(mine[:-1], state) and torch.equal(mine[-1], buffer[-1])
+
+
+@pytest.mark.parametrize("which", ["x", "g"])
+def test_the_same_memory_under_another_storage(which):
+    start = -torch.rand(N, N, generator=torch.Generator().manual_seed(4)).cuda()
+    other = torch.randn(N, N, generator=torch.Generator().manual_seed(5)).cuda().abs().neg()
+    mine, want = start.clone(), start.clone()
+    view = torch.from_dlpack(mine).t()
+    assert view.untyped_storage().data_ptr() == mine.data_ptr()
+    same = start.t().contiguous()
+    h = ops.diag_scan_step(*((view, other) if which == "x" else (other, view)), mine)
+    wh = ops.diag_scan_step(*((same, other) if which == "x" else (other, same)), want)
+    assert torch.equal(h, wh) and torch.equal(mine, want)
+
+
+def test_neighbours_in_one_buffer():
+    """Input, decay and state as parts of one allocation that do not overlap."""
+    buffer = -torch.rand(3, 8, 64, generator=torch.Generator().manual_seed(6)).cuda()
+    x, g, state = buffer.clone().unbind(0)
+    want = buffer[2].clone()
+    h = ops.diag_scan_step(x, g, state)
+    assert torch.equal(h, ops.diag_scan_step(buffer[0].clone(), buffer[1].clone(), want)) and torch.equal(state, want)
+    assert torch.equal(x, buffer[0]) and torch.equal(g, buffer[1])
