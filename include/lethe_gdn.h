@@ -356,6 +356,72 @@ size_t lethe_gdn_norm_work_bytes(int64_t rows, int32_t D, int32_t vectors);
 int lethe_gdn_residual_norm(const LetheGdnResidualNormArgs* args, void* cuda_stream);
 int lethe_gdn_residual_norm_vjp(const LetheGdnResidualNormArgs* args, void* cuda_stream);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * Decoding with several hypotheses: choosing tokens, and moving the states that belong to them.  No counterpart in the reference.
+ * These calls work on the GPU that owns `logits`, the first tensor of states (fork and compact: `live`), or `state`, and otherwise as the ones above.
+ * ------------------------------------------------------------------------------------------------------------------ */
+
+/* Beam search's selection: for B groups of W beams over V tokens,
+ *   c_wv = scores_w + l_wv / temperature - log sum_u exp(l_wu / temperature)   over the allowed tokens,
+ * the k candidates (w, v) with the largest c_wv / penalty_w, in order, of equal ones the lowest (w, v) first.  A finished beam offers
+ * itself, with its score, at the token eos and nothing else.  A beam offers nothing whose score is not finite, whose penalty is not
+ * above zero and finite, or that has no distribution (no allowed token above minus infinity, NaN or plus infinity at an allowed one).
+ * Candidates are ordered as in 64 bits.  Where there are fewer than k the rest has score minus infinity, parent 0, token eos
+ * (0 without eos) and counts as finished.
+ * logits [B, W, V] x_type, allowed bytes (non-zero: allowed), both with strides for group and beam (0: shared) in elements;
+ * scores, penalty fp32 [B, W], finished bytes [B, W], out_* [B, k].  W, k from 1 to 64, V to 2^30, temperature 1e-6 to 1e6.
+ * work: lethe_gdn_beam_work_bytes bytes on a 16-byte boundary, scratch of one call. */
+typedef struct LetheGdnBeamArgs {
+  int64_t B, V;
+  int32_t W, k, x_type;
+  double temperature;
+  const void* logits;
+  int64_t logits_batch, logits_beam;
+  const uint8_t* allowed;   /* NULL: every token                                              */
+  int64_t allowed_batch, allowed_beam;
+  const float* scores;
+  const uint8_t* finished;  /* NULL: none                                                     */
+  const float* penalty;     /* NULL: one                                                      */
+  int64_t eos;              /* -1: none (neither finished nor out_finished then)              */
+  float* out_scores;        /* c, not divided by the penalty                                  */
+  int64_t* parents;
+  int64_t* tokens;
+  uint8_t* out_finished;    /* NULL: not wanted.  Whether the parent was, or the token is eos  */
+  void* work;
+  size_t work_bytes;
+} LetheGdnBeamArgs;
+size_t lethe_gdn_beam_work_bytes(int64_t B, int32_t W, int64_t V, int32_t k, int32_t x_type);
+int lethe_gdn_beam_select(const LetheGdnBeamArgs* args, void* cuda_stream);
+
+/* States of sequences: for each of `count` tensors a row of row_bytes bytes per sequence, of any type, at
+ * data + group * group_stride + i * stride (bytes; whole rows do not overlap).  `states` is host memory, read during the call. */
+typedef struct LetheGdnStates {
+  void* data;
+  int64_t row_bytes, stride, group_stride;
+} LetheGdnStates;
+
+/* Row (b, w) becomes what row (b, parents[b, w]) was, in every tensor at once and in place, for B groups of W rows (W to 256).
+ * parents [B, W], int64 or (parents_64 = 0) int32.  A parent outside [0, W) leaves its row as it was and a code in *status. */
+int lethe_gdn_reorder_states(const LetheGdnStates* states, int32_t count, int64_t B, int32_t W, const void* parents, int32_t parents_64,
+                             int32_t* status, void* cuda_stream);
+
+/* A pool of slots (rows i of every tensor, to 65536; group_stride unused), live[i] non-zero for the ones in use.
+ * fork: n entries (to 4096); entry e takes the lowest free slot that no entry in front of it takes, target[e], which gets the values of
+ *   slot source[e] (zeros where that is -1).  Where source[e] is neither -1 nor a live slot, or no slot is left, target[e] = -1 and
+ *   nothing is taken.  live_after = live and the slots taken.  source int64 or (source_64 = 0) int32.
+ * compact: the m live slots become slots 0 to m - 1: the ones at or behind m, in their order, move to the free ones in front of m, in
+ *   theirs; what lies behind is left as it was.  place[i] = the new slot of live slot i, -1 for others; *live_count = m. */
+int lethe_gdn_fork_states(const LetheGdnStates* states, int32_t count, int64_t slots, const uint8_t* live, const void* source, int32_t source_64,
+                          int64_t n, int64_t* target, uint8_t* live_after, void* cuda_stream);
+int lethe_gdn_compact_states(const LetheGdnStates* states, int32_t count, int64_t slots, const uint8_t* live, int64_t* place,
+                             int64_t* live_count, void* cuda_stream);
+
+/* lethe_gdn_decode_step with a state of its own for what it writes: row b goes on from row source[b] of args->state [slots, H, K, V]
+ * (-1: from zeros), and its new state is row b of out [B, H, K, V], memory apart from args->state.  source [B], int64 or
+ * (source_64 = 0) int32; one outside [-1, slots) gives NaN and a code in *status. */
+int lethe_gdn_decode_step_from(const LetheGdnDecodeArgs* args, int64_t slots, const void* source, int32_t source_64, float* out,
+                               int32_t* status, void* cuda_stream);
+
 /* Text for a return code of the calls above or for a device status code. */
 const char* lethe_gdn_strerror(int code);
 

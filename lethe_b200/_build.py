@@ -24,7 +24,7 @@ PROBE_SRC = os.path.join(ROOT, "tests", "native", "probe.cu")
 PROBE_SRCS = [PROBE_SRC, os.path.join(ROOT, "tests", "native", "look_probe.cu")]
 PROBE_LIBDIR = os.path.join(ROOT, "tests", "native", "_lib")
 PROBE_LIB = os.path.join(PROBE_LIBDIR, "libletheprobe.so")
-TORCH_SRCS = [os.path.join(CSRC, f) for f in ("torch_ops.cpp", "torch_block.cpp")]
+TORCH_SRCS = [os.path.join(CSRC, f) for f in ("torch_ops.cpp", "torch_block.cpp", "torch_beam.cpp")]
 TORCH_LIB = os.path.join(LIBDIR, "lethe_gdn_torch.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 # -use_fast_math: subnormal results flush to zero and division / square root are the approximate forms.
@@ -34,7 +34,7 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-use_fast_math",
          "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr", "-I", os.path.join(ROOT, "include"), "-I", CSRC]
 # Not for these: their exponentials and roots stand in fp32 results.
-EXACT_MATH = {"diag_scan.cu", "block_norm.cu", "residual_norm.cu", "residual_norm_vjp.cu"}
+EXACT_MATH = {"diag_scan.cu", "block_norm.cu", "residual_norm.cu", "residual_norm_vjp.cu", "beam_select.cu"}
 FLAGS += os.environ.get("LETHE_NVCC_FLAGS", "").split()
 
 

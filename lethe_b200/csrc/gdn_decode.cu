@@ -25,7 +25,28 @@ struct DecodeProblem {
   const float *g, *beta;
   float* state;
   __nv_bfloat16* o;
+  // steps that go on from another row: `state` is what they write
+  int B;
+  long long slots;
+  const float* from;
+  const void* source;
+  int source64;
+  int* status;
 };
+
+// The step that goes on from other rows takes the rows of a head one after the other, where the plain one takes the heads of a row: rows
+// with one source read its state at about the same time, from L2 all but once.
+template <bool FROM> __device__ __forceinline__ int pair_of(const DecodeProblem& p, int i) {
+  return FROM ? i % p.B * p.H + i / p.B : i;
+}
+// what a row starts from: a slot, zeros (-1), or nothing that there is (-2)
+__device__ __forceinline__ long long slot_of(const DecodeProblem& p, int bh) {
+  const int b = bh / p.H;
+  const long long s = p.source64 ? static_cast<const long long*>(p.source)[b] : static_cast<const int*>(p.source)[b];
+  if (s >= -1 && s < p.slots) return s;
+  *p.status = kErrIndex;
+  return -2;
+}
 
 // kSplit threads share a column of S (kDK / kSplit rows each).
 constexpr int kSplit = 4;
@@ -36,11 +57,11 @@ __device__ __forceinline__ float token_in(const void* x, size_t i) {
   return __bfloat162float(static_cast<const __nv_bfloat16*>(x)[i]);
 }
 
-template <int V, bool F32>
+template <int V, bool F32, bool FROM>
 __global__ void __launch_bounds__(kSplit * V, 1024 / (kSplit * V))
 decode_step_kernel(const DecodeProblem p) {
   __shared__ float ks[kDK], qs[kDK], as[kDK], part[kSplit][V];
-  const int bh = blockIdx.x, c = threadIdx.x % V, part_id = threadIdx.x / V;   // rows [kRows part_id, + kRows)
+  const int bh = pair_of<FROM>(p, blockIdx.x), c = threadIdx.x % V, part_id = threadIdx.x / V;   // rows [kRows part_id, + kRows)
   for (int d = threadIdx.x; d < kDK; d += kSplit * V) {
     ks[d] = token_in<F32>(p.k, static_cast<size_t>(bh) * kDK + d);
     qs[d] = p.scale * token_in<F32>(p.q, static_cast<size_t>(bh) * kDK + d);
@@ -52,8 +73,17 @@ decode_step_kernel(const DecodeProblem p) {
   constexpr int kRows = kDK / kSplit;
   float* S = p.state + (static_cast<size_t>(bh) * kDK + part_id * kRows) * V + c;
   float col[kRows];
+  const float* in = S;
+  if (FROM) {
+    const long long slot = slot_of(p, bh);
+    in = slot < 0 ? nullptr : p.from + ((slot * p.H + bh % p.H) * kDK + part_id * kRows) * V + c;
 #pragma unroll
-  for (int d = 0; d < kRows; ++d) col[d] = S[static_cast<size_t>(d) * V];   // all loads in flight at once
+    for (int d = 0; d < kRows; ++d) col[d] = slot == -2 ? __int_as_float(0x7fffffff) : 0.f;
+  }
+  if (!FROM || in) {
+#pragma unroll
+    for (int d = 0; d < kRows; ++d) col[d] = in[static_cast<size_t>(d) * V];   // all loads in flight at once
+  }
   __syncthreads();
   const float* kh = ks + part_id * kRows;
   const float* qh = qs + part_id * kRows;
@@ -101,7 +131,7 @@ __device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
-template <bool F32>
+template <bool F32, bool FROM>
 __global__ void __launch_bounds__(kRingThreads, kRingCtas)
 decode_ring_kernel(const DecodeProblem p) {
   constexpr int V = 128;
@@ -111,9 +141,19 @@ decode_ring_kernel(const DecodeProblem p) {
   __shared__ __align__(16) float kpart[kRingWarps][V], opart[kRingWarps][V];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;         // rows [kRingRows warp, +), columns [4 lane, +4)
   const size_t own = static_cast<size_t>(warp * kRingRows) * 32 + lane;
-  auto fetch = [&](int bh) {
-    if (bh < p.BH) {
-      const float4* src = reinterpret_cast<const float4*>(p.state + static_cast<size_t>(bh) * kDK * V) + own;
+  // (the source of the state after the next comes while the next is fetched)
+  long long slot = 0;
+  auto look = [&](int i) {
+    if (FROM && i < p.BH) slot = slot_of(p, pair_of<FROM>(p, i));
+  };
+  auto fetch = [&](int i) {
+    if (i < p.BH && FROM && slot < 0) {
+      const float x = slot == -2 ? __int_as_float(0x7fffffff) : 0.f;
+#pragma unroll
+      for (int r = 0; r < kRingRows; ++r) slots[r * kRingThreads + tid] = make_float4(x, x, x, x);
+    } else if (i < p.BH) {
+      const size_t pair = FROM ? static_cast<size_t>(slot) * p.H + i / p.B : static_cast<size_t>(i);
+      const float4* src = reinterpret_cast<const float4*>((FROM ? p.from : p.state) + pair * kDK * V) + own;
       const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(slots + tid));
 #pragma unroll
       for (int r = 0; r < kRingRows; ++r) copy_async16(dst + r * kRingThreads * 16, src + r * 32);
@@ -122,8 +162,9 @@ decode_ring_kernel(const DecodeProblem p) {
   };
   // the token's vectors: k, q, decay by threads 0-127, v and beta by the others
   float t0 = 0.f, t1 = 0.f, t2 = 1.f;
-  auto token = [&](int bh) {
-    if (bh >= p.BH) return;
+  auto token = [&](int i) {
+    if (i >= p.BH) return;
+    const int bh = pair_of<FROM>(p, i);
     if (tid < kDK) {
       t0 = token_in<F32>(p.k, static_cast<size_t>(bh) * kDK + tid);
       t1 = p.scale * token_in<F32>(p.q, static_cast<size_t>(bh) * kDK + tid);
@@ -146,20 +187,23 @@ decode_ring_kernel(const DecodeProblem p) {
     if (tid == kDK) bs = t1;
   };
   const int step = gridDim.x;
+  look(blockIdx.x);
   fetch(blockIdx.x);
+  look(blockIdx.x + step);
   token(blockIdx.x);
   put_k(0);
   __syncthreads();
   int it = 0;
-  for (int bh = blockIdx.x; bh < p.BH; bh += step, ++it) {
-    const int buf = it & 1;
+  for (int i = blockIdx.x; i < p.BH; i += step, ++it) {
+    const int buf = it & 1, bh = pair_of<FROM>(p, i);
     put_qv();
-    token(bh + step);
+    token(i + step);
     float4 col[kRingRows];
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
     for (int r = 0; r < kRingRows; ++r) col[r] = slots[r * kRingThreads + tid];
-    fetch(bh + step);                                  // a slot is its thread's own: free once read
+    fetch(i + step);                                   // a slot is its thread's own: free once read
+    look(i + 2 * step);
     const float *kh = ks[buf] + warp * kRingRows, *qh = qs + warp * kRingRows, *ah = as + warp * kRingRows;
     float4 ksum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -208,20 +252,20 @@ decode_ring_kernel(const DecodeProblem p) {
 }
 
 // d_v = 64 stays with one CTA per pair: eight of half the size per SM overlap as well (2048 pairs: 26.8 us, ring 27.5).
-template <bool F32>
+template <bool F32, bool FROM>
 static int launch_decode(const DecodeProblem& p, cudaStream_t st) {
   if (p.V == 64) {
-    decode_step_kernel<64, F32><<<p.BH, kSplit * 64, 0, st>>>(p);
+    decode_step_kernel<64, F32, FROM><<<p.BH, kSplit * 64, 0, st>>>(p);
   } else {
     const int sms = sm_count();
     if (sms <= 0) return kErrDevice;
-    const bool aligned = reinterpret_cast<uintptr_t>(p.state) % 16 == 0 && reinterpret_cast<uintptr_t>(p.o) % 4 == 0;
+    const bool aligned = (reinterpret_cast<uintptr_t>(p.state) | reinterpret_cast<uintptr_t>(p.from)) % 16 == 0 && reinterpret_cast<uintptr_t>(p.o) % 4 == 0;
     if (p.BH >= 4 * sms && aligned) {
       static SmemAttr attr;
-      if (attr.set(decode_ring_kernel<F32>, kRingBytes)) return kErrLaunch;
-      decode_ring_kernel<F32><<<kRingCtas * sms, kRingThreads, kRingBytes, st>>>(p);
+      if (attr.set(decode_ring_kernel<F32, FROM>, kRingBytes)) return kErrLaunch;
+      decode_ring_kernel<F32, FROM><<<kRingCtas * sms, kRingThreads, kRingBytes, st>>>(p);
     } else {
-      decode_step_kernel<128, F32><<<p.BH, kSplit * 128, 0, st>>>(p);
+      decode_step_kernel<128, F32, FROM><<<p.BH, kSplit * 128, 0, st>>>(p);
     }
   }
   return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
@@ -229,16 +273,15 @@ static int launch_decode(const DecodeProblem& p, cudaStream_t st) {
 
 }  // namespace lg
 
-extern "C" int lethe_gdn_decode_step(const LetheGdnDecodeArgs* a, void* stream) {
+// a call's arguments, checked; 0 or an error code
+static int decode_problem(const LetheGdnDecodeArgs* a, lg::DecodeProblem* out) {
   using namespace lg;
   if (!a || !a->q || !a->k || !a->v || !a->state || !a->o) return kErrNull;
   if (a->B <= 0 || a->H <= 0 || a->K != kDK || (a->V != 64 && a->V != 128)) return kErrDims;
   if (a->gate != LETHE_GATE_NONE && a->gate != LETHE_GATE_SCALAR && a->gate != LETHE_GATE_CHANNEL) return kErrFlags;
   if (a->gate != LETHE_GATE_NONE && !a->g) return kErrNull;
   if (a->delta && !a->beta) return kErrNull;
-  DeviceGuard guard(a->state);
-  if (!guard.ok) return kErrDevice;
-  DecodeProblem p;
+  DecodeProblem p = {};
   p.BH = a->B * a->H;
   p.H = a->H;
   p.V = a->V;
@@ -252,6 +295,42 @@ extern "C" int lethe_gdn_decode_step(const LetheGdnDecodeArgs* a, void* stream) 
   p.beta = a->beta;
   p.state = a->state;
   p.o = static_cast<__nv_bfloat16*>(a->o);
+  *out = p;
+  return kOk;
+}
+
+extern "C" int lethe_gdn_decode_step(const LetheGdnDecodeArgs* a, void* stream) {
+  using namespace lg;
+  DecodeProblem p;
+  const int bad = decode_problem(a, &p);
+  if (bad) return bad;
+  DeviceGuard guard(a->state);
+  if (!guard.ok) return kErrDevice;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return a->in_f32 ? launch_decode<true>(p, st) : launch_decode<false>(p, st);
+  return a->in_f32 ? launch_decode<true, false>(p, st) : launch_decode<false, false>(p, st);
+}
+
+extern "C" int lethe_gdn_decode_step_from(const LetheGdnDecodeArgs* a, int64_t slots, const void* source, int32_t source_64, float* out,
+                                          int32_t* status, void* stream) {
+  using namespace lg;
+  DecodeProblem p;
+  const int bad = decode_problem(a, &p);
+  if (bad) return bad;
+  if (!source || !out || !status) return kErrNull;
+  const int64_t row = static_cast<int64_t>(a->H) * kDK * a->V * 4, most = (int64_t(1) << 56) / row;
+  if (slots <= 0 || slots > most || static_cast<int64_t>(a->B) * a->H > (int64_t(1) << 30)) return kErrDims;
+  if (reinterpret_cast<uintptr_t>(source) % (source_64 ? 8 : 4) || reinterpret_cast<uintptr_t>(out) % 4 || reinterpret_cast<uintptr_t>(a->state) % 4) return kErrAlign;
+  const uintptr_t in0 = reinterpret_cast<uintptr_t>(a->state), out0 = reinterpret_cast<uintptr_t>(out);
+  if (out0 < in0 + slots * row && in0 < out0 + a->B * row) return kErrFlags;      // (a row may be read after another is written)
+  DeviceGuard guard(a->state);
+  if (!guard.ok) return kErrDevice;
+  p.B = a->B;
+  p.slots = slots;
+  p.from = a->state;
+  p.state = out;
+  p.source = source;
+  p.source64 = source_64;
+  p.status = status;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return a->in_f32 ? launch_decode<true, true>(p, st) : launch_decode<false, true>(p, st);
 }

@@ -21,6 +21,7 @@ enum : int {
   kErrTooLarge = 8,    // problem larger than a fixed-capacity entry point accepts
   kErrDevice = 9,      // the device that owns the tensors could not be made current, or a buffer lives elsewhere
   kErrSymbol = 10,     // the address of the library's built-in workspace could not be looked up
+  kErrIndex = 11,      // (status word) an index on the device lay outside its range
 };
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,

@@ -48,31 +48,11 @@ bool wants_grad(std::initializer_list<Tensor> ts) {
   return false;
 }
 
-void need_cuda(const Tensor& t) {
-  if (!t.is_cuda()) fail("inputs must live on a CUDA device (there is no CPU path)");
-}
-bool known(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16 || t == at::kHalf; }
-int32_t code(at::ScalarType t) { return t == at::kFloat ? LETHE_F32 : t == at::kBFloat16 ? LETHE_BF16 : LETHE_F16; }
-void need_type(const Tensor& t, const char* name) {
-  if (!known(t.scalar_type())) fail(std::string(name) + " must be fp32, bf16 or fp16");
-}
-void need_float(const Tensor& t, const char* name) {
-  if (t.defined() && !at::isFloatingType(t.scalar_type())) fail(std::string(name) + " must be a real floating-point tensor");
-}
 // a tensor that may be in 32 bits or in the type of the activations; anything else is read as fp32
 Tensor in_type(const Tensor& t, at::ScalarType dt) {
   return t.scalar_type() == dt || t.scalar_type() == at::kFloat ? t : t.to(at::kFloat);
 }
 
-// whether dimensions [from, end) of t lie in memory as one contiguous piece per index of those in front
-bool packed_from(const Tensor& t, int64_t from) {
-  int64_t want = 1;
-  for (int64_t i = t.dim() - 1; i >= from; --i) {
-    if (t.size(i) != 1 && t.stride(i) != want) return false;
-    want *= t.size(i);
-  }
-  return true;
-}
 // stride between neighbours over dimensions [from, to) taken as one; -1: there is none
 int64_t joint_stride(const Tensor& t, int64_t from, int64_t to) {
   int64_t stride = 0, want = 0;
@@ -92,9 +72,6 @@ int64_t joint_stride(const Tensor& t, int64_t from, int64_t to) {
 // ---------------------------------------------------------------------------------------------
 // readable as [B, L, D] with strides for batch and token
 Tensor tokens(const Tensor& t) { return lazy(t) || !packed_from(t, 2) ? as(t, t.scalar_type()) : t; }
-
-// stride of a dimension; one of a single index is never gone by, and its stride says nothing
-int64_t step_of(const Tensor& t, int64_t dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
 
 LetheGdnDiagArgs diag_args(const Tensor& x, const Tensor& g, bool complement) {
   LetheGdnDiagArgs a;

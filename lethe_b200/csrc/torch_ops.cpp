@@ -633,27 +633,48 @@ Tensor six_inputs(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
 // ---------------------------------------------------------------------------------------------
 // One token
 // ---------------------------------------------------------------------------------------------
+// With `source`, row b goes on from row source[b] of the state and leaves its new one in `out`, which lies apart.
 Tensor decode_step(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& g_, const OptTensor& beta_,
-                   const Tensor& state, double scale) {
+                   const Tensor& state, double scale, const OptTensor& source_, const OptTensor& out_) {
   return guarded([&] {
     if (!state.is_cuda()) fail("inputs must live on a CUDA device (there is no CPU path)");
     if (state.scalar_type() != at::kFloat || !state.is_contiguous() || state.dim() != 4)
       fail("the decode state must be a contiguous fp32 tensor (it is updated in place)");
     at::NoGradGuard no_grad;
-    const int64_t B = state.size(0), H = state.size(1), K = state.size(2), V = state.size(3);
+    const Tensor source_in = opt(source_), out = opt(out_);
+    if (source_in.defined() != out.defined()) fail("decode step takes source and out together");
+    const bool from = out.defined();
+    if (from && out.dim() != 4) fail("decode step expects out [B,H,K,V]");
+    const int64_t B = from ? out.size(0) : state.size(0), H = state.size(1), K = state.size(2), V = state.size(3);
     if (q.sizes() != at::IntArrayRef({B, H, K}) || k.sizes() != q.sizes() || v.sizes() != at::IntArrayRef({B, H, V}))
       fail("decode step expects q, k [B,H,K] and v [B,H,V] matching the state");
     const Tensor g_in = opt(g_), beta_in = opt(beta_);
-    need_device(state, q, k, v, g_in, beta_in);
-    const Tensor g = as32(g_in), beta = as32(beta_in);
+    need_device(state, q, k, v, g_in, beta_in, source_in, out);
+    Tensor g = as32(g_in), beta = as32(beta_in);
     if (g.defined() && g.sizes() != at::IntArrayRef({B, H}) && g.sizes() != q.sizes())
       fail("decode step expects g [B,H] or [B,H,K]");
     if (beta.defined() && beta.sizes() != at::IntArrayRef({B, H})) fail("decode step expects beta [B,H]");
+    if (from) {
+      if (out.sizes() != at::IntArrayRef({B, H, K, V}) || out.scalar_type() != at::kFloat || !out.is_contiguous() || lazy(out) || out.requires_grad())
+        fail("out must be a contiguous fp32 tensor [B,H,K,V] without a gradient (it is written)");
+      if (lazy(state)) fail("the decode state must hold its values");
+      need_index(source_in, "source");
+      need_shape(source_in.sizes() == at::IntArrayRef({B}), "source [B]");
+      refuse_tangents({q, k, v, g_in, beta_in, state, out});
+      if (B && spans(state, out)) fail("out must not share memory with the state that other rows go on from");
+    }
     c10::cuda::CUDAGuard guard(state.device());
     const bool f32 = q.scalar_type() == at::kFloat && k.scalar_type() == at::kFloat && v.scalar_type() == at::kFloat;
     const at::ScalarType dt = f32 ? at::kFloat : at::kBFloat16;
-    const Tensor qc = as(q, dt), kc = as(k, dt), vc = as(v, dt);
+    Tensor qc = as(q, dt), kc = as(k, dt), vc = as(v, dt), source;
     Tensor o = at::empty({B, H, V}, state.options().dtype(at::kBFloat16));
+    if (from) {
+      if (!B) return o;
+      need_shape(state.numel() > 0, "state [slots,H,K,V] with a slot at least");
+      source = as(source_in, source_in.scalar_type());
+      for (Tensor* t : {&qc, &kc, &vc, &g, &beta, &source})      // what lies in the memory of `out` is read before any of it is written
+        if (t->defined() && spans(*t, out)) *t = t->clone();
+    }
     LetheGdnDecodeArgs a;
     memset(&a, 0, sizeof(a));
     a.B = static_cast<int32_t>(B); a.H = static_cast<int32_t>(H); a.K = static_cast<int32_t>(K); a.V = static_cast<int32_t>(V);
@@ -665,7 +686,13 @@ Tensor decode_step(const Tensor& q, const Tensor& k, const Tensor& v, const OptT
     a.state = ptr<float>(state);
     a.o = ptr(o);
     a.in_f32 = f32 ? 1u : 0u;
-    check(lethe_gdn_decode_step(&a, stream_of(state)));
+    if (!from) {
+      check(lethe_gdn_decode_step(&a, stream_of(state)));
+      return o;
+    }
+    check(lethe_gdn_decode_step_from(&a, state.size(0), ptr(source), source.scalar_type() == at::kLong, ptr<float>(out),
+                                     status_word(state.device().index()), stream_of(state)));
+    if (!out.is_inference()) torch::autograd::impl::bump_version(out);
     return o;
   });
 }
@@ -683,6 +710,12 @@ PYBIND11_MODULE(lethe_gdn_torch, m) {
     return reinterpret_cast<uintptr_t>(host_words().status + dev);
   });
   m.def("gate_test_slots", [] { return regime_pool().count(); });
-  m.def("decode_step", &decode_step);
+  using pybind11::arg;
+  m.def("decode_step", &decode_step, arg("q"), arg("k"), arg("v"), arg("g"), arg("beta"), arg("state"), arg("scale"), arg("source") = pybind11::none(),
+        arg("out") = pybind11::none());
+  m.def("decode_step_from", [](const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& g, const OptTensor& beta, const Tensor& state,
+                               const OptTensor& source, const OptTensor& out, double scale) { return decode_step(q, k, v, g, beta, state, scale, source, out); },
+        arg("q"), arg("k"), arg("v"), arg("g"), arg("beta"), arg("state"), arg("source"), arg("out"), arg("scale"));
   bind_block(m);
+  bind_beam(m);
 }

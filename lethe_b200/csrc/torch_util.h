@@ -78,6 +78,8 @@ inline int32_t* status_word(int dev) {
   const int32_t code = *w;
   if (code != 0) {
     *w = 0;
+    if (code < 100)
+      fail(std::string(lethe_gdn_strerror(code)) + " in an earlier call; the rows it was given for are not valid (code " + std::to_string(code) + ")");
     fail("a device-side wait of an earlier call timed out at site " + std::to_string(code) +
          "; the results of that call are invalid");
   }
@@ -139,6 +141,46 @@ inline void refuse_tangents(std::initializer_list<Tensor> ts) {
       fail("forward-mode differentiation is not implemented", PyExc_NotImplementedError);
 }
 
+inline void need_cuda(const Tensor& t) {
+  if (!t.is_cuda()) fail("inputs must live on a CUDA device (there is no CPU path)");
+}
+inline bool known(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16 || t == at::kHalf; }
+inline int32_t code(at::ScalarType t) { return t == at::kFloat ? LETHE_F32 : t == at::kBFloat16 ? LETHE_BF16 : LETHE_F16; }
+inline void need_type(const Tensor& t, const char* name) {
+  if (!known(t.scalar_type())) fail(std::string(name) + " must be fp32, bf16 or fp16");
+}
+inline void need_float(const Tensor& t, const char* name) {
+  if (t.defined() && !at::isFloatingType(t.scalar_type())) fail(std::string(name) + " must be a real floating-point tensor");
+}
+// whether dimensions [from, end) of t lie in memory as one contiguous piece per index of those in front
+inline bool packed_from(const Tensor& t, int64_t from) {
+  int64_t want = 1;
+  for (int64_t i = t.dim() - 1; i >= from; --i) {
+    if (t.size(i) != 1 && t.stride(i) != want) return false;
+    want *= t.size(i);
+  }
+  return true;
+}
+// stride of a dimension; one of a single index is never gone by, and its stride says nothing
+inline int64_t step_of(const Tensor& t, int64_t dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
+
+// places of tensors' memory from first to last byte, and whether two of them meet: by addresses, since two storages can stand for the same memory
+inline std::pair<const char*, const char*> span_of(const Tensor& t) {
+  const char* p = static_cast<const char*>(t.data_ptr());
+  if (t.numel() == 0) return {p, p};
+  int64_t last = 0;
+  for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+  return {p, p + (last + 1) * t.element_size()};
+}
+inline bool spans(const Tensor& a, const Tensor& b) {
+  const auto x = span_of(a), y = span_of(b);
+  return x.first < y.second && y.first < x.second;
+}
+inline void need_index(const Tensor& t, const char* name) {
+  if (t.scalar_type() != at::kInt && t.scalar_type() != at::kLong) fail(std::string(name) + " must be int32 or int64");
+}
+
 void bind_block(pybind11::module_& m);      // torch_block.cpp
+void bind_beam(pybind11::module_& m);       // torch_beam.cpp
 
 }  // namespace lethe_torch

@@ -569,6 +569,23 @@ class _TracedStep(torch.autograd.Function):
         return (None,) * len(ctx.needs_input_grad)
 
 
+class _TracedCall(torch.autograd.Function):
+    """The same for a call that chooses or moves: its tensors come in a list where `listed` says how many in front are one."""
+
+    @staticmethod
+    def forward(ctx, call, options, listed, *tensors):
+        args = tensors if listed is None else (list(tensors[:listed]), *tensors[listed:])
+        out = getattr(native.ext(), call)(*args, **options)
+        out = (args[-1].new_empty(0),) if out is None else out if isinstance(out, tuple) else (out,)
+        out = tuple(t for t in out if t is not None)
+        ctx.mark_non_differentiable(*out)
+        return out
+
+    @staticmethod
+    def backward(ctx, *grads):      # (never asked for)
+        return (None,) * len(ctx.needs_input_grad)
+
+
 def gdn_chunk(q: Tensor, k: Tensor, v: Tensor, g: Tensor | None, beta: Tensor | None,
               h0: Tensor | None = None, *, scale: float | None = None,
               use_qk_l2norm: bool = False) -> tuple[Tensor, Tensor]:
@@ -600,7 +617,7 @@ class _DecodeArgs(ctypes.Structure):
 
 
 def gdn_decode_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor | None, beta: Tensor | None, state: Tensor,
-                    *, scale: float | None = None) -> Tensor:
+                    *, scale: float | None = None, source: Tensor | None = None, out: Tensor | None = None) -> Tensor:
     """One token of the recurrence for every (batch, head) pair, for generation: the body of the
     reference's token loop (``src/lethe/kernels/references/gdn_backward.py:45-53``).
 
@@ -608,11 +625,18 @@ def gdn_decode_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor | None, beta: Ten
     ``beta [B,H]`` or None (no delta term); ``state [B,H,K,V]`` fp32 contiguous, **updated in place**
     (start from the ``h_T`` that ``gdn_chunk`` returned for the prompt).  Returns ``o [B,H,V]`` bf16.
     Not differentiable.  K must be 128, V 64 or 128.
+
+    With ``source [B]`` (int32 or int64) and ``out [B,H,K,V]`` (fp32, contiguous, apart from the state) row b goes on from row
+    ``source[b]`` of ``state [slots,H,K,V]``, from zeros where that is -1, and its new state is row b of ``out``; ``state`` is left as it
+    was.  A beam search that swaps two buffers after every token so hands states on without moving them.  A source outside gives NaN, and an
+    error at a later call.
     """
     if torch._C._is_tracing():
         scale = int(state.shape[2]) ** -0.5 if scale is None else scale      # (a traced size is a tensor)
+        if source is not None or out is not None:
+            return _TracedCall.apply("decode_step_from", dict(scale=float(scale)), None, q, k, v, g, beta, state, source, out)[0]
         return _TracedStep.apply("decode_step", float(scale), q, k, v, g, beta, state)
-    return native.ext().decode_step(q, k, v, g, beta, state, state.shape[2] ** -0.5 if scale is None else scale)
+    return native.ext().decode_step(q, k, v, g, beta, state, state.shape[2] ** -0.5 if scale is None else scale, source, out)
 
 
 def gdn_chunk_full(q: Tensor, k: Tensor, v: Tensor, g: Tensor, b: Tensor, w: Tensor, h0: Tensor | None = None, *,
@@ -684,6 +708,83 @@ def residual_norm(x: Tensor, residual: Tensor | None, weight: Tensor, *, scale: 
     if torch._C._is_tracing():
         return _Traced.apply("residual_norm", float(eps), num, x, residual, weight, post_weight, vec)
     return native.ext().residual_norm(x, residual, weight, post_weight, vec, eps, num)
+
+
+# ------------------------------------------------------------------------------------------------
+# Decoding with several hypotheses
+# ------------------------------------------------------------------------------------------------
+class BeamChoice(NamedTuple):
+    """``[B, k]`` each, best first.  ``finished`` is None where no ``eos`` was given."""
+    scores: Tensor
+    parents: Tensor
+    tokens: Tensor
+    finished: Tensor | None
+
+
+def beam_select(logits: Tensor, scores: Tensor, k: int | None = None, *, temperature: float = 1.0, allowed: Tensor | None = None,
+                finished: Tensor | None = None, eos: int | None = None, penalty: Tensor | None = None) -> BeamChoice:
+    """Beam search's selection: for B groups of W beams the ``k`` best continuations (W where not given) over all beams and the
+    vocabulary, in one pass over the logits.
+
+    ``logits [B, W, V]``: fp32, bf16 or fp16.  ``scores [B, W]``: log probabilities of the beams so far, fp32.  A candidate is token v behind
+    beam w, with score ``scores[w] + log_softmax(logits[w] / temperature)[v]``; ``allowed`` (truth values that broadcast to the logits)
+    leaves tokens out, of the softmax too.  Candidates are ranked by score, or by score / ``penalty [B, W]`` (fp32, above zero; a length penalty), as in 64 bits,
+    of equal ones the lowest beam and token first.  ``scores`` of the result are not divided, rounded to fp32; ``parents`` (the beam gone on
+    from) and ``tokens`` are int64.
+
+    ``eos``: the token that ends a hypothesis; ``finished`` of the result is whether the parent was or the token is it.  A beam that
+    ``finished [B, W]`` marks offers itself, with its score, at the token ``eos``, and nothing else; its logits are not read.  A beam whose score is
+    not finite (``-inf``: not in use, as all but the first of equal ones at the start), whose penalty is not above zero and finite, or
+    whose allowed logits are all ``-inf`` or hold NaN or ``+inf``, offers nothing.  Places that are left have score ``-inf``, parent 0, token ``eos`` or 0,
+    and count as finished.
+
+    W and k from 1 to 64, V up to 2^30, temperature 1e-6 to 1e6.  Beams may have any strides.  Not differentiable."""
+    options = dict(k=-1 if k is None else int(k), temperature=float(temperature), eos=None if eos is None else int(eos))
+    if torch._C._is_tracing():
+        got = _TracedCall.apply("beam_select", options, None, logits, scores, allowed, finished, penalty)
+    else:
+        got = native.ext().beam_select(logits, scores, allowed, finished, penalty, **options)
+    return BeamChoice(*got[:3], None if eos is None else got[3])
+
+
+def reorder_states(states: Tensor | list[Tensor], parents: Tensor) -> None:
+    """Every beam takes over the states of the beam that it continues, **in place**: row (b, w) becomes what row ``(b, parents[b, w])`` was.
+
+    ``states``: a tensor or a list of them, ``[B W, ...]`` or ``[B, W, ...]``, of any types; the row of a sequence contiguous, rows with any
+    strides, no two in one place.  Rows that stay are not touched, one that several take over is read once, and there is one launch for
+    all (up to 32) tensors.  ``parents [B, W]``: int32 or int64, W up to 256; the tokens so far can go along as one of the states.  A parent outside
+    ``[0, W)`` leaves its row as it was, and gives an error at a later call.  Not differentiable."""
+    states = [states] if isinstance(states, Tensor) else list(states)
+    if torch._C._is_tracing():
+        _TracedCall.apply("reorder_states", {}, len(states), *states, parents)
+    else:
+        native.ext().reorder_states(states, parents)
+
+
+def fork_states(states: Tensor | list[Tensor], live: Tensor, source: Tensor) -> tuple[Tensor, Tensor]:
+    """Slots of a pool for new sequences, each with a copy of another's states.  Returns ``(target [n] int64, live)``: the slot that entry i
+    got, and which slots are in use now.
+
+    ``states``: a tensor or a list of them, ``[slots, ...]``, of any types, written **in place**; ``live [slots]``: truth values, the slots in use
+    (give one back by clearing its mark).  ``source [n]`` (int32 or int64): the live slot that entry i starts from, or -1 for a new sequence, whose states
+    are zero.  Entries take the lowest free slots in their order; one whose source is neither, or for which no slot is
+    left, gets -1.  Nothing waits for the host.  Up to 65536 slots and 4096 entries.  Not differentiable."""
+    states = [states] if isinstance(states, Tensor) else list(states)
+    if torch._C._is_tracing():
+        return _TracedCall.apply("fork_states", {}, len(states), *states, live, source)
+    return native.ext().fork_states(states, live, source)
+
+
+def compact_states(states: Tensor | list[Tensor], live: Tensor) -> tuple[Tensor, Tensor]:
+    """The live slots of a pool move together at its front, **in place**, with as few copies as there can be: of n live slots those at n or behind
+    move, in their order, to the free ones in front of n.  Returns ``(place [slots] int64, count)``: where each live slot is now (-1 for the
+    others; ``table = place[table]`` mends a table of slots), and n as a tensor.  What lies in the slots behind is left as it was.
+
+    ``states`` and ``live`` as for ``fork_states``; the marks afterwards are ``torch.arange(slots) < count``.  Not differentiable."""
+    states = [states] if isinstance(states, Tensor) else list(states)
+    if torch._C._is_tracing():
+        return _TracedCall.apply("compact_states", {}, len(states), *states, live)
+    return native.ext().compact_states(states, live)
 
 
 # ------------------------------------------------------------------------------------------------

@@ -94,7 +94,8 @@ class DiagBlock(nn.Module):
 
 
 class TinyDiagLM(nn.Module):
-    """``ops``: ``lethe_b200.ops`` or anything with its ``diag_scan``, ``diag_scan_step``, ``gated_norm`` and ``residual_norm``."""
+    """``ops``: ``lethe_b200.ops`` or anything with its ``diag_scan``, ``diag_scan_step``, ``gated_norm`` and ``residual_norm`` (``beam_search``: ``beam_select`` and
+    ``reorder_states`` too)."""
 
     def __init__(self, ops, vocab: int = 40, d_model: int = 64, H: int = 2, V: int = 64, layers: int = 2):
         super().__init__()
@@ -113,3 +114,23 @@ class TinyDiagLM(nn.Module):
             after.append(state)
         y, _ = self.ops.residual_norm(x, stream, self.norm)
         return self.head(y), after
+
+    @torch.no_grad()
+    def beam_search(self, prompt: Tensor, steps: int, beams: int, eos: int | None = None) -> tuple[Tensor, Tensor]:
+        """The ``beams`` best continuations found for every ``prompt [B, L]``: tokens ``[B, beams, steps]`` and log probabilities
+        ``[B, beams]``, best first.  Every beam has its own states, which follow the beams that are gone on from."""
+        B = prompt.shape[0]
+        logits, states = self(prompt)
+        scores = torch.full((B, beams), float("-inf"), device=prompt.device)
+        scores[:, 0] = 0.0                                          # (all beams are the same one)
+        states = [s.repeat_interleave(beams, 0) for s in states]
+        logits = logits[:, -1:].expand(B, beams, -1)
+        written = torch.zeros(B * beams, steps, dtype=torch.long, device=prompt.device)
+        finished = None
+        for t in range(steps):
+            if t:
+                logits = self(written[:, t - 1], states)[0].view(B, beams, -1)
+            scores, parents, tokens, finished = self.ops.beam_select(logits, scores, finished=finished, eos=eos)
+            self.ops.reorder_states([*states, written], parents)
+            written[:, t] = tokens.flatten()
+        return written.view(B, beams, steps), scores
