@@ -12,6 +12,8 @@
 // different beams that decide the result are closer than two such errors, the merge sums the exponentials of those beams again in 64 bits.
 #include <math.h>
 
+#include <type_traits>
+
 #include "elem.cuh"
 #include "host_util.h"
 #include "umma.cuh"
@@ -20,8 +22,9 @@ namespace lg {
 
 constexpr int kBeamMost = 64;                     // beams of a group, and candidates asked for
 constexpr int kTileLogits = 1024, kMostTiles = 8; // a warp takes that many logits at a time, and so many times
-constexpr int kScanWarps = 8, kFillWarps = 148 * 24;
-constexpr int kCands = 256;                       // candidates of a segment that are put in order together
+constexpr int kScanWarps = 4, kFillWarps = 148 * 24;
+constexpr int kCands = 128;                       // candidates of a segment that are looked at together
+constexpr int kSpare = 16;                        // more than asked for that a list may have
 constexpr int kMergeThreads = 512, kBins = 128, kMergeRoom = 2 * kMergeThreads;
 constexpr int kBehind = 8;                        // candidates behind the last chosen one that are looked at for equals
 // A term of a sum: exp2 by the hardware 2^-22, its argument (two roundings of |t| 2^-24, weighted by 2^t) 2^-23.5, twice (tile to
@@ -30,7 +33,7 @@ constexpr double kLseError = 2 * 2.4e-7 + 1e-7 + 7 * 6e-8;
 
 struct ScanStat {
   float m;          // largest logit
-  int n;            // candidates in the list
+  int n;            // candidates in the list, the k largest of the segment among them, in no order
   double s;         // sum of exp((l - m) / T); NaN: the beam has no distribution
 };
 
@@ -46,7 +49,7 @@ struct BeamProblem {
   float over;                             // log2(e) / T
   double temperature;
   ScanStat* stat;                         // [B, W, lists]
-  unsigned long long* keys;               // [B, W, lists, k]
+  unsigned long long* keys;               // [B, W, lists, k + kSpare]
   float* out_scores;
   long long *parents, *tokens;
   uint8_t* out_finished;
@@ -96,29 +99,60 @@ template <int TY> struct Row {
   }
   __device__ __forceinline__ T least() const { return from_f32<TY>(-INFINITY); }
   __device__ __forceinline__ T at(int v) const { return v >= 0 && v < V && (!ok || ok[v]) ? x[v] : least(); }
+  // minus infinity in the place of what is not allowed of [v, v + N)
+  __device__ __forceinline__ void mask(Vec& r, int v) const {
+    const uint8_t* const m = ok + v;
+    uint32_t keep[N / 4];                         // a byte of ones for each allowed token
+    if (reinterpret_cast<uintptr_t>(m) % N == 0) {
+#pragma unroll
+      for (int i = 0; i < N / 4; ++i) keep[i] = __vcmpne4(reinterpret_cast<const uint32_t*>(m)[i], 0u);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N / 4; ++i) keep[i] = __vcmpne4(m[4 * i] | m[4 * i + 1] << 8 | m[4 * i + 2] << 16 | static_cast<uint32_t>(m[4 * i + 3]) << 24, 0u);
+    }
+    constexpr uint32_t kNone = TY == LETHE_F32 ? 0xff800000u : TY == LETHE_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t k = N == 4 ? __byte_perm(keep[0], 0, i * 0x1111) : __byte_perm(keep[i / 2], 0, i % 2 ? 0x3322 : 0x1100);
+      r.w[i] = (r.w[i] & k) | (kNone & ~k);
+    }
+  }
   // logits [v, v + N), minus infinity in the place of what is not there or not allowed; v + past is a multiple of N
   template <bool MASK> __device__ __forceinline__ Vec load(int v) const {
     Vec r;
     if (v >= 0 && v <= V - N) {
       r.load(x + v);
-      if (MASK) {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-          if (!ok[v + i]) raw_put<TY, N>(r, i, least());
-      }
+      if (MASK) mask(r, v);
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i) raw_put<TY, N>(r, i, at(v + i));
     }
     return r;
   }
+  // the largest of a lane's part of a tile; NaN is none
+  static __device__ __forceinline__ float largest(const Vec (&x)[kVecs]) {
+    if constexpr (TY == LETHE_F32) {
+      float m = x[0].get(0);
+#pragma unroll
+      for (int i = 1; i < 32; ++i) m = fmaxf(m, x[i / N].get(i % N));
+      return fmaxf(m, -INFINITY);
+    } else {
+      using T2 = typename std::conditional<TY == LETHE_BF16, __nv_bfloat162, __half2>::type;
+      auto two = [&](int i) { return *reinterpret_cast<const T2*>(&x[i / 4].w[i % 4]); };
+      T2 m = two(0);
+#pragma unroll
+      for (int i = 1; i < 16; ++i) m = __hmax2(m, two(i));
+      return fmaxf(fmaxf(to_f32(m.x), to_f32(m.y)), -INFINITY);
+    }
+  }
 };
 
 // Segment of a row: the lanes' tiles lie 16 bytes a lane beside one another, so element e of vector n of a lane is token
 // first + tile kTileLogits + n 32 N + lane N + e.
 template <int TY, bool MASK>
-__global__ void __launch_bounds__(32 * kScanWarps) beam_scan_kernel(const BeamProblem p) {
+__global__ void __launch_bounds__(32 * kScanWarps, TY == LETHE_F32 ? 8 : MASK ? 10 : 12) beam_scan_kernel(const BeamProblem p) {
   using R = Row<TY>;
+  constexpr int N = R::N, E = N / 4;                              // E: logits of 4 bytes
   __shared__ float2 bins[kScanWarps][kMostTiles][32];             // maximum and sum of a lane's part of a tile
   __shared__ unsigned long long cands[kScanWarps][kCands];
   __shared__ uint16_t passed[kScanWarps][kMostTiles * 32];
@@ -136,17 +170,13 @@ __global__ void __launch_bounds__(32 * kScanWarps) beam_scan_kernel(const BeamPr
   for (int j = 0; j < p.tiles; ++j) {
     typename R::Vec x[R::kVecs];
 #pragma unroll
-    for (int n = 0; n < R::kVecs; ++n) x[n] = r.template load<MASK>(first + j * kTileLogits + (n * 32 + lane) * R::N);
-    float m = -INFINITY;
-#pragma unroll
-    for (int n = 0; n < R::kVecs; ++n)
-#pragma unroll
-      for (int i = 0; i < R::N; ++i) m = fmaxf(m, x[n].get(i));
+    for (int n = 0; n < R::kVecs; ++n) x[n] = r.template load<MASK>(first + j * kTileLogits + (n * 32 + lane) * N);
+    const float m = R::largest(x);
     const F2 less = f2(m == -INFINITY ? 0.f : -m), over = f2(p.over);
     F2 sum[4];
 #pragma unroll
     for (int n = 0; n < 16; ++n) {
-      const F2 t = (x[n / (R::N / 2)].get2(n % (R::N / 2)) + less) * over;
+      const F2 t = (x[n / (N / 2)].get2(n % (N / 2)) + less) * over;
       const F2 e = f2(ex2(lo(t)), ex2(hi(t)));
       sum[n % 4] = n < 4 ? e : sum[n % 4] + e;
     }
@@ -154,91 +184,108 @@ __global__ void __launch_bounds__(32 * kScanWarps) beam_scan_kernel(const BeamPr
     bins[warp][j][lane] = make_float2(m, lo(s) + hi(s));
     top = fmaxf(top, m);
   }
+  const float mine = top;
 #pragma unroll
   for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
   double s = 0.;
-  uint32_t best = 0, taken = 0;
-  int best_at = 0;
-  for (int j = 0; j < p.tiles; ++j) {
-    const float2 bin = bins[warp][j][lane];
-    s += static_cast<double>(bin.y * (bin.x == -INFINITY ? 0.f : ex2((bin.x - top) * p.over)));
-    const uint32_t u = ordered(bin.x);
-    if (u > best) best = u, best_at = j;
+  uint32_t key[kMostTiles];
+#pragma unroll
+  for (int j = 0; j < kMostTiles; ++j) {
+    key[j] = 0;
+    if (j < p.tiles) {
+      const float2 bin = bins[warp][j][lane];
+      s += static_cast<double>(bin.y * (bin.x == -INFINITY ? 0.f : ex2((bin.x - top) * p.over)));
+      key[j] = ordered(bin.x);
+    }
   }
 #pragma unroll
   for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
 
-  // The k-th largest of the bins' maxima: what is below it is not among the k largest logits, and only bins that reach it have any of those.
-  uint32_t least = 0;
-  for (int i = 0; i < p.k; ++i) {
-    least = __reduce_max_sync(~0u, best);
-    if (least <= kLeast) break;
-    if (lane == __ffs(__ballot_sync(~0u, best == least)) - 1) {
-      taken |= 1u << best_at;
-      best = 0;
-      for (int j = 0; j < p.tiles; ++j) {
-        const uint32_t u = (taken >> j) & 1u ? 0u : ordered(bins[warp][j][lane].x);
-        if (u > best) best = u, best_at = j;
+  // A logit that k bins or a few more have something as large as, by halving: what is below it is not among the k largest, and only
+  // those bins have any of them.
+  auto reach = [&](uint32_t least) {
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < kMostTiles; ++j) n += key[j] >= least;
+    return __reduce_add_sync(~0u, n);
+  };
+  constexpr int kMore = 4;
+  uint32_t least = kLeast + 1, over = ordered(top) + 1;
+  if (p.k <= 32) least = max(least, __reduce_min_sync(~0u, ordered(mine)));
+  if (reach(least) > p.k + kMore)
+    while (over - least > 1) {
+      const uint32_t mid = least + (over - least) / 2;
+      const int n = reach(mid);
+      if (n >= p.k) {
+        least = mid;
+        if (n <= p.k + kMore) break;
+      } else {
+        over = mid;
       }
     }
-  }
-  least = max(least, kLeast + 1);
   int reached = 0;
-  for (int j = 0; j < p.tiles; ++j) {
-    const bool mine = ordered(bins[warp][j][lane].x) >= least;
-    const uint32_t who = __ballot_sync(~0u, mine);
-    if (mine) passed[warp][reached + __popc(who & ((1u << lane) - 1))] = static_cast<uint16_t>(j * 32 + lane);
+#pragma unroll
+  for (int j = 0; j < kMostTiles; ++j) {
+    const uint32_t who = __ballot_sync(~0u, key[j] >= least);
+    if (key[j] >= least) passed[warp][reached + __popc(who & ((1u << lane) - 1))] = static_cast<uint16_t>(j * 32 + lane);
     reached += __popc(who);
   }
   __syncwarp();
-  // their logits, one of a bin for each lane
+  // their logits, four bytes for each lane: E bins at a time
   unsigned long long* const cand = cands[warp];
+  const float floor = from_ordered(least);
   int n = 0;
-  constexpr int kAhead = 8;
-  for (int i = 0; i < reached; i += kAhead) {
-    uint32_t u[kAhead];
+  constexpr int kAhead = 4;
+  for (int i = 0; i < reached && n <= kCands; i += kAhead * E) {
+    float x[kAhead][E];
     int v[kAhead];
 #pragma unroll
     for (int h = 0; h < kAhead; ++h) {
-      const int bin = i + h < reached ? passed[warp][i + h] : 0;
-      v[h] = first + bin / 32 * kTileLogits + (lane / R::N * 32 + bin % 32) * R::N + lane % R::N;
-      u[h] = i + h < reached ? ordered(to_f32(r.at(v[h]))) : 0u;
+      const int c = i + h * E + lane / (32 / E), word = lane % (32 / E);
+      const int bin = passed[warp][min(c, reached - 1)];
+      v[h] = first + bin / 32 * kTileLogits + (word / 4 * 32 + bin % 32) * N + word % 4 * E;
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[h][e] = c < reached ? to_f32(r.at(v[h] + e)) : -INFINITY;
     }
 #pragma unroll
-    for (int h = 0; h < kAhead; ++h) {
-      const uint32_t who = __ballot_sync(~0u, u[h] >= least);
-      const int at = n + __popc(who & ((1u << lane) - 1));
-      if (u[h] >= least && at < kCands) cand[at] = static_cast<unsigned long long>(u[h]) << 32 | static_cast<uint32_t>(~v[h]);
-      n += __popc(who);
-    }
-    if (n > kCands) break;
+    for (int h = 0; h < kAhead; ++h)
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const bool in = x[h][e] >= floor;
+        const uint32_t who = __ballot_sync(~0u, in);
+        const int at = n + __popc(who & ((1u << lane) - 1));
+        if (in && at < kCands) cand[at] = static_cast<unsigned long long>(ordered(x[h][e])) << 32 | static_cast<uint32_t>(~(v[h] + e));
+        n += __popc(who);
+      }
   }
   __syncwarp();
-  unsigned long long* const list = p.keys + task * p.k;
-  if (n <= kCands) {
+  unsigned long long* const list = p.keys + task * (p.k + kSpare);
+  if (n <= p.k + kSpare) {
+    for (int i = lane; i < n; i += 32) list[i] = cand[i];
+  } else if (n <= kCands) {
     for (int i = lane; i < n; i += 32) {
-      const unsigned long long key = cand[i];
+      const unsigned long long c = cand[i];
       int before = 0;
-      for (int j = 0; j < n; ++j) before += cand[j] > key;
-      if (before < p.k) list[before] = key;
+      for (int j = 0; j < n; ++j) before += cand[j] > c;
+      if (before < p.k) list[before] = c;
     }
-    n = min(n, p.k);
+    n = p.k;
   } else {
     // Too many equal ones, or large ones side by side: the largest of the segment, then the largest behind it, k times.
     unsigned long long last = ~0ull;
     for (n = 0; n < p.k; ++n) {
-      unsigned long long key = 0;
+      unsigned long long best = 0;
       for (int j = 0; j < p.tiles * kTileLogits / 32; ++j) {
         const int v = first + j * 32 + lane;
         const uint32_t u = ordered(to_f32(r.at(v)));
         const unsigned long long c = static_cast<unsigned long long>(u) << 32 | static_cast<uint32_t>(~v);
-        if (u > kLeast && c < last && c > key) key = c;
+        if (u > kLeast && c < last && c > best) best = c;
       }
 #pragma unroll
-      for (int d = 16; d; d >>= 1) key = max(key, __shfl_xor_sync(~0u, key, d));
-      if (!key) break;
-      if (lane == 0) list[n] = key;
-      last = key;
+      for (int d = 16; d; d >>= 1) best = max(best, __shfl_xor_sync(~0u, best, d));
+      if (!best) break;
+      if (lane == 0) list[n] = best;
+      last = best;
     }
   }
   if (lane == 0) p.stat[task] = ScanStat{top, n, s};
@@ -252,123 +299,163 @@ __device__ __forceinline__ bool larger(const Entry& a, const Entry& b) { return 
 
 struct MergeMemory {
   Entry room[kMergeRoom], sorted[kBins];
-  double lse[kBeamMost], part[kMergeThreads / 32], widest;      // (largest 1 / penalty)
+  double score[kBeamMost], inverse[kBeamMost], lse[kBeamMost], part[kMergeThreads / 32];      // inverse: 1 / penalty
   float top[kBeamMost];
-  bool on[kBeamMost], again[kBeamMost];
-  int n, any;
+  uint32_t bins[kBins], least;
+  int todo[kMergeThreads];
+  bool on[kBeamMost], ended[kBeamMost], again[kBeamMost];
+  int n, lists, any;
 };
 
 // The largest of room[0, n), at most `most`, in order; `least` becomes the last of them where there are so many.
 __device__ __forceinline__ void keep_largest(MergeMemory& m, int most, Entry* least) {
   __syncthreads();
-  const int n = m.n;
-  for (int i = threadIdx.x; i < n; i += kMergeThreads) {
-    const Entry e = m.room[i];
+  const int n = m.n, tid = threadIdx.x;
+  if (n <= kMergeThreads / 8) {
+    const int i = tid / 8;
+    const Entry e = m.room[min(i, n - 1 < 0 ? 0 : n - 1)];
     int before = 0;
-    for (int j = 0; j < n; ++j) before += larger(m.room[j], e);
-    if (before < most) m.sorted[before] = e;
+    for (int j = tid % 8; j < n; j += 8) before += larger(m.room[j], e);
+#pragma unroll
+    for (int d = 4; d; d >>= 1) before += __shfl_xor_sync(~0u, before, d);
+    if (i < n && before < most && tid % 8 == 0) m.sorted[before] = e;
+  } else {
+    for (int i = tid; i < n; i += kMergeThreads) {
+      const Entry e = m.room[i];
+      int before = 0;
+      for (int j = 0; j < n; ++j) before += larger(m.room[j], e);
+      if (before < most) m.sorted[before] = e;
+    }
   }
   __syncthreads();
   const int left = min(n, most);
-  for (int i = threadIdx.x; i < left; i += kMergeThreads) m.room[i] = m.sorted[i];
-  if (threadIdx.x == 0) m.n = left;
+  for (int i = tid; i < left; i += kMergeThreads) m.room[i] = m.sorted[i];
+  if (tid == 0) m.n = left;
   if (left == most) *least = m.sorted[most - 1];
   __syncthreads();
+}
+
+// exp(t) for t <= 0 in 64 bits: 2^n e^f with n the nearest whole number to t / ln 2, and e^f by its power series to the twelfth power (the
+// next term is below 2^-52); what is below e^-700 is zero.
+__device__ __forceinline__ double exp_below(double t) {
+  t = fmax(t, -700.);
+  const double n = rint(t * 1.4426950408889634), f = fma(n, -2.3190468138462996e-17, fma(n, -0.69314718055994529, t));
+  double e = 1. / 479001600.;
+  const double over[] = {1. / 39916800., 1. / 3628800., 1. / 362880., 1. / 40320., 1. / 5040., 1. / 720., 1. / 120., 1. / 24., 1. / 6., .5, 1., 1.};
+#pragma unroll
+  for (int i = 0; i < 12; ++i) e = fma(e, f, over[i]);
+  return t <= -700. ? 0. : __longlong_as_double(__double_as_longlong(e) + (static_cast<long long>(n) << 52));
 }
 
 template <int TY>
 __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamProblem p) {
   __shared__ MergeMemory m;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, row0 = blockIdx.x * p.W;
-  const int lists = p.W * p.lists, most = p.k + kBehind;
+  const int lists = p.W * p.lists, most = p.k + kBehind, line = p.k + kSpare;
+  const double over = 1. / p.temperature;
   const ScanStat* const stat = p.stat + static_cast<long long>(row0) * p.lists;
-  const unsigned long long* const keys = p.keys + static_cast<long long>(row0) * p.lists * p.k;
+  const unsigned long long* const keys = p.keys + static_cast<long long>(row0) * p.lists * line;
+  if (tid < p.W) {
+    const bool in = counts(p, row0 + tid), ended = p.finished && p.finished[row0 + tid];
+    m.score[tid] = p.scores[row0 + tid];
+    m.inverse[tid] = in ? (p.penalty ? 1. / p.penalty[row0 + tid] : 1.) : 0.;
+    m.on[tid] = in && !ended;
+    m.ended[tid] = in && ended;
+    m.again[tid] = false;
+  }
+  __syncthreads();
   griddep_wait();
   for (int w = warp; w < p.W; w += kMergeThreads / 32) {
-    bool on = goes_on(p, row0 + w);
+    if (!m.on[w]) continue;
+    const ScanStat* const a = stat + w * p.lists;
     float top = -INFINITY;
+    for (int i = lane; i < p.lists; i += 32) top = fmaxf(top, a[i].m);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
     double s = 0.;
-    if (on) {
-      const ScanStat* const a = stat + w * p.lists;
-      for (int i = lane; i < p.lists; i += 32) top = fmaxf(top, a[i].m);
-#pragma unroll
-      for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-      for (int i = lane; i < p.lists; i += 32) {
-        const ScanStat t = a[i];
-        s += t.m == -INFINITY ? t.s : t.s * exp((static_cast<double>(t.m) - top) / p.temperature);
-      }
-#pragma unroll
-      for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
-      on = s > 0. && s < INFINITY && top < INFINITY;
+    for (int i = lane; i < p.lists; i += 32) {
+      const ScanStat t = a[i];
+      s += t.m == -INFINITY ? t.s : t.s * exp_below((static_cast<double>(t.m) - top) * over);
     }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
     if (lane == 0) {
-      m.on[w] = on;
+      m.on[w] = s > 0. && s < INFINITY && top < INFINITY;
       m.top[w] = top;
-      m.lse[w] = on ? top / p.temperature + log(s) : 0.;
-      m.again[w] = false;
+      m.lse[w] = top * over + log(s);
     }
   }
-  auto penalty = [&](int w) { return p.penalty ? static_cast<double>(p.penalty[row0 + w]) : 1.; };
+  auto rank = [&](int w, float x) { return (m.score[w] + (x * over - m.lse[w])) * m.inverse[w]; };
   auto entry = [&](int l, unsigned long long key) {
     const int w = l / p.lists;
-    const double x = static_cast<double>(from_ordered(static_cast<uint32_t>(key >> 32))) / p.temperature;
-    const double c = static_cast<double>(p.scores[row0 + w]) + (x - m.lse[w]);
-    return Entry{ordered(c / penalty(w)), ~(static_cast<unsigned long long>(w) * p.V + static_cast<uint32_t>(~static_cast<uint32_t>(key)))};
+    return Entry{ordered(rank(w, from_ordered(static_cast<uint32_t>(key >> 32)))),
+                 ~(static_cast<unsigned long long>(w) * p.V + (~static_cast<uint32_t>(key)))};
   };
+  auto narrow = [](double x) { return ordered(static_cast<float>(x)); };      // in the same order, equal ones more
   for (int pass = 0;; ++pass) {
     __syncthreads();
-    if (tid == 0) {
-      m.n = m.any = 0;
-      m.widest = 0.;
-      for (int w = 0; w < p.W; ++w)
-        if (counts(p, row0 + w)) m.widest = fmax(m.widest, 1. / penalty(w));
-    }
+    if (tid == 0) m.n = m.lists = m.least = 0;
+    if (tid < kBins) m.bins[tid] = 0;
     __syncthreads();
-    if (tid < p.W && p.finished && p.finished[row0 + tid] && counts(p, row0 + tid))
-      m.room[atomicAdd(&m.n, 1)] = Entry{ordered(p.scores[row0 + tid] / penalty(tid)), ~(static_cast<unsigned long long>(tid) * p.V + p.eos)};
-    // The `most`-th largest of the bins' first candidates, of which none of those behind it is among the `most` largest.
-    Entry least{0, 0}, head{0, 0};
+    if (tid < p.W && m.ended[tid])
+      m.room[atomicAdd(&m.n, 1)] = Entry{ordered(m.score[tid] * m.inverse[tid]), ~(static_cast<unsigned long long>(tid) * p.V + p.eos)};
+    // `least`: as many bins as candidates are wanted have a list whose largest logit reaches it.  What is below is not wanted.
+    uint32_t head = 0;
     for (int l = tid; l < lists; l += kMergeThreads)
-      if (m.on[l / p.lists] && stat[l].n > 0) {
-        const Entry e = entry(l, keys[static_cast<long long>(l) * p.k]);
-        if (larger(e, head)) head = e;
-      }
-#pragma unroll
-    for (int d = kMergeThreads / kBins / 2; d; d >>= 1) {
-      const Entry e{__shfl_xor_sync(~0u, head.rank, d), __shfl_xor_sync(~0u, head.place, d)};
-      if (larger(e, head)) head = e;
-    }
-    if (tid % (kMergeThreads / kBins) == 0) m.sorted[tid / (kMergeThreads / kBins)] = head;
+      if (m.on[l / p.lists] && stat[l].n > 0) head = max(head, narrow(rank(l / p.lists, stat[l].m)));
+    if (head) atomicMax(&m.bins[tid % kBins], head);
     __syncthreads();
-    if (tid < kBins) {
-      const Entry e = m.sorted[tid];
+    {
+      constexpr int kShare = kMergeThreads / kBins;
+      const int i = tid / kShare;
+      const uint32_t b = m.bins[i];
       int before = 0;
-      for (int j = 0; j < kBins; ++j) before += larger(m.sorted[j], e);
-      if (before == most - 1 && e.rank) m.room[kMergeRoom - 1] = e, m.any = 1;
+#pragma unroll 8
+      for (int j = tid % kShare; j < kBins; j += kShare) before += m.bins[j] > b || (m.bins[j] == b && j < i);
+#pragma unroll
+      for (int d = kShare / 2; d; d >>= 1) before += __shfl_xor_sync(~0u, before, d);
+      if (before == most - 1 && tid % kShare == 0) m.least = b;
     }
     __syncthreads();
-    if (m.any) least = m.room[kMergeRoom - 1];
+    const uint32_t floor = max(m.least, 1u);
+    for (int l = tid; l < lists; l += kMergeThreads)
+      if (m.on[l / p.lists] && stat[l].n > 0 && narrow(rank(l / p.lists, stat[l].m)) >= floor) {
+        const int at = atomicAdd(&m.lists, 1);
+        if (at < kMergeThreads) m.todo[at] = l;
+      }
     __syncthreads();
-    // every thread's lists, each to its first candidate below `least`
-    int l = tid, at = 0;
-    for (;;) {
-      Entry e{0, 0};
-      bool have = false;
-      while (l < lists && !have) {
-        if (m.on[l / p.lists] && at < stat[l].n) {
-          e = entry(l, keys[static_cast<long long>(l) * p.k + at]);
-          have = !larger(least, e);
+    // their candidates that reach it
+    for (int i = warp; i < min(m.lists, kMergeThreads); i += kMergeThreads / 32) {
+      const int l = m.todo[i], n = stat[l].n;
+      for (int c = lane; c < n; c += 32) {
+        const Entry e = entry(l, keys[static_cast<long long>(l) * line + c]);
+        if (narrow(from_ordered(e.rank)) >= floor) {
+          const int at = atomicAdd(&m.n, 1);
+          if (at < kMergeRoom) m.room[at] = e;
         }
-        if (!have) l += kMergeThreads, at = 0;
       }
-      if (have) {
-        m.room[atomicAdd(&m.n, 1)] = e;
-        ++at;
-      }
-      if (!__syncthreads_or(have)) break;
-      const int n = m.n;
+    }
+    __syncthreads();
+    Entry least{0, 0};
+    if (m.lists > kMergeThreads || m.n > kMergeRoom) {
+      // So many equal ones: all candidates in turn, as many at a time as there is room for.
       __syncthreads();
-      if (n > kMergeRoom - kMergeThreads) keep_largest(m, most, &least);
+      if (tid == 0) m.n = 0;
+      __syncthreads();
+      if (tid < p.W && m.ended[tid])
+        m.room[atomicAdd(&m.n, 1)] = Entry{ordered(m.score[tid] * m.inverse[tid]), ~(static_cast<unsigned long long>(tid) * p.V + p.eos)};
+      const long long all = static_cast<long long>(lists) * line;
+      for (long long i = 0; i < all; i += kMergeThreads) {
+        const int l = static_cast<int>((i + tid) / line), c = static_cast<int>((i + tid) % line);
+        if (l < lists && m.on[l / p.lists] && c < stat[l].n) {
+          const Entry e = entry(l, keys[static_cast<long long>(l) * line + c]);
+          if (!larger(least, e)) m.room[atomicAdd(&m.n, 1)] = e;
+        }
+        __syncthreads();
+        const int n = m.n;
+        __syncthreads();
+        if (n > kMergeRoom - kMergeThreads) keep_largest(m, most, &least);
+      }
     }
     keep_largest(m, most, &least);
     if (pass) break;
@@ -377,17 +464,23 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamPro
     __syncthreads();
     const int n = m.n;
     auto beam = [&](const Entry& e) { return static_cast<int>(~e.place / p.V); };
-    auto doubt = [&](const Entry& a, const Entry& b) {
-      const int u = beam(a), w = beam(b);
-      const double gap = from_ordered(a.rank) - from_ordered(b.rank);
-      return gap > 0. && u != w && gap < kLseError * (1. / penalty(u) + 1. / penalty(w));
-    };
     if (tid < n && tid < p.k) {
       const Entry a = m.sorted[tid];
-      const double far = 2. * kLseError * m.widest;
+      const int u = beam(a);
+      double far = 0.;
+      if (p.penalty) {
+        for (int w = 0; w < p.W; ++w) far = fmax(far, m.inverse[w]);
+      } else {
+        far = 1.;
+      }
+      far *= 2. * kLseError;
       int j = tid + 1;
-      for (; j < n && from_ordered(a.rank) - from_ordered(m.sorted[j].rank) < far; ++j)
-        if (doubt(a, m.sorted[j])) m.again[beam(a)] = m.again[beam(m.sorted[j])] = m.any = 1;
+      for (; j < n; ++j) {
+        const double gap = from_ordered(a.rank) - from_ordered(m.sorted[j].rank);
+        if (!(gap < far)) break;
+        const int w = beam(m.sorted[j]);
+        if (gap > 0. && u != w && gap < kLseError * (m.inverse[u] + m.inverse[w])) m.again[u] = m.again[w] = m.any = 1;
+      }
       // as many equals behind the last of this beam's: another beam's may lie behind them
       if (j == most && p.W > 1) {
         for (int w = 0; w < p.W; ++w) m.again[w] = true;
@@ -400,8 +493,8 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamPro
       if (!m.again[w] || !m.on[w]) continue;
       const Row<TY> r(p, row0 + w);
       double s = 0.;
-      for (int v = tid; v < p.V; v += kMergeThreads)
-        s += exp((static_cast<double>(to_f32(r.at(v))) - m.top[w]) / p.temperature);
+#pragma unroll 4
+      for (int v = tid; v < p.V; v += kMergeThreads) s += exp_below((static_cast<double>(to_f32(r.at(v))) - m.top[w]) * over);
 #pragma unroll
       for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
       if (lane == 0) m.part[warp] = s;
@@ -409,7 +502,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamPro
       if (tid == 0) {
         s = 0.;
         for (int i = 0; i < kMergeThreads / 32; ++i) s += m.part[i];
-        m.lse[w] = m.top[w] / p.temperature + log(s);
+        m.lse[w] = m.top[w] * over + log(s);
       }
       __syncthreads();
     }
@@ -419,10 +512,10 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamPro
     const bool there = tid < m.n;
     const unsigned long long place = there ? ~m.sorted[tid].place : 0;
     const int w = static_cast<int>(place / p.V), v = there ? static_cast<int>(place % p.V) : max(p.eos, 0);
-    p.out_scores[o] = there ? static_cast<float>(from_ordered(m.sorted[tid].rank) * penalty(w)) : -INFINITY;
+    p.out_scores[o] = there ? static_cast<float>(from_ordered(m.sorted[tid].rank) * (p.penalty ? p.penalty[row0 + w] : 1.f)) : -INFINITY;
     p.parents[o] = w;
     p.tokens[o] = v;
-    if (p.out_finished) p.out_finished[o] = !there || v == p.eos || (p.finished && p.finished[row0 + w]);
+    if (p.out_finished) p.out_finished[o] = !there || v == p.eos || m.ended[w];
   }
 }
 
@@ -430,14 +523,17 @@ struct ScanPlan {
   int tiles;
   long long lists, tasks;
 };
-// Segments short enough for kFillWarps of them, where there are so many; more bins than candidates in each.
-static ScanPlan scan_plan(long long B, int W, long long V, int k, int ty) {
-  const long long n = 16 / elem_bytes(ty), row = (V + n - 1 + kTileLogits - 1) / kTileLogits;
+// Segments short enough for kFillWarps of them, where there are so many; more bins than candidates in each.  A row that does not begin on a
+// 16-byte boundary may reach into one more tile.
+static ScanPlan scan_plan(long long B, int W, long long V, int k, int ty, bool aligned) {
+  const long long past = aligned ? 0 : 16 / elem_bytes(ty) - 1, row = (V + past + kTileLogits - 1) / kTileLogits;
+  const long long want = B * W * ((V + kTileLogits - 1) / kTileLogits) / kFillWarps;
   ScanPlan s;
-  const long long want = B * W * row / kFillWarps;
   s.tiles = static_cast<int>(want < kMostTiles ? want : kMostTiles);
   if (s.tiles * 32 < k) s.tiles = (k + 31) / 32;
   s.lists = (row + s.tiles - 1) / s.tiles;
+  s.tiles = static_cast<int>((row + s.lists - 1) / s.lists);
+  if (s.tiles * 32 < k) s.tiles = (k + 31) / 32;
   s.tasks = B * W * s.lists;
   return s;
 }
@@ -460,7 +556,7 @@ static int launch_beam(const BeamProblem& p, long long tasks, cudaStream_t st) {
 extern "C" size_t lethe_gdn_beam_work_bytes(int64_t B, int32_t W, int64_t V, int32_t k, int32_t x_type) {
   using namespace lg;
   if (!beam_sizes(B, W, V, k, x_type)) return 0;
-  return static_cast<size_t>(scan_plan(B, W, V, k, x_type).tasks) * (sizeof(ScanStat) + 8 * static_cast<size_t>(k));
+  return static_cast<size_t>(scan_plan(B, W, V, k, x_type, false).tasks) * (sizeof(ScanStat) + 8 * static_cast<size_t>(k + kSpare));
 }
 
 extern "C" int lethe_gdn_beam_select(const LetheGdnBeamArgs* a, void* stream) {
@@ -473,7 +569,9 @@ extern "C" int lethe_gdn_beam_select(const LetheGdnBeamArgs* a, void* stream) {
   if ((reinterpret_cast<uintptr_t>(a->parents) | reinterpret_cast<uintptr_t>(a->tokens)) % 8) return kErrAlign;
   if (!a->work) return kErrNull;
   if (reinterpret_cast<uintptr_t>(a->work) % 16) return kErrAlign;
-  const ScanPlan plan = scan_plan(a->B, a->W, a->V, a->k, a->x_type);
+  const int e = elem_bytes(a->x_type);
+  const bool aligned = (reinterpret_cast<uintptr_t>(a->logits) | static_cast<uintptr_t>(a->logits_batch * e) | static_cast<uintptr_t>(a->logits_beam * e)) % 16 == 0;
+  const ScanPlan plan = scan_plan(a->B, a->W, a->V, a->k, a->x_type, aligned);
   if (a->work_bytes < lethe_gdn_beam_work_bytes(a->B, a->W, a->V, a->k, a->x_type)) return kErrWorkspace;
   DeviceGuard guard(a->logits);
   if (!guard.ok) return kErrDevice;
