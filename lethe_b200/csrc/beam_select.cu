@@ -21,15 +21,16 @@
 namespace lg {
 
 constexpr int kBeamMost = 64;                     // beams of a group, and candidates asked for
-constexpr int kTileLogits = 1024, kMostTiles = 8; // a warp takes that many logits at a time, and so many times
-constexpr int kScanWarps = 4, kFillWarps = 148 * 24;
+constexpr int kTileLogits = 1024, kMostTiles = 16; // a warp takes that many logits at a time, and so many times
+constexpr int kScanWarps = 4;
 constexpr int kCands = 128;                       // candidates of a segment that are looked at together
 constexpr int kSpare = 16;                        // more than asked for that a list may have
 constexpr int kMergeThreads = 512, kBins = 128, kMergeRoom = 2 * kMergeThreads;
 constexpr int kBehind = 8;                        // candidates behind the last chosen one that are looked at for equals
-// A term of a sum: exp2 by the hardware 2^-22, its argument (two roundings of |t| 2^-24, weighted by 2^t) 2^-23.5, twice (tile to
-// segment) the former, seven roundings of sums in 32 bits; the rest is in 64 bits.
-constexpr double kLseError = 2 * 2.4e-7 + 1e-7 + 7 * 6e-8;
+// A term of a sum: exp2 by the hardware 2^-22; its argument t has two roundings of |t| 2^-24, which count with 2^t relative to the
+// largest term, |t| up to kSlack there, together below 2^-22; seven roundings of sums in 32 bits.  The rest is in 64 bits.
+constexpr double kLseError = 2 * 2.4e-7 + 7 * 6e-8;
+constexpr float kSlack = 2.f;                     // how far (as a power of two) terms may be above what they are relative to
 
 struct ScanStat {
   float m;          // largest logit
@@ -47,7 +48,7 @@ struct BeamProblem {
   int B, W, k, V, eos;
   int tiles, lists;                       // of a segment; of a row
   float over;                             // log2(e) / T
-  double temperature;
+  double inverse;                         // 1 / T
   ScanStat* stat;                         // [B, W, lists]
   unsigned long long* keys;               // [B, W, lists, k + kSpare]
   float* out_scores;
@@ -72,6 +73,18 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// exp(t) for t <= 0 in 64 bits: 2^n e^f with n the nearest whole number to t / ln 2, and e^f by its power series to the twelfth power (the
+// next term is below 2^-52); what is below e^-700 is zero.
+__device__ __forceinline__ double exp_below(double t) {
+  t = fmax(t, -700.);
+  const double n = rint(t * 1.4426950408889634), f = fma(n, -2.3190468138462996e-17, fma(n, -0.69314718055994529, t));
+  double e = 1. / 479001600.;
+  const double over[] = {1. / 39916800., 1. / 3628800., 1. / 362880., 1. / 40320., 1. / 5040., 1. / 720., 1. / 120., 1. / 24., 1. / 6., .5, 1., 1.};
+#pragma unroll
+  for (int i = 0; i < 12; ++i) e = fma(e, f, over[i]);
+  return t <= -700. ? 0. : __longlong_as_double(__double_as_longlong(e) + (static_cast<long long>(n) << 52));
 }
 
 // whether the beam goes on: one that does not offers nothing, or only itself
@@ -148,31 +161,49 @@ template <int TY> struct Row {
 };
 
 // Segment of a row: the lanes' tiles lie 16 bytes a lane beside one another, so element e of vector n of a lane is token
-// first + tile kTileLogits + n 32 N + lane N + e.
+// first + tile kTileLogits + n 32 N + lane N + e.  A lane's part of a tile is a bin.
+template <int TY> constexpr int scan_ctas(bool mask) { return TY == LETHE_F32 ? 8 : mask ? 10 : 12; }
 template <int TY, bool MASK>
-__global__ void __launch_bounds__(32 * kScanWarps, TY == LETHE_F32 ? 8 : MASK ? 10 : 12) beam_scan_kernel(const BeamProblem p) {
+__global__ void __launch_bounds__(32 * kScanWarps, scan_ctas<TY>(MASK)) beam_scan_kernel(const BeamProblem p) {
   using R = Row<TY>;
-  constexpr int N = R::N, E = N / 4;                              // E: logits of 4 bytes
-  __shared__ float2 bins[kScanWarps][kMostTiles][32];             // maximum and sum of a lane's part of a tile
+  constexpr int N = R::N;
+  __shared__ uint32_t tops[kScanWarps][kMostTiles][32];           // maxima of the bins
   __shared__ unsigned long long cands[kScanWarps][kCands];
-  __shared__ uint16_t passed[kScanWarps][kMostTiles * 32];
+  __shared__ uint16_t passed[kScanWarps][kCands];
   griddep_launch();      // (the merge waits for the lists)
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const long long task = static_cast<long long>(blockIdx.x) * kScanWarps + warp;
-  if (task >= static_cast<long long>(p.B) * p.W * p.lists) return;
-  const int row = static_cast<int>(task / p.lists), seg = static_cast<int>(task % p.lists);
+  const unsigned task = blockIdx.x * kScanWarps + warp, lists = p.lists, row = task / lists;
+  if (row >= static_cast<unsigned>(p.B) * p.W) return;
   if (!goes_on(p, row)) return;
   const R r(p, row);
-  const int first = seg * p.tiles * kTileLogits - r.past;
+  const int first = static_cast<int>(task - row * lists) * p.tiles * kTileLogits - r.past;
 
-  // sums and maxima
-  float top = -INFINITY;
+  // The sum of 2^t, t = (l - ref) over: ref is the warp's largest logit so far, or up to kSlack behind it.
+  float ref = -INFINITY, mine = -INFINITY;
+  double s = 0.;
   for (int j = 0; j < p.tiles; ++j) {
     typename R::Vec x[R::kVecs];
+    const int v0 = first + j * kTileLogits;
+    if (v0 >= 0 && v0 <= r.V - kTileLogits) {
 #pragma unroll
-    for (int n = 0; n < R::kVecs; ++n) x[n] = r.template load<MASK>(first + j * kTileLogits + (n * 32 + lane) * N);
+      for (int n = 0; n < R::kVecs; ++n) x[n].load(r.x + v0 + (n * 32 + lane) * N);
+      if (MASK) {
+#pragma unroll
+        for (int n = 0; n < R::kVecs; ++n) r.mask(x[n], v0 + (n * 32 + lane) * N);
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < R::kVecs; ++n) x[n] = r.template load<MASK>(v0 + (n * 32 + lane) * N);
+    }
     const float m = R::largest(x);
-    const F2 less = f2(m == -INFINITY ? 0.f : -m), over = f2(p.over);
+    tops[warp][j][lane] = ordered(m);
+    mine = fmaxf(mine, m);
+    if (__any_sync(~0u, m > ref && !((m - ref) * p.over <= kSlack))) {
+      const float now = from_ordered(__reduce_max_sync(~0u, ordered(m)));
+      if (ref > -INFINITY) s *= exp_below((static_cast<double>(ref) - now) * p.inverse);
+      ref = now;
+    }
+    const F2 less = f2(ref == -INFINITY ? 0.f : -ref), over = f2(p.over);
     F2 sum[4];
 #pragma unroll
     for (int n = 0; n < 16; ++n) {
@@ -180,86 +211,87 @@ __global__ void __launch_bounds__(32 * kScanWarps, TY == LETHE_F32 ? 8 : MASK ? 
       const F2 e = f2(ex2(lo(t)), ex2(hi(t)));
       sum[n % 4] = n < 4 ? e : sum[n % 4] + e;
     }
-    const F2 s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    bins[warp][j][lane] = make_float2(m, lo(s) + hi(s));
-    top = fmaxf(top, m);
-  }
-  const float mine = top;
-#pragma unroll
-  for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-  double s = 0.;
-  uint32_t key[kMostTiles];
-#pragma unroll
-  for (int j = 0; j < kMostTiles; ++j) {
-    key[j] = 0;
-    if (j < p.tiles) {
-      const float2 bin = bins[warp][j][lane];
-      s += static_cast<double>(bin.y * (bin.x == -INFINITY ? 0.f : ex2((bin.x - top) * p.over)));
-      key[j] = ordered(bin.x);
-    }
+    const F2 t = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    s += static_cast<double>(lo(t) + hi(t));
   }
 #pragma unroll
   for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
+  const uint32_t own = ordered(mine), top = __reduce_max_sync(~0u, own);
 
   // A logit that k bins or a few more have something as large as, by halving: what is below it is not among the k largest, and only
-  // those bins have any of them.
-  auto reach = [&](uint32_t least) {
-    int n = 0;
-#pragma unroll
-    for (int j = 0; j < kMostTiles; ++j) n += key[j] >= least;
-    return __reduce_add_sync(~0u, n);
-  };
-  constexpr int kMore = 4;
-  uint32_t least = kLeast + 1, over = ordered(top) + 1;
-  if (p.k <= 32) least = max(least, __reduce_min_sync(~0u, ordered(mine)));
-  if (reach(least) > p.k + kMore)
-    while (over - least > 1) {
-      const uint32_t mid = least + (over - least) / 2;
+  // those bins have any of them.  Few candidates: by the lanes' maxima alone, which lets some more pass.
+  constexpr int kMore = 4, kFew = 16;
+  uint32_t least = kLeast + 1, above = top + 1;
+  auto halve = [&](auto reach) {
+    if (reach(least) <= p.k + kMore) return;
+    while (above - least > 1) {
+      const uint32_t mid = least + (above - least) / 2;
       const int n = reach(mid);
-      if (n >= p.k) {
+      if (n < p.k) {
+        above = mid;
+      } else {
         least = mid;
         if (n <= p.k + kMore) break;
-      } else {
-        over = mid;
       }
     }
-  int reached = 0;
-#pragma unroll
-  for (int j = 0; j < kMostTiles; ++j) {
-    const uint32_t who = __ballot_sync(~0u, key[j] >= least);
-    if (key[j] >= least) passed[warp][reached + __popc(who & ((1u << lane) - 1))] = static_cast<uint16_t>(j * 32 + lane);
-    reached += __popc(who);
+  };
+  if (p.k <= kFew) {
+    halve([&](uint32_t u) { return __popc(__ballot_sync(~0u, own >= u)); });
+  } else {
+    halve([&](uint32_t u) {
+      int n = 0;
+      for (int j = 0; j < p.tiles; ++j) n += tops[warp][j][lane] >= u;
+      return static_cast<int>(__reduce_add_sync(~0u, n));
+    });
   }
+  // places in front of the lanes' own
+  auto offset = [&](int n, int* all) {
+    int a = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int b = __shfl_up_sync(~0u, a, d);
+      if (lane >= d) a += b;
+    }
+    *all = __shfl_sync(~0u, a, 31);
+    return a - n;
+  };
+  uint32_t hit = 0;
+  if (own >= least)
+    for (int j = 0; j < p.tiles; ++j) hit |= static_cast<uint32_t>(tops[warp][j][lane] >= least) << j;
+  int reached, n = 0;
+  int at = offset(__popc(hit), &reached);
+  for (; hit; hit &= hit - 1, ++at)
+    if (at < kCands) passed[warp][at] = static_cast<uint16_t>((__ffs(hit) - 1) * 32 + lane);
   __syncwarp();
-  // their logits, four bytes for each lane: E bins at a time
+  // their logits, a bin for each lane
   unsigned long long* const cand = cands[warp];
   const float floor = from_ordered(least);
-  int n = 0;
-  constexpr int kAhead = 4;
-  for (int i = 0; i < reached && n <= kCands; i += kAhead * E) {
-    float x[kAhead][E];
-    int v[kAhead];
+  if (reached > kCands) {
+    n = kCands + 1;
+  } else {
+    for (int i = 0; i < reached; i += 32) {
+      int v = 0;
+      if (i + lane < reached) {
+        const int bin = passed[warp][i + lane];
+        v = first + bin / 32 * kTileLogits + bin % 32 * N;
 #pragma unroll
-    for (int h = 0; h < kAhead; ++h) {
-      const int c = i + h * E + lane / (32 / E), word = lane % (32 / E);
-      const int bin = passed[warp][min(c, reached - 1)];
-      v[h] = first + bin / 32 * kTileLogits + (word / 4 * 32 + bin % 32) * N + word % 4 * E;
+        for (int b = 0; b < R::kVecs; ++b) {
+          const typename R::Vec x = r.template load<MASK>(v + b * 32 * N);
 #pragma unroll
-      for (int e = 0; e < E; ++e) x[h][e] = c < reached ? to_f32(r.at(v[h] + e)) : -INFINITY;
-    }
-#pragma unroll
-    for (int h = 0; h < kAhead; ++h)
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const bool in = x[h][e] >= floor;
-        const uint32_t who = __ballot_sync(~0u, in);
-        const int at = n + __popc(who & ((1u << lane) - 1));
-        if (in && at < kCands) cand[at] = static_cast<unsigned long long>(ordered(x[h][e])) << 32 | static_cast<uint32_t>(~(v[h] + e));
-        n += __popc(who);
+          for (int e = 0; e < N; ++e) hit |= static_cast<uint32_t>(x.get(e) >= floor) << (b * N + e);
+        }
       }
+      int all;
+      at = n + offset(__popc(hit), &all);
+      n += all;
+      for (; hit; hit &= hit - 1, ++at) {
+        const int b = __ffs(hit) - 1, u = v + b / N * 32 * N + b % N;
+        if (at < kCands) cand[at] = static_cast<unsigned long long>(ordered(to_f32(r.x[u]))) << 32 | static_cast<uint32_t>(~u);
+      }
+    }
   }
   __syncwarp();
-  unsigned long long* const list = p.keys + task * (p.k + kSpare);
+  unsigned long long* const list = p.keys + static_cast<long long>(task) * (p.k + kSpare);
   if (n <= p.k + kSpare) {
     for (int i = lane; i < n; i += 32) list[i] = cand[i];
   } else if (n <= kCands) {
@@ -288,7 +320,11 @@ __global__ void __launch_bounds__(32 * kScanWarps, TY == LETHE_F32 ? 8 : MASK ? 
       last = best;
     }
   }
-  if (lane == 0) p.stat[task] = ScanStat{top, n, s};
+  if (lane == 0) {
+    const float m = from_ordered(top);
+    if (ref > -INFINITY) s *= exp_below((static_cast<double>(ref) - m) * p.inverse);
+    p.stat[task] = ScanStat{m, n, s};
+  }
 }
 
 // A candidate: larger ones come first.
@@ -335,24 +371,12 @@ __device__ __forceinline__ void keep_largest(MergeMemory& m, int most, Entry* le
   __syncthreads();
 }
 
-// exp(t) for t <= 0 in 64 bits: 2^n e^f with n the nearest whole number to t / ln 2, and e^f by its power series to the twelfth power (the
-// next term is below 2^-52); what is below e^-700 is zero.
-__device__ __forceinline__ double exp_below(double t) {
-  t = fmax(t, -700.);
-  const double n = rint(t * 1.4426950408889634), f = fma(n, -2.3190468138462996e-17, fma(n, -0.69314718055994529, t));
-  double e = 1. / 479001600.;
-  const double over[] = {1. / 39916800., 1. / 3628800., 1. / 362880., 1. / 40320., 1. / 5040., 1. / 720., 1. / 120., 1. / 24., 1. / 6., .5, 1., 1.};
-#pragma unroll
-  for (int i = 0; i < 12; ++i) e = fma(e, f, over[i]);
-  return t <= -700. ? 0. : __longlong_as_double(__double_as_longlong(e) + (static_cast<long long>(n) << 52));
-}
-
 template <int TY>
 __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamProblem p) {
   __shared__ MergeMemory m;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, row0 = blockIdx.x * p.W;
   const int lists = p.W * p.lists, most = p.k + kBehind, line = p.k + kSpare;
-  const double over = 1. / p.temperature;
+  const double over = p.inverse;
   const ScanStat* const stat = p.stat + static_cast<long long>(row0) * p.lists;
   const unsigned long long* const keys = p.keys + static_cast<long long>(row0) * p.lists * line;
   if (tid < p.W) {
@@ -523,11 +547,12 @@ struct ScanPlan {
   int tiles;
   long long lists, tasks;
 };
-// Segments short enough for kFillWarps of them, where there are so many; more bins than candidates in each.  A row that does not begin on a
-// 16-byte boundary may reach into one more tile.
+// As many segments as the GPU's SMs hold warps of the kernel, or fewer, where tiles are enough; more bins than candidates in each.  A row that
+// does not begin on a 16-byte boundary may reach into one more tile.
 static ScanPlan scan_plan(long long B, int W, long long V, int k, int ty, bool aligned) {
   const long long past = aligned ? 0 : 16 / elem_bytes(ty) - 1, row = (V + past + kTileLogits - 1) / kTileLogits;
-  const long long want = B * W * ((V + kTileLogits - 1) / kTileLogits) / kFillWarps;
+  const long long held = 148 * kScanWarps * (ty == LETHE_F32 ? scan_ctas<LETHE_F32>(false) : scan_ctas<LETHE_BF16>(false));
+  const long long want = (B * W * ((V + kTileLogits - 1) / kTileLogits) + held - 1) / held;
   ScanPlan s;
   s.tiles = static_cast<int>(want < kMostTiles ? want : kMostTiles);
   if (s.tiles * 32 < k) s.tiles = (k + 31) / 32;
@@ -592,8 +617,8 @@ extern "C" int lethe_gdn_beam_select(const LetheGdnBeamArgs* a, void* stream) {
   p.eos = static_cast<int>(a->eos);
   p.tiles = plan.tiles;
   p.lists = static_cast<int>(plan.lists);
-  p.temperature = a->temperature;
-  p.over = static_cast<float>(1.4426950408889634 / p.temperature);
+  p.inverse = 1. / a->temperature;
+  p.over = static_cast<float>(1.4426950408889634 / a->temperature);
   p.stat = static_cast<ScanStat*>(a->work);
   p.keys = reinterpret_cast<unsigned long long*>(p.stat + plan.tasks);
   p.out_scores = a->out_scores;
