@@ -21,11 +21,14 @@
 namespace lg {
 
 constexpr int kBeamMost = 64;                     // beams of a group, and candidates asked for
-constexpr int kTileLogits = 1024, kMostTiles = 16; // a warp takes that many logits at a time, and so many times
-constexpr int kScanWarps = 4;
+constexpr int kTileLogits = 1024;                 // a warp takes that many at a time, a lane 32 of them
+constexpr int kScanWarps = 2, kScanCtas = 14;
+constexpr int kMostTiles = 8;                     // of a segment
 constexpr int kCands = 128;                       // candidates of a segment that are looked at together
 constexpr int kSpare = 16;                        // more than asked for that a list may have
+__host__ __device__ constexpr int list_room(int k) { return (k + kSpare + 1) / 2 * 2; }      // keys come in pairs
 constexpr int kMergeThreads = 512, kBins = 128, kMergeRoom = 2 * kMergeThreads;
+constexpr int kMergeKeys = 4096;                  // of a group's lists, that are fetched before it is known which are wanted
 constexpr int kBehind = 8;                        // candidates behind the last chosen one that are looked at for equals
 // A term of a sum: exp2 by the hardware 2^-22; its argument t has two roundings of |t| 2^-24, which count with 2^t relative to the
 // largest term, |t| up to kSlack there, together below 2^-22; seven roundings of sums in 32 bits.  The rest is in 64 bits.
@@ -50,7 +53,7 @@ struct BeamProblem {
   float over;                             // log2(e) / T
   double inverse;                         // 1 / T
   ScanStat* stat;                         // [B, W, lists]
-  unsigned long long* keys;               // [B, W, lists, k + kSpare]
+  unsigned long long* keys;               // [B, W, lists, list_room(k)]
   float* out_scores;
   long long *parents, *tokens;
   uint8_t* out_finished;
@@ -98,6 +101,7 @@ template <int TY> struct Row {
   using T = typename Elem<TY>::T;
   static constexpr int N = 16 / sizeof(T);        // logits of 16 bytes
   static constexpr int kVecs = 32 / N;            // of a lane and tile
+  static constexpr int kDepth = N == 4 ? 2 : 3;   // tiles on their way
   using Vec = Raw<TY, N>;
   const T* x;
   const uint8_t* ok;                              // NULL: every token is allowed
@@ -142,6 +146,30 @@ template <int TY> struct Row {
     }
     return r;
   }
+  // the same for vector n of a tile, by selections: n is not known to the compiler
+  template <bool MASK> __device__ __forceinline__ void edge(Vec (&x)[kVecs], int n, int v) const {
+    const Vec r = load<MASK>(v);
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i)
+      if (i == n) x[i] = r;
+  }
+  // which of a lane's part of a tile are not below `floor`, one of them at least is not; the place of a bit's element
+  static __device__ __forceinline__ uint32_t reaching(const Vec (&x)[kVecs], float floor) {
+    uint32_t hit = 0;
+    if constexpr (TY == LETHE_F32) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) hit |= static_cast<uint32_t>(x[i / N].get(i % N) >= floor) << i;
+    } else {
+      using T2 = typename std::conditional<TY == LETHE_BF16, __nv_bfloat162, __half2>::type;
+      T2 f;
+      if constexpr (TY == LETHE_BF16) f.x = f.y = __float2bfloat16_ru(floor);
+      else f.x = f.y = __float2half_ru(floor);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) hit |= __hge2_mask(*reinterpret_cast<const T2*>(&x[i / 4].w[i % 4]), f) & (0x10001u << i);
+    }
+    return hit;
+  }
+  static __device__ __forceinline__ int element(int bit) { return TY == LETHE_F32 ? bit : bit % 16 * 2 + bit / 16; }
   // the largest of a lane's part of a tile; NaN is none
   static __device__ __forceinline__ float largest(const Vec (&x)[kVecs]) {
     if constexpr (TY == LETHE_F32) {
@@ -162,41 +190,63 @@ template <int TY> struct Row {
 
 // Segment of a row: the lanes' tiles lie 16 bytes a lane beside one another, so element e of vector n of a lane is token
 // first + tile kTileLogits + n 32 N + lane N + e.  A lane's part of a tile is a bin.
-template <int TY> constexpr int scan_ctas(bool mask) { return TY == LETHE_F32 ? 8 : mask ? 10 : 12; }
 template <int TY, bool MASK>
-__global__ void __launch_bounds__(32 * kScanWarps, scan_ctas<TY>(MASK)) beam_scan_kernel(const BeamProblem p) {
+__global__ void __launch_bounds__(32 * kScanWarps, TY == LETHE_F32 ? 11 : kScanCtas) beam_scan_kernel(const BeamProblem p) {
   using R = Row<TY>;
-  constexpr int N = R::N;
-  __shared__ uint32_t tops[kScanWarps][kMostTiles][32];           // maxima of the bins
-  __shared__ unsigned long long cands[kScanWarps][kCands];
-  __shared__ uint16_t passed[kScanWarps][kCands];
-  griddep_launch();      // (the merge waits for the lists)
+  using T = typename R::T;
+  constexpr int N = R::N, kDepth = R::kDepth, kTile = R::kVecs * 32;
+  __shared__ T tops[kScanWarps][kMostTiles][32];                  // maxima of the bins
+  __shared__ uint4 rings[kScanWarps][kDepth * kTile];             // tiles on their way; afterwards a bin for each lane, and candidates
+  static_assert(kCands * (sizeof(unsigned long long) + sizeof(uint16_t)) <= (kDepth - 1) * kTile * sizeof(uint4), "candidates lie where tiles were");
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const unsigned task = blockIdx.x * kScanWarps + warp, lists = p.lists, row = task / lists;
+  griddep_wait();
+  griddep_launch();      // (the merge waits for the lists)
   if (row >= static_cast<unsigned>(p.B) * p.W) return;
-  if (!goes_on(p, row)) return;
   const R r(p, row);
   const int first = static_cast<int>(task - row * lists) * p.tiles * kTileLogits - r.past;
-
+  // A lane's part of a tile lies where only that lane reads it, so it waits for nobody else.
+  typename R::Vec x[R::kVecs];
+  uint4* const ring = rings[warp] + lane;
+  auto fetch = [&](int j) {
+    if (j < p.tiles) {
+      uint4* const slot = ring + j % kDepth * kTile;
+      const int v = first + j * kTileLogits + lane * N;
+      if (v >= lane * N && v <= r.V - kTileLogits + lane * N) {
+#pragma unroll
+        for (int n = 0; n < R::kVecs; ++n)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(slot + n * 32))), "l"(r.x + v + n * 32 * N) : "memory");
+      } else {
+#pragma unroll 1
+        for (int n = 0; n < R::kVecs; ++n) {
+          const typename R::Vec y = r.template load<MASK>(v + n * 32 * N);
+          slot[n * 32] = make_uint4(y.w[0], y.w[1], y.w[2], y.w[3]);
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int j = 0; j < kDepth - 1; ++j) fetch(j);
+  if (!goes_on(p, row)) {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    return;
+  }
   // The sum of 2^t, t = (l - ref) over: ref is the warp's largest logit so far, or up to kSlack behind it.
   float ref = -INFINITY, mine = -INFINITY;
   double s = 0.;
   for (int j = 0; j < p.tiles; ++j) {
-    typename R::Vec x[R::kVecs];
-    const int v0 = first + j * kTileLogits;
-    if (v0 >= 0 && v0 <= r.V - kTileLogits) {
+    fetch(j + kDepth - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
 #pragma unroll
-      for (int n = 0; n < R::kVecs; ++n) x[n].load(r.x + v0 + (n * 32 + lane) * N);
-      if (MASK) {
-#pragma unroll
-        for (int n = 0; n < R::kVecs; ++n) r.mask(x[n], v0 + (n * 32 + lane) * N);
-      }
-    } else {
-#pragma unroll
-      for (int n = 0; n < R::kVecs; ++n) x[n] = r.template load<MASK>(v0 + (n * 32 + lane) * N);
+    for (int n = 0; n < R::kVecs; ++n) {
+      const uint4 y = ring[j % kDepth * kTile + n * 32];
+      x[n].w[0] = y.x, x[n].w[1] = y.y, x[n].w[2] = y.z, x[n].w[3] = y.w;
+      const int v = first + j * kTileLogits + (n * 32 + lane) * N;
+      if (MASK && v >= 0 && v <= r.V - N) r.mask(x[n], v);
     }
     const float m = R::largest(x);
-    tops[warp][j][lane] = ordered(m);
+    tops[warp][j][lane] = from_f32<TY>(m);
     mine = fmaxf(mine, m);
     if (__any_sync(~0u, m > ref && !((m - ref) * p.over <= kSlack))) {
       const float now = from_ordered(__reduce_max_sync(~0u, ordered(m)));
@@ -214,14 +264,17 @@ __global__ void __launch_bounds__(32 * kScanWarps, scan_ctas<TY>(MASK)) beam_sca
     const F2 t = (sum[0] + sum[1]) + (sum[2] + sum[3]);
     s += static_cast<double>(lo(t) + hi(t));
   }
-#pragma unroll
-  for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
+  __syncwarp();
+  unsigned long long* const cand = reinterpret_cast<unsigned long long*>(rings[warp] + kTile);
+  uint16_t* const passed = reinterpret_cast<uint16_t*>(cand + kCands);
+  auto top_of = [&](int j) { return ordered(to_f32(tops[warp][j][lane])); };
   const uint32_t own = ordered(mine), top = __reduce_max_sync(~0u, own);
 
   // A logit that k bins or a few more have something as large as, by halving: what is below it is not among the k largest, and only
   // those bins have any of them.  Few candidates: by the lanes' maxima alone, which lets some more pass.
   constexpr int kMore = 4, kFew = 16;
   uint32_t least = kLeast + 1, above = top + 1;
+  if (p.k <= 32) least = max(least, __reduce_min_sync(~0u, own));
   auto halve = [&](auto reach) {
     if (reach(least) <= p.k + kMore) return;
     while (above - least > 1) {
@@ -240,7 +293,7 @@ __global__ void __launch_bounds__(32 * kScanWarps, scan_ctas<TY>(MASK)) beam_sca
   } else {
     halve([&](uint32_t u) {
       int n = 0;
-      for (int j = 0; j < p.tiles; ++j) n += tops[warp][j][lane] >= u;
+      for (int j = 0; j < p.tiles; ++j) n += top_of(j) >= u;
       return static_cast<int>(__reduce_add_sync(~0u, n));
     });
   }
@@ -257,42 +310,56 @@ __global__ void __launch_bounds__(32 * kScanWarps, scan_ctas<TY>(MASK)) beam_sca
   };
   uint32_t hit = 0;
   if (own >= least)
-    for (int j = 0; j < p.tiles; ++j) hit |= static_cast<uint32_t>(tops[warp][j][lane] >= least) << j;
+#pragma unroll
+    for (int j = 0; j < kMostTiles; ++j)
+      if (j < p.tiles) hit |= static_cast<uint32_t>(top_of(j) >= least) << j;
   int reached, n = 0;
   int at = offset(__popc(hit), &reached);
   for (; hit; hit &= hit - 1, ++at)
-    if (at < kCands) passed[warp][at] = static_cast<uint16_t>((__ffs(hit) - 1) * 32 + lane);
+    if (at < kCands) passed[at] = static_cast<uint16_t>((__ffs(hit) - 1) * 32 + lane);
   __syncwarp();
   // their logits, a bin for each lane
-  unsigned long long* const cand = cands[warp];
   const float floor = from_ordered(least);
-  if (reached > kCands) {
-    n = kCands + 1;
-  } else {
-    for (int i = 0; i < reached; i += 32) {
-      int v = 0;
-      if (i + lane < reached) {
-        const int bin = passed[warp][i + lane];
-        v = first + bin / 32 * kTileLogits + bin % 32 * N;
+  if (reached > kCands) n = kCands + 1;
+  for (int i = 0; i == 0 || (i < reached && n <= kCands); i += 32) {
+    int v = 0;
+    const bool any = i + lane < reached && n <= kCands;
+    if (any) {
+      const int bin = passed[i + lane];
+      v = first + bin / 32 * kTileLogits + bin % 32 * N;
+      if (v >= 0 && v + (R::kVecs - 1) * 32 * N <= r.V - N) {
 #pragma unroll
-        for (int b = 0; b < R::kVecs; ++b) {
-          const typename R::Vec x = r.template load<MASK>(v + b * 32 * N);
+        for (int b = 0; b < R::kVecs; ++b) x[b].load(r.x + v + b * 32 * N);
+        if (MASK) {
 #pragma unroll
-          for (int e = 0; e < N; ++e) hit |= static_cast<uint32_t>(x.get(e) >= floor) << (b * N + e);
+          for (int b = 0; b < R::kVecs; ++b) r.mask(x[b], v + b * 32 * N);
         }
+      } else {
+#pragma unroll 1
+        for (int b = 0; b < R::kVecs; ++b) r.template edge<MASK>(x, b, v + b * 32 * N);
       }
-      int all;
-      at = n + offset(__popc(hit), &all);
-      n += all;
-      for (; hit; hit &= hit - 1, ++at) {
-        const int b = __ffs(hit) - 1, u = v + b / N * 32 * N + b % N;
-        if (at < kCands) cand[at] = static_cast<unsigned long long>(ordered(to_f32(r.x[u]))) << 32 | static_cast<uint32_t>(~u);
-      }
+    }
+    if (i == 0) {      // (while they come)
+#pragma unroll
+      for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
+    }
+    if (any) {
+      hit = R::reaching(x, floor);
+#pragma unroll
+      for (int b = 0; b < R::kVecs; ++b) ring[b * 32] = make_uint4(x[b].w[0], x[b].w[1], x[b].w[2], x[b].w[3]);
+    }
+    int all;
+    at = n + offset(__popc(hit), &all);
+    n += all;
+    for (; hit; hit &= hit - 1, ++at) {
+      const int b = R::element(__ffs(hit) - 1);
+      const float l = to_f32(reinterpret_cast<const T*>(ring + b / N * 32)[b % N]);
+      if (at < kCands) cand[at] = static_cast<unsigned long long>(ordered(l)) << 32 | static_cast<uint32_t>(~(v + b / N * 32 * N + b % N));
     }
   }
   __syncwarp();
-  unsigned long long* const list = p.keys + static_cast<long long>(task) * (p.k + kSpare);
-  if (n <= p.k + kSpare) {
+  unsigned long long* const list = p.keys + static_cast<long long>(task) * list_room(p.k);
+  if (n <= list_room(p.k)) {
     for (int i = lane; i < n; i += 32) list[i] = cand[i];
   } else if (n <= kCands) {
     for (int i = lane; i < n; i += 32) {
@@ -322,63 +389,63 @@ __global__ void __launch_bounds__(32 * kScanWarps, scan_ctas<TY>(MASK)) beam_sca
   }
   if (lane == 0) {
     const float m = from_ordered(top);
-    if (ref > -INFINITY) s *= exp_below((static_cast<double>(ref) - m) * p.inverse);
+    if (ref < m) s *= exp_below((static_cast<double>(ref) - m) * p.inverse);
     p.stat[task] = ScanStat{m, n, s};
   }
 }
 
 // A candidate: larger ones come first.
 struct Entry {
-  unsigned long long rank, place;      // ordered(r); ~(w V + v)
+  unsigned long long rank, place;      // ordered(r); ~(w 2^32 + v)
 };
-__device__ __forceinline__ bool larger(const Entry& a, const Entry& b) { return a.rank > b.rank || (a.rank == b.rank && a.place > b.place); }
+__device__ __forceinline__ bool larger(const Entry& a, const Entry& b) { return (a.rank > b.rank) | ((a.rank == b.rank) & (a.place > b.place)); }
+__device__ __forceinline__ int beam_of(const Entry& e) { return static_cast<int>(~e.place >> 32); }
+__device__ __forceinline__ int token_of(const Entry& e) { return static_cast<int>(~static_cast<uint32_t>(e.place)); }
 
 struct MergeMemory {
+  unsigned long long keys[kMergeKeys];
+  ScanStat stat[kMergeThreads];
   Entry room[kMergeRoom], sorted[kBins];
+  uint4 bins[kBins / 4];
   double score[kBeamMost], inverse[kBeamMost], lse[kBeamMost], part[kMergeThreads / 32];      // inverse: 1 / penalty
   float top[kBeamMost];
-  uint32_t bins[kBins], least;
-  int todo[kMergeThreads];
+  int2 todo[kMergeThreads];             // list, beam
+  uint32_t least;
+  int n, lists;
   bool on[kBeamMost], ended[kBeamMost], again[kBeamMost];
-  int n, lists, any;
 };
 
-// The largest of room[0, n), at most `most`, in order; `least` becomes the last of them where there are so many.
-__device__ __forceinline__ void keep_largest(MergeMemory& m, int most, Entry* least) {
+// The largest of room[0, n), at most `most`, in order, as sorted[0, n).
+__device__ __forceinline__ int sort_largest(MergeMemory& m, int most) {
   __syncthreads();
   const int n = m.n, tid = threadIdx.x;
-  if (n <= kMergeThreads / 8) {
-    const int i = tid / 8;
-    const Entry e = m.room[min(i, n - 1 < 0 ? 0 : n - 1)];
+  // as many threads for an entry as there are; they count those that are larger
+  const int share = n <= 32 ? 16 : n <= 64 ? 8 : n <= 128 ? 4 : n <= 256 ? 2 : 1;
+  for (int i = tid / share; i < (n + 31) / 32 * 32; i += kMergeThreads / share) {      // (whole warps)
+    const Entry e = m.room[min(i, n - 1)];
     int before = 0;
-    for (int j = tid % 8; j < n; j += 8) before += larger(m.room[j], e);
-#pragma unroll
-    for (int d = 4; d; d >>= 1) before += __shfl_xor_sync(~0u, before, d);
-    if (i < n && before < most && tid % 8 == 0) m.sorted[before] = e;
-  } else {
-    for (int i = tid; i < n; i += kMergeThreads) {
-      const Entry e = m.room[i];
-      int before = 0;
-      for (int j = 0; j < n; ++j) before += larger(m.room[j], e);
-      if (before < most) m.sorted[before] = e;
-    }
+#pragma unroll 4
+    for (int j = tid % share; j < n; j += share) before += larger(m.room[j], e);
+    for (int d = share / 2; d; d >>= 1) before += __shfl_xor_sync(~0u, before, d);
+    if (i < n && before < most && tid % share == 0) m.sorted[before] = e;
   }
   __syncthreads();
-  const int left = min(n, most);
-  for (int i = tid; i < left; i += kMergeThreads) m.room[i] = m.sorted[i];
-  if (tid == 0) m.n = left;
-  if (left == most) *least = m.sorted[most - 1];
-  __syncthreads();
+  return min(n, most);
+}
+
+__device__ __forceinline__ void fetch16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from) : "memory");
 }
 
 template <int TY>
 __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamProblem p) {
-  __shared__ MergeMemory m;
+  extern __shared__ __align__(16) unsigned char memory[];
+  MergeMemory& m = *reinterpret_cast<MergeMemory*>(memory);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, row0 = blockIdx.x * p.W;
-  const int lists = p.W * p.lists, most = p.k + kBehind, line = p.k + kSpare;
+  const int lists = p.W * p.lists, most = p.k + kBehind, line = list_room(p.k);
   const double over = p.inverse;
-  const ScanStat* const stat = p.stat + static_cast<long long>(row0) * p.lists;
-  const unsigned long long* const keys = p.keys + static_cast<long long>(row0) * p.lists * line;
+  const ScanStat* stat = p.stat + static_cast<long long>(row0) * p.lists;
+  const unsigned long long* keys = p.keys + static_cast<long long>(row0) * p.lists * line;
   if (tid < p.W) {
     const bool in = counts(p, row0 + tid), ended = p.finished && p.finished[row0 + tid];
     m.score[tid] = p.scores[row0 + tid];
@@ -387,15 +454,34 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamPro
     m.ended[tid] = in && ended;
     m.again[tid] = false;
   }
-  __syncthreads();
+  const int w_of_tid = tid / p.lists;
+  auto beam_of_list = [&](int l) { return l == tid ? w_of_tid : l / p.lists; };
+  auto begin = [&] {      // finished beams offer themselves
+    if (tid == 0) m.n = m.lists = m.least = 0;
+    if (tid < kBins / 4) m.bins[tid] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    if (tid < p.W && m.ended[tid])
+      m.room[atomicAdd(&m.n, 1)] = Entry{ordered(m.score[tid] * m.inverse[tid]), ~(static_cast<unsigned long long>(tid) << 32 | static_cast<uint32_t>(p.eos))};
+  };
+  begin();
   griddep_wait();
+  if (lists <= kMergeThreads) {
+    if (tid < lists) fetch16(&m.stat[tid], &stat[tid]);
+    stat = m.stat;
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
+  if (lists * line <= kMergeKeys) {
+    for (int i = 2 * tid; i < lists * line; i += 2 * kMergeThreads) fetch16(&m.keys[i], &keys[i]);
+    keys = m.keys;
+  }
+  asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 1;" ::: "memory");
+  __syncthreads();
   for (int w = warp; w < p.W; w += kMergeThreads / 32) {
     if (!m.on[w]) continue;
     const ScanStat* const a = stat + w * p.lists;
     float top = -INFINITY;
     for (int i = lane; i < p.lists; i += 32) top = fmaxf(top, a[i].m);
-#pragma unroll
-    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+    top = from_ordered(__reduce_max_sync(~0u, ordered(top)));
     double s = 0.;
     for (int i = lane; i < p.lists; i += 32) {
       const ScanStat t = a[i];
@@ -410,109 +496,116 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamPro
     }
   }
   auto rank = [&](int w, float x) { return (m.score[w] + (x * over - m.lse[w])) * m.inverse[w]; };
-  auto entry = [&](int l, unsigned long long key) {
-    const int w = l / p.lists;
-    return Entry{ordered(rank(w, from_ordered(static_cast<uint32_t>(key >> 32)))),
-                 ~(static_cast<unsigned long long>(w) * p.V + (~static_cast<uint32_t>(key)))};
+  auto entry = [&](int w, unsigned long long key) {
+    return Entry{ordered(rank(w, from_ordered(static_cast<uint32_t>(key >> 32)))), ~(static_cast<unsigned long long>(w) << 32) ^ (~static_cast<uint32_t>(key))};
   };
   auto narrow = [](double x) { return ordered(static_cast<float>(x)); };      // in the same order, equal ones more
+  int n;
   for (int pass = 0;; ++pass) {
+    if (pass) begin();
     __syncthreads();
-    if (tid == 0) m.n = m.lists = m.least = 0;
-    if (tid < kBins) m.bins[tid] = 0;
-    __syncthreads();
-    if (tid < p.W && m.ended[tid])
-      m.room[atomicAdd(&m.n, 1)] = Entry{ordered(m.score[tid] * m.inverse[tid]), ~(static_cast<unsigned long long>(tid) * p.V + p.eos)};
     // `least`: as many bins as candidates are wanted have a list whose largest logit reaches it.  What is below is not wanted.
     uint32_t head = 0;
-    for (int l = tid; l < lists; l += kMergeThreads)
-      if (m.on[l / p.lists] && stat[l].n > 0) head = max(head, narrow(rank(l / p.lists, stat[l].m)));
-    if (head) atomicMax(&m.bins[tid % kBins], head);
+    for (int l = tid; l < lists; l += kMergeThreads) {
+      const int w = beam_of_list(l);
+      if (m.on[w] && stat[l].n > 0) head = max(head, narrow(rank(w, stat[l].m)));
+    }
+    if (head) atomicMax(reinterpret_cast<uint32_t*>(m.bins) + tid % kBins, head);
+    if (!pass) asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
     {
       constexpr int kShare = kMergeThreads / kBins;
       const int i = tid / kShare;
-      const uint32_t b = m.bins[i];
+      const uint32_t b = reinterpret_cast<const uint32_t*>(m.bins)[i];
       int before = 0;
-#pragma unroll 8
-      for (int j = tid % kShare; j < kBins; j += kShare) before += m.bins[j] > b || (m.bins[j] == b && j < i);
+      auto count = [&](uint32_t o, int j) { before += (o > b) | ((o == b) & (j < i)); };
+#pragma unroll
+      for (int k = 0; k < kBins / 4 / kShare; ++k) {
+        const int j = k * kShare + tid % kShare;
+        const uint4 o = m.bins[j];
+        count(o.x, 4 * j), count(o.y, 4 * j + 1), count(o.z, 4 * j + 2), count(o.w, 4 * j + 3);
+      }
 #pragma unroll
       for (int d = kShare / 2; d; d >>= 1) before += __shfl_xor_sync(~0u, before, d);
       if (before == most - 1 && tid % kShare == 0) m.least = b;
     }
     __syncthreads();
     const uint32_t floor = max(m.least, 1u);
-    for (int l = tid; l < lists; l += kMergeThreads)
-      if (m.on[l / p.lists] && stat[l].n > 0 && narrow(rank(l / p.lists, stat[l].m)) >= floor) {
+    for (int l = tid; l < lists; l += kMergeThreads) {
+      const int w = beam_of_list(l);
+      if (m.on[w] && stat[l].n > 0 && (lists <= kMergeThreads ? head : narrow(rank(w, stat[l].m))) >= floor) {
         const int at = atomicAdd(&m.lists, 1);
-        if (at < kMergeThreads) m.todo[at] = l;
-      }
-    __syncthreads();
-    // their candidates that reach it
-    for (int i = warp; i < min(m.lists, kMergeThreads); i += kMergeThreads / 32) {
-      const int l = m.todo[i], n = stat[l].n;
-      for (int c = lane; c < n; c += 32) {
-        const Entry e = entry(l, keys[static_cast<long long>(l) * line + c]);
-        if (narrow(from_ordered(e.rank)) >= floor) {
-          const int at = atomicAdd(&m.n, 1);
-          if (at < kMergeRoom) m.room[at] = e;
-        }
+        if (at < kMergeThreads) m.todo[at] = make_int2(l, w);
       }
     }
     __syncthreads();
-    Entry least{0, 0};
+    // their candidates that reach it, of two lists at a time
+    for (int i = warp; i < min(m.lists, kMergeThreads); i += kMergeThreads / 16) {
+      const int2 a = m.todo[i], b = i + kMergeThreads / 32 < min(m.lists, kMergeThreads) ? m.todo[i + kMergeThreads / 32] : make_int2(-1, 0);
+      const int an = stat[a.x].n, bn = b.x >= 0 ? stat[b.x].n : 0;
+      for (int c = lane; c < max(an, bn); c += 32) {
+        unsigned long long ak = 0, bk = 0;
+        if (c < an) ak = keys[static_cast<long long>(a.x) * line + c];
+        if (c < bn) bk = keys[static_cast<long long>(b.x) * line + c];
+        auto put = [&](int w, unsigned long long key) {
+          const Entry e = entry(w, key);
+          if (narrow(from_ordered(e.rank)) < floor) return;
+          const int at = atomicAdd(&m.n, 1);
+          if (at < kMergeRoom) m.room[at] = e;
+        };
+        if (c < an) put(a.y, ak);
+        if (c < bn) put(b.y, bk);
+      }
+    }
+    __syncthreads();
     if (m.lists > kMergeThreads || m.n > kMergeRoom) {
-      // So many equal ones: all candidates in turn, as many at a time as there is room for.
+      // So many equal ones: all candidates in turn, as many at a time as there is room for, and no more of those below the last wanted one.
+      Entry least{0, 0};
       __syncthreads();
-      if (tid == 0) m.n = 0;
+      begin();
       __syncthreads();
-      if (tid < p.W && m.ended[tid])
-        m.room[atomicAdd(&m.n, 1)] = Entry{ordered(m.score[tid] * m.inverse[tid]), ~(static_cast<unsigned long long>(tid) * p.V + p.eos)};
       const long long all = static_cast<long long>(lists) * line;
       for (long long i = 0; i < all; i += kMergeThreads) {
         const int l = static_cast<int>((i + tid) / line), c = static_cast<int>((i + tid) % line);
         if (l < lists && m.on[l / p.lists] && c < stat[l].n) {
-          const Entry e = entry(l, keys[static_cast<long long>(l) * line + c]);
+          const Entry e = entry(l / p.lists, keys[static_cast<long long>(l) * line + c]);
           if (!larger(least, e)) m.room[atomicAdd(&m.n, 1)] = e;
         }
         __syncthreads();
-        const int n = m.n;
+        if (m.n > kMergeRoom - kMergeThreads) {
+          const int left = sort_largest(m, most);
+          if (tid < left) m.room[tid] = m.sorted[tid];
+          if (tid == 0) m.n = left;
+          if (left == most) least = m.sorted[most - 1];
+        }
         __syncthreads();
-        if (n > kMergeRoom - kMergeThreads) keep_largest(m, most, &least);
       }
     }
-    keep_largest(m, most, &least);
+    n = sort_largest(m, most);
     if (pass) break;
     // Candidates of different beams next to one another, closer than the sums are known.
-    if (tid == 0) m.any = 0;
-    __syncthreads();
-    const int n = m.n;
-    auto beam = [&](const Entry& e) { return static_cast<int>(~e.place / p.V); };
+    bool close = false;
     if (tid < n && tid < p.k) {
       const Entry a = m.sorted[tid];
-      const int u = beam(a);
-      double far = 0.;
-      if (p.penalty) {
-        for (int w = 0; w < p.W; ++w) far = fmax(far, m.inverse[w]);
-      } else {
-        far = 1.;
-      }
+      const int u = beam_of(a);
+      double far = 1.;
+      if (p.penalty)
+        for (int w = 0; w < p.W; ++w) far = fmax(w ? far : 0., m.inverse[w]);
       far *= 2. * kLseError;
       int j = tid + 1;
       for (; j < n; ++j) {
         const double gap = from_ordered(a.rank) - from_ordered(m.sorted[j].rank);
         if (!(gap < far)) break;
-        const int w = beam(m.sorted[j]);
-        if (gap > 0. && u != w && gap < kLseError * (m.inverse[u] + m.inverse[w])) m.again[u] = m.again[w] = m.any = 1;
+        const int w = beam_of(m.sorted[j]);
+        if (gap > 0. && u != w && gap < kLseError * (m.inverse[u] + m.inverse[w])) m.again[u] = m.again[w] = close = true;
       }
       // as many equals behind the last of this beam's: another beam's may lie behind them
       if (j == most && p.W > 1) {
         for (int w = 0; w < p.W; ++w) m.again[w] = true;
-        m.any = 1;
+        close = true;
       }
     }
-    __syncthreads();
-    if (!m.any) break;
+    if (!__syncthreads_or(close)) break;
     for (int w = 0; w < p.W; ++w) {
       if (!m.again[w] || !m.on[w]) continue;
       const Row<TY> r(p, row0 + w);
@@ -533,10 +626,10 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamPro
   }
   if (tid < p.k) {
     const long long o = static_cast<long long>(blockIdx.x) * p.k + tid;
-    const bool there = tid < m.n;
-    const unsigned long long place = there ? ~m.sorted[tid].place : 0;
-    const int w = static_cast<int>(place / p.V), v = there ? static_cast<int>(place % p.V) : max(p.eos, 0);
-    p.out_scores[o] = there ? static_cast<float>(from_ordered(m.sorted[tid].rank) * (p.penalty ? p.penalty[row0 + w] : 1.f)) : -INFINITY;
+    const bool there = tid < n;
+    const Entry e = m.sorted[tid];
+    const int w = there ? beam_of(e) : 0, v = there ? token_of(e) : max(p.eos, 0);
+    p.out_scores[o] = there ? static_cast<float>(from_ordered(e.rank) * (p.penalty ? p.penalty[row0 + w] : 1.f)) : -INFINITY;
     p.parents[o] = w;
     p.tokens[o] = v;
     if (p.out_finished) p.out_finished[o] = !there || v == p.eos || m.ended[w];
@@ -547,14 +640,14 @@ struct ScanPlan {
   int tiles;
   long long lists, tasks;
 };
-// As many segments as the GPU's SMs hold warps of the kernel, or fewer, where tiles are enough; more bins than candidates in each.  A row that
-// does not begin on a 16-byte boundary may reach into one more tile.
+// Segments so many that the GPU's SMs hold their warps all at once, where there is enough for them to do; more bins than candidates in each.
+// A row that does not begin on a 16-byte boundary may reach into one more tile.
 static ScanPlan scan_plan(long long B, int W, long long V, int k, int ty, bool aligned) {
   const long long past = aligned ? 0 : 16 / elem_bytes(ty) - 1, row = (V + past + kTileLogits - 1) / kTileLogits;
-  const long long held = 148 * kScanWarps * (ty == LETHE_F32 ? scan_ctas<LETHE_F32>(false) : scan_ctas<LETHE_BF16>(false));
-  const long long want = (B * W * ((V + kTileLogits - 1) / kTileLogits) + held - 1) / held;
+  const long long even = (V + kTileLogits - 1) / kTileLogits, held = 148 * kScanWarps * kScanCtas / (B * W);      // (for every row)
+  const long long most = kMostTiles, want = held ? (even + held - 1) / held : most;
   ScanPlan s;
-  s.tiles = static_cast<int>(want < kMostTiles ? want : kMostTiles);
+  s.tiles = static_cast<int>(want < most ? want : most);
   if (s.tiles * 32 < k) s.tiles = (k + 31) / 32;
   s.lists = (row + s.tiles - 1) / s.tiles;
   s.tiles = static_cast<int>((row + s.lists - 1) / s.lists);
@@ -570,10 +663,10 @@ static bool beam_sizes(long long B, int W, long long V, int k, int ty) {
 template <int TY>
 static int launch_beam(const BeamProblem& p, long long tasks, cudaStream_t st) {
   const dim3 grid(static_cast<unsigned>((tasks + kScanWarps - 1) / kScanWarps));
-  if (p.allowed) beam_scan_kernel<TY, true><<<grid, 32 * kScanWarps, 0, st>>>(p);
-  else beam_scan_kernel<TY, false><<<grid, 32 * kScanWarps, 0, st>>>(p);
-  if (cudaGetLastError() != cudaSuccess) return kErrLaunch;
-  return launch_dependent(beam_merge_kernel<TY>, dim3(p.B), dim3(kMergeThreads), 0, st, p) == cudaSuccess ? kOk : kErrLaunch;
+  if (launch_dependent(p.allowed ? beam_scan_kernel<TY, true> : beam_scan_kernel<TY, false>, grid, dim3(32 * kScanWarps), 0, st, p) != cudaSuccess) return kErrLaunch;
+  static SmemAttr attr;
+  if (attr.set(beam_merge_kernel<TY>, sizeof(MergeMemory))) return kErrLaunch;
+  return launch_dependent(beam_merge_kernel<TY>, dim3(p.B), dim3(kMergeThreads), sizeof(MergeMemory), st, p) == cudaSuccess ? kOk : kErrLaunch;
 }
 
 }  // namespace lg
@@ -581,7 +674,7 @@ static int launch_beam(const BeamProblem& p, long long tasks, cudaStream_t st) {
 extern "C" size_t lethe_gdn_beam_work_bytes(int64_t B, int32_t W, int64_t V, int32_t k, int32_t x_type) {
   using namespace lg;
   if (!beam_sizes(B, W, V, k, x_type)) return 0;
-  return static_cast<size_t>(scan_plan(B, W, V, k, x_type, false).tasks) * (sizeof(ScanStat) + 8 * static_cast<size_t>(k + kSpare));
+  return static_cast<size_t>(scan_plan(B, W, V, k, x_type, false).tasks) * (sizeof(ScanStat) + 8 * static_cast<size_t>(list_room(k)));
 }
 
 extern "C" int lethe_gdn_beam_select(const LetheGdnBeamArgs* a, void* stream) {

@@ -57,12 +57,12 @@ def test_beam_select(lib):
 
 
 def test_beam_work_bytes(lib):
-    assert lib.lethe_gdn_beam_work_bytes(2, 3, 100, 3, 0) == 6 * (16 + 8 * 19)           # a list a row, of 16 more than asked for
-    assert lib.lethe_gdn_beam_work_bytes(2, 3, 1021, 3, 0) == 6 * (16 + 8 * 19)          # 1024 logits a list, the row up to 3 behind a 16-byte boundary
-    assert lib.lethe_gdn_beam_work_bytes(2, 3, 1022, 3, 0) == 12 * (16 + 8 * 19)
-    assert lib.lethe_gdn_beam_work_bytes(2, 3, 1017, 3, 1) == 6 * (16 + 8 * 19)          # 16 bits: up to 7
-    assert lib.lethe_gdn_beam_work_bytes(2, 3, 1018, 3, 1) == 12 * (16 + 8 * 19)
-    assert lib.lethe_gdn_beam_work_bytes(1, 1, 2000, 33, 1) == 16 + 8 * 49                # more candidates than lanes: two tiles at least
+    assert lib.lethe_gdn_beam_work_bytes(2, 3, 100, 3, 0) == 6 * (16 + 8 * 20)           # a list a row, of 16 more than asked for, made even
+    assert lib.lethe_gdn_beam_work_bytes(2, 3, 1021, 3, 0) == 6 * (16 + 8 * 20)          # 1024 logits a list, the row up to 3 behind a 16-byte boundary
+    assert lib.lethe_gdn_beam_work_bytes(2, 3, 1022, 3, 0) == 12 * (16 + 8 * 20)
+    assert lib.lethe_gdn_beam_work_bytes(2, 3, 1017, 3, 1) == 6 * (16 + 8 * 20)          # 16 bits: up to 7
+    assert lib.lethe_gdn_beam_work_bytes(2, 3, 1018, 3, 1) == 12 * (16 + 8 * 20)
+    assert lib.lethe_gdn_beam_work_bytes(1, 1, 2000, 33, 1) == 16 + 8 * 50                # more candidates than lanes: two tiles at least
     for bad in ((0, 1, 1, 1, 0), (1, 0, 1, 1, 0), (1, 65, 1, 1, 0), (1, 1, 0, 1, 0), (1, 1, 1, 0, 0), (1, 1, 1, 65, 0), (1, 1, 1, 1, 3)):
         assert lib.lethe_gdn_beam_work_bytes(*bad) == 0
 
