@@ -412,9 +412,9 @@ int lethe_gdn_reorder_states(const LetheGdnStates* states, int32_t count, int64_
  * compact: the m live slots become slots 0 to m - 1: the ones at or behind m, in their order, move to the free ones in front of m, in
  *   theirs; what lies behind is left as it was.  place[i] = the new slot of live slot i, -1 for others; *live_count = m. */
 int lethe_gdn_fork_states(const LetheGdnStates* states, int32_t count, int64_t slots, const uint8_t* live, const void* source, int32_t source_64,
-                          int64_t n, int64_t* target, uint8_t* live_after, void* cuda_stream);
+                          int64_t n, int64_t* target, uint8_t* live_after, int32_t* status, void* cuda_stream);
 int lethe_gdn_compact_states(const LetheGdnStates* states, int32_t count, int64_t slots, const uint8_t* live, int64_t* place,
-                             int64_t* live_count, void* cuda_stream);
+                             int64_t* live_count, int32_t* status, void* cuda_stream);
 
 /* lethe_gdn_decode_step with a state of its own for what it writes: row b goes on from row source[b] of args->state [slots, H, K, V]
  * (-1: from zeros), and its new state is row b of out [B, H, K, V], memory apart from args->state.  source [B], int64 or

@@ -13,6 +13,7 @@
 
 #include "../../include/lethe_gdn.h"
 #include "host_util.h"
+#include "umma.cuh"
 
 namespace lg {
 
@@ -61,6 +62,7 @@ template <int V, bool F32, bool FROM>
 __global__ void __launch_bounds__(kSplit * V, 1024 / (kSplit * V))
 decode_step_kernel(const DecodeProblem p) {
   __shared__ float ks[kDK], qs[kDK], as[kDK], part[kSplit][V];
+  if (FROM) griddep_wait();
   const int bh = pair_of<FROM>(p, blockIdx.x), c = threadIdx.x % V, part_id = threadIdx.x / V;   // rows [kRows part_id, + kRows)
   for (int d = threadIdx.x; d < kDK; d += kSplit * V) {
     ks[d] = token_in<F32>(p.k, static_cast<size_t>(bh) * kDK + d);
@@ -141,6 +143,7 @@ decode_ring_kernel(const DecodeProblem p) {
   __shared__ __align__(16) float kpart[kRingWarps][V], opart[kRingWarps][V];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;         // rows [kRingRows warp, +), columns [4 lane, +4)
   const size_t own = static_cast<size_t>(warp * kRingRows) * 32 + lane;
+  if (FROM) griddep_wait();
   // (the source of the state after the next comes while the next is fetched)
   long long slot = 0;
   auto look = [&](int i) {
@@ -252,23 +255,24 @@ decode_ring_kernel(const DecodeProblem p) {
 }
 
 // d_v = 64 stays with one CTA per pair: eight of half the size per SM overlap as well (2048 pairs: 26.8 us, ring 27.5).
+// The step from other rows starts while the kernel before it ends.
+template <bool FROM>
+static int launch_step(void (*kernel)(const DecodeProblem), int grid, int block, size_t smem, cudaStream_t st, const DecodeProblem& p) {
+  if (FROM) return launch_dependent(kernel, dim3(grid), dim3(block), smem, st, p) == cudaSuccess ? kOk : kErrLaunch;
+  kernel<<<grid, block, smem, st>>>(p);
+  return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
+}
+
 template <bool F32, bool FROM>
 static int launch_decode(const DecodeProblem& p, cudaStream_t st) {
-  if (p.V == 64) {
-    decode_step_kernel<64, F32, FROM><<<p.BH, kSplit * 64, 0, st>>>(p);
-  } else {
-    const int sms = sm_count();
-    if (sms <= 0) return kErrDevice;
-    const bool aligned = (reinterpret_cast<uintptr_t>(p.state) | reinterpret_cast<uintptr_t>(p.from)) % 16 == 0 && reinterpret_cast<uintptr_t>(p.o) % 4 == 0;
-    if (p.BH >= 4 * sms && aligned) {
-      static SmemAttr attr;
-      if (attr.set(decode_ring_kernel<F32, FROM>, kRingBytes)) return kErrLaunch;
-      decode_ring_kernel<F32, FROM><<<kRingCtas * sms, kRingThreads, kRingBytes, st>>>(p);
-    } else {
-      decode_step_kernel<128, F32, FROM><<<p.BH, kSplit * 128, 0, st>>>(p);
-    }
-  }
-  return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
+  if (p.V == 64) return launch_step<FROM>(decode_step_kernel<64, F32, FROM>, p.BH, kSplit * 64, 0, st, p);
+  const int sms = sm_count();
+  if (sms <= 0) return kErrDevice;
+  const bool aligned = (reinterpret_cast<uintptr_t>(p.state) | reinterpret_cast<uintptr_t>(p.from)) % 16 == 0 && reinterpret_cast<uintptr_t>(p.o) % 4 == 0;
+  if (p.BH < 4 * sms || !aligned) return launch_step<FROM>(decode_step_kernel<128, F32, FROM>, p.BH, kSplit * 128, 0, st, p);
+  static SmemAttr attr;
+  if (attr.set(decode_ring_kernel<F32, FROM>, kRingBytes)) return kErrLaunch;
+  return launch_step<FROM>(decode_ring_kernel<F32, FROM>, kRingCtas * sms, kRingThreads, kRingBytes, st, p);
 }
 
 }  // namespace lg

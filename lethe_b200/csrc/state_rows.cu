@@ -2,22 +2,29 @@
 // another's (fork), the rows in use move together (compact).  Nothing is computed: what bounds these is reading every row
 // that somebody takes over once and writing every row that changes once.  Which rows those are stands on the device; every CTA works it
 // out for itself (bytes against megabytes) instead of waiting for a launch that does.
+//
+// Rows of 16-byte multiples go through shared memory by bulk copies, one CTA per SM: up to four warps issue them, each with a ring of its own,
+// and no thread touches the data.  Rows of other sizes go through registers in the other warps meanwhile.
 #include "elem.cuh"
 #include "host_util.h"
 #include "umma.cuh"
 
 namespace lg {
 
-constexpr int kRowThreads = 256, kRowCtas = 4;
+constexpr int kRowThreads = 256, kCopyWarps = 4, kPlainWarps = kRowThreads / 32 - kCopyWarps;
 constexpr int kMostTensors = 32;            // of one launch
 constexpr int kMostBeams = 256, kMostSlots = 65536, kMostEntries = 4096;
-constexpr int kReorderBytes = 32768, kCopyStrip = 16384;
+constexpr int kGroupBytes = 32768;          // a wide group's strips
+// Stages of a ring: as many strips on their way in as out.  With half the strips on their way out a compaction of 518 MB took 101 us for NNN.
+constexpr int kStages = 6, kOut = kStages / 2;
+constexpr int kAllBytes = 218112, kMostStage = 8192;      // dynamic shared memory of a CTA; bytes of a stage where there are four rings
+constexpr int kSiteReorder = 811, kSiteCopy = 812;
 
 struct StateTensor {
   char* data;
   long long row, stride, group;     // bytes
-  int unit, strip;                  // what is moved at once; bytes of a row that a CTA takes
-  long long first;                  // places of the tensors in front
+  int unit, strip;                  // what is moved at once; bytes of a row that are an item's
+  long long first;                  // strips of the tensors in front
 };
 struct StateTensors {
   StateTensor t[kMostTensors];
@@ -70,40 +77,232 @@ __device__ __forceinline__ unsigned block_scan(unsigned x, unsigned* total) {
   return before + s - x;
 }
 
-__device__ __forceinline__ long long index_at(const void* p, int is64, long long i) {
-  return is64 ? static_cast<const long long*>(p)[i] : static_cast<const int*>(p)[i];
-}
-
-// ------------------------------------------------------------------------------------------------------------------
-// Reorder: a CTA has a strip of the rows of one group.  The strips that somebody takes over are in shared memory before any is written.
-// ------------------------------------------------------------------------------------------------------------------
-struct ReorderProblem {
-  StateTensors s;
-  const void* parents;
-  int parents64, W;
-  int* status;
-};
-
 template <typename T> __device__ __forceinline__ void fetch(T* to, const T* from) {
-  if constexpr (sizeof(T) >= 4) {
-    const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(to));
-    if constexpr (sizeof(T) == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(from) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(from), "n"(sizeof(T)) : "memory");
+  if constexpr (sizeof(T) == 4 || sizeof(T) == 8) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(to)), "l"(from), "n"(sizeof(T)) : "memory");
+  } else if constexpr (sizeof(T) == 16) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
   } else {
     *to = *from;
   }
 }
 
+// a / b, and what is left
+__device__ __forceinline__ unsigned long long divide(unsigned long long a, unsigned b, unsigned* rest) {
+  const unsigned long long q = a >> 32 ? a / b : static_cast<unsigned>(a) / b;
+  *rest = static_cast<unsigned>(a - q * b);
+  return q;
+}
+
+__device__ __forceinline__ long long index_at(const void* p, int is64, long long i) {
+  return is64 ? static_cast<const long long*>(p)[i] : static_cast<const int*>(p)[i];
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// A warp's ring.  Lane 0 expects what comes; a stage is filled again when the stores out of it have read it.
+// ------------------------------------------------------------------------------------------------------------------
+struct LaneCopy {           // what a lane stores out of a stage
+  char* to;
+  uint32_t from, bytes;     // (0: nothing)
+};
+struct RingMemory {
+  uint64_t full[kCopyWarps][kStages];
+  LaneCopy copies[kCopyWarps][kStages][32];
+  int abort_flag;
+};
+
+struct Ring {
+  unsigned char* bytes;
+  uint64_t* full;
+  LaneCopy (*copies)[32];
+  CtaCtl ctl;
+  int stage_bytes, site;
+  uint32_t phases = 0, filled = 0;      // bit s: the parity that stage s is waited for next; loads into it that nobody has waited for
+
+  // (all threads of the CTA, in front of a barrier)
+  __device__ __forceinline__ Ring(RingMemory& m, unsigned char* memory, int stage_bytes, int* status, int site)
+      : bytes(memory + threadIdx.x / 32 % kCopyWarps * kStages * stage_bytes), full(m.full[threadIdx.x / 32 % kCopyWarps]),
+        copies(m.copies[threadIdx.x / 32 % kCopyWarps]), ctl{status, &m.abort_flag}, stage_bytes(stage_bytes), site(site) {
+    if (threadIdx.x < kCopyWarps * kStages) mbar_init(&m.full[0][0] + threadIdx.x, 1);
+    if (threadIdx.x == 0) m.abort_flag = 0;
+    fence_mbar_init();
+  }
+  __device__ __forceinline__ unsigned char* stage(int s) const { return bytes + s * stage_bytes; }
+  __device__ __forceinline__ void expect(int s, uint32_t n) {
+    if (threadIdx.x % 32 == 0) mbar_expect_tx(full + s, n);
+    filled |= 1u << s;
+    __syncwarp();
+  }
+  __device__ __forceinline__ void arrive(int s) {
+    if (!((filled >> s) & 1)) return;
+    mbar_wait_warp(full + s, (phases >> s) & 1, ctl, site);
+    phases ^= 1u << s;
+    filled &= ~(1u << s);
+  }
+  // Whether a wait gave up.  What is still on its way is waited for, with a limit, before the CTA may end.
+  __device__ __forceinline__ bool gave_up() {
+    if (!*ctl.abort_flag) return false;
+    const long long t0 = clock64();
+    for (int s = 0; s < kStages; ++s)
+      while (((filled >> s) & 1) && !mbar_try(full + s, (phases >> s) & 1) && clock64() - t0 < ctl.limit) {
+      }
+    return true;
+  }
+
+  // Step after step: load(s, &copy) issues the next one's copies into stage s and says what the lane stores out of it, or that there is none.
+  template <typename Load> __device__ __forceinline__ void run(Load load) {
+    const int lane = threadIdx.x % 32;
+    int loaded = 0, into = 0, at = 0;
+    bool more = true;
+    auto one = [&] {
+      LaneCopy c;
+      more = load(into, &c);
+      if (!more) return;
+      copies[into][lane] = c;
+      into = into + 1 == kStages ? 0 : into + 1;
+      ++loaded;
+    };
+    while (more && loaded < kStages - kOut) one();
+    for (int stored = 0; stored < loaded; ++stored) {
+      if (more) {      // (the stage that `kOut` steps ago was stored from)
+        asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kOut - 1) : "memory");
+        __syncwarp();
+        one();
+      }
+      arrive(at);
+      if (gave_up()) break;
+      const LaneCopy c = copies[at][lane];
+      if (c.bytes) asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(c.to), "r"(c.from), "r"(c.bytes) : "memory");
+      bulk_commit();
+      at = at + 1 == kStages ? 0 : at + 1;
+    }
+    bulk_wait_read();
+  }
+};
+// the copying warps' items: first those of one warp of every CTA
+__device__ __forceinline__ long long first_item() { return static_cast<long long>(threadIdx.x / 32) * gridDim.x + blockIdx.x; }
+
+// ------------------------------------------------------------------------------------------------------------------
+// Reorder.  An item is a strip of the rows of one group, a step as much of it as a stage holds: those that somebody takes over are in
+// shared memory before any is written.
+// ------------------------------------------------------------------------------------------------------------------
+struct ReorderProblem {
+  StateTensors bulk, plain;
+  long long bulk_items, plain_items;
+  const void* parents;
+  int parents64, W, copy_warps, stage_bytes;
+  int* status;
+};
+
+struct Parents {              // of a group of up to 32, in a warp's lanes
+  int parent;
+  uint32_t used;              // rows that others take over
+  bool moves;
+  __device__ __forceinline__ int place(int row) const { return __popc(used & ((1u << row) - 1)); }
+};
+__device__ __forceinline__ long long parent_of(const ReorderProblem& p, long long b) {
+  const int lane = threadIdx.x % 32;
+  return lane < p.W ? index_at(p.parents, p.parents64, b * p.W + lane) : lane;
+}
+__device__ __forceinline__ Parents parents_of(const ReorderProblem& p, long long x) {
+  const int lane = threadIdx.x % 32;
+  if (x < 0 || (lane < p.W && x >= p.W)) {
+    *p.status = kErrIndex;
+    x = lane;
+  }
+  Parents r;
+  r.parent = static_cast<int>(x);
+  r.moves = r.parent != lane;
+  r.used = __reduce_or_sync(~0u, r.moves ? 1u << r.parent : 0u);
+  return r;
+}
+
+struct Strip {
+  const StateTensor* t;
+  long long group, begin;
+  int width;
+};
+__device__ __forceinline__ Strip strip_of(const StateTensors& s, long long item) {
+  const StateTensor& t = tensor_of(s, item);
+  unsigned rest;
+  Strip r;
+  r.t = &t;
+  r.group = divide(item - t.first, static_cast<unsigned>((t.row + t.strip - 1) / t.strip), &rest);
+  r.begin = static_cast<long long>(rest) * t.strip;
+  r.width = static_cast<int>(min(static_cast<long long>(t.strip), t.row - r.begin));
+  return r;
+}
+
 __global__ void __launch_bounds__(kRowThreads) reorder_kernel(const __grid_constant__ ReorderProblem p) {
-  extern __shared__ __align__(16) char strips[];
+  extern __shared__ __align__(128) unsigned char memory[];
+  __shared__ RingMemory rings;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  Ring ring(rings, memory, p.stage_bytes, p.status, kSiteReorder);
+  __syncthreads();
+  griddep_wait();
+  if (warp < p.copy_warps) {
+    long long item = first_item(), ahead = 0;      // ahead: the lane's parent in the next item
+    const long long step = static_cast<long long>(p.copy_warps) * gridDim.x;
+    if (item < p.bulk_items) ahead = parent_of(p, strip_of(p.bulk, item).group);
+    Strip x;
+    Parents r;
+    int done = 0, width = 0;
+    x.width = 0;
+    ring.run([&](int s, LaneCopy* c) {
+      while (done >= x.width) {
+        if (item >= p.bulk_items) return false;
+        x = strip_of(p.bulk, item);
+        r = parents_of(p, ahead);
+        item += step;
+        if (item < p.bulk_items) ahead = parent_of(p, strip_of(p.bulk, item).group);
+        const int reads = __popc(r.used);
+        done = reads ? 0 : x.width;
+        width = reads ? ring.stage_bytes / reads / 128 * 128 : 0;
+      }
+      const int n = min(width, x.width - done);
+      char* const row = x.t->data + x.group * x.t->group + lane * x.t->stride + x.begin + done;
+      ring.expect(s, __popc(r.used) * n);
+      if ((r.used >> lane) & 1) bulk_g2s(ring.stage(s) + r.place(lane) * width, row, n, ring.full + s);
+      *c = LaneCopy{row, smem_u32(ring.stage(s) + r.place(r.parent) * width), r.moves ? static_cast<uint32_t>(n) : 0u};
+      done += n;
+      return true;
+    });
+    return;
+  }
+  if (warp < kCopyWarps) return;
+  // The others: a column of units for each lane, which has all rows of it in its own places of shared memory before it writes one.
+  unsigned char* const own = memory + kStages * p.copy_warps * p.stage_bytes + (warp - kCopyWarps) * p.W * 32 * 8;
+  for (long long item = static_cast<long long>(blockIdx.x) * kPlainWarps + warp - kCopyWarps; item < p.plain_items; item += static_cast<long long>(gridDim.x) * kPlainWarps) {
+    const Strip x = strip_of(p.plain, item);
+    const Parents r = parents_of(p, parent_of(p, x.group));
+    const uint32_t moved = __ballot_sync(~0u, r.moves);
+    char* const rows = x.t->data + x.group * x.t->group + x.begin;
+    with_unit(x.t->unit, [&](auto u) {
+      using T = typename decltype(u)::T;
+      T* const mine = reinterpret_cast<T*>(own) + lane;
+      for (int c = lane; c < (x.width / static_cast<int>(sizeof(T)) + 31) / 32 * 32; c += 32) {
+        const bool in = c < x.width / static_cast<int>(sizeof(T));
+        int n = 0;
+        for (uint32_t m = r.used; m; m &= m - 1, ++n)
+          if (in) fetch(mine + n * 32, reinterpret_cast<const T*>(rows + (__ffs(m) - 1) * x.t->stride) + c);
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        for (uint32_t m = moved; m; m &= m - 1) {
+          const int row = __ffs(m) - 1, from = r.place(__shfl_sync(~0u, r.parent, row));
+          if (in) reinterpret_cast<T*>(rows + row * x.t->stride)[c] = mine[from * 32];
+        }
+      }
+    });
+  }
+}
+
+// Groups of more than 32 rows: an item for each CTA, all of its threads.
+__global__ void __launch_bounds__(kRowThreads) reorder_wide_kernel(const __grid_constant__ ReorderProblem p) {
+  extern __shared__ __align__(128) unsigned char memory[];
   __shared__ int used[kMostBeams], sources[kMostBeams], to[kMostBeams], from[kMostBeams];
   const int tid = threadIdx.x;
-  const StateTensor& t = tensor_of(p.s, blockIdx.x);
-  const long long item = blockIdx.x - t.first, per = (t.row + t.strip - 1) / t.strip;
-  const long long b = item / per, begin = item % per * t.strip;
-  const int width = static_cast<int>(min(static_cast<long long>(t.strip), t.row - begin));
-
-  long long parent = tid < p.W ? index_at(p.parents, p.parents64, b * p.W + tid) : tid;
+  griddep_wait();
+  const Strip x = strip_of(p.plain, blockIdx.x);
+  long long parent = tid < p.W ? index_at(p.parents, p.parents64, x.group * p.W + tid) : tid;
   if (parent < 0 || (tid < p.W && parent >= p.W)) {
     *p.status = kErrIndex;
     parent = tid;
@@ -126,28 +325,31 @@ __global__ void __launch_bounds__(kRowThreads) reorder_kernel(const __grid_const
     from[at & 0xffff] = used[parent];
   }
   const int n = both & 0xffff, reads = static_cast<int>(both >> 16);
-  char* const rows = t.data + b * t.group + begin;
-  with_unit(t.unit, [&](auto u) {
+  char* const rows = x.t->data + x.group * x.t->group + x.begin;
+  with_unit(x.t->unit, [&](auto u) {
     using T = typename decltype(u)::T;
-    const int columns = width / static_cast<int>(sizeof(T));
-    T* const mine = reinterpret_cast<T*>(strips);
+    const int columns = x.width / static_cast<int>(sizeof(T));
+    T* const mine = reinterpret_cast<T*>(memory);
     for (int i = tid; i < reads * columns; i += kRowThreads)
-      fetch(mine + i, reinterpret_cast<const T*>(rows + sources[i / columns] * t.stride) + i % columns);
+      fetch(mine + i, reinterpret_cast<const T*>(rows + sources[i / columns] * x.t->stride) + i % columns);
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
     for (int i = tid; i < n * columns; i += kRowThreads)
-      reinterpret_cast<T*>(rows + to[i / columns] * t.stride)[i % columns] = mine[from[i / columns] * columns + i % columns];
+      reinterpret_cast<T*>(rows + to[i / columns] * x.t->stride)[i % columns] = mine[from[i / columns] * columns + i % columns];
   });
 }
 
 // ------------------------------------------------------------------------------------------------------------------
 // Fork and compact: a list of rows that are read and rows that are written, none of them both
 // ------------------------------------------------------------------------------------------------------------------
+constexpr int kGroupSlots = 4096, kGroupEntries = 1024, kMostTargets = 8;      // moves are put together by their source up to here; of one load
+
 struct PoolProblem {
-  StateTensors s;
-  long long strips;                 // of all tensors' rows
+  StateTensors bulk, plain;
+  long long bulk_strips, plain_strips;      // of all tensors' rows
   const uint8_t* live;
-  int slots;
+  int slots, stage_bytes;               // (a strip of a bulk row is a stage)
+  int* status;
   // fork
   const void* source;
   int source64, n;
@@ -156,42 +358,74 @@ struct PoolProblem {
   // compact
   long long *place, *live_count;
 };
+// shared memory: the ring, a strip of zeros (fork), lists
+__host__ __device__ constexpr int fork_list_bytes(int slots, int n) {
+  return 8 * n + (slots <= kGroupSlots && n <= kGroupEntries ? 4 * (slots + 2) + 14 * n + 8 : 0);
+}
 
-// Strip after strip of every move: the rows that share a source read the same strip of it at about the same time, from L2 all but once.
-template <typename Src, typename Dst>
-__device__ __forceinline__ void copy_rows(const PoolProblem& p, int moves, Src src, Dst dst) {
-  for (long long item = blockIdx.x; item < p.strips * moves; item += gridDim.x) {
-    const long long strip = item / moves;
-    const int m = static_cast<int>(item % moves);
-    const StateTensor& t = tensor_of(p.s, strip);
-    const long long begin = (strip - t.first) * t.strip;
-    const int width = static_cast<int>(min(static_cast<long long>(t.strip), t.row - begin));
-    const long long s = src(m);
-    with_unit(t.unit, [&](auto u) {
+// `chunks` of moves: row src(i) goes to rows dst(i, 0 ... len(i) - 1); `moves` single ones for rows that are not of 16-byte multiples.
+// Strip after strip of every chunk: rows that share a source read the same strip of it at about the same time.
+template <typename Src, typename Len, typename Dst, typename From, typename To>
+__device__ __forceinline__ void copy_rows(const PoolProblem& p, Ring& ring, const unsigned char* zeros, int chunks, Src src, Len len, Dst dst, int moves, From from, To to) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  auto strip = [](const StateTensors& s, long long i) {
+    const StateTensor& t = tensor_of(s, i);
+    const long long begin = (i - t.first) * t.strip;
+    return Strip{&t, 0, begin, static_cast<int>(min(static_cast<long long>(t.strip), t.row - begin))};
+  };
+  if (warp < kCopyWarps) {
+    long long item = first_item();
+    ring.run([&](int s, LaneCopy* out) {
+      if (item >= p.bulk_strips * chunks) return false;
+      unsigned c;
+      const Strip x = strip(p.bulk, divide(item, chunks, &c));
+      item += kCopyWarps * gridDim.x;
+      const long long row = src(c);
+      if (row >= 0) {
+        ring.expect(s, x.width);
+        if (lane == 0) bulk_g2s(ring.stage(s), x.t->data + row * x.t->stride + x.begin, x.width, ring.full + s);
+      }
+      *out = LaneCopy{nullptr, 0, 0};
+      if (lane < len(c)) *out = LaneCopy{x.t->data + static_cast<long long>(dst(c, lane)) * x.t->stride + x.begin, smem_u32(row < 0 ? zeros : ring.stage(s)), static_cast<uint32_t>(x.width)};
+      return true;
+    });
+    return;
+  }
+  for (long long item = static_cast<long long>(blockIdx.x) * kPlainWarps + warp - kCopyWarps; item < p.plain_strips * moves; item += static_cast<long long>(gridDim.x) * kPlainWarps) {
+    unsigned m;
+    const Strip x = strip(p.plain, divide(item, moves, &m));
+    const long long row = from(m);
+    with_unit(x.t->unit, [&](auto u) {
       using T = typename decltype(u)::T;
-      constexpr int kAhead = 4;
-      const int columns = width / static_cast<int>(sizeof(T));
-      const T* const in = reinterpret_cast<const T*>(t.data + s * t.stride + begin);
-      T* const out = reinterpret_cast<T*>(t.data + dst(m) * t.stride + begin);
-      for (int c = threadIdx.x; c < columns; c += kAhead * kRowThreads) {
-        T x[kAhead];
+      constexpr int kAhead = 8;
+      const int columns = x.width / static_cast<int>(sizeof(T));
+      const T* const in = reinterpret_cast<const T*>(x.t->data + row * x.t->stride + x.begin);
+      T* const out = reinterpret_cast<T*>(x.t->data + static_cast<long long>(to(m)) * x.t->stride + x.begin);
+      for (int c = lane; c < columns; c += kAhead * 32) {
+        T y[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-          x[i] = T{};
-          if (s >= 0 && c + i * kRowThreads < columns) x[i] = in[c + i * kRowThreads];
+          y[i] = T{};
+          if (row >= 0 && c + i * 32 < columns) y[i] = in[c + i * 32];
         }
 #pragma unroll
         for (int i = 0; i < kAhead; ++i)
-          if (c + i * kRowThreads < columns) out[c + i * kRowThreads] = x[i];
+          if (c + i * 32 < columns) out[c + i * 32] = y[i];
       }
     });
   }
 }
 
-__global__ void __launch_bounds__(kRowThreads, kRowCtas) fork_kernel(const __grid_constant__ PoolProblem p) {
-  extern __shared__ int lists[];
-  int *const slot = lists, *const src = lists + p.n;
+__global__ void __launch_bounds__(kRowThreads) fork_kernel(const __grid_constant__ PoolProblem p) {
+  extern __shared__ __align__(128) unsigned char memory[];
+  __shared__ RingMemory rings;
+  Ring ring(rings, memory, p.stage_bytes, p.status, kSiteCopy);
+  unsigned char* const zeros = memory + kStages * kCopyWarps * p.stage_bytes;
+  int *const slot = reinterpret_cast<int*>(zeros + p.stage_bytes), *const src = slot + p.n;
   const int tid = threadIdx.x;
+  for (int i = tid; i < p.stage_bytes / 16; i += kRowThreads) reinterpret_cast<uint4*>(zeros)[i] = make_uint4(0, 0, 0, 0);
+  fence_proxy_async();
+  griddep_wait();
   // the lowest n free slots
   const int each = (p.slots + kRowThreads - 1) / kRowThreads, s0 = min(p.slots, tid * each), s1 = min(p.slots, s0 + each);
   int free = 0;
@@ -228,13 +462,52 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) fork_kernel(const __gri
     for (int s = s0; s < s1; ++s) p.after[s] = p.live[s] || at++ < moves;
   }
   __syncthreads();
-  copy_rows(p, moves, [&](int m) { return static_cast<long long>(src[m]); }, [&](int m) { return static_cast<long long>(slot[m]); });
+  auto from = [&](int m) { return static_cast<long long>(src[m]); };
+  auto to = [&](int m) { return slot[m]; };
+  if (p.slots > kGroupSlots || p.n > kGroupEntries) {
+    copy_rows(p, ring, zeros, moves, from, [](int) { return 1; }, [&](int c, int) { return slot[c]; }, moves, from, to);
+    return;
+  }
+  // Together by their source, so that it is read once for up to kMostTargets of them: places by counting, in every CTA the same.
+  int2* const chunk = reinterpret_cast<int2*>((reinterpret_cast<uintptr_t>(src + p.n) + 7) / 8 * 8);      // source; first place and how many
+  int* const count = reinterpret_cast<int*>(chunk + p.n);                                                 // [slots + 1], by source + 1
+  uint16_t *const order = reinterpret_cast<uint16_t*>(count + p.slots + 1), *const rank = order + p.n;
+  for (int s = tid; s <= p.slots; s += kRowThreads) count[s] = 0;
+  __syncthreads();
+  for (int m = tid; m < moves; m += kRowThreads) {
+    const int of = src[m];
+    int earlier = 0;
+#pragma unroll 8
+    for (int j = 0; j < m; ++j) earlier += src[j] == of;
+    rank[m] = static_cast<uint16_t>(earlier);
+    atomicAdd(count + of + 1, 1);
+  }
+  __syncthreads();
+  const int keys = p.slots + 1, share = (keys + kRowThreads - 1) / kRowThreads, k0 = min(keys, tid * share), k1 = min(keys, k0 + share);
+  unsigned sums = 0;      // places and chunks of the sources in front
+  for (int k = k0; k < k1; ++k) sums += count[k] | ((count[k] + kMostTargets - 1) / kMostTargets) << 16;
+  sums = block_scan(sums, &total);
+  const int chunks = total >> 16;
+  for (int k = k0; k < k1; ++k) {
+    const int c = count[k];
+    for (int i = 0; i < c; i += kMostTargets) chunk[(sums >> 16) + i / kMostTargets] = make_int2(k - 1, ((sums & 0xffff) + i) << 8 | min(kMostTargets, c - i));
+    count[k] = sums & 0xffff;
+    sums += c | ((c + kMostTargets - 1) / kMostTargets) << 16;
+  }
+  __syncthreads();
+  for (int m = tid; m < moves; m += kRowThreads) order[count[src[m] + 1] + rank[m]] = static_cast<uint16_t>(slot[m]);
+  __syncthreads();
+  copy_rows(p, ring, zeros, chunks, [&](int c) { return static_cast<long long>(chunk[c].x); }, [&](int c) { return chunk[c].y & 0xff; },
+            [&](int c, int i) { return order[(chunk[c].y >> 8) + i]; }, moves, from, to);
 }
 
-__global__ void __launch_bounds__(kRowThreads, kRowCtas) compact_kernel(const __grid_constant__ PoolProblem p) {
-  extern __shared__ uint16_t rows[];
-  uint16_t *const src = rows, *const dst = rows + p.slots / 2;
+__global__ void __launch_bounds__(kRowThreads) compact_kernel(const __grid_constant__ PoolProblem p) {
+  extern __shared__ __align__(128) unsigned char memory[];
+  __shared__ RingMemory rings;
+  Ring ring(rings, memory, p.stage_bytes, p.status, kSiteCopy);
+  uint16_t *const src = reinterpret_cast<uint16_t*>(memory + kStages * kCopyWarps * p.stage_bytes), *const dst = src + p.slots / 2;
   const int tid = threadIdx.x;
+  griddep_wait();
   const int each = (p.slots + kRowThreads - 1) / kRowThreads, s0 = min(p.slots, tid * each), s1 = min(p.slots, s0 + each);
   unsigned live = 0, total;
   for (int s = s0; s < s1; ++s) live += p.live[s] != 0;
@@ -261,16 +534,18 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtas) compact_kernel(const __
     if (static_cast<unsigned>(s) % gridDim.x == blockIdx.x) p.place[s] = to;
   }
   if (blockIdx.x == 0 && tid == 0) *p.live_count = count;
-  copy_rows(p, moves, [&](int m) { return static_cast<long long>(src[m]); }, [&](int m) { return static_cast<long long>(dst[m]); });
+  auto from = [&](int m) { return static_cast<long long>(src[m]); };
+  auto to = [&](int m) { return dst[m]; };
+  copy_rows(p, ring, nullptr, moves, from, [](int) { return 1; }, [&](int c, int) { return dst[c]; }, moves, from, to);
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// The tensors [begin, ...) of a call that go into one launch; `groups`: how often each is counted.  Returns an error code.
-static int take_states(const LetheGdnStates* s, int count, int strip, long long groups, StateTensors* out, long long* items) {
+// The tensors of a call that go into one launch, with rows of 16-byte multiples or of others; `groups`: how often each is counted.
+static void take_states(const LetheGdnStates* s, int count, bool bulk, int strip, long long groups, StateTensors* out, long long* items) {
   long long n = 0;
-  out->count = count;
+  out->count = 0;
   for (int i = 0; i < count; ++i) {
-    StateTensor& t = out->t[i];
+    StateTensor t;
     t.data = static_cast<char*>(s[i].data);
     t.row = s[i].row_bytes;
     t.stride = s[i].stride;
@@ -278,12 +553,13 @@ static int take_states(const LetheGdnStates* s, int count, int strip, long long 
     const unsigned long long bits = reinterpret_cast<uintptr_t>(t.data) | t.row | t.stride | t.group;
     t.unit = 16;
     while (bits % t.unit) t.unit /= 2;
+    if ((t.unit == 16) != bulk) continue;
     t.strip = strip;
     t.first = n;
     n += groups * ((t.row + strip - 1) / strip);
+    out->t[out->count++] = t;
   }
   *items = n;
-  return kOk;
 }
 static int check_states(const LetheGdnStates* s, int count) {
   if (count < 0 || (count && !s)) return kErrNull;
@@ -293,17 +569,25 @@ static int check_states(const LetheGdnStates* s, int count) {
   }
   return kOk;
 }
-
-template <typename Launch>
-static int in_launches(const LetheGdnStates* states, int count, int strip, long long groups, Launch launch) {
+template <typename Launch> static int in_launches(const LetheGdnStates* states, int count, Launch launch) {
   for (int i = 0; i == 0 || i < count; i += kMostTensors) {
-    StateTensors s;
-    long long items;
-    take_states(states + i, count - i < kMostTensors ? count - i : kMostTensors, strip, groups, &s, &items);
-    const int rc = launch(s, items);
+    const int rc = launch(states + i, count - i < kMostTensors ? count - i : kMostTensors);
     if (rc != kOk) return rc;
   }
   return kOk;
+}
+constexpr int kPlainStrip = 2048;
+// bytes of a strip, `most` or halves of it, so that there are `items` of `rows` rows of every tensor
+static int balanced(const LetheGdnStates* s, int count, long long rows, int most, long long items) {
+  long long bytes = 0;
+  for (int i = 0; i < count; ++i) bytes += rows * s[i].row_bytes;
+  int strip = most;
+  while (strip >= 4096 && strip % 1024 == 0 && bytes / strip < items) strip /= 2;
+  return strip;
+}
+static unsigned ctas_for(long long bulk, long long plain, int sms) {
+  const long long p = (plain + kPlainWarps - 1) / kPlainWarps, n = bulk > p ? bulk : p;
+  return static_cast<unsigned>(n < 1 ? 1 : n < sms ? n : sms);
 }
 
 }  // namespace lg
@@ -316,49 +600,73 @@ extern "C" int lethe_gdn_reorder_states(const LetheGdnStates* states, int32_t co
   if (bad) return bad;
   if (B <= 0 || W <= 0 || W > kMostBeams || B > (1ll << 30)) return kErrDims;
   if (reinterpret_cast<uintptr_t>(parents) % (parents_64 ? 8 : 4)) return kErrAlign;
-  int strip = 128;
-  while (strip < kCopyStrip && 2 * strip * W <= kReorderBytes) strip *= 2;
   for (int i = 0; i < count; ++i)
-    if ((states[i].row_bytes + strip - 1) / strip > (1ll << 30) / kMostTensors / B) return kErrDims;
+    if (states[i].row_bytes / 128 + 1 > (1ll << 30) / kMostTensors / B) return kErrDims;
   DeviceGuard guard(states[0].data);
   if (!guard.ok) return kErrDevice;
-  return in_launches(states, count, strip, B, [&](const StateTensors& s, long long items) {
-    ReorderProblem p;
-    p.s = s;
+  const int sms = sm_count();
+  if (sms <= 0) return kErrDevice;
+  static SmemAttr attr;
+  if (attr.set(reorder_kernel, kAllBytes)) return kErrLaunch;
+  const bool wide = W > 32;
+  return in_launches(states, count, [&](const LetheGdnStates* s, int n) {
+    ReorderProblem p = {};
     p.parents = parents;
     p.parents64 = parents_64;
     p.W = W;
     p.status = status;
-    reorder_kernel<<<static_cast<unsigned>(items), kRowThreads, kReorderBytes, static_cast<cudaStream_t>(stream)>>>(p);
-    return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (wide) {
+      int part = 128;
+      while (2 * part * W <= kGroupBytes) part *= 2;
+      long long more;
+      take_states(s, n, false, part, B, &p.plain, &p.plain_items);
+      StateTensors& all = p.plain;      // those of 16-byte multiples behind them
+      take_states(s, n, true, part, B, &p.bulk, &more);
+      for (int i = 0; i < p.bulk.count; ++i) {
+        all.t[all.count] = p.bulk.t[i];
+        all.t[all.count++].first += p.plain_items;
+      }
+      return launch_dependent(reorder_wide_kernel, dim3(static_cast<unsigned>(p.plain_items + more)), dim3(kRowThreads), kGroupBytes, st, p) == cudaSuccess ? kOk : kErrLaunch;
+    }
+    take_states(s, n, false, kPlainStrip, B, &p.plain, &p.plain_items);
+    const int plain_bytes = p.plain_items ? kPlainWarps * W * 32 * 8 : 0;      // (units of 8 bytes at most)
+    // fewer and larger rings for wide groups, whose strips share a stage; strips short enough for all rings
+    p.copy_warps = W <= 8 ? kCopyWarps : W <= 16 ? kCopyWarps / 2 : 1;
+    const int strip = balanced(s, n, B, 4 * kMostStage, 2LL * p.copy_warps * sms);
+    take_states(s, n, true, strip, B, &p.bulk, &p.bulk_items);
+    p.stage_bytes = p.bulk_items ? (kAllBytes - plain_bytes) / (kStages * p.copy_warps) / 512 * 512 : 0;
+    if (p.stage_bytes * p.copy_warps > kMostStage * kCopyWarps) p.stage_bytes = kMostStage * kCopyWarps / p.copy_warps;
+    return launch_dependent(reorder_kernel, dim3(ctas_for(p.bulk_items, p.plain_items, sms)), dim3(kRowThreads), kStages * p.copy_warps * p.stage_bytes + plain_bytes, st, p) == cudaSuccess ? kOk : kErrLaunch;
   });
 }
 
-static int pool_call(const LetheGdnStates* states, int count, long long slots, const uint8_t* live, lg::PoolProblem* p, bool fork, size_t smem,
-                     long long most, void* stream) {
+static int pool_call(const LetheGdnStates* states, int count, long long slots, const uint8_t* live, lg::PoolProblem* p, bool fork, int lists,
+                     long long most, int* status, void* stream) {
   using namespace lg;
   DeviceGuard guard(live);
   if (!guard.ok) return kErrDevice;
   const int sms = sm_count();
   if (sms <= 0) return kErrDevice;
   static SmemAttr attrs[2];
-  if (attrs[fork].set(fork ? fork_kernel : compact_kernel, fork ? 8 * kMostEntries : 2 * kMostSlots)) return kErrLaunch;
+  if (attrs[fork].set(fork ? fork_kernel : compact_kernel, kAllBytes)) return kErrLaunch;
   p->live = live;
   p->slots = static_cast<int>(slots);
-  return in_launches(states, count, kCopyStrip, 1, [&](const StateTensors& s, long long strips) {
-    p->s = s;
-    p->strips = strips;
-    const long long items = strips * most, ctas = static_cast<long long>(kRowCtas) * sms;
-    const unsigned grid = static_cast<unsigned>(items < 1 ? 1 : items < ctas ? items : ctas);
-    (fork ? fork_kernel : compact_kernel)<<<grid, kRowThreads, smem, static_cast<cudaStream_t>(stream)>>>(*p);
-    return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
+  p->status = status;
+  const int stages = kStages * kCopyWarps + (fork ? 1 : 0), room = (kAllBytes - lists) / stages / 512 * 512;
+  return in_launches(states, count, [&](const LetheGdnStates* s, int n) {
+    p->stage_bytes = balanced(s, n, most, room < kMostStage ? room : kMostStage, 2LL * kCopyWarps * sms);
+    take_states(s, n, true, p->stage_bytes, 1, &p->bulk, &p->bulk_strips);
+    take_states(s, n, false, kPlainStrip, 1, &p->plain, &p->plain_strips);
+    const unsigned grid = ctas_for(p->bulk_strips * most, p->plain_strips * most, sms);
+    return launch_dependent(fork ? fork_kernel : compact_kernel, dim3(grid), dim3(kRowThreads), stages * p->stage_bytes + lists, static_cast<cudaStream_t>(stream), *p) == cudaSuccess ? kOk : kErrLaunch;
   });
 }
 
 extern "C" int lethe_gdn_fork_states(const LetheGdnStates* states, int32_t count, int64_t slots, const uint8_t* live, const void* source,
-                                     int32_t source_64, int64_t n, int64_t* target, uint8_t* live_after, void* stream) {
+                                     int32_t source_64, int64_t n, int64_t* target, uint8_t* live_after, int32_t* status, void* stream) {
   using namespace lg;
-  if (!live || !source || !target || !live_after) return kErrNull;
+  if (!live || !source || !target || !live_after || !status) return kErrNull;
   const int bad = check_states(states, count);
   if (bad) return bad;
   if (slots <= 0 || slots > kMostSlots || n <= 0 || n > kMostEntries) return kErrDims;
@@ -369,13 +677,13 @@ extern "C" int lethe_gdn_fork_states(const LetheGdnStates* states, int32_t count
   p.n = static_cast<int>(n);
   p.target = reinterpret_cast<long long*>(target);
   p.after = live_after;
-  return pool_call(states, count, slots, live, &p, true, 8 * static_cast<size_t>(n), n < slots ? n : slots, stream);
+  return pool_call(states, count, slots, live, &p, true, fork_list_bytes(static_cast<int>(slots), p.n), n < slots ? n : slots, status, stream);
 }
 
 extern "C" int lethe_gdn_compact_states(const LetheGdnStates* states, int32_t count, int64_t slots, const uint8_t* live, int64_t* place,
-                                        int64_t* live_count, void* stream) {
+                                        int64_t* live_count, int32_t* status, void* stream) {
   using namespace lg;
-  if (!live || !place || !live_count) return kErrNull;
+  if (!live || !place || !live_count || !status) return kErrNull;
   const int bad = check_states(states, count);
   if (bad) return bad;
   if (slots <= 0 || slots > kMostSlots) return kErrDims;
@@ -383,5 +691,5 @@ extern "C" int lethe_gdn_compact_states(const LetheGdnStates* states, int32_t co
   PoolProblem p = {};
   p.place = reinterpret_cast<long long*>(place);
   p.live_count = reinterpret_cast<long long*>(live_count);
-  return pool_call(states, count, slots, live, &p, false, 2 * static_cast<size_t>(slots), slots / 2, stream);
+  return pool_call(states, count, slots, live, &p, false, 2 * static_cast<int>(slots), slots / 2, status, stream);
 }

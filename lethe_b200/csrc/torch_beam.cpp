@@ -196,7 +196,7 @@ std::pair<Tensor, Tensor> fork_states(const std::vector<Tensor>& states, const T
     if (n == 0) return {target, live.clone()};
     Tensor after = at::empty({S}, live.options());
     check(lethe_gdn_fork_states(r.s.data(), static_cast<int32_t>(r.s.size()), S, ptr<uint8_t>(live), ptr(source), source.scalar_type() == at::kLong, n,
-                                ptr<int64_t>(target), ptr<uint8_t>(after), stream_of(live)));
+                                ptr<int64_t>(target), ptr<uint8_t>(after), status_word(live.device().index()), stream_of(live)));
     changed(r);
     return {target, after};
   });
@@ -210,7 +210,8 @@ std::pair<Tensor, Tensor> compact_states(const std::vector<Tensor>& states, cons
     const Rows r = rows_of(states, live_in, 1, S, false, "states [slots, ...] for live [slots]");
     const Tensor live = apart(live_in, r);
     Tensor place = at::empty({S}, live.options().dtype(at::kLong)), count = at::empty({}, live.options().dtype(at::kLong));
-    check(lethe_gdn_compact_states(r.s.data(), static_cast<int32_t>(r.s.size()), S, ptr<uint8_t>(live), ptr<int64_t>(place), ptr<int64_t>(count), stream_of(live)));
+    check(lethe_gdn_compact_states(r.s.data(), static_cast<int32_t>(r.s.size()), S, ptr<uint8_t>(live), ptr<int64_t>(place), ptr<int64_t>(count),
+                                   status_word(live.device().index()), stream_of(live)));
     changed(r);
     return {place, count};
   });

@@ -25,8 +25,8 @@ def lib():
     L = native.lib()
     L.lethe_gdn_beam_work_bytes.restype, L.lethe_gdn_beam_work_bytes.argtypes = Z, [I64, I32, I64, I32, I32]
     L.lethe_gdn_reorder_states.argtypes = [P, I32, I64, I32, P, I32, P, P]
-    L.lethe_gdn_fork_states.argtypes = [P, I32, I64, P, P, I32, I64, P, P, P]
-    L.lethe_gdn_compact_states.argtypes = [P, I32, I64, P, P, P, P]
+    L.lethe_gdn_fork_states.argtypes = [P, I32, I64, P, P, I32, I64, P, P, P, P]
+    L.lethe_gdn_compact_states.argtypes = [P, I32, I64, P, P, P, P, P]
     L.lethe_gdn_decode_step_from.argtypes = [P, I64, P, I32, P, P, P]
     return L
 
@@ -82,8 +82,8 @@ def test_reorder_states(lib):
 
 
 def test_fork_states(lib):
-    call = lambda s=ONE, n=1, S=8, live=0x20000, src=0x30000, s64=1, e=3, t=0x40000, after=0x50000: lib.lethe_gdn_fork_states(s, n, S, live, src, s64, e, t, after, None)      # noqa: E731
-    for bad in (dict(s=None), dict(live=None), dict(src=None), dict(t=None), dict(after=None), dict(n=-1)):
+    call = lambda s=ONE, n=1, S=8, live=0x20000, src=0x30000, s64=1, e=3, t=0x40000, after=0x50000, status=0x60000: lib.lethe_gdn_fork_states(s, n, S, live, src, s64, e, t, after, status, None)      # noqa: E731
+    for bad in (dict(s=None), dict(live=None), dict(src=None), dict(t=None), dict(after=None), dict(status=None), dict(n=-1)):
         refused(lib, call(**bad), b"null")
     for bad in (dict(S=0), dict(S=65537), dict(e=0), dict(e=4097), dict(s=(States * 1)(States(0x10000, 0, 64, 0)))):
         refused(lib, call(**bad), b"sizes")
@@ -92,8 +92,8 @@ def test_fork_states(lib):
 
 
 def test_compact_states(lib):
-    call = lambda s=ONE, n=1, S=8, live=0x20000, place=0x30000, count=0x40000: lib.lethe_gdn_compact_states(s, n, S, live, place, count, None)      # noqa: E731
-    for bad in (dict(s=None), dict(live=None), dict(place=None), dict(count=None), dict(n=-1)):
+    call = lambda s=ONE, n=1, S=8, live=0x20000, place=0x30000, count=0x40000, status=0x50000: lib.lethe_gdn_compact_states(s, n, S, live, place, count, status, None)      # noqa: E731
+    for bad in (dict(s=None), dict(live=None), dict(place=None), dict(count=None), dict(status=None), dict(n=-1)):
         refused(lib, call(**bad), b"null")
     for bad in (dict(S=0), dict(S=65537)):
         refused(lib, call(**bad), b"sizes")
