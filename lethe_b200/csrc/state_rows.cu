@@ -17,7 +17,7 @@ constexpr int kMostBeams = 256, kMostSlots = 65536, kMostEntries = 4096;
 constexpr int kGroupBytes = 32768;          // a wide group's strips
 // Stages of a ring: as many strips on their way in as out.  With half the strips on their way out a compaction of 518 MB took 101 us for NNN.
 constexpr int kStages = 6, kOut = kStages / 2;
-constexpr int kAllBytes = 218112, kMostStage = 8192;      // dynamic shared memory of a CTA; bytes of a stage where there are four rings
+constexpr int kAllBytes = 208896, kMostStage = 8192;      // dynamic shared memory of a CTA; bytes of a stage where there are four rings
 constexpr int kSiteReorder = 811, kSiteCopy = 812;
 
 struct StateTensor {
@@ -364,7 +364,7 @@ __host__ __device__ constexpr int fork_list_bytes(int slots, int n) {
 }
 
 // `chunks` of moves: row src(i) goes to rows dst(i, 0 ... len(i) - 1); `moves` single ones for rows that are not of 16-byte multiples.
-// Strip after strip of every chunk: rows that share a source read the same strip of it at about the same time.
+// The strips of a chunk one after another, so that the CTAs are near one another in memory.
 template <typename Src, typename Len, typename Dst, typename From, typename To>
 __device__ __forceinline__ void copy_rows(const PoolProblem& p, Ring& ring, const unsigned char* zeros, int chunks, Src src, Len len, Dst dst, int moves, From from, To to) {
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -377,8 +377,9 @@ __device__ __forceinline__ void copy_rows(const PoolProblem& p, Ring& ring, cons
     long long item = first_item();
     ring.run([&](int s, LaneCopy* out) {
       if (item >= p.bulk_strips * chunks) return false;
-      unsigned c;
-      const Strip x = strip(p.bulk, divide(item, chunks, &c));
+      unsigned i;
+      const int c = static_cast<int>(divide(item, static_cast<unsigned>(p.bulk_strips), &i));
+      const Strip x = strip(p.bulk, i);
       item += kCopyWarps * gridDim.x;
       const long long row = src(c);
       if (row >= 0) {
@@ -392,8 +393,9 @@ __device__ __forceinline__ void copy_rows(const PoolProblem& p, Ring& ring, cons
     return;
   }
   for (long long item = static_cast<long long>(blockIdx.x) * kPlainWarps + warp - kCopyWarps; item < p.plain_strips * moves; item += static_cast<long long>(gridDim.x) * kPlainWarps) {
-    unsigned m;
-    const Strip x = strip(p.plain, divide(item, moves, &m));
+    unsigned i;
+    const int m = static_cast<int>(divide(item, static_cast<unsigned>(p.plain_strips), &i));
+    const Strip x = strip(p.plain, i);
     const long long row = from(m);
     with_unit(x.t->unit, [&](auto u) {
       using T = typename decltype(u)::T;
@@ -426,21 +428,35 @@ __global__ void __launch_bounds__(kRowThreads) fork_kernel(const __grid_constant
   for (int i = tid; i < p.stage_bytes / 16; i += kRowThreads) reinterpret_cast<uint4*>(zeros)[i] = make_uint4(0, 0, 0, 0);
   fence_proxy_async();
   griddep_wait();
+  // marks and sources of pools that are not large come to shared memory at once: several passes go over them
+  __shared__ uint8_t marks[kGroupSlots];
+  __shared__ int sources[kGroupEntries];
+  const bool small = p.slots <= kGroupSlots && p.n <= kGroupEntries;
+  if (small) {
+    for (int s = tid; s < p.slots; s += kRowThreads) marks[s] = p.live[s];
+    for (int e = tid; e < p.n; e += kRowThreads) {
+      const long long s = index_at(p.source, p.source64, e);
+      sources[e] = s >= -1 && s < p.slots ? static_cast<int>(s) : -2;
+    }
+    __syncthreads();
+  }
+  const uint8_t* const live = small ? marks : p.live;
+  auto source = [&](int e) { return small ? sources[e] : index_at(p.source, p.source64, e); };
   // the lowest n free slots
   const int each = (p.slots + kRowThreads - 1) / kRowThreads, s0 = min(p.slots, tid * each), s1 = min(p.slots, s0 + each);
   int free = 0;
-  for (int s = s0; s < s1; ++s) free += !p.live[s];
+  for (int s = s0; s < s1; ++s) free += !live[s];
   unsigned frees, total;
   const int before = block_scan(free, &frees);
   int at = before;
   for (int s = s0; s < s1 && at < p.n; ++s)
-    if (!p.live[s]) slot[at++] = s;
+    if (!live[s]) slot[at++] = s;
   __syncthreads();
   // the entries that take one
   const int per = (p.n + kRowThreads - 1) / kRowThreads, e0 = min(p.n, tid * per), e1 = min(p.n, e0 + per);
   auto takes = [&](int e) {
-    const long long s = index_at(p.source, p.source64, e);
-    return s == -1 || (s >= 0 && s < p.slots && p.live[s]);
+    const long long s = source(e);
+    return s == -1 || (s >= 0 && s < p.slots && live[s]);
   };
   int mine = 0;
   for (int e = e0; e < e1; ++e) mine += takes(e);
@@ -451,7 +467,7 @@ __global__ void __launch_bounds__(kRowThreads) fork_kernel(const __grid_constant
     if (takes(e)) {
       if (at < moves) {
         got = slot[at];
-        src[at] = static_cast<int>(index_at(p.source, p.source64, e));
+        src[at] = static_cast<int>(source(e));
       }
       ++at;
     }
@@ -459,12 +475,12 @@ __global__ void __launch_bounds__(kRowThreads) fork_kernel(const __grid_constant
   }
   if (blockIdx.x == 0) {
     at = before;
-    for (int s = s0; s < s1; ++s) p.after[s] = p.live[s] || at++ < moves;
+    for (int s = s0; s < s1; ++s) p.after[s] = live[s] || at++ < moves;
   }
   __syncthreads();
   auto from = [&](int m) { return static_cast<long long>(src[m]); };
   auto to = [&](int m) { return slot[m]; };
-  if (p.slots > kGroupSlots || p.n > kGroupEntries) {
+  if (!small) {
     copy_rows(p, ring, zeros, moves, from, [](int) { return 1; }, [&](int c, int) { return slot[c]; }, moves, from, to);
     return;
   }
@@ -508,19 +524,26 @@ __global__ void __launch_bounds__(kRowThreads) compact_kernel(const __grid_const
   uint16_t *const src = reinterpret_cast<uint16_t*>(memory + kStages * kCopyWarps * p.stage_bytes), *const dst = src + p.slots / 2;
   const int tid = threadIdx.x;
   griddep_wait();
+  __shared__ uint8_t marks[kGroupSlots];
+  const bool small = p.slots <= kGroupSlots;
+  if (small) {
+    for (int s = tid; s < p.slots; s += kRowThreads) marks[s] = p.live[s];
+    __syncthreads();
+  }
+  const uint8_t* const live_at = small ? marks : p.live;
   const int each = (p.slots + kRowThreads - 1) / kRowThreads, s0 = min(p.slots, tid * each), s1 = min(p.slots, s0 + each);
   unsigned live = 0, total;
-  for (int s = s0; s < s1; ++s) live += p.live[s] != 0;
+  for (int s = s0; s < s1; ++s) live += live_at[s] != 0;
   block_scan(live, &total);
   const int count = total;
   // those behind the place of the last live slot to be, and the holes in front of it: as many of one as of the other
   unsigned both = 0;
-  for (int s = s0; s < s1; ++s) both += p.live[s] ? s >= count : (s < count ? 1u << 16 : 0u);
+  for (int s = s0; s < s1; ++s) both += live_at[s] ? s >= count : (s < count ? 1u << 16 : 0u);
   const unsigned before = block_scan(both, &total);
   const int moves = total & 0xffff;
   int leave = before & 0xffff, hole = before >> 16;
   for (int s = s0; s < s1; ++s) {
-    if (p.live[s]) {
+    if (live_at[s]) {
       if (s >= count) src[leave++] = static_cast<uint16_t>(s);
     } else if (s < count) {
       dst[hole++] = static_cast<uint16_t>(s);
@@ -530,7 +553,7 @@ __global__ void __launch_bounds__(kRowThreads) compact_kernel(const __grid_const
   leave = before & 0xffff;
   for (int s = s0; s < s1; ++s) {
     long long to = -1;
-    if (p.live[s]) to = s < count ? s : dst[leave++];
+    if (live_at[s]) to = s < count ? s : dst[leave++];
     if (static_cast<unsigned>(s) % gridDim.x == blockIdx.x) p.place[s] = to;
   }
   if (blockIdx.x == 0 && tid == 0) *p.live_count = count;

@@ -43,10 +43,13 @@ std::tuple<Tensor, Tensor, Tensor, OptTensor> beam_select(const Tensor& logits, 
     refuse_tangents({logits, scores, penalty_in});
     at::NoGradGuard no_grad;
     c10::cuda::CUDAGuard guard(logits.device());
-    const auto longs = logits.options().dtype(at::kLong);
-    Tensor best = at::empty({B, k}, logits.options().dtype(at::kFloat)), parents = at::empty({B, k}, longs), tokens = at::empty({B, k}, longs), ended;
-    if (eos) ended = at::empty({B, k}, logits.options().dtype(at::kBool));
-    const OptTensor ended_out = ended.defined() ? OptTensor(ended) : std::nullopt;
+    Parts all;
+    const int64_t n = B * k, at_best = all.reserve(4 * n), at_parents = all.reserve(8 * n), at_tokens = all.reserve(8 * n), at_ended = all.reserve(eos ? n : 0);
+    all.make(logits);
+    const int64_t shape_out[] = {B, k};
+    const Tensor best = all.part(at_best, shape_out, at::kFloat), parents = all.part(at_parents, shape_out, at::kLong), tokens = all.part(at_tokens, shape_out, at::kLong);
+    const Tensor ended = eos ? all.part(at_ended, shape_out, at::kBool) : Tensor();
+    const OptTensor ended_out = eos ? OptTensor(ended) : std::nullopt;
     if (B == 0) return {best, parents, tokens, ended_out};
     const Tensor x = lazy(logits) || !packed_from(logits, 2) ? as(logits, logits.scalar_type()) : logits;
     const Tensor s = as32(scores), pen = as32(penalty_in);
@@ -192,9 +195,11 @@ std::pair<Tensor, Tensor> fork_states(const std::vector<Tensor>& states, const T
     c10::cuda::CUDAGuard guard(live_in.device());
     const Rows r = rows_of(states, live_in, 1, S, false, "states [slots, ...] for live [slots]");
     const Tensor live = apart(live_in, r), source = apart(source_in, r);
-    Tensor target = at::empty({n}, live.options().dtype(at::kLong));
-    if (n == 0) return {target, live.clone()};
-    Tensor after = at::empty({S}, live.options());
+    if (n == 0) return {at::empty({n}, live.options().dtype(at::kLong)), live.clone()};
+    Parts all;
+    const int64_t at_target = all.reserve(8 * n), at_after = all.reserve(S);
+    all.make(live);
+    const Tensor target = all.part(at_target, {n}, at::kLong), after = all.part(at_after, {S}, at::kBool);
     check(lethe_gdn_fork_states(r.s.data(), static_cast<int32_t>(r.s.size()), S, ptr<uint8_t>(live), ptr(source), source.scalar_type() == at::kLong, n,
                                 ptr<int64_t>(target), ptr<uint8_t>(after), status_word(live.device().index()), stream_of(live)));
     changed(r);
@@ -209,7 +214,10 @@ std::pair<Tensor, Tensor> compact_states(const std::vector<Tensor>& states, cons
     c10::cuda::CUDAGuard guard(live_in.device());
     const Rows r = rows_of(states, live_in, 1, S, false, "states [slots, ...] for live [slots]");
     const Tensor live = apart(live_in, r);
-    Tensor place = at::empty({S}, live.options().dtype(at::kLong)), count = at::empty({}, live.options().dtype(at::kLong));
+    Parts all;
+    const int64_t at_place = all.reserve(8 * S), at_count = all.reserve(8);
+    all.make(live);
+    const Tensor place = all.part(at_place, {S}, at::kLong), count = all.part(at_count, {}, at::kLong);
     check(lethe_gdn_compact_states(r.s.data(), static_cast<int32_t>(r.s.size()), S, ptr<uint8_t>(live), ptr<int64_t>(place), ptr<int64_t>(count),
                                    status_word(live.device().index()), stream_of(live)));
     changed(r);

@@ -176,6 +176,23 @@ inline bool spans(const Tensor& a, const Tensor& b) {
   const auto x = span_of(a), y = span_of(b);
   return x.first < y.second && y.first < x.second;
 }
+// Several results in one allocation: bytes first, then tensors that are parts of them.  (An allocation costs the host about a microsecond.)
+struct Parts {
+  int64_t bytes = 0;
+  Tensor whole;
+  int64_t reserve(int64_t n) {
+    const int64_t at = bytes;
+    bytes += (n + 15) / 16 * 16;
+    return at;
+  }
+  void make(const Tensor& like) { whole = at::empty({bytes}, like.options().dtype(at::kByte)); }
+  Tensor part(int64_t at, at::IntArrayRef sizes, at::ScalarType dt) const {
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), c10::scalarTypeToTypeMeta(dt));
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    t.unsafeGetTensorImpl()->set_storage_offset(at / static_cast<int64_t>(c10::elementSize(dt)));
+    return t;
+  }
+};
 inline void need_index(const Tensor& t, const char* name) {
   if (t.scalar_type() != at::kInt && t.scalar_type() != at::kLong) fail(std::string(name) + " must be int32 or int64");
 }
