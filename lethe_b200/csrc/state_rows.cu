@@ -343,6 +343,7 @@ __global__ void __launch_bounds__(kRowThreads) reorder_wide_kernel(const __grid_
 // Fork and compact: a list of rows that are read and rows that are written, none of them both
 // ------------------------------------------------------------------------------------------------------------------
 constexpr int kGroupSlots = 4096, kGroupEntries = 1024, kMostTargets = 8;      // moves are put together by their source up to here; of one load
+constexpr double kTogetherBytes = 32e6;
 
 struct PoolProblem {
   StateTensors bulk, plain;
@@ -352,16 +353,14 @@ struct PoolProblem {
   int* status;
   // fork
   const void* source;
-  int source64, n;
+  int source64, n, together;            // together: moves of one source share its loads
   long long* target;
   uint8_t* after;
   // compact
   long long *place, *live_count;
 };
 // shared memory: the ring, a strip of zeros (fork), lists
-__host__ __device__ constexpr int fork_list_bytes(int slots, int n) {
-  return 8 * n + (slots <= kGroupSlots && n <= kGroupEntries ? 4 * (slots + 2) + 14 * n + 8 : 0);
-}
+constexpr int fork_list_bytes(int slots, int n, bool together) { return 8 * n + (together ? 4 * (slots + 2) + 14 * n + 8 : 0); }
 
 // `chunks` of moves: row src(i) goes to rows dst(i, 0 ... len(i) - 1); `moves` single ones for rows that are not of 16-byte multiples.
 // The strips of a chunk one after another, so that the CTAs are near one another in memory.
@@ -480,7 +479,7 @@ __global__ void __launch_bounds__(kRowThreads) fork_kernel(const __grid_constant
   __syncthreads();
   auto from = [&](int m) { return static_cast<long long>(src[m]); };
   auto to = [&](int m) { return slot[m]; };
-  if (!small) {
+  if (!p.together) {
     copy_rows(p, ring, zeros, moves, from, [](int) { return 1; }, [&](int c, int) { return slot[c]; }, moves, from, to);
     return;
   }
@@ -700,7 +699,11 @@ extern "C" int lethe_gdn_fork_states(const LetheGdnStates* states, int32_t count
   p.n = static_cast<int>(n);
   p.target = reinterpret_cast<long long*>(target);
   p.after = live_after;
-  return pool_call(states, count, slots, live, &p, true, fork_list_bytes(static_cast<int>(slots), p.n), n < slots ? n : slots, status, stream);
+  // What L2 holds may be read once for each target: the plan that puts moves together takes 2 us longer.
+  double bytes = 0;
+  for (int i = 0; i < count; ++i) bytes += static_cast<double>(n) * states[i].row_bytes;
+  p.together = bytes > kTogetherBytes && slots <= kGroupSlots && n <= kGroupEntries;
+  return pool_call(states, count, slots, live, &p, true, fork_list_bytes(static_cast<int>(slots), p.n, p.together), n < slots ? n : slots, status, stream);
 }
 
 extern "C" int lethe_gdn_compact_states(const LetheGdnStates* states, int32_t count, int64_t slots, const uint8_t* live, int64_t* place,
