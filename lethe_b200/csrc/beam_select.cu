@@ -90,12 +90,22 @@ __device__ __forceinline__ double exp_below(double t) {
   return t <= -700. ? 0. : __longlong_as_double(__double_as_longlong(e) + (static_cast<long long>(n) << 52));
 }
 
+// log(s) for s >= 1 in 64 bits: what fp32 says, and log(s e^-y) = log(1 + d) behind it, d below 2^-19
+__device__ __forceinline__ double log_above(double s) {
+  const double y = logf(static_cast<float>(s)), d = fma(s, exp_below(-y), -1.);
+  return y + (d - .5 * d * d);
+}
+
 // whether the beam goes on: one that does not offers nothing, or only itself
 __device__ __forceinline__ bool counts(const BeamProblem& p, int row) {
   const float pen = p.penalty ? p.penalty[row] : 1.f;
   return isfinite(p.scores[row]) && pen > 0.f && pen < INFINITY;
 }
 __device__ __forceinline__ bool goes_on(const BeamProblem& p, int row) { return counts(p, row) && !(p.finished && p.finished[row]); }
+
+__device__ __forceinline__ void fetch16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+}
 
 template <int TY> struct Row {
   using T = typename Elem<TY>::T;
@@ -116,42 +126,45 @@ template <int TY> struct Row {
   }
   __device__ __forceinline__ T least() const { return from_f32<TY>(-INFINITY); }
   __device__ __forceinline__ T at(int v) const { return v >= 0 && v < V && (!ok || ok[v]) ? x[v] : least(); }
-  // minus infinity in the place of what is not allowed of [v, v + N)
-  __device__ __forceinline__ void mask(Vec& r, int v) const {
-    const uint8_t* const m = ok + v;
-    uint32_t keep[N / 4];                         // a byte of ones for each allowed token
-    if (reinterpret_cast<uintptr_t>(m) % N == 0) {
-#pragma unroll
-      for (int i = 0; i < N / 4; ++i) keep[i] = __vcmpne4(reinterpret_cast<const uint32_t*>(m)[i], 0u);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N / 4; ++i) keep[i] = __vcmpne4(m[4 * i] | m[4 * i + 1] << 8 | m[4 * i + 2] << 16 | static_cast<uint32_t>(m[4 * i + 3]) << 24, 0u);
-    }
-    constexpr uint32_t kNone = TY == LETHE_F32 ? 0xff800000u : TY == LETHE_BF16 ? 0xff80ff80u : 0xfc00fc00u;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t k = N == 4 ? __byte_perm(keep[0], 0, i * 0x1111) : __byte_perm(keep[i / 2], 0, i % 2 ? 0x3322 : 0x1100);
-      r.w[i] = (r.w[i] & k) | (kNone & ~k);
-    }
-  }
-  // logits [v, v + N), minus infinity in the place of what is not there or not allowed; v + past is a multiple of N
-  template <bool MASK> __device__ __forceinline__ Vec load(int v) const {
+  __device__ __forceinline__ bool inside(int v) const { return v >= 0 && v <= V - N; }
+  __device__ __forceinline__ bool astride(int v) const { return !inside(v) && v > -N && v < V; }      // at an end of the row
+  static constexpr uint32_t kNone = TY == LETHE_F32 ? 0xff800000u : TY == LETHE_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+  static __device__ __forceinline__ Vec none() {
     Vec r;
-    if (v >= 0 && v <= V - N) {
-      r.load(x + v);
-      if (MASK) mask(r, v);
+    r.w[0] = r.w[1] = r.w[2] = r.w[3] = kNone;
+    return r;
+  }
+  // the mask's bytes for [v, v + N)
+  struct Marks {
+    uint32_t w[N / 4];
+  };
+  __device__ __forceinline__ Marks marks(int v) const {
+    const uint8_t* const m = ok + v;
+    Marks r;
+    if (reinterpret_cast<uintptr_t>(ok - past) % N == 0) {      // (every v + past is a multiple of N)
+#pragma unroll
+      for (int i = 0; i < N / 4; ++i) r.w[i] = reinterpret_cast<const uint32_t*>(m)[i];
     } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i) raw_put<TY, N>(r, i, at(v + i));
+      for (int i = 0; i < N / 4; ++i) r.w[i] = m[4 * i] | m[4 * i + 1] << 8 | m[4 * i + 2] << 16 | static_cast<uint32_t>(m[4 * i + 3]) << 24;
     }
     return r;
   }
-  // the same for vector n of a tile, by selections: n is not known to the compiler
-  template <bool MASK> __device__ __forceinline__ void edge(Vec (&x)[kVecs], int n, int v) const {
-    const Vec r = load<MASK>(v);
+  // minus infinity in the place of what is not allowed
+  static __device__ __forceinline__ void mask(Vec& r, const Marks& marks) {
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i)
-      if (i == n) x[i] = r;
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t b = __vcmpne4(marks.w[N == 4 ? 0 : i / 2], 0u);
+      const uint32_t k = N == 4 ? __byte_perm(b, 0, i * 0x1111) : __byte_perm(b, 0, i % 2 ? 0x3322 : 0x1100);
+      r.w[i] = (r.w[i] & k) | (kNone & ~k);
+    }
+  }
+  // logits [v, v + N) at an end of the row, one by one, minus infinity in the place of what is not there or not allowed
+  __device__ __forceinline__ Vec end(int v) const {
+    Vec r;
+#pragma unroll
+    for (int i = 0; i < N; ++i) raw_put<TY, N>(r, i, at(v + i));
+    return r;
   }
   // which of a lane's part of a tile are not below `floor`, one of them at least is not; the place of a bit's element
   static __device__ __forceinline__ uint32_t reaching(const Vec (&x)[kVecs], float floor) {
@@ -211,17 +224,26 @@ __global__ void __launch_bounds__(32 * kScanWarps, TY == LETHE_F32 ? 11 : kScanC
   auto fetch = [&](int j) {
     if (j < p.tiles) {
       uint4* const slot = ring + j % kDepth * kTile;
-      const int v = first + j * kTileLogits + lane * N;
-      if (v >= lane * N && v <= r.V - kTileLogits + lane * N) {
+      const int v0 = first + j * kTileLogits, v = v0 + lane * N;
+      auto copy = [&](int n) { fetch16(slot + n * 32, r.x + v + n * 32 * N); };
+      if (v0 >= 0 && v0 <= r.V - kTileLogits) {
 #pragma unroll
-        for (int n = 0; n < R::kVecs; ++n)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(slot + n * 32))), "l"(r.x + v + n * 32 * N) : "memory");
+        for (int n = 0; n < R::kVecs; ++n) copy(n);
       } else {
-#pragma unroll 1
+        bool ends = false;
+#pragma unroll
         for (int n = 0; n < R::kVecs; ++n) {
-          const typename R::Vec y = r.template load<MASK>(v + n * 32 * N);
-          slot[n * 32] = make_uint4(y.w[0], y.w[1], y.w[2], y.w[3]);
+          if (r.inside(v + n * 32 * N)) copy(n);
+          else slot[n * 32] = make_uint4(R::kNone, R::kNone, R::kNone, R::kNone);
+          ends |= r.astride(v + n * 32 * N);
         }
+        if (ends)
+#pragma unroll 1
+          for (int n = 0; n < R::kVecs; ++n)
+            if (r.astride(v + n * 32 * N)) {
+              const typename R::Vec y = r.end(v + n * 32 * N);
+              slot[n * 32] = make_uint4(y.w[0], y.w[1], y.w[2], y.w[3]);
+            }
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -237,13 +259,18 @@ __global__ void __launch_bounds__(32 * kScanWarps, TY == LETHE_F32 ? 11 : kScanC
   double s = 0.;
   for (int j = 0; j < p.tiles; ++j) {
     fetch(j + kDepth - 1);
+    const int v = first + j * kTileLogits + lane * N;
+    typename R::Marks marks[R::kVecs];
+    if (MASK)
+#pragma unroll
+      for (int n = 0; n < R::kVecs; ++n)
+        if (r.inside(v + n * 32 * N)) marks[n] = r.marks(v + n * 32 * N);
     asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
 #pragma unroll
     for (int n = 0; n < R::kVecs; ++n) {
       const uint4 y = ring[j % kDepth * kTile + n * 32];
       x[n].w[0] = y.x, x[n].w[1] = y.y, x[n].w[2] = y.z, x[n].w[3] = y.w;
-      const int v = first + j * kTileLogits + (n * 32 + lane) * N;
-      if (MASK && v >= 0 && v <= r.V - N) r.mask(x[n], v);
+      if (MASK && r.inside(v + n * 32 * N)) R::mask(x[n], marks[n]);
     }
     const float m = R::largest(x);
     tops[warp][j][lane] = from_f32<TY>(m);
@@ -327,16 +354,34 @@ __global__ void __launch_bounds__(32 * kScanWarps, TY == LETHE_F32 ? 11 : kScanC
     if (any) {
       const int bin = passed[i + lane];
       v = first + bin / 32 * kTileLogits + bin % 32 * N;
-      if (v >= 0 && v + (R::kVecs - 1) * 32 * N <= r.V - N) {
+      typename R::Marks marks[R::kVecs];
+      if (v >= 0 && v <= r.V - N - (R::kVecs - 1) * 32 * N) {
 #pragma unroll
-        for (int b = 0; b < R::kVecs; ++b) x[b].load(r.x + v + b * 32 * N);
-        if (MASK) {
-#pragma unroll
-          for (int b = 0; b < R::kVecs; ++b) r.mask(x[b], v + b * 32 * N);
+        for (int b = 0; b < R::kVecs; ++b) {
+          x[b].load(r.x + v + b * 32 * N);
+          if (MASK) marks[b] = r.marks(v + b * 32 * N);
         }
+        if (MASK)
+#pragma unroll
+          for (int b = 0; b < R::kVecs; ++b) R::mask(x[b], marks[b]);
       } else {
+#pragma unroll
+        for (int b = 0; b < R::kVecs; ++b) {
+          const int u = v + b * 32 * N;
+          x[b] = R::none();
+          if (r.inside(u)) {
+            x[b].load(r.x + u);
+            if (MASK) R::mask(x[b], r.marks(u));
+          }
+        }
 #pragma unroll 1
-        for (int b = 0; b < R::kVecs; ++b) r.template edge<MASK>(x, b, v + b * 32 * N);
+        for (int b = 0; b < R::kVecs; ++b)
+          if (r.astride(v + b * 32 * N)) {
+            const typename R::Vec y = r.end(v + b * 32 * N);
+#pragma unroll
+            for (int c = 0; c < R::kVecs; ++c)
+              if (c == b) x[c] = y;
+          }
       }
     }
     if (i == 0) {      // (while they come)
@@ -420,21 +465,17 @@ __device__ __forceinline__ int sort_largest(MergeMemory& m, int most) {
   __syncthreads();
   const int n = m.n, tid = threadIdx.x;
   // as many threads for an entry as there are; they count those that are larger
-  const int share = n <= 32 ? 16 : n <= 64 ? 8 : n <= 128 ? 4 : n <= 256 ? 2 : 1;
-  for (int i = tid / share; i < (n + 31) / 32 * 32; i += kMergeThreads / share) {      // (whole warps)
+  const int bits = n <= 32 ? 4 : n <= 64 ? 3 : n <= 128 ? 2 : n <= 256 ? 1 : 0, share = 1 << bits, part = tid & (share - 1);
+  for (int i = tid >> bits; i < (n + 31) / 32 * 32; i += kMergeThreads >> bits) {      // (whole warps)
     const Entry e = m.room[min(i, n - 1)];
     int before = 0;
 #pragma unroll 4
-    for (int j = tid % share; j < n; j += share) before += larger(m.room[j], e);
+    for (int j = part; j < n; j += share) before += larger(m.room[j], e);
     for (int d = share / 2; d; d >>= 1) before += __shfl_xor_sync(~0u, before, d);
-    if (i < n && before < most && tid % share == 0) m.sorted[before] = e;
+    if (i < n && before < most && part == 0) m.sorted[before] = e;
   }
   __syncthreads();
   return min(n, most);
-}
-
-__device__ __forceinline__ void fetch16(void* to, const void* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from) : "memory");
 }
 
 template <int TY>
@@ -492,7 +533,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamPro
     if (lane == 0) {
       m.on[w] = s > 0. && s < INFINITY && top < INFINITY;
       m.top[w] = top;
-      m.lse[w] = top * over + log(s);
+      m.lse[w] = top * over + log_above(s);
     }
   }
   auto rank = [&](int w, float x) { return (m.score[w] + (x * over - m.lse[w])) * m.inverse[w]; };
@@ -517,17 +558,15 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamPro
       constexpr int kShare = kMergeThreads / kBins;
       const int i = tid / kShare;
       const uint32_t b = reinterpret_cast<const uint32_t*>(m.bins)[i];
-      int before = 0;
-      auto count = [&](uint32_t o, int j) { before += (o > b) | ((o == b) & (j < i)); };
+      int reach = 0;
 #pragma unroll
       for (int k = 0; k < kBins / 4 / kShare; ++k) {
-        const int j = k * kShare + tid % kShare;
-        const uint4 o = m.bins[j];
-        count(o.x, 4 * j), count(o.y, 4 * j + 1), count(o.z, 4 * j + 2), count(o.w, 4 * j + 3);
+        const uint4 o = m.bins[k * kShare + tid % kShare];
+        reach += (o.x >= b) + (o.y >= b) + (o.z >= b) + (o.w >= b);
       }
 #pragma unroll
-      for (int d = kShare / 2; d; d >>= 1) before += __shfl_xor_sync(~0u, before, d);
-      if (before == most - 1 && tid % kShare == 0) m.least = b;
+      for (int d = kShare / 2; d; d >>= 1) reach += __shfl_xor_sync(~0u, reach, d);
+      if (reach >= most && tid % kShare == 0) atomicMax(&m.least, b);
     }
     __syncthreads();
     const uint32_t floor = max(m.least, 1u);
@@ -619,7 +658,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamPro
       if (tid == 0) {
         s = 0.;
         for (int i = 0; i < kMergeThreads / 32; ++i) s += m.part[i];
-        m.lse[w] = m.top[w] * over + log(s);
+        m.lse[w] = m.top[w] * over + log_above(s);
       }
       __syncthreads();
     }

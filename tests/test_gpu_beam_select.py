@@ -125,6 +125,20 @@ def test_layouts(layout, dtype):
     assert torch.equal(got.tokens, want.tokens)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [1019, 3001, 9001])
+def test_every_place_of_a_row_in_memory(V, dtype):
+    """Rows that begin and end at every distance from a 16-byte boundary, the largest logits at their ends."""
+    for past in range(8):
+        buffer = torch.full((2, 3, V + 16), 50.0, dtype=dtype, device="cuda")
+        x = buffer[..., past:past + V]
+        y, s = some(2, 3, V, dtype, past)
+        x.copy_(y)
+        x[..., 0], x[..., -1] = 9.0, 8.5
+        check(x, s, 6)
+        check(x, s, 6, allowed=torch.arange(V, device="cuda") % 3 != 1)
+
+
 def test_one_row_for_all_beams():
     x, _ = some(2, 1, 5000)
     scores = torch.tensor([[0.0, DEAD, DEAD], [0.0, DEAD, DEAD]], device="cuda")

@@ -231,6 +231,28 @@ def test_fork_one_for_many():
     assert same(t, t[:1].expand(64, 3000))
 
 
+@pytest.mark.parametrize("sources", [1, 3, 40])
+def test_fork_more_than_l2_holds_at_once(sources):
+    """Moves of one source share its loads: more, and fewer, than eight of them, zeros, and rows of no particular size beside them."""
+    S, n = 150, 90
+    live = torch.zeros(S, dtype=torch.bool, device="cuda")
+    live[torch.randperm(S, generator=gen(1), device="cuda")[:45]] = True
+    of = torch.cat([live.nonzero().flatten()[:sources], torch.tensor([-1, -2, S + 3], device="cuda"), (~live).nonzero().flatten()[:1]])
+    for seed in range(2):
+        source = of[torch.randint(0, len(of), (n,), generator=gen(seed), device="cuda")]
+        check_fork([values((S, 8, 128, 128), torch.float32), values((S, 7, 9), torch.bfloat16), values((S, 4, 128, 64), torch.float32)], live, source)
+
+
+@pytest.mark.parametrize("W", [9, 16, 17, 24, 32])
+def test_reorder_wide_groups_of_large_rows(W):
+    for seed, few in ((0, W), (1, 2)):
+        parents = torch.randint(0, few, (3, W), generator=gen(seed), device="cuda")
+        ts = [values((3 * W, 100000), torch.uint8), values((3, W, 4, 128, 64), torch.float32), values((3 * W, 999), torch.uint8)]
+        want = [reordered(t, parents) for t in ts]
+        ops.reorder_states(ts, parents)
+        assert all(same(a, b) for a, b in zip(ts, want))
+
+
 @pytest.mark.parametrize("S", [4096, 65535, 65536])
 def test_large_pools(S):
     live = torch.rand(S, generator=gen(S), device="cuda") < 0.5
