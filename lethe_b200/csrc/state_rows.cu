@@ -3,6 +3,10 @@
 // that somebody takes over once and writing every row that changes once.  Which rows those are stands on the device; every CTA works it
 // out for itself (bytes against megabytes) instead of waiting for a launch that does.
 //
+// Measured, a pass through the public call: reorder of 64 x 8 rows of 2 MB, 6 moved from 3 in each group (1.23 GB, 187 us at the copy rate) 218 us; 272 rows of
+// 2 MB forked from 32 and from zeros (0.65 GB, 98 us) 125 us; 128 rows moved (0.54 GB, 83 us) 93 us; a few small rows 5 to 7 us, which is
+// the host's time.  HBM moves what the rows have and no more (409 MB in and 757 out, 80 and 514, 272 and 218); two writes for a read run at 5.6 TB/s.
+//
 // Rows of 16-byte multiples go through shared memory by bulk copies, one CTA per SM: up to four warps issue them, each with a ring of its own,
 // and no thread touches the data.  Rows of other sizes go through registers in the other warps meanwhile.
 #include "elem.cuh"
@@ -15,7 +19,8 @@ constexpr int kRowThreads = 256, kCopyWarps = 4, kPlainWarps = kRowThreads / 32 
 constexpr int kMostTensors = 32;            // of one launch
 constexpr int kMostBeams = 256, kMostSlots = 65536, kMostEntries = 4096;
 constexpr int kGroupBytes = 32768;          // a wide group's strips
-// Stages of a ring: as many strips on their way in as out.  With half the strips on their way out a compaction of 518 MB took 101 us for NNN.
+// Stages of a ring: as many strips on their way in as out.  A compaction of 543 MB (83 us at the copy rate) in us:
+// four rings of 8 KB strips 93, two of 16 KB 92, four of 2 KB 134, one of 16 KB with two strips on their way out 101, without rings, through registers, 98.
 constexpr int kStages = 6, kOut = kStages / 2;
 constexpr int kAllBytes = 208896, kMostStage = 8192;      // dynamic shared memory of a CTA; bytes of a stage where there are four rings
 constexpr int kSiteReorder = 811, kSiteCopy = 812;
@@ -343,7 +348,7 @@ __global__ void __launch_bounds__(kRowThreads) reorder_wide_kernel(const __grid_
 // Fork and compact: a list of rows that are read and rows that are written, none of them both
 // ------------------------------------------------------------------------------------------------------------------
 constexpr int kGroupSlots = 4096, kGroupEntries = 1024, kMostTargets = 8;      // moves are put together by their source up to here; of one load
-constexpr double kTogetherBytes = 32e6;
+constexpr double kTogetherBytes = 32e6;      // (272 rows of 2 MB: 140 us one by one, 125 together)
 
 struct PoolProblem {
   StateTensors bulk, plain;
@@ -699,7 +704,7 @@ extern "C" int lethe_gdn_fork_states(const LetheGdnStates* states, int32_t count
   p.n = static_cast<int>(n);
   p.target = reinterpret_cast<long long*>(target);
   p.after = live_after;
-  // What L2 holds may be read once for each target: the plan that puts moves together takes 2 us longer.
+  // What L2 holds may be read once for each target.
   double bytes = 0;
   for (int i = 0; i < count; ++i) bytes += static_cast<double>(n) * states[i].row_bytes;
   p.together = bytes > kTogetherBytes && slots <= kGroupSlots && n <= kGroupEntries;

@@ -733,7 +733,7 @@ def beam_select(logits: Tensor, scores: Tensor, k: int | None = None, *, tempera
     from) and ``tokens`` are int64.
 
     ``eos``: the token that ends a hypothesis; ``finished`` of the result is whether the parent was or the token is it.  A beam that
-    ``finished [B, W]`` marks offers itself, with its score, at the token ``eos``, and nothing else; its logits are not read.  A beam whose score is
+    ``finished [B, W]`` marks offers itself, with its score, at the token ``eos``, and nothing else, whatever its logits.  A beam whose score is
     not finite (``-inf``: not in use, as all but the first of equal ones at the start), whose penalty is not above zero and finite, or
     whose allowed logits are all ``-inf`` or hold NaN or ``+inf``, offers nothing.  Places that are left have score ``-inf``, parent 0, token ``eos`` or 0,
     and count as finished.
