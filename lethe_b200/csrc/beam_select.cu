@@ -539,10 +539,11 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamPro
     if (lane == 0) {
       m.on[w] = s > 0. && s < INFINITY && top < INFINITY;
       m.top[w] = top;
-      m.lse[w] = top * over + log_above(s);
+      m.lse[w] = __dmul_rn(top, over) + log_above(s);
     }
   }
-  auto rank = [&](int w, float x) { return (m.score[w] + (x * over - m.lse[w])) * m.inverse[w]; };
+  // (the products rounded by themselves: the one token of a beam that may say one only has log probability zero)
+  auto rank = [&](int w, float x) { return (m.score[w] + (__dmul_rn(x, over) - m.lse[w])) * m.inverse[w]; };
   auto entry = [&](int w, unsigned long long key) {
     return Entry{ordered(rank(w, from_ordered(static_cast<uint32_t>(key >> 32)))), ~(static_cast<unsigned long long>(w) << 32) ^ (~static_cast<uint32_t>(key))};
   };
@@ -642,7 +643,8 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamPro
         const double gap = from_ordered(a.rank) - from_ordered(m.sorted[j].rank);
         if (!(gap < far)) break;
         const int w = beam_of(m.sorted[j]);
-        if (gap > 0. && u != w && gap < kLseError * (m.inverse[u] + m.inverse[w])) m.again[u] = m.again[w] = close = true;
+        // (sums that differ may be rounded to the same; finished beams have none)
+        if (u != w && gap < kLseError * ((m.on[u] ? m.inverse[u] : 0.) + (m.on[w] ? m.inverse[w] : 0.))) m.again[u] = m.again[w] = close = true;
       }
       // as many equals behind the last of this beam's: another beam's may lie behind them
       if (j == most && p.W > 1) {
@@ -664,7 +666,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamPro
       if (tid == 0) {
         s = 0.;
         for (int i = 0; i < kMergeThreads / 32; ++i) s += m.part[i];
-        m.lse[w] = m.top[w] * over + log_above(s);
+        m.lse[w] = __dmul_rn(m.top[w], over) + log_above(s);
       }
       __syncthreads();
     }

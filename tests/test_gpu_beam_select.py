@@ -206,6 +206,20 @@ def test_beams_one_step_of_fp32_apart(V, k):
                 assert (values == row.sort(descending=True).values[i]).all()
 
 
+@pytest.mark.parametrize("V", [5, 700, 40000])
+def test_beams_that_are_all_but_sure(V):
+    """One token of every beam has all but 1e-7 to 1e-13 of the probability, which is nothing beside one in 32 bits, and decides."""
+    W = 12
+    for seed in range(3):
+        rest = -torch.rand(1, W, 1, generator=gen(seed), device="cuda") * 14 - 16 - math.log(V)
+        x = rest + torch.rand(1, W, V, generator=gen(seed + 5), device="cuda")
+        x.scatter_(2, torch.randint(0, V, (1, W, 1), generator=gen(seed + 9), device="cuda"), 1.0)
+        for scores in (torch.zeros(1, W, device="cuda"), torch.full((1, W), -7.0, device="cuda")):
+            check(x, scores, W)
+            check(x, scores, 5, finished=torch.arange(W, device="cuda")[None] % 5 == 2, eos=0)
+            check(x, scores, 20, penalty=torch.full((1, W), 1.7, device="cuda"))
+
+
 def test_equals_behind_the_cut_hide_another_beams():
     """Many equals of one beam around the last candidate, and one of another beam that lies between them by less than the sums are known."""
     V = 4000
@@ -233,6 +247,16 @@ def test_masks(V, dtype):
     check(x, s, 6, allowed=m[..., 3:V + 3])
     check(x, s, 6, allowed=(torch.rand(B, W, 2 * V, generator=gen(2), device="cuda") < 0.3)[..., ::2])
     check(x[..., 1:], s, 6, allowed=m[..., :V - 1])
+
+
+@pytest.mark.parametrize("temperature", [1.0, 0.9, 1.7])
+def test_masks_that_leave_one_token(temperature):
+    """Whose log probability is zero, so that the scores decide, and among equal ones the beam."""
+    x, _ = some(2, 9, 700, torch.float32)
+    m = torch.zeros(2, 9, 700, dtype=torch.bool, device="cuda").scatter_(2, torch.randint(0, 700, (2, 9, 1), generator=gen(8), device="cuda"), True)
+    for scores in (torch.zeros(2, 9, device="cuda"), torch.full((2, 9), -3.7, device="cuda"), -torch.arange(9, device="cuda").float().div(3).floor().expand(2, 9)):
+        got = check(x, scores, 9, allowed=m, temperature=temperature)
+        assert torch.equal(got.scores, scores) and torch.equal(got.parents[0], torch.arange(9, device="cuda"))
 
 
 def test_masks_that_leave_little_or_nothing():
