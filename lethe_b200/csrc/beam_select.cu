@@ -96,6 +96,27 @@ __device__ __forceinline__ double exp_below(double t) {
   return t <= -700. ? 0. : __longlong_as_double(__double_as_longlong(e) + (static_cast<long long>(n) << 52));
 }
 
+// The same by eighths of powers of two, roots[i] = 2^(i / 8): the seventh power of what is left is below 2^-43 of the result.  For many terms, so
+// without conversions to and from 64 bits, which the GPU has few units for: the whole number is read off a sum with 1.5 2^52.
+__device__ __forceinline__ double exp_below(double t, const double* roots) {
+  constexpr double kWhole = 6755399441055744.;
+  t = fmax(t, -700.);
+  const double m = fma(t, 8 * 1.4426950408889634, kWhole), n = m - kWhole;
+  const int k = static_cast<int>(__double2loint(m));
+  const double f = fma(n, -2.3190468138462996e-17 / 8, fma(n, -0.69314718055994529 / 8, t));
+  double e = 1. / 720.;
+  const double over[] = {1. / 120., 1. / 24., 1. / 6., .5, 1., 1.};
+#pragma unroll
+  for (int i = 0; i < 6; ++i) e = fma(e, f, over[i]);
+  e *= roots[k & 7];
+  return t <= -700. ? 0. : __hiloint2double(__double2hiint(e) + (k >> 3) * (1 << 20), __double2loint(e));
+}
+// x in 64 bits, where what is below the normal numbers is zero and minus infinity some number below -2^127
+__device__ __forceinline__ double widen(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return u & 0x7f800000u ? __hiloint2double(static_cast<int>((u & 0x80000000u) | (((u & 0x7fffffffu) >> 3) + (896u << 20))), static_cast<int>(u << 29)) : 0.;
+}
+
 // log(s) for s >= 1 in 64 bits: what fp32 says, and log(s e^-y) = log(1 + d) behind it, d below 2^-19
 __device__ __forceinline__ double log_above(double s) {
   const double y = logf(static_cast<float>(s)), d = fma(s, exp_below(-y), -1.);
@@ -459,6 +480,7 @@ struct MergeMemory {
   Entry room[kMergeRoom], sorted[kBins];
   uint4 bins[kBins / 4];
   double score[kBeamMost], inverse[kBeamMost], lse[kBeamMost], part[kMergeThreads / 32];      // inverse: 1 / penalty
+  double roots[8];
   float top[kBeamMost];
   int2 todo[kMergeThreads];             // list, beam
   uint32_t least;
@@ -652,13 +674,25 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamPro
         close = true;
       }
     }
+    if (tid < 8) m.roots[tid] = exp2(tid / 8.);
     if (!__syncthreads_or(close)) break;
     for (int w = 0; w < p.W; ++w) {
       if (!m.again[w] || !m.on[w]) continue;
       const Row<TY> r(p, row0 + w);
       double s = 0.;
-#pragma unroll 4
-      for (int v = tid; v < p.V; v += kMergeThreads) s += exp_below((static_cast<double>(to_f32(r.at(v))) - m.top[w]) * over);
+      constexpr int kAhead = 8;      // (by the token's number, wherever the row lies: equal rows have equal sums)
+      for (int v = tid; v < p.V; v += kAhead * kMergeThreads) {
+        float x[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {      // (no branch around a load: they are under way together)
+          const int u = min(v + i * kMergeThreads, p.V - 1);
+          const float l = to_f32(r.x[u]);
+          const bool in = (u == v + i * kMergeThreads) & (r.ok ? r.ok[u] != 0 : true);
+          x[i] = in ? l : -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) s += exp_below((widen(x[i]) - m.top[w]) * over, m.roots);
+      }
 #pragma unroll
       for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
       if (lane == 0) m.part[warp] = s;
