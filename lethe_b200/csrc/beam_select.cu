@@ -479,7 +479,8 @@ struct MergeMemory {
   ScanStat stat[kMergeThreads];
   Entry room[kMergeRoom], sorted[kBins];
   uint4 bins[kBins / 4];
-  double score[kBeamMost], inverse[kBeamMost], lse[kBeamMost], part[kMergeThreads / 32];      // inverse: 1 / penalty
+  double score[kBeamMost], penalty[kBeamMost], lse[kBeamMost], part[kMergeThreads / 32];
+  double inverse[kBeamMost];            // 1 / penalty, for how far ranks can be off; 0: the beam offers nothing
   double roots[8];
   float top[kBeamMost];
   int2 todo[kMergeThreads];             // list, beam
@@ -518,19 +519,22 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamPro
   if (tid < p.W) {      // (older than the scan, which has waited for what was before it when this kernel starts)
     const bool in = counts(p, row0 + tid), ended = p.finished && p.finished[row0 + tid];
     m.score[tid] = p.scores[row0 + tid];
-    m.inverse[tid] = in ? (p.penalty ? 1. / p.penalty[row0 + tid] : 1.) : 0.;
+    m.penalty[tid] = p.penalty ? p.penalty[row0 + tid] : 1.;
+    m.inverse[tid] = in ? 1. / m.penalty[tid] : 0.;
     m.on[tid] = in && !ended;
     m.ended[tid] = in && ended;
     m.again[tid] = false;
   }
   const int w_of_tid = tid / p.lists;
   auto beam_of_list = [&](int l) { return l == tid ? w_of_tid : l / p.lists; };
+  // (a product with 1 / penalty would be another number: 49 and 1 / 49 make less than one)
+  auto ranked = [&](int w, double c) { return p.penalty ? __ddiv_rn(c, m.penalty[w]) : c; };
   auto begin = [&] {      // finished beams offer themselves
     if (tid == 0) m.n = m.lists = m.least = 0;
     if (tid < kBins / 4) m.bins[tid] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     if (tid < p.W && m.ended[tid])
-      m.room[atomicAdd(&m.n, 1)] = Entry{ordered(m.score[tid] * m.inverse[tid]), ~(static_cast<unsigned long long>(tid) << 32 | static_cast<uint32_t>(p.eos))};
+      m.room[atomicAdd(&m.n, 1)] = Entry{ordered(ranked(tid, m.score[tid])), ~(static_cast<unsigned long long>(tid) << 32 | static_cast<uint32_t>(p.eos))};
   };
   begin();
   griddep_wait();
@@ -565,7 +569,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamPro
     }
   }
   // (the products rounded by themselves: the one token of a beam that may say one only has log probability zero)
-  auto rank = [&](int w, float x) { return (m.score[w] + (__dmul_rn(x, over) - m.lse[w])) * m.inverse[w]; };
+  auto rank = [&](int w, float x) { return ranked(w, m.score[w] + (__dmul_rn(x, over) - m.lse[w])); };
   auto entry = [&](int w, unsigned long long key) {
     return Entry{ordered(rank(w, from_ordered(static_cast<uint32_t>(key >> 32)))), ~(static_cast<unsigned long long>(w) << 32) ^ (~static_cast<uint32_t>(key))};
   };
