@@ -8,7 +8,7 @@
 // suffices: a warp takes a segment of a row, sums exponentials relative to the largest logit it has seen, and leaves the k largest of the
 // segment among a few more, in no order (beam_scan_kernel); a CTA per group adds up the sums and merges the lists (beam_merge_kernel).
 //
-// Between beams candidates can be as close as they like.  The sums are within kLseError of the formula (below); where two candidates of
+// Between beams candidates can be as close as they like.  The logarithms of the sums are within kLseError of the formula (below); where two candidates of
 // different beams that decide the result are closer than two such errors, the merge sums the exponentials of those beams again in 64 bits.
 //
 // Measured, a pass through the public call: 64 x 8 x 131072 bf16, k = 16 (134 MB, 20.5 us at the copy rate) 36 us, of it the scan 30 and the merge 5;
@@ -36,9 +36,14 @@ __host__ __device__ constexpr int list_room(int k) { return (k + kSpare + 1) / 2
 constexpr int kMergeThreads = 512, kBins = 128, kMergeRoom = 2 * kMergeThreads;
 constexpr int kMergeKeys = 4096;                  // of a group's lists, that are fetched before it is known which are wanted
 constexpr int kBehind = 8;                        // candidates behind the last chosen one that are looked at for equals
-// A term of a sum: exp2 by the hardware 2^-22; its argument t has two roundings of |t| 2^-24, which count with 2^t relative to the
-// largest term, |t| up to kSlack there, together below 2^-22; seven roundings of sums in 32 bits.  The rest is in 64 bits.
-constexpr double kLseError = 2 * 2.4e-7 + 7 * 6e-8;
+// How far the logarithm of a beam's sum can be off.  A term: exp2 by the hardware 2^-22; its argument t is rounded three times (the difference,
+// log2(e) / T, their product), 2^-24 |t| each; six roundings of sums in 32 bits.  The rest is in 64 bits.  What the arguments add to a sum, relative to it, is the
+// mean of |t| weighted with 2^t.  Of n terms, one t = 0 and the others not above it, that mean m is largest with all others at t = -(m + 1 / ln 2), where
+// n - 1 = ln 2 e m 2^m: 8.93 for a segment's 8192 (terms up to kSlack above what they are relative to lower it; several references of a segment,
+// several segments: the worst of them).  A token far above a flat tail comes to 1.1e-6 of the 1.72e-6.
+constexpr int kMostSummed = kMostTiles * kTileLogits;
+static_assert(kMostSummed <= 8192, "the mean of |t| is below 9 up to here");
+constexpr double kLseError = .693148 * 3 * 9 * 5.9605e-8 + 2.3842e-7 + 6 * 5.9605e-8;
 constexpr float kSlack = 2.f;                     // how far (as a power of two) terms may be above what they are relative to
 
 struct ScanStat {
