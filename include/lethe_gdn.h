@@ -410,7 +410,8 @@ int lethe_gdn_reorder_states(const LetheGdnStates* states, int32_t count, int64_
  *   slot source[e] (zeros where that is -1).  Where source[e] is neither -1 nor a live slot, or no slot is left, target[e] = -1 and
  *   nothing is taken.  live_after = live and the slots taken.  source int64 or (source_64 = 0) int32.
  * compact: the m live slots become slots 0 to m - 1: the ones at or behind m, in their order, move to the free ones in front of m, in
- *   theirs; what lies behind is left as it was.  place[i] = the new slot of live slot i, -1 for others; *live_count = m. */
+ *   theirs; what lies behind is left as it was.  place[i] = the new slot of live slot i, -1 for others; *live_count = m.
+ * Results lie apart from live and source and from one another (refused otherwise), and all of these apart from the states' rows. */
 int lethe_gdn_fork_states(const LetheGdnStates* states, int32_t count, int64_t slots, const uint8_t* live, const void* source, int32_t source_64,
                           int64_t n, int64_t* target, uint8_t* live_after, int32_t* status, void* cuda_stream);
 int lethe_gdn_compact_states(const LetheGdnStates* states, int32_t count, int64_t slots, const uint8_t* live, int64_t* place,

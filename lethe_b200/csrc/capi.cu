@@ -313,6 +313,7 @@ extern "C" const char* lethe_gdn_strerror(int code) {
     case kErrDevice: return "the device that owns q could not be made current, or a buffer is not device memory of that GPU";
     case kErrSymbol: return "the address of the library's built-in workspace could not be looked up on this GPU";
     case kErrIndex: return "an index lay outside its range (status word: a parent or a source of states)";
+    case kErrShared: return "a result lies in the memory of what is read while it is written, or of another result";
     case kErrTooLarge: return "problem needs more workspace than the library's built-in 16 MiB (use lethe_gdn_forward)";
     default: break;
   }

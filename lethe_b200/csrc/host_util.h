@@ -22,7 +22,14 @@ enum : int {
   kErrDevice = 9,      // the device that owns the tensors could not be made current, or a buffer lives elsewhere
   kErrSymbol = 10,     // the address of the library's built-in workspace could not be looked up
   kErrIndex = 11,      // (status word) an index on the device lay outside its range
+  kErrShared = 12,     // a result lies in the memory of what is read while it is written, or of another result
 };
+
+// whether bytes [a, a + n) and [b, b + m) meet
+inline bool meet(const void* a, long long n, const void* b, long long m) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + m && y < x + n;
+}
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,

@@ -698,6 +698,11 @@ extern "C" int lethe_gdn_fork_states(const LetheGdnStates* states, int32_t count
   if (bad) return bad;
   if (slots <= 0 || slots > kMostSlots || n <= 0 || n > kMostEntries) return kErrDims;
   if (reinterpret_cast<uintptr_t>(source) % (source_64 ? 8 : 4) || reinterpret_cast<uintptr_t>(target) % 8) return kErrAlign;
+  // (one CTA writes the results while others still work out the plan)
+  const long long source_bytes = n * (source_64 ? 8 : 4);
+  if (meet(live_after, slots, live, slots) || meet(live_after, slots, source, source_bytes) || meet(target, 8 * n, live, slots) ||
+      meet(target, 8 * n, source, source_bytes) || meet(target, 8 * n, live_after, slots))
+    return kErrShared;
   PoolProblem p = {};
   p.source = source;
   p.source64 = source_64;
@@ -719,6 +724,7 @@ extern "C" int lethe_gdn_compact_states(const LetheGdnStates* states, int32_t co
   if (bad) return bad;
   if (slots <= 0 || slots > kMostSlots) return kErrDims;
   if ((reinterpret_cast<uintptr_t>(place) | reinterpret_cast<uintptr_t>(live_count)) % 8) return kErrAlign;
+  if (meet(place, 8 * slots, live, slots) || meet(live_count, 8, live, slots) || meet(live_count, 8, place, 8 * slots)) return kErrShared;
   PoolProblem p = {};
   p.place = reinterpret_cast<long long*>(place);
   p.live_count = reinterpret_cast<long long*>(live_count);
