@@ -370,7 +370,9 @@ int lethe_gdn_residual_norm_vjp(const LetheGdnResidualNormArgs* args, void* cuda
  * (0 without eos) and counts as finished.
  * logits [B, W, V] x_type, allowed bytes (non-zero: allowed), both with strides for group and beam (0: shared) in elements;
  * scores, penalty fp32 [B, W], finished bytes [B, W], out_* [B, k].  W, k from 1 to 64, V to 2^30, temperature 1e-6 to 1e6.
- * work: lethe_gdn_beam_work_bytes bytes on a 16-byte boundary, scratch of one call. */
+ * work: lethe_gdn_beam_work_bytes bytes on a 16-byte boundary, scratch of one call.
+ * Results and work lie apart from one another and from the inputs (refused otherwise for all but logits and allowed); with k = W out_scores may be scores
+ * or penalty, and out_finished may be finished. */
 typedef struct LetheGdnBeamArgs {
   int64_t B, V;
   int32_t W, k, x_type;

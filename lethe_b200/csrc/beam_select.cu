@@ -719,7 +719,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamPro
     const bool there = tid < n;
     const Entry e = m.sorted[tid];
     const int w = there ? beam_of(e) : 0, v = there ? token_of(e) : max(p.eos, 0);
-    p.out_scores[o] = there ? static_cast<float>(from_ordered(e.rank) * (p.penalty ? p.penalty[row0 + w] : 1.f)) : -INFINITY;
+    p.out_scores[o] = there ? static_cast<float>(from_ordered(e.rank) * m.penalty[w]) : -INFINITY;
     p.parents[o] = w;
     p.tokens[o] = v;
     if (p.out_finished) p.out_finished[o] = !there || v == p.eos || m.ended[w];
@@ -750,6 +750,29 @@ static ScanPlan scan_plan(long long B, int W, long long V, int k, int ty, bool a
 static bool beam_sizes(long long B, int W, long long V, int k, int ty) {
   return B > 0 && W > 0 && W <= kBeamMost && k > 0 && k <= kBeamMost && V > 0 && V <= (1ll << 30) && B <= (1ll << 24) && B * W <= (1ll << 24) &&
          ty >= LETHE_F32 && ty <= LETHE_F16 && B * W * ((V + 7) / kTileLogits + 1) < (1ll << 31);
+}
+
+// Whether a result lies where another group's input may still be read.  A group's CTA has its own in shared memory before it writes anything, so with as
+// many candidates as beams new scores may take the place of the old ones, and the same with marks.
+static bool beam_meets(const LetheGdnBeamArgs& a) {
+  struct Part {
+    const void* at;
+    long long bytes;
+    int e;
+  };
+  const long long beams = a.B * a.W, n = a.B * a.k;
+  const Part part[] = {{a.out_scores, 4 * n, 4}, {a.out_finished, n, 1}, {a.parents, 8 * n, 8}, {a.tokens, 8 * n, 8},
+                       {a.scores, 4 * beams, 4}, {a.penalty, 4 * beams, 4}, {a.finished, beams, 1}};
+  const long long work = static_cast<long long>(lethe_gdn_beam_work_bytes(a.B, a.W, a.V, a.k, a.x_type));
+  for (int i = 0; i < 7; ++i) {
+    if (!part[i].at) continue;
+    if (meet(part[i].at, part[i].bytes, a.work, work)) return true;
+    for (int j = i + 1; i < 4 && j < 7; ++j) {
+      const bool own = j >= 4 && part[i].at == part[j].at && part[i].e == part[j].e && a.k == a.W;
+      if (part[j].at && !own && meet(part[i].at, part[i].bytes, part[j].at, part[j].bytes)) return true;
+    }
+  }
+  return false;
 }
 
 template <int TY>
@@ -783,6 +806,7 @@ extern "C" int lethe_gdn_beam_select(const LetheGdnBeamArgs* a, void* stream) {
   const bool aligned = (reinterpret_cast<uintptr_t>(a->logits) | static_cast<uintptr_t>(a->logits_batch * e) | static_cast<uintptr_t>(a->logits_beam * e)) % 16 == 0;
   const ScanPlan plan = scan_plan(a->B, a->W, a->V, a->k, a->x_type, aligned);
   if (a->work_bytes < lethe_gdn_beam_work_bytes(a->B, a->W, a->V, a->k, a->x_type)) return kErrWorkspace;
+  if (beam_meets(*a)) return kErrShared;
   DeviceGuard guard(a->logits);
   if (!guard.ok) return kErrDevice;
   BeamProblem p;

@@ -6,7 +6,7 @@ import torch
 
 from lethe_b200 import _build, native
 
-from .test_beam_cabi_cpu import ONE, refused
+from .test_beam_cabi_cpu import ONE, beam, refused
 
 # The addresses are none: with a GPU, a call that is not refused would run on them.
 pytestmark = pytest.mark.skipif(torch.cuda.is_available(), reason="only where no kernel can be launched")
@@ -46,3 +46,31 @@ def test_compact_states(lib):
         refused(lib, call(**bad), b"memory of what is read")
     for good in (dict(), dict(place=0x20000 + S), dict(place=0x20000 - 8 * S), dict(count=0x20000 + S), dict(count=0x20000 - 8), dict(count=0x30000 + 8 * S)):
         passed(lib, call(**good))
+
+
+def test_beam_select(lib):
+    B, W = 2, 3
+    size = dict(scores=4, penalty=4, finished=1, out_scores=4, parents=8, tokens=8, out_finished=1)
+    at = dict(scores=0x20000, penalty=0x21000, finished=0x22000, out_scores=0x30000, parents=0x40000, tokens=0x50000, out_finished=0x60000, work=0x70000)
+    work_bytes = lambda k: lib.lethe_gdn_beam_work_bytes(B, W, 100, k, 0)      # noqa: E731
+    call = lambda k, **kw: lib.lethe_gdn_beam_select(ctypes.byref(beam(**{**at, **dict(B=B, W=W, k=k, eos=7, work_bytes=work_bytes(k)), **kw})), None)      # noqa: E731
+    rows = lambda n, k: size[n] * B * (W if n in ("scores", "penalty", "finished") else k)      # noqa: E731
+    outs, ins = ("out_scores", "parents", "tokens", "out_finished"), ("scores", "penalty", "finished")
+    for k in (3, 5):
+        passed(lib, call(k))
+        need = work_bytes(k)
+        for o in outs:
+            for other in (*ins, *outs):
+                if o == other:
+                    continue
+                # (results of eight bytes lie on boundaries of eight)
+                for place in (at[other], at[other] + (rows(other, k) - 1) // 8 * 8, at[other] - (rows(o, k) - 1) // 8 * 8):
+                    own = place == at[other] and k == W and (o, other) in (("out_scores", "scores"), ("out_scores", "penalty"), ("out_finished", "finished"))
+                    if own:
+                        passed(lib, call(k, **{o: place}))
+                    else:
+                        refused(lib, call(k, **{o: place}), b"memory of what is read")
+                passed(lib, call(k, **{o: at[other] + (rows(other, k) + 7) // 8 * 8}))
+        for n in (*ins, *outs):
+            refused(lib, call(k, **{n: at["work"] + need // 8 * 8 - 8}), b"memory of what is read")
+            passed(lib, call(k, **{n: at["work"] + need}))
