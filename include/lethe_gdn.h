@@ -420,7 +420,7 @@ int lethe_gdn_compact_states(const LetheGdnStates* states, int32_t count, int64_
                              int64_t* live_count, int32_t* status, void* cuda_stream);
 
 /* lethe_gdn_decode_step with a state of its own for what it writes: row b goes on from row source[b] of args->state [slots, H, K, V]
- * (-1: from zeros), and its new state is row b of out [B, H, K, V], memory apart from args->state.  source [B], int64 or
+ * (-1: from zeros), and its new state is row b of out [B, H, K, V], memory apart from everything else of the call (refused otherwise).  source [B], int64 or
  * (source_64 = 0) int32; one outside [-1, slots) gives NaN and a code in *status. */
 int lethe_gdn_decode_step_from(const LetheGdnDecodeArgs* args, int64_t slots, const void* source, int32_t source_64, float* out,
                                int32_t* status, void* cuda_stream);

@@ -328,6 +328,12 @@ extern "C" int lethe_gdn_decode_step_from(const LetheGdnDecodeArgs* a, int64_t s
   if (reinterpret_cast<uintptr_t>(source) % (source_64 ? 8 : 4) || reinterpret_cast<uintptr_t>(out) % 4 || reinterpret_cast<uintptr_t>(a->state) % 4) return kErrAlign;
   const uintptr_t in0 = reinterpret_cast<uintptr_t>(a->state), out0 = reinterpret_cast<uintptr_t>(out);
   if (out0 < in0 + slots * row && in0 < out0 + a->B * row) return kErrFlags;      // (a row may be read after another is written)
+  const int64_t heads = static_cast<int64_t>(a->B) * a->H, e = a->in_f32 ? 4 : 2, wide = heads * kDK, out_bytes = a->B * row;
+  if (meet(source, a->B * (source_64 ? 8 : 4), out, out_bytes) || meet(a->q, wide * e, out, out_bytes) || meet(a->k, wide * e, out, out_bytes) ||
+      meet(a->v, heads * a->V * e, out, out_bytes) || meet(a->o, heads * a->V * 2, out, out_bytes) ||
+      (a->gate != LETHE_GATE_NONE && meet(a->g, 4 * (a->gate == LETHE_GATE_CHANNEL ? wide : heads), out, out_bytes)) ||
+      (a->delta && meet(a->beta, 4 * heads, out, out_bytes)))
+    return kErrShared;
   DeviceGuard guard(a->state);
   if (!guard.ok) return kErrDevice;
   p.B = a->B;

@@ -4,7 +4,7 @@ import ctypes
 import pytest
 import torch
 
-from lethe_b200 import _build, native
+from lethe_b200 import _build, native, ops
 
 from .test_beam_cabi_cpu import ONE, beam, refused
 
@@ -19,6 +19,7 @@ def lib():
     L = native.lib()
     L.lethe_gdn_fork_states.argtypes = [P, I32, I64, P, P, I32, I64, P, P, P, P]
     L.lethe_gdn_compact_states.argtypes = [P, I32, I64, P, P, P, P, P]
+    L.lethe_gdn_decode_step_from.argtypes = [P, I64, P, I32, P, P, P]
     return L
 
 
@@ -74,3 +75,24 @@ def test_beam_select(lib):
         for n in (*ins, *outs):
             refused(lib, call(k, **{n: at["work"] + need // 8 * 8 - 8}), b"memory of what is read")
             passed(lib, call(k, **{n: at["work"] + need}))
+
+
+def test_decode_step_from(lib):
+    B, H, V = 2, 2, 64
+    base = dict(B=B, H=H, K=128, V=V, gate=2, delta=1, scale=1.0, q=0x1000000, k=0x1100000, v=0x1200000, g=0x1300000, beta=0x1400000, state=0x2000000, o=0x1500000)
+    out, row = 0x9000000, H * 128 * V * 4
+
+    def call(source=0x1600000, s64=1, **kw):
+        a = ops._DecodeArgs(**{**base, **kw})
+        return lib.lethe_gdn_decode_step_from(ctypes.byref(a), 4, source, s64, out, 0x1700000, None)
+    passed(lib, call())
+    size = dict(q=2 * B * H * 128, k=2 * B * H * 128, v=2 * B * H * V, g=4 * B * H * 128, beta=4 * B * H, o=2 * B * H * V)
+    for n, e in size.items():
+        for place in (out, out + B * row - 4, out - e + 4):
+            refused(lib, call(**{n: place}), b"memory of what is read")
+        for place in (out + B * row, out - e):
+            passed(lib, call(**{n: place}))
+    refused(lib, call(in_f32=1, q=out - size["q"]), b"memory of what is read")
+    refused(lib, call(source=out + 8), b"memory of what is read")
+    refused(lib, call(source=out - 8), b"memory of what is read")
+    passed(lib, call(source=out - 8, s64=0))
