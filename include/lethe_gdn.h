@@ -396,7 +396,7 @@ size_t lethe_gdn_beam_work_bytes(int64_t B, int32_t W, int64_t V, int32_t k, int
 int lethe_gdn_beam_select(const LetheGdnBeamArgs* args, void* cuda_stream);
 
 /* States of sequences: for each of `count` tensors a row of row_bytes bytes per sequence, of any type, at
- * data + group * group_stride + i * stride (bytes; whole rows do not overlap).  `states` is host memory, read during the call. */
+ * data + group * group_stride + i * stride (bytes; whole rows do not overlap), row_bytes up to 2^38.  `states` is host memory, read during the call. */
 typedef struct LetheGdnStates {
   void* data;
   int64_t row_bytes, stride, group_stride;

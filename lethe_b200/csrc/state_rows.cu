@@ -300,48 +300,52 @@ __global__ void __launch_bounds__(kRowThreads) reorder_kernel(const __grid_const
   }
 }
 
-// Groups of more than 32 rows: an item for each CTA, all of its threads.
+// Groups of more than 32 rows: an item at a time for each CTA, all of its threads.
+constexpr long long kMostWideCtas = 65536;
 __global__ void __launch_bounds__(kRowThreads) reorder_wide_kernel(const __grid_constant__ ReorderProblem p) {
   extern __shared__ __align__(128) unsigned char memory[];
   __shared__ int used[kMostBeams], sources[kMostBeams], to[kMostBeams], from[kMostBeams];
   const int tid = threadIdx.x;
   griddep_wait();
-  const Strip x = strip_of(p.plain, blockIdx.x);
-  long long parent = tid < p.W ? index_at(p.parents, p.parents64, x.group * p.W + tid) : tid;
-  if (parent < 0 || (tid < p.W && parent >= p.W)) {
-    *p.status = kErrIndex;
-    parent = tid;
-  }
-  used[tid] = 0;
-  __syncthreads();
-  const bool moves = tid < p.W && parent != tid;
-  if (moves) used[parent] = 1;
-  __syncthreads();
-  const bool source = used[tid];
-  unsigned both;
-  const unsigned at = block_scan(moves | source << 16, &both);
-  if (source) {
-    sources[at >> 16] = tid;
-    used[tid] = at >> 16;
-  }
-  __syncthreads();
-  if (moves) {
-    to[at & 0xffff] = tid;
-    from[at & 0xffff] = used[parent];
-  }
-  const int n = both & 0xffff, reads = static_cast<int>(both >> 16);
-  char* const rows = x.t->data + x.group * x.t->group + x.begin;
-  with_unit(x.t->unit, [&](auto u) {
-    using T = typename decltype(u)::T;
-    const int columns = x.width / static_cast<int>(sizeof(T));
-    T* const mine = reinterpret_cast<T*>(memory);
-    for (int i = tid; i < reads * columns; i += kRowThreads)
-      fetch(mine + i, reinterpret_cast<const T*>(rows + sources[i / columns] * x.t->stride) + i % columns);
-    asm volatile("cp.async.wait_all;" ::: "memory");
+  for (long long item = blockIdx.x; item < p.plain_items; item += gridDim.x) {
+    const Strip x = strip_of(p.plain, item);
+    long long parent = tid < p.W ? index_at(p.parents, p.parents64, x.group * p.W + tid) : tid;
+    if (parent < 0 || (tid < p.W && parent >= p.W)) {
+      *p.status = kErrIndex;
+      parent = tid;
+    }
+    used[tid] = 0;
     __syncthreads();
-    for (int i = tid; i < n * columns; i += kRowThreads)
-      reinterpret_cast<T*>(rows + to[i / columns] * x.t->stride)[i % columns] = mine[from[i / columns] * columns + i % columns];
-  });
+    const bool moves = tid < p.W && parent != tid;
+    if (moves) used[parent] = 1;
+    __syncthreads();
+    const bool source = used[tid];
+    unsigned both;
+    const unsigned at = block_scan(moves | source << 16, &both);
+    if (source) {
+      sources[at >> 16] = tid;
+      used[tid] = at >> 16;
+    }
+    __syncthreads();
+    if (moves) {
+      to[at & 0xffff] = tid;
+      from[at & 0xffff] = used[parent];
+    }
+    const int n = both & 0xffff, reads = static_cast<int>(both >> 16);
+    char* const rows = x.t->data + x.group * x.t->group + x.begin;
+    with_unit(x.t->unit, [&](auto u) {
+      using T = typename decltype(u)::T;
+      const int columns = x.width / static_cast<int>(sizeof(T));
+      T* const mine = reinterpret_cast<T*>(memory);
+      for (int i = tid; i < reads * columns; i += kRowThreads)
+        fetch(mine + i, reinterpret_cast<const T*>(rows + sources[i / columns] * x.t->stride) + i % columns);
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncthreads();
+      for (int i = tid; i < n * columns; i += kRowThreads)
+        reinterpret_cast<T*>(rows + to[i / columns] * x.t->stride)[i % columns] = mine[from[i / columns] * columns + i % columns];
+    });
+    __syncthreads();      // (the next item's lists and columns go where these are)
+  }
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -627,8 +631,8 @@ extern "C" int lethe_gdn_reorder_states(const LetheGdnStates* states, int32_t co
   if (bad) return bad;
   if (B <= 0 || W <= 0 || W > kMostBeams || B > (1ll << 30)) return kErrDims;
   if (reinterpret_cast<uintptr_t>(parents) % (parents_64 ? 8 : 4)) return kErrAlign;
-  for (int i = 0; i < count; ++i)
-    if (states[i].row_bytes / 128 + 1 > (1ll << 30) / kMostTensors / B) return kErrDims;
+  for (int i = 0; i < count; ++i)      // strips of a row are counted in 32 bits, those of all tensors in 64
+    if (states[i].row_bytes > (1ll << 38) || states[i].row_bytes / 128 + 1 > (1ll << 57) / B) return kErrDims;
   DeviceGuard guard(states[0].data);
   if (!guard.ok) return kErrDevice;
   const int sms = sm_count();
@@ -654,7 +658,8 @@ extern "C" int lethe_gdn_reorder_states(const LetheGdnStates* states, int32_t co
         all.t[all.count] = p.bulk.t[i];
         all.t[all.count++].first += p.plain_items;
       }
-      return launch_dependent(reorder_wide_kernel, dim3(static_cast<unsigned>(p.plain_items + more)), dim3(kRowThreads), kGroupBytes, st, p) == cudaSuccess ? kOk : kErrLaunch;
+      p.plain_items += more;
+      return launch_dependent(reorder_wide_kernel, dim3(static_cast<unsigned>(p.plain_items < kMostWideCtas ? p.plain_items : kMostWideCtas)), dim3(kRowThreads), kGroupBytes, st, p) == cudaSuccess ? kOk : kErrLaunch;
     }
     take_states(s, n, false, kPlainStrip, B, &p.plain, &p.plain_items);
     const int plain_bytes = p.plain_items ? kPlainWarps * W * 32 * 8 : 0;      // (units of 8 bytes at most)

@@ -1,4 +1,5 @@
-"""CPU: the C calls of decoding with several hypotheses refuse results in the memory of what other CTAs still read, before they touch a GPU."""
+"""CPU: the C calls of decoding with several hypotheses refuse results in the memory of what other CTAs still read, before they touch a GPU, and take
+states of any size that a GPU holds."""
 import ctypes
 
 import pytest
@@ -6,7 +7,7 @@ import torch
 
 from lethe_b200 import _build, native, ops
 
-from .test_beam_cabi_cpu import ONE, beam, refused
+from .test_beam_cabi_cpu import ONE, States, beam, refused
 
 # The addresses are none: with a GPU, a call that is not refused would run on them.
 pytestmark = pytest.mark.skipif(torch.cuda.is_available(), reason="only where no kernel can be launched")
@@ -17,6 +18,7 @@ I32, I64, P = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p
 def lib():
     _build.build()
     L = native.lib()
+    L.lethe_gdn_reorder_states.argtypes = [P, I32, I64, I32, P, I32, P, P]
     L.lethe_gdn_fork_states.argtypes = [P, I32, I64, P, P, I32, I64, P, P, P, P]
     L.lethe_gdn_compact_states.argtypes = [P, I32, I64, P, P, P, P, P]
     L.lethe_gdn_decode_step_from.argtypes = [P, I64, P, I32, P, P, P]
@@ -96,3 +98,13 @@ def test_decode_step_from(lib):
     refused(lib, call(source=out + 8), b"memory of what is read")
     refused(lib, call(source=out - 8), b"memory of what is read")
     passed(lib, call(source=out - 8, s64=0))
+
+
+def test_large_states(lib):
+    """12 MB rows of 512 groups, one row of 100 GB, more groups than a grid has CTAs."""
+    for W in (2, 4, 32, 33, 256):
+        for B, row in ((512, 12 << 20), (128, 32 << 20), (1, 100 << 30), (2, 1 << 37), (1 << 30, 1 << 10), (3, (5 << 30) + 4)):
+            s = (States * 2)(States(0x10000, row, row, row * W), States(0x10000 + row * W * B, 64, 64, 64 * W))
+            passed(lib, lib.lethe_gdn_reorder_states(s, 2, B, W, 0x20000, 1, 0x30000, None))
+        for B, row in ((1, (1 << 38) + 1), (1 << 30, 1 << 36)):
+            refused(lib, lib.lethe_gdn_reorder_states((States * 1)(States(0x10000, row, row, row * W)), 1, B, W, 0x20000, 1, 0x30000, None), b"sizes")
