@@ -17,7 +17,7 @@ void need_bool(const Tensor& t, const char* name) {
 // Selection
 // ---------------------------------------------------------------------------------------------
 std::tuple<Tensor, Tensor, Tensor, OptTensor> beam_select(const Tensor& logits, const Tensor& scores, const OptTensor& allowed_, const OptTensor& finished_,
-                                                          const OptTensor& penalty_, int64_t k, double temperature, std::optional<int64_t> eos) {
+                                                          const OptTensor& penalty_, std::optional<int64_t> k_, double temperature, std::optional<int64_t> eos) {
   return guarded([&]() -> std::tuple<Tensor, Tensor, Tensor, OptTensor> {
     need_cuda(logits);
     const Tensor allowed_in = opt(allowed_), finished_in = opt(finished_), penalty_in = opt(penalty_);
@@ -33,7 +33,7 @@ std::tuple<Tensor, Tensor, Tensor, OptTensor> beam_select(const Tensor& logits, 
     const at::IntArrayRef beams(shape2);
     need_shape(scores.sizes() == beams && (!finished_in.defined() || finished_in.sizes() == beams) && (!penalty_in.defined() || penalty_in.sizes() == beams),
                "scores, finished, penalty [B, W] for logits [B, W, V]");
-    if (k < 0) k = W;
+    const int64_t k = k_.value_or(W);
     if (W < 1 || W > kMostBeams || k < 1 || k > kMostBeams)
       fail("beam_select takes 1 to " + std::to_string(kMostBeams) + " beams and as many candidates (got " + std::to_string(W) + " and " + std::to_string(k) + ")");
     if (V < 1) fail("beam_select needs a vocabulary");

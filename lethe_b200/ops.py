@@ -739,7 +739,7 @@ def beam_select(logits: Tensor, scores: Tensor, k: int | None = None, *, tempera
     and count as finished.
 
     W and k from 1 to 64, V up to 2^30, temperature 1e-6 to 1e6.  Beams may have any strides.  Not differentiable."""
-    k, eos = -1 if k is None else int(k), None if eos is None else int(eos)
+    k, eos = None if k is None else int(k), None if eos is None else int(eos)
     if not torch._C._is_tracing():
         return BeamChoice(*native.ext().beam_select(logits, scores, allowed, finished, penalty, k, temperature, eos))
     got = _TracedCall.apply("beam_select", dict(k=k, temperature=float(temperature), eos=eos), None, logits, scores, allowed, finished, penalty)
