@@ -21,7 +21,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "_lib")
 LIB = os.path.join(LIBDIR, "liblethe_gdn.so")
 PROBE_SRC = os.path.join(ROOT, "tests", "native", "probe.cu")
-PROBE_SRCS = [PROBE_SRC, os.path.join(ROOT, "tests", "native", "look_probe.cu")]
+PROBE_SRCS = [PROBE_SRC, *(os.path.join(ROOT, "tests", "native", f) for f in ("look_probe.cu", "ring_probe.cu"))]
 PROBE_LIBDIR = os.path.join(ROOT, "tests", "native", "_lib")
 PROBE_LIB = os.path.join(PROBE_LIBDIR, "libletheprobe.so")
 TORCH_SRCS = [os.path.join(CSRC, f) for f in ("torch_ops.cpp", "torch_block.cpp", "torch_beam.cpp")]

@@ -11,17 +11,14 @@
 // and no thread touches the data.  Rows of other sizes go through registers in the other warps meanwhile.
 #include "elem.cuh"
 #include "host_util.h"
-#include "umma.cuh"
+#include "state_ring.cuh"
 
 namespace lg {
 
-constexpr int kRowThreads = 256, kCopyWarps = 4, kPlainWarps = kRowThreads / 32 - kCopyWarps;
+constexpr int kRowThreads = 256, kPlainWarps = kRowThreads / 32 - kCopyWarps;
 constexpr int kMostTensors = 32;            // of one launch
 constexpr int kMostBeams = 256, kMostSlots = 65536, kMostEntries = 4096;
 constexpr int kGroupBytes = 32768;          // a wide group's strips
-// Stages of a ring: as many strips on their way in as out.  A compaction of 543 MB (83 us at the copy rate) in us:
-// four rings of 8 KB strips 93, two of 16 KB 92, four of 2 KB 134, one of 16 KB with two strips on their way out 101, without rings, through registers, 98.
-constexpr int kStages = 6, kOut = kStages / 2;
 constexpr int kAllBytes = 208896, kMostStage = 8192;      // dynamic shared memory of a CTA; bytes of a stage where there are four rings
 constexpr int kSiteReorder = 811, kSiteCopy = 812;
 
@@ -103,87 +100,6 @@ __device__ __forceinline__ long long index_at(const void* p, int is64, long long
   return is64 ? static_cast<const long long*>(p)[i] : static_cast<const int*>(p)[i];
 }
 
-// ------------------------------------------------------------------------------------------------------------------
-// A warp's ring.  Lane 0 expects what comes; a stage is filled again when the stores out of it have read it.
-// ------------------------------------------------------------------------------------------------------------------
-struct LaneCopy {           // what a lane stores out of a stage
-  char* to;
-  uint32_t from, bytes;     // (0: nothing)
-};
-struct RingMemory {
-  uint64_t full[kCopyWarps][kStages];
-  LaneCopy copies[kCopyWarps][kStages][32];
-  int abort_flag;
-};
-
-struct Ring {
-  unsigned char* bytes;
-  uint64_t* full;
-  LaneCopy (*copies)[32];
-  CtaCtl ctl;
-  int stage_bytes, site;
-  uint32_t phases = 0, filled = 0;      // bit s: the parity that stage s is waited for next; loads into it that nobody has waited for
-
-  // (all threads of the CTA, in front of a barrier)
-  __device__ __forceinline__ Ring(RingMemory& m, unsigned char* memory, int stage_bytes, int* status, int site)
-      : bytes(memory + threadIdx.x / 32 % kCopyWarps * kStages * stage_bytes), full(m.full[threadIdx.x / 32 % kCopyWarps]),
-        copies(m.copies[threadIdx.x / 32 % kCopyWarps]), ctl{status, &m.abort_flag}, stage_bytes(stage_bytes), site(site) {
-    if (threadIdx.x < kCopyWarps * kStages) mbar_init(&m.full[0][0] + threadIdx.x, 1);
-    if (threadIdx.x == 0) m.abort_flag = 0;
-    fence_mbar_init();
-  }
-  __device__ __forceinline__ unsigned char* stage(int s) const { return bytes + s * stage_bytes; }
-  __device__ __forceinline__ void expect(int s, uint32_t n) {
-    if (threadIdx.x % 32 == 0) mbar_expect_tx(full + s, n);
-    filled |= 1u << s;
-    __syncwarp();
-  }
-  __device__ __forceinline__ void arrive(int s) {
-    if (!((filled >> s) & 1)) return;
-    mbar_wait_warp(full + s, (phases >> s) & 1, ctl, site);
-    phases ^= 1u << s;
-    filled &= ~(1u << s);
-  }
-  // Whether a wait gave up.  What is still on its way is waited for, with a limit, before the CTA may end.
-  __device__ __forceinline__ bool gave_up() {
-    if (!*ctl.abort_flag) return false;
-    const long long t0 = clock64();
-    for (int s = 0; s < kStages; ++s)
-      while (((filled >> s) & 1) && !mbar_try(full + s, (phases >> s) & 1) && clock64() - t0 < ctl.limit) {
-      }
-    return true;
-  }
-
-  // Step after step: load(s, &copy) issues the next one's copies into stage s and says what the lane stores out of it, or that there is none.
-  template <typename Load> __device__ __forceinline__ void run(Load load) {
-    const int lane = threadIdx.x % 32;
-    int loaded = 0, into = 0, at = 0;
-    bool more = true;
-    auto one = [&] {
-      LaneCopy c;
-      more = load(into, &c);
-      if (!more) return;
-      copies[into][lane] = c;
-      into = into + 1 == kStages ? 0 : into + 1;
-      ++loaded;
-    };
-    while (more && loaded < kStages - kOut) one();
-    for (int stored = 0; stored < loaded; ++stored) {
-      if (more) {      // (the stage that `kOut` steps ago was stored from)
-        asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kOut - 1) : "memory");
-        __syncwarp();
-        one();
-      }
-      arrive(at);
-      if (gave_up()) break;
-      const LaneCopy c = copies[at][lane];
-      if (c.bytes) asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(c.to), "r"(c.from), "r"(c.bytes) : "memory");
-      bulk_commit();
-      at = at + 1 == kStages ? 0 : at + 1;
-    }
-    bulk_wait_read();
-  }
-};
 // the copying warps' items: first those of one warp of every CTA
 __device__ __forceinline__ long long first_item() { return static_cast<long long>(threadIdx.x / 32) * gridDim.x + blockIdx.x; }
 
