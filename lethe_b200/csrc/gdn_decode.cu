@@ -47,7 +47,7 @@ __device__ __forceinline__ long long slot_of(const DecodeProblem& p, int bh) {
   const int b = bh / p.H;
   const long long s = p.source64 ? static_cast<const long long*>(p.source)[b] : static_cast<const int*>(p.source)[b];
   if (s >= -1 && s < p.slots) return s;
-  *p.status = kErrIndex;
+  report(p.status, kErrIndex);
   return -2;
 }
 

@@ -1,6 +1,7 @@
 // Rings of strips in shared memory, global memory to global memory by bulk copies: a warp that issues them has a ring of its own, and no thread touches
 // the data.
 #pragma once
+#include "host_util.h"
 #include "umma.cuh"
 
 namespace lg {
@@ -50,6 +51,7 @@ struct Ring {
     const uint32_t bit = filled & (1u << s);
     if (bit) mbar_wait_warp(full + s, (phases >> s) & 1, ctl, site);
     if (__any_sync(~0u, *ctl.abort_flag)) {
+      atomicCAS(ctl.status, kErrIndex, site);      // (an index outside spoils its own rows only: the wait is what the host has to hear of)
       const long long t0 = clock64();
       for (int i = 0; i < kStages; ++i)
         while (((filled >> i) & 1) && !mbar_try(full + i, (phases >> i) & 1) && clock64() - t0 < ctl.limit) {

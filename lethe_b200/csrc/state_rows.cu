@@ -128,7 +128,7 @@ __device__ __forceinline__ long long parent_of(const ReorderProblem& p, long lon
 __device__ __forceinline__ Parents parents_of(const ReorderProblem& p, long long x) {
   const int lane = threadIdx.x % 32;
   if (x < 0 || (lane < p.W && x >= p.W)) {
-    *p.status = kErrIndex;
+    report(p.status, kErrIndex);
     x = lane;
   }
   Parents r;
@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(kRowThreads) reorder_wide_kernel(const __grid_
     const Strip x = strip_of(p.plain, item);
     long long parent = tid < p.W ? index_at(p.parents, p.parents64, x.group * p.W + tid) : tid;
     if (parent < 0 || (tid < p.W && parent >= p.W)) {
-      *p.status = kErrIndex;
+      report(p.status, kErrIndex);
       parent = tid;
     }
     used[tid] = 0;

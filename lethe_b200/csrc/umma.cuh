@@ -30,6 +30,9 @@ struct CtaCtl {
   long long limit = kWaitLimitCycles;   // cycles a wait may spin before it gives up
 };
 
+// The first code stays until the host has read it.
+__device__ __forceinline__ void report(int* status, int code) { atomicCAS(status, 0, code); }
+
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
@@ -83,7 +86,7 @@ __device__ __forceinline__ void mbar_wait(uint64_t* bar, uint32_t parity, const 
   while (!mbar_try(bar, parity)) {
     if (*ctl.abort_flag) return;
     if (clock64() - t0 > ctl.limit) {
-      atomicCAS(ctl.status, 0, code);
+      report(ctl.status, code);
       *ctl.abort_flag = 1;
       return;
     }

@@ -8,12 +8,13 @@ namespace lg {
 
 constexpr int kProbeStrip = 512, kProbeStrips = 8;
 
-__global__ void __launch_bounds__(256) ring_kernel(const char* in, char* out, int* status, int steps, int starved, int hole, long long limit, int* steps_of) {
+__global__ void __launch_bounds__(256) ring_kernel(const char* in, char* out, int* status, int steps, int starved, int hole, long long limit, int* steps_of, int index) {
   __shared__ __align__(128) unsigned char memory[kCopyWarps * kStages * kProbeStrip];
   __shared__ RingMemory rings;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   Ring ring(rings, memory, kProbeStrip, status, 812);
   ring.ctl.limit = limit;
+  if (index == 1 && threadIdx.x == 255) report(status, kErrIndex);
   __syncthreads();
   if (warp >= kCopyWarps) return;
   int i = 0;
@@ -29,15 +30,16 @@ __global__ void __launch_bounds__(256) ring_kernel(const char* in, char* out, in
     return true;
   });
   steps_of[threadIdx.x] = i;
+  if (index == 2) report(status, kErrIndex);
 }
 
 }  // namespace lg
 
-extern "C" int lethe_probe_ring(const void* in, void* out, int* status, int steps, int starved, int hole, long long limit_cycles, int* steps_of, void* stream) {
+extern "C" int lethe_probe_ring(const void* in, void* out, int* status, int steps, int starved, int hole, long long limit_cycles, int* steps_of, int index, void* stream) {
   using namespace lg;
   if (!in || !out || !status || !steps_of) return kErrNull;
   if (steps < 1 || steps > 200000 || starved < -1 || starved > kCopyWarps || limit_cycles < 1000 || limit_cycles > 200000000LL) return kErrDims;
   if ((reinterpret_cast<uintptr_t>(in) | reinterpret_cast<uintptr_t>(out)) % 16) return kErrAlign;
-  ring_kernel<<<1, 256, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<const char*>(in), static_cast<char*>(out), status, steps, starved, hole, limit_cycles, steps_of);
+  ring_kernel<<<1, 256, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<const char*>(in), static_cast<char*>(out), status, steps, starved, hole, limit_cycles, steps_of, index);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
 }
