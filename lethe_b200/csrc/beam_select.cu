@@ -89,8 +89,8 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// exp(t) for t <= 0 in 64 bits: 2^n e^f with n the nearest whole number to t / ln 2, and e^f by its power series to the twelfth power (the
-// next term is below 2^-52); what is below e^-700 is zero.
+// exp(t) for t <= 0 in 64 bits: 2^n e^f with n the nearest whole number to t / ln 2, f = t - n ln 2 by Cody and Waite's reduction (ln 2 as its value in
+// 64 bits and what that leaves out), and e^f by its power series to the twelfth power (the next term is below 2^-52); what is below e^-700 is zero.
 __device__ __forceinline__ double exp_below(double t) {
   t = fmax(t, -700.);
   const double n = rint(t * 1.4426950408889634), f = fma(n, -2.3190468138462996e-17, fma(n, -0.69314718055994529, t));
@@ -733,7 +733,8 @@ struct ScanPlan {
 // Segments as long as they can be with a warp for each on the GPU at once, up to kMostTiles; more bins than candidates in each.  Every list costs
 // its look for candidates, so one tile each is too short, and longer ones than 8 leave too little to share out.  Passes in us with 1, 2, 4, 6, 8 tiles:
 // 64 x 8 x 131072 78, 53, 41, 42, 36 (chosen: 8; an earlier form with 14 and 26: 49, 60); 16 x 8 x 65536 15.8, 13.5, 13.0, 14.8, 13.4 (2).
-// A row that does not begin on a 16-byte boundary may reach into one more tile.
+// A row that does not begin on a 16-byte boundary may reach into one more tile.  "At once" is counted with a B200's 148 SMs, whatever GPU is current, and with the CTAs of
+// 16-bit types, since the workspace has to be the same wherever it is asked for: fp32 rows, 11 CTAs an SM, with 3256 to 4144 segments take a second wave.
 static ScanPlan scan_plan(long long B, int W, long long V, int k, int ty, bool aligned) {
   const long long past = aligned ? 0 : 16 / elem_bytes(ty) - 1, row = (V + past + kTileLogits - 1) / kTileLogits;
   const long long even = (V + kTileLogits - 1) / kTileLogits, held = 148 * kScanWarps * kScanCtas / (B * W);      // (for every row)
